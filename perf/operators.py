@@ -203,7 +203,8 @@ def prepare(case, seed):
             st["pools"] = [torch.randint(0, 256, (pool, PAGE), generator=g, device=dev, dtype=torch.uint8) for _ in range(2)]
         else:
             st["pools"] = [torch.randn((pool, BLOCK, D), generator=g, device=dev).to(torch.bfloat16) for _ in range(2)]
-        perm = torch.randperm(pool, generator=g, device=dev)[:2 * n].tolist()
+        # page ids as an allocator on the host keeps them
+        perm = torch.randperm(pool, generator=g, device=dev)[:2 * n].to(torch.int32).cpu().numpy()
         st["src"], st["dst"] = perm[:n], perm[n:]
         return st
     hq, hkv, L = case["hq"], case["hkv"], case["length"]
@@ -316,7 +317,7 @@ def _attend(st):
 
 def _copy(st):
     dev = st["pools"][0].device
-    src, dst = torch.tensor(st["src"], device=dev), torch.tensor(st["dst"], device=dev)
+    src, dst = (torch.from_numpy(st[n]).to(dev, torch.int64) for n in ("src", "dst"))
     for pool in st["pools"]:
         pool[dst] = pool[src]
     return list(st["pools"])
@@ -431,7 +432,7 @@ def exact(case, seed):
         out = []
         for pool in st["pools"]:
             new = pool.clone()
-            for a, b in zip(st["src"], st["dst"]):
+            for a, b in zip(st["src"].tolist(), st["dst"].tolist()):
                 new[b].copy_(pool[a])
             out.append(new)
         return out
