@@ -20,6 +20,8 @@ HEAD_DIM = 128
 BLOCK = 64
 MAX_BATCH = 64
 STATIC_SCRATCH_BYTES = 48 << 20
+PAGE4_BYTES = 4352  # a 64-token page of one KV head held in 4 bits: codes, then scales
+MAX_POOLS = 8
 
 CA_OK = 0
 CA_ERR_INVALID = -1
@@ -60,8 +62,14 @@ EXPORTED = (
     "ca_attn_fwd_noalloc",
     "ca_attn_decode",
     "ca_attn_decode_workspace_size",
+    "ca_append_q4",
+    "ca_gather_q4",
+    "ca_attn_fwd_q4",
+    "ca_attn_decode_q4",
+    "ca_copy_pages",
     "ca_rope_apply",
     "ca_rope_qk",
+    "ca_norm_rope_qk",
     "ca_rmsnorm",
     "ca_swiglu",
 )
@@ -104,6 +112,25 @@ class SeqLayout(ctypes.Structure):
         ("stride_b", ctypes.c_int64),
         ("stride_t", ctypes.c_int64),
         ("stride_h", ctypes.c_int64),
+    ]
+
+
+class Kv4Layout(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("stride_page", ctypes.c_int64),
+        ("page_table", ctypes.c_void_p),
+        ("page_table_stride", ctypes.c_int64),
+        ("num_pages", ctypes.c_int64),
+    ]
+
+
+class PagePool(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("page_bytes", ctypes.c_int64),
+        ("stride_page", ctypes.c_int64),
+        ("num_pages", ctypes.c_int64),
     ]
 
 
@@ -161,6 +188,15 @@ _SIGNATURES = {
     "ca_rope_apply": (ctypes.c_int, [_P(SeqLayout), _P(SeqLayout), _i32, _i32, _i32, _vp, _vp, _vp]),
     "ca_rope_qk": (ctypes.c_int, [_P(SeqLayout), _P(SeqLayout), _i32, _P(SeqLayout), _P(SeqLayout), _i32, _i32, _i32,
                                   _vp, _vp, _vp]),
+    "ca_norm_rope_qk": (ctypes.c_int, [_P(SeqLayout), _P(SeqLayout), _i32, _vp, _P(SeqLayout), _P(SeqLayout), _i32,
+                                       _vp, _i32, _i32, _vp, _vp, _i64, _f32, _vp]),
+    "ca_append_q4": (ctypes.c_int, [_P(Dims), _P(SeqLayout), _P(SeqLayout), _P(Kv4Layout), _P(Kv4Layout), _vp, _vp]),
+    "ca_gather_q4": (ctypes.c_int, [_P(Dims), _P(Kv4Layout), _P(Kv4Layout), _vp, _vp, _vp, _vp]),
+    "ca_attn_fwd_q4": (ctypes.c_int, [_P(Dims), _P(SeqLayout), _P(Kv4Layout), _P(Kv4Layout), _vp, _i64, _vp, _vp,
+                                      _f32, _P(SeqLayout), _vp, _i32, _vp, _i64, _vp]),
+    "ca_attn_decode_q4": (ctypes.c_int, [_P(Dims), _P(SeqLayout), _P(Kv4Layout), _P(Kv4Layout), _vp, _f32,
+                                         _P(SeqLayout), _vp, _i32, _vp, _i64, _vp]),
+    "ca_copy_pages": (ctypes.c_int, [_P(PagePool), _i32, _vp, _vp, _i32, _vp]),
     "ca_rmsnorm": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i32, _f32, _vp]),
     "ca_swiglu": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _vp]),
 }

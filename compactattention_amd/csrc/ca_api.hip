@@ -6,12 +6,14 @@
 
 #include <cstdarg>
 #include <cstdio>
+#include <cstdlib>
 #include <cstring>
 #include <mutex>
 #include <string>
 
 #include "../../include/compactattn.h"
 #include "ca_kernels.h"
+#include "ca_kv4.h"
 
 namespace {
 
@@ -226,6 +228,66 @@ int scratch_for_stream(hipStream_t stream, void** ptr) {
     }
     *ptr = g_scratch_ptr[dev];
     return CA_OK;
+}
+
+}  // namespace
+
+namespace {
+
+int check_kv4(const ca_kv4_layout* l, const char* name, int blocks, ca::Kv4Addr* out) {
+    if (l == nullptr || l->data == nullptr || l->page_table == nullptr)
+        return fail(CA_ERR_INVALID, "%s, its data or its page_table is NULL", name);
+    if (!aligned16(l->data)) return fail(CA_ERR_INVALID, "%s data must be 16-byte aligned", name);
+    if (!aligned4(l->page_table)) return fail(CA_ERR_INVALID, "%s page_table misaligned", name);
+    if (l->stride_page < CA_PAGE4_BYTES || l->stride_page % 16)
+        return fail(CA_ERR_INVALID, "%s stride_page=%lld must be a multiple of 16 and at least %d", name,
+                    (long long)l->stride_page, CA_PAGE4_BYTES);
+    if (l->page_table_stride < blocks)
+        return fail(CA_ERR_INVALID, "%s page_table_stride=%lld < blocks per row %d", name, (long long)l->page_table_stride, blocks);
+    if (l->num_pages < 1 || l->num_pages > INT32_MAX)
+        return fail(CA_ERR_INVALID, "%s num_pages=%lld outside [1, 2^31)", name, (long long)l->num_pages);
+    *out = ca::Kv4Addr{static_cast<uint8_t*>(l->data), l->stride_page, l->page_table, l->page_table_stride,
+                       static_cast<int32_t>(l->num_pages - 1)};
+    return CA_OK;
+}
+
+// The rows of an append to or a read from a 4-bit cache; blocks: how many a row must have.
+int check_rows4(const ca_dims* d, const int32_t* start, int* blocks) {
+    if (d == nullptr || start == nullptr) return fail(CA_ERR_INVALID, "dims or start_host is NULL");
+    if (d->batch < 1 || d->batch > CA_MAX_BATCH)
+        return fail(d->batch < 1 ? CA_ERR_INVALID : CA_ERR_LIMIT, "batch=%d outside [1, %d]", d->batch, CA_MAX_BATCH);
+    if (d->q_len < 1 || d->num_kv_heads < 1)
+        return fail(CA_ERR_INVALID, "q_len=%d and num_kv_heads=%d must be positive", d->q_len, d->num_kv_heads);
+    if (d->kv_cap < 1 || (int64_t)d->kv_cap * CA_BLOCK > (int64_t)1 << 30)
+        return fail(d->kv_cap < 1 ? CA_ERR_INVALID : CA_ERR_LIMIT, "kv_cap=%d blocks outside [1, 2^24]", d->kv_cap);
+    if ((int64_t)d->batch * d->num_kv_heads > INT32_MAX / d->q_len) return fail(CA_ERR_LIMIT, "too many rows");
+    *blocks = 0;
+    for (int b = 0; b < d->batch; ++b) {
+        const int64_t end = (int64_t)start[b] + d->q_len;
+        if (start[b] < 0 || end > (int64_t)d->kv_cap * CA_BLOCK)
+            return fail(CA_ERR_INVALID, "tokens [%d, %lld) of request %d outside a cache of %d blocks", start[b],
+                        (long long)end, b, d->kv_cap);
+        *blocks = max(*blocks, static_cast<int>((end + CA_BLOCK - 1) / CA_BLOCK));
+    }
+    return CA_OK;
+}
+
+// The arguments that the two attention entry points over a 4-bit cache share, and the launch.
+int attn4(ca::AttnArgs& a, const ca::Kv4Addr& k, const ca::Kv4Addr& v, float scale, float* lse, int num_splits,
+          int max_splits, int most, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (!(scale > 0.0f)) return fail(CA_ERR_INVALID, "scale must be positive");
+    if (num_splits < 0 || num_splits > most) return fail(CA_ERR_INVALID, "num_splits=%d outside [0, %d]", num_splits, most);
+    const int64_t need = ca::attn_workspace_bytes(a.s, max_splits);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
+        return fail(CA_ERR_WORKSPACE, "num_splits=%d needs a 16-byte aligned workspace of %lld bytes (got %lld)",
+                    num_splits, (long long)need, (long long)workspace_bytes);
+    a.scale = scale;
+    a.lse = lse;
+    a.num_splits = num_splits;
+    a.workspace = workspace;
+    hipError_t e = ca::launch_attn4(a, k, v, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "4-bit attn launch");
+    return ok();
 }
 
 }  // namespace
@@ -630,6 +692,124 @@ int ca_attn_fwd(const ca_dims* dims, const ca_seq_layout* q, const ca_kv_layout*
     return ok();
 }
 
+int ca_attn_fwd_q4(const ca_dims* dims, const ca_seq_layout* q, const ca_kv4_layout* k, const ca_kv4_layout* v,
+                   const int32_t* table, int64_t table_stride, const int32_t* counts,
+                   const int32_t* past_blocks_host, float scale, const ca_seq_layout* out, float* lse,
+                   int32_t num_splits, void* workspace, int64_t workspace_bytes, void* stream) {
+    ca::AttnArgs a{};
+    ca::Kv4Addr ka, va;
+    int max_nkb = 0, rc;
+    if ((rc = check_dims(dims, past_blocks_host, &a.s, &a.pb, &max_nkb)) != CA_OK) return rc;
+    if ((rc = check_seq(q, "q", &a.q)) != CA_OK) return rc;
+    if ((rc = check_seq(out, "out", &a.out)) != CA_OK) return rc;
+    if ((rc = check_kv4(k, "k", max_nkb, &ka)) != CA_OK) return rc;
+    if ((rc = check_kv4(v, "v", max_nkb, &va)) != CA_OK) return rc;
+    if (table == nullptr || counts == nullptr) return fail(CA_ERR_INVALID, "table and counts are required");
+    if (!aligned4(table) || !aligned4(counts)) return fail(CA_ERR_INVALID, "table and counts must be 4-byte aligned");
+    if (table_stride < a.s.cap) return fail(CA_ERR_INVALID, "table_stride=%lld < kv_cap=%d", (long long)table_stride, a.s.cap);
+    if ((int64_t)a.s.Lq * a.s.G > (int64_t)1 << 24) return fail(CA_ERR_LIMIT, "q_len * group too large");
+    a.table = table;
+    a.table_stride = table_stride;
+    a.counts = counts;
+    const int max_splits = num_splits == 0 ? ca::attn_pick_splits(a.s, a.pb, nullptr) : num_splits;
+    return attn4(a, ka, va, scale, lse, num_splits, max_splits, ca::kMaxPrefillSplits, workspace, workspace_bytes, stream);
+}
+
+int ca_attn_decode_q4(const ca_dims* dims, const ca_seq_layout* q, const ca_kv4_layout* k, const ca_kv4_layout* v,
+                      const int32_t* kv_len_host, float scale, const ca_seq_layout* out, float* lse,
+                      int32_t num_splits, void* workspace, int64_t workspace_bytes, void* stream) {
+    ca::AttnArgs a{};
+    ca::Kv4Addr ka, va;
+    int max_nkb = 0, rc;
+    if ((rc = check_decode_dims(dims, kv_len_host, &a.s, &a.pb, &max_nkb)) != CA_OK) return rc;
+    if ((rc = check_seq(q, "q", &a.q)) != CA_OK) return rc;
+    if ((rc = check_seq(out, "out", &a.out)) != CA_OK) return rc;
+    if ((rc = check_kv4(k, "k", max_nkb, &ka)) != CA_OK) return rc;
+    if ((rc = check_kv4(v, "v", max_nkb, &va)) != CA_OK) return rc;
+    a.kv_len = kv_len_host;
+    const int max_splits = num_splits == 0 ? ca::attn_pick_splits(a.s, a.pb, kv_len_host) : num_splits;
+    return attn4(a, ka, va, scale, lse, num_splits, max_splits, ca::kMaxDecodeSplits, workspace, workspace_bytes, stream);
+}
+
+int ca_append_q4(const ca_dims* dims, const ca_seq_layout* k_new, const ca_seq_layout* v_new,
+                 const ca_kv4_layout* k_cache, const ca_kv4_layout* v_cache, const int32_t* start_host,
+                 void* stream) {
+    ca::SeqAddr kn, vn;
+    ca::Kv4Addr kc, vc;
+    int blocks = 0, rc;
+    if ((rc = check_rows4(dims, start_host, &blocks)) != CA_OK) return rc;
+    if ((rc = check_seq(k_new, "k_new", &kn)) != CA_OK) return rc;
+    if ((rc = check_seq(v_new, "v_new", &vn)) != CA_OK) return rc;
+    if ((rc = check_kv4(k_cache, "k_cache", blocks, &kc)) != CA_OK) return rc;
+    if ((rc = check_kv4(v_cache, "v_cache", blocks, &vc)) != CA_OK) return rc;
+    hipError_t e = ca::launch_append4(dims->batch, dims->q_len, dims->num_kv_heads, start_host, kn, vn, kc, vc,
+                                      static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "append_q4 launch");
+    return ok();
+}
+
+int ca_gather_q4(const ca_dims* dims, const ca_kv4_layout* k_cache, const ca_kv4_layout* v_cache,
+                 const int32_t* start_host, void* k_out, void* v_out, void* stream) {
+    ca::Kv4Addr kc, vc;
+    int blocks = 0, rc;
+    if ((rc = check_rows4(dims, start_host, &blocks)) != CA_OK) return rc;
+    if ((v_cache == nullptr) != (v_out == nullptr))
+        return fail(CA_ERR_INVALID, "v_cache and v_out are given together or not at all");
+    if ((rc = check_kv4(k_cache, "k_cache", blocks, &kc)) != CA_OK) return rc;
+    if (v_cache != nullptr && (rc = check_kv4(v_cache, "v_cache", blocks, &vc)) != CA_OK) return rc;
+    if (k_out == nullptr || !aligned16(k_out) || !aligned16(v_out))
+        return fail(CA_ERR_INVALID, "k_out is required, and the outputs must be 16-byte aligned");
+    hipError_t e = ca::launch_gather4(dims->batch, dims->q_len, dims->num_kv_heads, start_host, kc,
+                                      v_cache != nullptr ? &vc : nullptr, static_cast<uint16_t*>(k_out),
+                                      static_cast<uint16_t*>(v_out), static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "gather_q4 launch");
+    return ok();
+}
+
+int ca_copy_pages(const ca_page_pool* pools, int32_t n_pools, const int32_t* src_host, const int32_t* dst_host,
+                  int32_t n, void* stream) {
+    if (pools == nullptr || n_pools < 1 || n_pools > CA_MAX_POOLS)
+        return fail(CA_ERR_INVALID, "n_pools=%d outside [1, %d] or pools NULL", n_pools, CA_MAX_POOLS);
+    if (n < 0) return fail(CA_ERR_INVALID, "n=%d < 0", n);
+    ca::PagePool addr[CA_MAX_POOLS];
+    int64_t pages = INT64_MAX;
+    for (int i = 0; i < n_pools; ++i) {
+        const ca_page_pool& p = pools[i];
+        if (p.data == nullptr || !aligned16(p.data)) return fail(CA_ERR_INVALID, "pool %d: data is NULL or not 16-byte aligned", i);
+        if (p.page_bytes < 16 || p.page_bytes % 16 || p.stride_page % 16 || p.stride_page < p.page_bytes)
+            return fail(CA_ERR_INVALID, "pool %d: page_bytes=%lld and stride_page=%lld must be multiples of 16, the stride no less",
+                        i, (long long)p.page_bytes, (long long)p.stride_page);
+        if (p.page_bytes > (int64_t)1 << 22) return fail(CA_ERR_LIMIT, "pool %d: page_bytes=%lld above 2^22", i, (long long)p.page_bytes);
+        if (p.num_pages < 1) return fail(CA_ERR_INVALID, "pool %d has no pages", i);
+        addr[i] = ca::PagePool{static_cast<uint8_t*>(p.data), p.page_bytes, p.stride_page};
+        if (p.num_pages < pages) pages = p.num_pages;
+    }
+    if (n == 0) return ok();
+    if (src_host == nullptr || dst_host == nullptr) return fail(CA_ERR_INVALID, "src_host and dst_host are required");
+    for (int i = 0; i < n; ++i)
+        if (src_host[i] < 0 || src_host[i] >= pages || dst_host[i] < 0 || dst_host[i] >= pages)
+            return fail(CA_ERR_INVALID, "copy %d: page %d to page %d outside [0, %lld)", i, src_host[i], dst_host[i], (long long)pages);
+    // one bit a page: written
+    const int64_t words = (pages + 63) / 64;
+    uint64_t* written = static_cast<uint64_t*>(std::calloc(static_cast<size_t>(words), sizeof(uint64_t)));
+    if (written == nullptr) return fail(CA_ERR_LIMIT, "no host memory to check %lld pages", (long long)pages);
+    auto bit = [](int32_t page) { return uint64_t{1} << (page & 63); };
+    int twice = -1, both = -1;
+    for (int i = 0; i < n && twice < 0; ++i) {
+        uint64_t& w = written[dst_host[i] >> 6];
+        if (w & bit(dst_host[i])) twice = dst_host[i];
+        w |= bit(dst_host[i]);
+    }
+    for (int i = 0; i < n && both < 0; ++i)
+        if (written[src_host[i] >> 6] & bit(src_host[i])) both = src_host[i];
+    std::free(written);
+    if (twice >= 0) return fail(CA_ERR_INVALID, "page %d is written twice", twice);
+    if (both >= 0) return fail(CA_ERR_INVALID, "page %d is read and written", both);
+    hipError_t e = ca::launch_copy_pages(addr, n_pools, src_host, dst_host, n, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "copy_pages launch");
+    return ok();
+}
+
 int ca_attn_fwd_noalloc(const ca_dims* dims, const ca_seq_layout* q, const ca_kv_layout* k,
                         const ca_kv_layout* v, const int32_t* table, int64_t table_stride,
                         const int32_t* counts, const int32_t* past_blocks_host, float scale,
@@ -746,6 +926,33 @@ int ca_rope_qk(const ca_seq_layout* q, const ca_seq_layout* q_out, int32_t q_hea
                const float* sin, void* stream) {
     if (k_heads < 1) return fail(CA_ERR_INVALID, "k_heads must be positive");
     return rope(q, q_out, q_heads, k, k_out, k_heads, batch, len, cos, sin, stream);
+}
+
+int ca_norm_rope_qk(const ca_seq_layout* q, const ca_seq_layout* q_out, int32_t q_heads, const uint16_t* q_weight,
+                    const ca_seq_layout* k, const ca_seq_layout* k_out, int32_t k_heads, const uint16_t* k_weight,
+                    int32_t batch, int32_t len, const float* cos, const float* sin, int64_t cs_stride_b, float eps,
+                    void* stream) {
+    ca::SeqAddr qa, qo, ka, ko;
+    int rc;
+    if ((rc = check_seq(q, "q", &qa)) != CA_OK) return rc;
+    if ((rc = check_seq(q_out, "q_out", &qo)) != CA_OK) return rc;
+    if ((rc = check_seq(k, "k", &ka)) != CA_OK) return rc;
+    if ((rc = check_seq(k_out, "k_out", &ko)) != CA_OK) return rc;
+    if (batch < 1 || len < 1 || q_heads < 1 || k_heads < 1)
+        return fail(CA_ERR_INVALID, "batch, len and heads must be positive");
+    if (q_heads > 65535 || k_heads > 65535 ||
+        (int64_t)batch * len >= ((int64_t)1 << 31) / ((q_heads + 7) / 8 + (k_heads + 7) / 8))
+        return fail(CA_ERR_LIMIT, "too many heads");
+    if (q_weight == nullptr || k_weight == nullptr || cos == nullptr || sin == nullptr)
+        return fail(CA_ERR_INVALID, "the weights, cos and sin are required");
+    if (!aligned16(q_weight) || !aligned16(k_weight) || !aligned16(cos) || !aligned16(sin))
+        return fail(CA_ERR_INVALID, "the weights, cos and sin must be 16-byte aligned");
+    if (cs_stride_b < 0 || cs_stride_b % 4) return fail(CA_ERR_INVALID, "cs_stride_b must be a non-negative multiple of 4");
+    if (!(eps >= 0.0f)) return fail(CA_ERR_INVALID, "eps must be >= 0");
+    hipError_t e = ca::launch_norm_rope(qa, qo, q_heads, q_weight, ka, ko, k_heads, k_weight, cos, sin, cs_stride_b,
+                                        batch, len, eps, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "norm_rope launch");
+    return ok();
 }
 
 int ca_rmsnorm(const uint16_t* x, int64_t x_stride, const uint16_t* residual, int64_t r_stride, uint16_t* sum_out,

@@ -34,180 +34,16 @@
 //  - Workgroup ids are remapped so consecutive work items (same KV row) share an XCD and
 //    its L2.
 
-#include "ca_common.h"
-#include "ca_kernels.h"
+#include "ca_attn.h"
 
 namespace ca {
 namespace {
 
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
-typedef float f32x8_t __attribute__((ext_vector_type(8)));
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
-typedef float f32x2_t __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
-typedef short i16x4_t __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) void lds_void_t;
-typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
-
-constexpr int kNW = 8;     // waves per workgroup (32 packed query rows each)
 constexpr int kStages = 4;  // places of the K and of the V ring in LDS: 128 KB per workgroup
-constexpr int kBM = 32 * kNW;        // packed query rows per workgroup
 constexpr int kKBytes = 64 * 256;  // K rows of one block in LDS (swizzled, unpadded)
 constexpr int kVBytes = 64 * 256;  // V rows of one block in LDS (swizzled, unpadded)
 constexpr int kVRing = kStages * kKBytes;  // LDS byte offset of the V ring
-constexpr float kRescale = 8.0f;      // lazy-rescale slack (log2 units)
 
-struct AttnParams {
-    Shape s;
-    SeqAddr q;
-    KvAddr k, v;
-    const int32_t* table;
-    int64_t table_stride;
-    const int32_t* counts;
-    PastBlocks pb;
-    float scale_log2;  // softmax scale * log2(e)
-    SeqAddr out;
-    float* lse;
-    int ntiles;       // packed-row tiles per KV row
-    int sp0;          // kPlaceSplits: splits of every request
-    int rows_total;   // Lq * G
-    int total_items;  // B*Hkv*ntiles*splits
-    int per_xcd;      // ceil(total_items / 8)
-    float* ws_o;      // [max splits][B*Hkv][rows_total][128]
-    float* ws_lse;    // [max splits][B*Hkv][rows_total]  (log2 domain)
-    // Ragged prefill whose row tiles fill 3/4 of the CUs: the kernel runs unsplit when every
-    // row's selected count is within 1.5x of their mean (workgroup 0 records the choice
-    // here for the merge); null otherwise
-    int32_t* ws_unsplit;
-    int32_t qpos0[CA_MAX_BATCH];     // absolute position of each request's query row 0
-    int32_t nkb[CA_MAX_BATCH];       // valid logical blocks of each request
-    int32_t sp[CA_MAX_BATCH];        // splits of each request's block lists
-    int32_t ioff[CA_MAX_BATCH + 1];  // first work item of each request (linear placement)
-    int placement;                   // kPlace*: where a workgroup finds its unit
-    int units;                       // kPlaceSplits: units in all
-    int unit_splits;                 // kPlaceRows, kPlaceTable: the splits of every unit, 0 when they differ
-    int32_t xoff[9];                 // kPlaceTable
-    uint32_t unit[kPlanRows];
-};
-
-// The work item of a workgroup: KV row, request, split of the row's list (of p.sp[b]) and, for
-// kernels with row tiles, the tile.
-struct Item {
-    int row, b, split, tile;
-};
-// Workgroup L runs on XCD L % 8 and is that XCD's (L / 8)-th; false when the XCD has no such
-// item.  Where all units hold the same number of splits the unit's place is computed: equal
-// requests need no table (kPlaceRows, kPlaceSplits), a ragged launch reads one entry.  The units
-// of a ragged launch differ only when a decode has more than kPlanRows splits in all; those are
-// read 64 at a time, one per lane, and found by a prefix sum over their items.
-// Every workgroup starts with this, so its latency shows in short launches (decode, from graph
-// replays: a scalar scan over the units, the prefix sum in all ragged launches, this): 5 requests
-// of 254-23110 tokens, 8 / 8 heads 33.6, 34.6, 33.9 us; 4 of 460-42073, 16 / 2 heads 26.1, 26.5,
-// 25.8; 7 of 136-8722, 16 / 2 heads 15.8, 14.7, 14.1.
-__device__ __forceinline__ bool find_item(const AttnParams& p, int ntiles, Item* it) {
-    const int x = blockIdx.x & 7;
-    int k = blockIdx.x >> 3;
-    const int Hkv = p.s.Hkv;
-    int lo = 0, cnt = p.unit_splits;
-    auto unit = [&](uint32_t word) {
-        it->row = word & (kPlanRows - 1);
-        it->b = (word >> kUnitReq) & (CA_MAX_BATCH - 1);
-        lo = (word >> kUnitLo) & 0xffu;
-        cnt = word >> kUnitCnt;
-    };
-    if (cnt > 0) {
-        const int per = ntiles * cnt;
-        int u = k;
-        if (per != 1) u = k / per;  // (an integer division is a chain of about 0.1 us)
-        k -= u * per;
-        if (p.placement == kPlaceRows) {
-            it->row = x + 8 * u;
-            if (it->row >= p.s.B * Hkv) return false;
-            it->b = it->row / Hkv;
-        } else {
-            if (p.xoff[x] + u >= p.xoff[x + 1]) return false;
-            unit(p.unit[p.xoff[x] + u]);
-        }
-    } else if (p.placement == kPlaceTable) {
-        const int lane = threadIdx.x & 63;
-        const int end = p.xoff[x + 1];
-        for (int base = p.xoff[x];; base += 64) {
-            if (base >= end) return false;
-            const uint32_t w = base + lane < end ? p.unit[base + lane] : 0u;
-            int sum = ntiles * static_cast<int>(w >> kUnitCnt);  // inclusive prefix of the units' items
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int y = __shfl_up(sum, o, 64);
-                if (lane >= o) sum += y;
-            }
-            const int total = __builtin_amdgcn_readlane(sum, 63);
-            if (k < total) {
-                const int u = __popcll(__ballot(sum <= k));
-                unit(__builtin_amdgcn_readlane(w, u));
-                if (u > 0) k -= __builtin_amdgcn_readlane(sum, u - 1);
-                break;
-            }
-            k -= total;
-        }
-    } else {
-        if (p.placement == kPlaceSplits) {
-            cnt = 1;
-            const int u = x + 8 * (k / ntiles);
-            if (u >= p.units) return false;
-            it->row = u / p.sp0;
-            lo = u - it->row * p.sp0;
-            k %= ntiles;
-        } else {
-            const int W = x * p.per_xcd + k;
-            if (W >= p.total_items) return false;
-            int b = 0;
-            while (b + 1 < p.s.B && p.ioff[b + 1] <= W) ++b;
-            cnt = p.sp[b];
-            const int local = W - p.ioff[b];
-            const int u = local / (ntiles * cnt);
-            it->row = b * Hkv + u;
-            k = local - u * ntiles * cnt;
-        }
-        it->b = it->row / Hkv;
-    }
-    it->tile = k;
-    if (cnt != 1) it->tile = k / cnt;
-    it->split = lo + k - it->tile * cnt;
-    return true;
-}
-
-__device__ __forceinline__ int swap23(int m) {
-    return (m & ~12) | ((m & 4) << 1) | ((m & 8) >> 1);
-}
-
-__device__ __forceinline__ lds_void_t* to_lds(const uint8_t* p) {
-    return (lds_void_t*)(p);
-}
-__device__ __forceinline__ lds_i16x4_t* to_lds_v4(const uint8_t* p) {
-    return (lds_i16x4_t*)(p);
-}
-// max(x, x of lane ^ 32): v_permlane32_swap hands each half the other half's values, so
-// the max of its two outputs is the pair's max in every lane (no LDS round trip).
-__device__ __forceinline__ float xor32_max(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-// max(x, x of lane ^ 16), the same way with v_permlane16_swap
-__device__ __forceinline__ float xor16_max(float x) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-// Wave-uniform reads of tables the kernel never writes (block ids, counts, page tables) go
-// through the scalar data cache: s_load waits on lgkmcnt, so they do not queue behind the
-// LDS-DMA loads in flight on vmcnt.
-typedef const __attribute__((address_space(4))) int32_t const_i32_t;
-__device__ __forceinline__ int32_t sload(const int32_t* p) {
-    return *(const_i32_t*)p;
-}
 // Words of a raw buffer resource over `bytes` bytes at base (wave-uniform).
 __device__ __forceinline__ u32x4_t buffer_words(const uint16_t* base, int bytes) {
     const uint64_t a = reinterpret_cast<uint64_t>(base);
@@ -827,6 +663,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
 // the max and the weights take two loads per thread, then add the partial outputs eight
 // splits at a time with the loads issued together.
 static_assert(kMaxPrefillSplits <= 64 && kMaxDecodeSplits <= 64, "the merge holds two splits per lane");
+// kNan: a row whose sum is NaN keeps it as its lse (else -inf); its output is NaN either way.
+template <bool kNan>
 __global__ __launch_bounds__(256) void attn_merge_kernel(AttnParams p) {
     const Shape& s = p.s;
     const int64_t gid = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -890,7 +728,7 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(AttnParams p) {
     *reinterpret_cast<bf16x4_t*>(op) = __builtin_convertvector(o4, bf16x4_t);
     if (p.lse && lane == 0)
         p.lse[((int64_t)b * s.Hq + hq) * s.Lq + t] =
-            wsum > 0.0f ? (mx + __log2f(wsum)) * 0.69314718055994531f : -__builtin_inff();
+            (kNan ? wsum != 0.0f : wsum > 0.0f) ? (mx + __log2f(wsum)) * 0.69314718055994531f : -__builtin_inff();
 }
 
 // ---------------------------------------------------------------------------------------
@@ -1390,45 +1228,57 @@ int64_t attn_workspace_bytes(const Shape& s, int num_splits) {
     return (int64_t)num_splits * rows_all * (128 + 1) * (int64_t)sizeof(float) + 16;
 }
 
+void attn_fill(const AttnArgs& a, AttnParams* p, SplitPlan* plan) {
+    p->s = a.s;
+    p->q = a.q;
+    p->k = a.k;
+    p->v = a.v;
+    p->table = a.table;
+    p->table_stride = a.table_stride;
+    p->counts = a.counts;
+    p->pb = a.pb;
+    p->scale_log2 = a.scale * 1.4426950408889634f;
+    p->out = a.out;
+    p->lse = a.lse;
+    p->rows_total = a.s.Lq * a.s.G;
+    p->ntiles = (p->rows_total + kBM - 1) / kBM;
+    int32_t nkb[CA_MAX_BATCH];
+    attn_positions(a.s, a.pb, a.kv_len, p->qpos0, nkb);
+    for (int b = 0; b < CA_MAX_BATCH; ++b) p->nkb[b] = b < a.s.B ? nkb[b] : 0;
+    for (int b = a.s.B; b < CA_MAX_BATCH; ++b) p->qpos0[b] = 0;
+    attn_plan(a.s, nkb, a.num_splits, a.kv_len != nullptr, plan);
+    for (int b = 0; b < CA_MAX_BATCH; ++b) p->sp[b] = b < a.s.B ? plan->s[b] : 1;
+    for (int b = 0; b <= CA_MAX_BATCH; ++b) p->ioff[b] = b <= a.s.B ? plan->off[b] : plan->off[a.s.B];
+    p->total_items = plan->off[a.s.B];
+    p->per_xcd = plan->per_xcd;
+    p->placement = plan->placement;
+    p->sp0 = plan->sp0;
+    p->units = plan->units;
+    p->unit_splits = plan->unit_splits;
+    if (plan->placement == kPlaceTable) {  // the kernels read the table in this case only
+        for (int x = 0; x < 9; ++x) p->xoff[x] = plan->xoff[x];
+        for (int i = 0; i < plan->xoff[8]; ++i) p->unit[i] = plan->unit[i];
+    }
+    const int64_t rows_all = (int64_t)a.s.B * a.s.Hkv * p->rows_total;
+    p->ws_o = plan->max > 1 ? static_cast<float*>(a.workspace) : nullptr;
+    p->ws_lse = plan->max > 1 ? p->ws_o + (int64_t)plan->max * rows_all * 128 : nullptr;
+    p->ws_unsplit = plan->max > 1 && plan->may_unsplit && a.table
+                       ? reinterpret_cast<int32_t*>(p->ws_lse + (int64_t)plan->max * rows_all)
+                       : nullptr;
+}
+
+hipError_t launch_attn_merge(const AttnParams& p, bool nan_lse, hipStream_t stream) {
+    const int64_t rows_all = (int64_t)p.s.B * p.s.Hkv * p.rows_total;
+    const int64_t blocks = (rows_all + 7) / 8;
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p); };
+    nan_lse ? launch(attn_merge_kernel<true>) : launch(attn_merge_kernel<false>);
+    return hipGetLastError();
+}
+
 hipError_t launch_attn(const AttnArgs& a, hipStream_t stream) {
     AttnParams p;
-    p.s = a.s;
-    p.q = a.q;
-    p.k = a.k;
-    p.v = a.v;
-    p.table = a.table;
-    p.table_stride = a.table_stride;
-    p.counts = a.counts;
-    p.pb = a.pb;
-    p.scale_log2 = a.scale * 1.4426950408889634f;
-    p.out = a.out;
-    p.lse = a.lse;
-    p.rows_total = a.s.Lq * a.s.G;
-    p.ntiles = (p.rows_total + kBM - 1) / kBM;
-    int32_t nkb[CA_MAX_BATCH];
-    attn_positions(a.s, a.pb, a.kv_len, p.qpos0, nkb);
-    for (int b = 0; b < CA_MAX_BATCH; ++b) p.nkb[b] = b < a.s.B ? nkb[b] : 0;
-    for (int b = a.s.B; b < CA_MAX_BATCH; ++b) p.qpos0[b] = 0;
     SplitPlan plan;
-    attn_plan(a.s, nkb, a.num_splits, a.kv_len != nullptr, &plan);
-    for (int b = 0; b < CA_MAX_BATCH; ++b) p.sp[b] = b < a.s.B ? plan.s[b] : 1;
-    for (int b = 0; b <= CA_MAX_BATCH; ++b) p.ioff[b] = b <= a.s.B ? plan.off[b] : plan.off[a.s.B];
-    p.total_items = plan.off[a.s.B];
-    p.per_xcd = plan.per_xcd;
-    p.placement = plan.placement;
-    p.sp0 = plan.sp0;
-    p.units = plan.units;
-    p.unit_splits = plan.unit_splits;
-    if (plan.placement == kPlaceTable) {  // the kernels read the table in this case only
-        for (int x = 0; x < 9; ++x) p.xoff[x] = plan.xoff[x];
-        for (int i = 0; i < plan.xoff[8]; ++i) p.unit[i] = plan.unit[i];
-    }
-    const int64_t rows_all = (int64_t)a.s.B * a.s.Hkv * p.rows_total;
-    p.ws_o = plan.max > 1 ? static_cast<float*>(a.workspace) : nullptr;
-    p.ws_lse = plan.max > 1 ? p.ws_o + (int64_t)plan.max * rows_all * 128 : nullptr;
-    p.ws_unsplit = plan.max > 1 && plan.may_unsplit && a.table
-                       ? reinterpret_cast<int32_t*>(p.ws_lse + (int64_t)plan.max * rows_all)
-                       : nullptr;
+    attn_fill(a, &p, &plan);
     bool row_res;
     {
         int max_tokens = 0;
@@ -1465,9 +1315,7 @@ hipError_t launch_attn(const AttnArgs& a, hipStream_t stream) {
         row_res ? launch(attn_fwd_kernel<kNW, false, true>) : launch(attn_fwd_kernel<kNW, false, false>);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || plan.max <= 1) return e;
-    const int64_t blocks = (rows_all + 7) / 8;
-    hipLaunchKernelGGL(attn_merge_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p);
-    return hipGetLastError();
+    return launch_attn_merge(p, false, stream);
 }
 
 }  // namespace ca

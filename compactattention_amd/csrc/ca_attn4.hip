@@ -1,0 +1,585 @@
+// Attention over a KV cache held in 4 bits (pages and conversions: ca_kv4.h): single tokens and short
+// drafts over the whole cache, and chunks over the selected blocks.  Queries, weights and outputs are as
+// in the bf16 kernels: S = Q K^T * scale in fp32 from exact bf16 operands, an online softmax in fp32, the
+// weights rounded to bf16 once for O = P V, their sum taken of the rounded weights, O in fp32.
+//
+// What a mask hides has no effect, whatever it holds: hidden scores are replaced by -inf, and in the
+// blocks that hold a hidden key (those that reach past the first query's position) values that no query
+// of the request may see are read as zero, while a NaN value that some may see is taken out of the
+// product and given to the rows that see it.  In all other blocks every row sees every key, and NaN goes
+// through the products.
+
+#include "ca_attn.h"
+#include "ca_kv4.h"
+
+namespace ca {
+namespace {
+
+struct Attn4Params {
+    AttnParams a;
+    Kv4Addr k, v;
+};
+static_assert(sizeof(Attn4Params) <= 4096, "the arguments of a launch");
+
+constexpr float kNegInf = -__builtin_inff();
+constexpr int kNoKey = 0x7fffffff;
+
+__device__ __forceinline__ u32x4_t load16(const uint8_t* p) { return *reinterpret_cast<const u32x4_t*>(p); }
+
+// 8 values of one word of codes under one scale: a row of 8 dims, bf16
+__device__ __forceinline__ u32x4_t decode_row(uint32_t w, float s) {
+    return u32x4_t{decode2<0>(w, s), decode2<1>(w, s), decode2<2>(w, s), decode2<3>(w, s)};
+}
+
+// ---------------------------------------------------------------------------------------
+// Single tokens: at most 16 packed query rows per KV row.  Bound by memory: every cached byte is read
+// once (68 bytes a token of K and of V).  16x16x32 MFMAs, S^T = K Q^T and O^T += V^T P^T, with the
+// packed rows as the N dimension.  Eight waves, each with pages of its own (e0 + w, e0 + w + 8, ...) and
+// its own softmax; their results meet in LDS at the end.
+//  - The contraction order of a product is free as long as both operands share it, so the page's layout
+//    decides it and nothing crosses lanes: lane (n = l % 16, g = l / 16) has token 16 kt + n's group g
+//    (16 bytes) as its share of K, and takes the dims 32 g + 8 s .. + 7 in step s; the scores then lie
+//    with the lane as tokens 16 kt + 4 g + i, and its share of V is dims 8 n .. 8 n + 7 of those tokens.
+//  - V's words are tokens, the MFMA wants tokens side by side: v_perm_b32 pairs them.  Output tile j
+//    holds the dims 8 m + j, so a lane ends with 8 consecutive dims of its row.
+constexpr int kWaves4 = 8;
+constexpr int kRows4 = 16;
+constexpr int kOStride4 = 132;  // floats per row of a wave's partial O in LDS (padded)
+
+struct Page4 {
+    u32x4_t k[4], v[4], vs;  // by tile of 16 tokens: K, V; V's scale bytes (word: tile)
+    uint32_t ks;             // K's scale bytes (byte: tile)
+};
+
+__global__ __launch_bounds__(kWaves4 * 64) void attn4_decode_kernel(Attn4Params p4) {
+    __shared__ __attribute__((aligned(16))) float mo[kWaves4 * kRows4 * kOStride4];
+    __shared__ float ml[kWaves4 * kRows4 * 2];
+    const AttnParams& p = p4.a;
+    Item it;
+    if (!find_item(p, 1, &it)) return;
+    const Shape& s = p.s;
+    const int row = __builtin_amdgcn_readfirstlane(it.row);
+    const int b = __builtin_amdgcn_readfirstlane(it.b);
+    const int split = __builtin_amdgcn_readfirstlane(it.split);
+    const int hk = row - b * s.Hkv;
+    const int nsplit = p.sp[b];
+    const int G = s.G;
+    const int R = p.rows_total;
+    const int qpos0 = p.qpos0[b];
+    const int nkb = p.nkb[b];
+    const int chunk = (nkb + nsplit - 1) / nsplit;
+    const int e0 = min(nkb, split * chunk);
+    const int e1 = min(nkb, e0 + chunk);
+    const int e_mask = (qpos0 + 1) >> 6;  // blocks from here on hold keys past query row 0
+    const int kv_tokens = qpos0 + s.Lq;
+
+    const int tid = threadIdx.x;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l = tid & 63;
+    const int n = l & 15;
+    const int g = l >> 4;
+
+    const bool qvalid = n < R;
+    const int qt = qvalid ? n / G : 0;
+    const int qg = qvalid ? n - qt * G : 0;
+    bf16x8_t qf[4];
+    {
+        const uint16_t* qp = p.q.data + b * p.q.sb + (int64_t)qt * p.q.st + (int64_t)(hk * G + qg) * p.q.sh + 32 * g;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const u32x4_t z = {0u, 0u, 0u, 0u};
+            qf[j] = qvalid ? *reinterpret_cast<const bf16x8_t*>(qp + 8 * j) : __builtin_bit_cast(bf16x8_t, z);
+        }
+    }
+    const int qpos = qpos0 + qt;
+
+    const int32_t* kpt = p4.k.page_table + (int64_t)row * p4.k.pts;
+    const int32_t* vpt = p4.v.page_table + (int64_t)row * p4.v.pts;
+    const int k_off = 64 * n + 16 * g;
+    const int v_off = 16 * l;
+    const int ks_off = k4_scale(n, g);
+    const int vs_off = v4_scale(4 * g, n >> 2);
+
+    // this wave's pages, 64 at a time, one per lane
+    const int nb_w = e0 + w < e1 ? (e1 - 1 - (e0 + w)) / kWaves4 + 1 : 0;
+    int kid = 0, vid = 0;
+    auto load_ids = [&](int c) {
+        const int e = e0 + w + kWaves4 * (64 * c + l);
+        if (e < e1) {
+            kid = static_cast<int>(clamp_page(kpt[e], p4.k.max_page));
+            vid = static_cast<int>(clamp_page(vpt[e], p4.v.max_page));
+        }
+    };
+    auto load_page = [&](int i) {
+        if ((i & 63) == 0) load_ids(i >> 6);
+        const uint8_t* kp = p4.k.data + (int64_t)__builtin_amdgcn_readlane(kid, i & 63) * p4.k.stride;
+        const uint8_t* vp = p4.v.data + (int64_t)__builtin_amdgcn_readlane(vid, i & 63) * p4.v.stride;
+        Page4 x;
+        x.ks = *reinterpret_cast<const uint32_t*>(kp + ks_off);
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) x.k[kt] = load16(kp + k_off + 1024 * kt);
+        x.vs = load16(vp + vs_off);
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) x.v[kt] = load16(vp + v_off + 1024 * kt);
+        return x;
+    };
+
+    const float sl2 = p.scale_log2;
+    f32x4_t oacc[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) oacc[j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    float m_run = kNegInf;
+    float l_run = 0.0f;
+    const bf16x2_t ones = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
+
+    auto k_scale = [&](const Page4& x, int kt) { return __uint_as_float(((x.ks >> (8 * kt)) & 0xffu) << 23); };
+    auto compute = [&](Page4& x, int i) {
+        const int kb = e0 + w + kWaves4 * i;
+        f32x4_t sc[4];
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+            sc[kt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            const float ks = k_scale(x, kt);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                sc[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, decode_row(x.k[kt][j], ks)),
+                                                                 qf[j], sc[kt], 0, 0, 0);
+        }
+        int nan_at = kNoKey;  // the first position with a NaN value in this lane's output dims
+        if (kb >= e_mask) {
+            // value i of tile kt is key 64 kb + 16 kt + 4 g + i
+            const int first = 64 * kb + 4 * g;
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int key = first + 16 * kt + e;
+                    if (key > qpos) sc[kt][e] = kNegInf;
+                    const bool bad = ((x.vs[kt] >> (8 * e)) & 0xffu) == kScaleNan;
+                    if (bad && key < kv_tokens) nan_at = min(nan_at, key);
+                    if (bad || key >= kv_tokens) {
+                        x.v[kt][e] = 0;
+                        x.vs[kt] &= ~(0xffu << (8 * e));
+                    }
+                }
+            if (__ballot(nan_at != kNoKey)) {
+                // over the four lanes and the four lane groups that hold this group of dims, then to the
+                // lanes whose output dims these are: 8 (4 g + i) + j, group g
+                nan_at = min(nan_at, __shfl_xor(nan_at, 1, 64));
+                nan_at = min(nan_at, __shfl_xor(nan_at, 2, 64));
+                nan_at = min(nan_at, __shfl_xor(nan_at, 16, 64));
+                nan_at = min(nan_at, __shfl_xor(nan_at, 32, 64));
+                nan_at = __shfl(nan_at, 4 * g, 64);
+            }
+        }
+        float mx = kNegInf;
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[kt][e]);
+        mx = xor32_max(xor16_max(mx)) * sl2;
+        float alpha = 1.0f;
+        if (mx > m_run + kRescale) {
+            alpha = __builtin_amdgcn_exp2f(m_run - mx);
+            m_run = mx;
+            l_run *= alpha;
+        }
+        if (__ballot(alpha != 1.0f)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) oacc[j] *= alpha;
+        }
+        const float m_use = m_run == kNegInf ? 0.0f : m_run;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            f32x8_t pv8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                pv8[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * half + (e >> 2)][e & 3], sl2, -m_use));
+            const bf16x8_t pf = __builtin_convertvector(pv8, bf16x8_t);
+            l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pf, pf, 0, 1), ones, l_run, false);
+            l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pf, pf, 2, 3), ones, l_run, false);
+            l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pf, pf, 4, 5), ones, l_run, false);
+            l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pf, pf, 6, 7), ones, l_run, false);
+            u32x4_t t[8];  // the 8 tokens' rows of 8 dims
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int kt = 2 * half + (e >> 2);
+                t[e] = decode_row(x.v[kt][e & 3], __uint_as_float(((x.vs[kt] >> (8 * (e & 3))) & 0xffu) << 23));
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
+                const u32x4_t a = {__builtin_amdgcn_perm(t[1][j >> 1], t[0][j >> 1], sel),
+                                   __builtin_amdgcn_perm(t[3][j >> 1], t[2][j >> 1], sel),
+                                   __builtin_amdgcn_perm(t[5][j >> 1], t[4][j >> 1], sel),
+                                   __builtin_amdgcn_perm(t[7][j >> 1], t[6][j >> 1], sel)};
+                oacc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), pf, oacc[j], 0, 0, 0);
+            }
+        }
+        if (nan_at <= qpos) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) oacc[j] = f32x4_t{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+        }
+    };
+
+    Page4 xa, xb;
+    if (nb_w > 0) xa = load_page(0);
+    for (int i = 0; i < nb_w; i += 2) {
+        if (i + 1 < nb_w) xb = load_page(i + 1);
+        compute(xa, i);
+        if (i + 2 < nb_w) xa = load_page(i + 2);
+        if (i + 1 < nb_w) compute(xb, i + 1);
+    }
+
+    // ---- the eight waves' results through LDS ----
+    l_run += __shfl_xor(l_run, 16, 64);
+    l_run += __shfl_xor(l_run, 32, 64);
+    // tile j, value i: dim 8 (4 g + i) + j of row n
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float* to = mo + (w * kRows4 + n) * kOStride4 + 8 * (4 * g + i);
+        *reinterpret_cast<f32x4_t*>(to) = f32x4_t{oacc[0][i], oacc[1][i], oacc[2][i], oacc[3][i]};
+        *reinterpret_cast<f32x4_t*>(to + 4) = f32x4_t{oacc[4][i], oacc[5][i], oacc[6][i], oacc[7][i]};
+    }
+    if (g == 0) {
+        ml[(w * kRows4 + n) * 2 + 0] = m_run;
+        ml[(w * kRows4 + n) * 2 + 1] = l_run;
+    }
+    __syncthreads();
+    const int orow = tid >> 5;  // 16 rows x 32 threads, 4 dims each
+    const int d4 = (tid & 31) * 4;
+    if (orow >= R) return;
+    float mx = kNegInf;
+#pragma unroll
+    for (int v = 0; v < kWaves4; ++v) mx = fmaxf(mx, ml[(v * kRows4 + orow) * 2]);
+    const float m_use = mx == kNegInf ? 0.0f : mx;
+    f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    float wsum = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kWaves4; ++v) {
+        const float wv = __builtin_amdgcn_exp2f(ml[(v * kRows4 + orow) * 2] - m_use);
+        wsum += wv * ml[(v * kRows4 + orow) * 2 + 1];
+        acc += wv * *reinterpret_cast<const f32x4_t*>(mo + (v * kRows4 + orow) * kOStride4 + d4);
+    }
+    // no key: zeros and -inf; a NaN sum stays
+    const float inv = wsum == 0.0f ? 0.0f : 1.0f / wsum;
+    const float lse2 = wsum == 0.0f ? kNegInf : mx + __log2f(wsum);
+    acc *= inv;
+    const int ot = orow / G;
+    const int og = orow - ot * G;
+    if (nsplit == 1) {
+        const int hq = hk * G + og;
+        uint16_t* op = p.out.data + b * p.out.sb + (int64_t)ot * p.out.st + (int64_t)hq * p.out.sh + d4;
+        *reinterpret_cast<bf16x4_t*>(op) = __builtin_convertvector(acc, bf16x4_t);
+        if (p.lse && (tid & 31) == 0) p.lse[((int64_t)b * s.Hq + hq) * s.Lq + ot] = lse2 * 0.69314718055994531f;
+    } else {
+        const int64_t prow = ((int64_t)split * (s.B * s.Hkv) + row) * R + orow;
+        *reinterpret_cast<f32x4_t*>(p.ws_o + prow * 128 + d4) = acc;
+        if ((tid & 31) == 0) p.ws_lse[prow] = lse2;
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// Chunks, and drafts with more than 16 packed rows: 256 packed rows a workgroup, 32 a wave, the
+// 32x32x16 products of the bf16 kernel.  A block's codes go from memory to registers (16 bytes a thread:
+// waves 0-3 a group of a token of K, waves 4-7 8 dims of four tokens of V), through 16 conversions to
+// bf16 and into LDS in the bf16 kernel's places, two blocks deep, while the block before is multiplied.
+// kTab: block lists come from the per-row table; otherwise they are the identity (drafts).
+constexpr int kKv4Bytes = 64 * 256;  // K or V rows of one block in LDS
+
+template <bool kTab>
+__global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn4_fwd_kernel(Attn4Params p4) {
+    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * 2 * kKv4Bytes];  // K and V of two blocks
+    // by block modulo 4 and group of dims: the first key in the block with a NaN value (masked blocks)
+    __shared__ int vnan[4][4];
+    const AttnParams& p = p4.a;
+    const Shape& s = p.s;
+    Item it;
+    if (!find_item(p, p.ntiles, &it)) return;
+    const int row = __builtin_amdgcn_readfirstlane(it.row);
+    const int b = __builtin_amdgcn_readfirstlane(it.b);
+    const int split = __builtin_amdgcn_readfirstlane(it.split);
+    const int tile = __builtin_amdgcn_readfirstlane(it.tile);
+    const int hk = row - b * s.Hkv;
+    const int nsplit = p.sp[b];
+    const int G = s.G;
+    const int qpos0 = p.qpos0[b];
+    const int nkb = p.nkb[b];
+    const int rows_total = p.rows_total;
+    const int r0 = tile * kBM;
+    const int t_first = r0 / G;
+    const int t_last = min(r0 + kBM - 1, rows_total - 1) / G;
+    const int32_t* tab = kTab ? p.table + (int64_t)row * p.table_stride : nullptr;
+    const int lim = (qpos0 + t_last) >> 6;  // last block the tile can see
+    const int kv_tokens = qpos0 + s.Lq;
+    const int tid = threadIdx.x;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l = tid & 63;
+    const int h = l >> 5;
+    const int n = l & 31;
+
+    const int qrow = r0 + 32 * w + n;
+    const bool qvalid = qrow < rows_total;
+    const int qt = qvalid ? qrow / G : 0;
+    const int qg = qvalid ? qrow - qt * G : 0;
+    bf16x8_t qf[8];
+    {
+        const uint16_t* qp = p.q.data + b * p.q.sb + (int64_t)qt * p.q.st + (int64_t)(hk * G + qg) * p.q.sh + 8 * h;
+#pragma unroll
+        for (int ds = 0; ds < 8; ++ds) {
+            const u32x4_t z = {0u, 0u, 0u, 0u};
+            qf[ds] = qvalid ? *reinterpret_cast<const bf16x8_t*>(qp + 16 * ds) : __builtin_bit_cast(bf16x8_t, z);
+        }
+    }
+    // entries up to the last one that the tile can see
+    int n_vis = kTab ? 0 : min(nkb, lim + 1);
+    if (kTab) {
+        for (int end = min(max(sload(p.counts + row), 0), s.cap); end > 0; end -= 64) {
+            const int e = end - 1 - l;
+            const uint64_t seen = __ballot(e >= 0 && max(tab[max(e, 0)], 0) <= lim);
+            if (seen != 0) {
+                n_vis = end - (__ffsll(static_cast<unsigned long long>(seen)) - 1);
+                break;
+            }
+        }
+    }
+    const int chunk = (n_vis + nsplit - 1) / nsplit;
+    const int e0 = min(n_vis, split * chunk);
+    const int nblk = min(n_vis, e0 + chunk) - e0;
+    const int qpos = qpos0 + qt;
+    const int first_q = qpos0 + t_first;  // blocks that reach past it are masked
+
+    f32x16_t oacc[4];
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) oacc[dt][j] = 0.0f;
+    float m_run = kNegInf;
+    float l_run = 0.0f;
+    float m_neg = 0.0f;  // -m_run, 0 while a row has seen no key
+
+    // ---- the list's blocks, 64 entries at a time, one per lane ----
+    // (logical id and this wave's page: K's for waves 0-3, V's for the others)
+    const bool is_v = w >= 4;
+    const Kv4Addr& kv = is_v ? p4.v : p4.k;
+    const int32_t* pt = kv.page_table + (int64_t)row * kv.pts;
+    int ids = 0, pages = 0;
+    auto load_ids = [&](int c) {
+        const int e = 64 * c + l;
+        if (e < nblk) {
+            ids = kTab ? min(max(tab[e0 + e], 0), nkb - 1) : e0 + e;
+            pages = static_cast<int>(clamp_page(pt[ids], kv.max_page));
+        }
+    };
+    // ---- a block's codes: memory -> registers ----
+    const int u = tid & 255;
+    const int st_t = is_v ? 4 * (u >> 4) : u >> 2;  // token (of V: the first of four)
+    const int st_c = is_v ? u & 15 : 4 * (u & 3);   // 16-byte chunk of the row in LDS (of K: the first of four)
+    const int sc_off = is_v ? v4_scale(st_t, st_c >> 2) : k4_scale(st_t, u & 3);
+    u32x4_t code;
+    uint32_t scale_w = 0;
+    int next_id = 0;  // of the block in the registers
+    auto fetch = [&](int j) {
+        if ((j & 63) == 0) load_ids(j >> 6);
+        next_id = __builtin_amdgcn_readlane(ids, j & 63);
+        const uint8_t* page = kv.data + (int64_t)__builtin_amdgcn_readlane(pages, j & 63) * kv.stride;
+        code = load16(page + 16 * u);
+        if (is_v)
+            scale_w = *reinterpret_cast<const uint32_t*>(page + sc_off);
+        else
+            scale_w = page[sc_off];
+    };
+    // ---- registers -> bf16 rows in LDS, block j in place j & 1 ----
+    //   K: 16-byte chunk c of row r sits at chunk c ^ (r & 15), V: at chunk c ^ 4 (r & 3)
+    auto stage = [&](int j) {
+        uint8_t* to = smem + (j & 1) * 2 * kKv4Bytes;
+        if (!is_v) {
+            const float sc = __uint_as_float(scale_w << 23);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<u32x4_t*>(to + st_t * 256 + ((st_c + i) ^ (st_t & 15)) * 16) = decode_row(code[i], sc);
+        } else {
+            if (64 * next_id + 63 > first_q) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool bad = ((scale_w >> (8 * i)) & 0xffu) == kScaleNan;
+                    const bool there = 64 * next_id + st_t + i < kv_tokens;
+                    if (bad && there) atomicMin(&vnan[j & 3][st_c >> 2], st_t + i);
+                    if (bad || !there) {
+                        code[i] = 0;
+                        scale_w &= ~(0xffu << (8 * i));
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<u32x4_t*>(to + kKv4Bytes + (st_t + i) * 256 + (st_c ^ (4 * i)) * 16) =
+                    decode_row(code[i], __uint_as_float(((scale_w >> (8 * i)) & 0xffu) << 23));
+        }
+    };
+
+    const float sl2 = p.scale_log2;
+    // Fragment addresses, as in the bf16 kernel: K rows swap23(n) (+32), 16 bytes at d = 16 ds + 8 h; V^T by
+    // transposing reads of 8 bytes at row 16 s4 + 8 h + 4 hh + (l & 15) / 4, d = 32 dt + 16 ((l >> 4) & 1) + 4 (l & 3).
+    const int k_r = swap23(n);
+    int k_off[8];
+#pragma unroll
+    for (int ds = 0; ds < 8; ++ds) k_off[ds] = k_r * 256 + (((2 * ds + h) ^ (k_r & 15)) * 16);
+    const int v_rq = (l & 15) >> 2;
+    const int v_x = 2 * ((l >> 4) & 1) + ((l & 3) >> 1);
+    int v_off[4];
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) v_off[dt] = kKv4Bytes + (8 * h + v_rq) * 256 + (4 * (dt ^ v_rq) + v_x) * 16 + (l & 1) * 8;
+    const i16x4_t ones = {0x3f80, 0x3f80, 0x3f80, 0x3f80};
+    auto add_weights = [&](uint32_t w0, uint32_t w1, f32x4_t acc) {
+        const u32x2_t ww = {w0, w1};
+        return __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(ones, __builtin_bit_cast(i16x4_t, ww), acc, 0, 0, 0);
+    };
+    auto compute = [&](int j, int kb) {
+        const uint8_t* at = smem + (j & 1) * 2 * kKv4Bytes;
+        f32x16_t sc[2];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[kt][e] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(at + k_off[i >> 1] + (i & 1) * 8192);
+            sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[i >> 1], sc[i & 1], 0, 0, 0);
+        }
+        const bool masked = 64 * kb + 63 > first_q;
+        if (masked) {
+            const int vis = qpos - 64 * kb - 8 * h;
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int key = kt * 32 + 16 * (e >> 3) + 4 * ((e >> 2) & 1) + (e & 3);
+                    if (key > vis) sc[kt][e] = kNegInf;
+                }
+        }
+        float mx = kNegInf;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[kt][e]);
+        mx = xor32_max(mx) * sl2;
+        if (__ballot(mx > m_run + kRescale)) {
+            float alpha = 1.0f;
+            if (mx > m_run + kRescale) {
+                alpha = __builtin_amdgcn_exp2f(m_run - mx);
+                m_run = mx;
+                m_neg = -mx;
+                l_run *= alpha;
+            }
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) oacc[dt][e] *= alpha;
+        }
+        bf16x8_t pf[4];
+        f32x4_t rs = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s4 = 0; s4 < 4; ++s4) {
+            f32x8_t pv8;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                pv8[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[s4 >> 1][8 * (s4 & 1) + i], sl2, m_neg));
+            pf[s4] = __builtin_convertvector(pv8, bf16x8_t);
+            const u32x4_t w4 = __builtin_bit_cast(u32x4_t, pf[s4]);
+            rs = add_weights(w4[0], w4[1], rs);
+            rs = add_weights(w4[2], w4[3], rs);
+        }
+        l_run += rs[0];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint8_t* vp = at + v_off[i & 3] + (i >> 2) * 4096;
+            const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(to_lds_v4(vp));
+            const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(to_lds_v4(vp + 1024));
+            const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            oacc[i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[i >> 2], oacc[i & 3], 0, 0, 0);
+        }
+        if (masked) {
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt)
+                if (64 * kb + vnan[j & 3][dt] <= qpos && vnan[j & 3][dt] < 64)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) oacc[dt][e] = __builtin_nanf("");
+        }
+    };
+
+    if (tid < 16) vnan[tid >> 2][tid & 3] = 64;
+    if (nblk > 0) {
+        fetch(0);
+        __syncthreads();
+        stage(0);
+        int kb = next_id;
+        if (nblk > 1) fetch(1);
+        for (int j = 0; j < nblk; ++j) {
+            // block j has been written, and place (j + 1) & 1 has been read
+            __syncthreads();
+            const int kb_next = next_id;
+            if (tid < 4) vnan[(j + 3) & 3][tid] = 64;  // read last for block j - 1, written next for j + 3
+            if (j + 1 < nblk) {
+                stage(j + 1);
+                if (j + 2 < nblk) fetch(j + 2);
+            }
+            compute(j, kb);
+            kb = kb_next;
+        }
+    }
+
+    // ---- epilogue ----
+    l_run += __shfl_xor(l_run, 32, 64);
+    if (qvalid) {
+        // no key: zeros and -inf; a NaN sum stays
+        const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
+        const float lse2 = l_run == 0.0f ? kNegInf : (m_run == kNegInf ? 0.0f : m_run) + __log2f(l_run);
+        const int hq = hk * G + qg;
+        const int64_t prow = ((int64_t)split * (s.B * s.Hkv) + row) * rows_total + qrow;
+        uint16_t* op = p.out.data + b * p.out.sb + (int64_t)qt * p.out.st + (int64_t)hq * p.out.sh;
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int jq = 0; jq < 4; ++jq) {
+                const int d0 = dt * 32 + 8 * jq + 4 * h;
+                f32x4_t o4;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o4[i] = oacc[dt][4 * jq + i] * inv;
+                if (nsplit == 1)
+                    *reinterpret_cast<bf16x4_t*>(op + d0) = __builtin_convertvector(o4, bf16x4_t);
+                else
+                    *reinterpret_cast<f32x4_t*>(p.ws_o + prow * 128 + d0) = o4;
+            }
+        if (h == 0) {
+            if (nsplit != 1)
+                p.ws_lse[prow] = lse2;
+            else if (p.lse)
+                p.lse[((int64_t)b * s.Hq + hq) * s.Lq + qt] = lse2 * 0.69314718055994531f;
+        }
+    }
+}
+
+}  // namespace
+
+hipError_t launch_attn4(const AttnArgs& a, const Kv4Addr& k, const Kv4Addr& v, hipStream_t stream) {
+    Attn4Params p;
+    SplitPlan plan;
+    attn_fill(a, &p.a, &plan);
+    p.a.ws_unsplit = nullptr;  // a launch with splits keeps them
+    p.k = k;
+    p.v = v;
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(plan.per_xcd * 8), dim3(kNW * 64), 0, stream, p); };
+    static_assert(kNW == kWaves4, "one workgroup size");
+    if (a.table)
+        launch(attn4_fwd_kernel<true>);
+    else if (attn_uses_decode_kernel(a.s, true))
+        launch(attn4_decode_kernel);
+    else
+        launch(attn4_fwd_kernel<false>);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || plan.max <= 1) return e;
+    return launch_attn_merge(p.a, true, stream);
+}
+
+}  // namespace ca

@@ -92,6 +92,23 @@ hipError_t launch_union_compact_pairs(const Shape& s, const uint32_t* rowmask, i
 hipError_t launch_append_tokens(int B, int L, int Hkv, const SeqAddr& k_new, const SeqAddr& v_new,
                                 const KvAddr& k_cache, const KvAddr& v_cache, int64_t start, hipStream_t stream);
 
+// Pages held in 4 bits (ca_kv4.h) and copies of pages (ca_pages.hip)
+struct Kv4Addr;
+struct PagePool {
+    uint8_t* data;
+    int64_t bytes;   // of a page, a multiple of 16
+    int64_t stride;  // bytes from page to page
+};
+// Quantises L tokens of every request at start[b] .. start[b] + L - 1 into its pages
+hipError_t launch_append4(int B, int L, int H, const int32_t* start, const SeqAddr& k_new, const SeqAddr& v_new,
+                          const Kv4Addr& k, const Kv4Addr& v, hipStream_t stream);
+// The tokens back as bf16 [B, H, L, 128]; v and v_out nullable
+hipError_t launch_gather4(int B, int L, int H, const int32_t* start, const Kv4Addr& k, const Kv4Addr* v,
+                          uint16_t* k_out, uint16_t* v_out, hipStream_t stream);
+// pool[dst[i]] = pool[src[i]] for every pool, in launches of a few hundred pages
+hipError_t launch_copy_pages(const PagePool* pools, int n_pools, const int32_t* src, const int32_t* dst, int n,
+                             hipStream_t stream);
+
 struct AttnArgs {
     Shape s;
     SeqAddr q;
@@ -148,11 +165,17 @@ void attn_positions(const Shape& s, const PastBlocks& pb, const int32_t* kv_len,
 int attn_pick_splits(const Shape& s, const PastBlocks& pb, const int32_t* kv_len);
 int64_t attn_workspace_bytes(const Shape& s, int num_splits);
 hipError_t launch_attn(const AttnArgs& a, hipStream_t stream);
+// The same over pages held in 4 bits (a.k and a.v unused; ca_attn4.hip)
+hipError_t launch_attn4(const AttnArgs& a, const Kv4Addr& k, const Kv4Addr& v, hipStream_t stream);
 
 // model plumbing (ca_model.hip)
 // x2 / y2 (nullable): a second tensor of H2 heads over the same tokens
 hipError_t launch_rope(const SeqAddr& x, const SeqAddr& y, int H, const SeqAddr* x2, const SeqAddr* y2, int H2,
                        const float* cos, const float* sin, int B, int L, hipStream_t stream);
+// cs_b: floats from a request's rows of cos and sin to the next one's (0: the same)
+hipError_t launch_norm_rope(const SeqAddr& q, const SeqAddr& q_out, int Hq, const uint16_t* qw, const SeqAddr& k,
+                            const SeqAddr& k_out, int Hk, const uint16_t* kw, const float* cos, const float* sin,
+                            int64_t cs_b, int B, int L, float eps, hipStream_t stream);
 hipError_t launch_rmsnorm(const uint16_t* x, int64_t x_stride, const uint16_t* r, int64_t r_stride, uint16_t* s,
                           int64_t s_stride, const uint16_t* w, uint16_t* y, int64_t y_stride, int64_t rows, int n,
                           float eps, hipStream_t stream);

@@ -11,7 +11,10 @@
 //    the mean's summation order is this kernel's own.  The residual form first adds the
 //    residual in bf16 (x + r rounded once, as the decoder's residual + h) and normalises
 //    that sum, returning both;
-//  - SwiGLU: out = bf16(bf16(silu(g)) * u), silu in fp32.
+//  - SwiGLU: out = bf16(bf16(silu(g)) * u), silu in fp32;
+//  - norm and rotation of a head: y = x * w / sqrt(mean(x^2) + eps) over its 128 dims and
+//    out = bf16(y * cos + rotate_half(y) * sin), all in fp32 and rounded once.  (The two kernels
+//    above in a row round three times.)
 
 #include "ca_common.h"
 #include "ca_kernels.h"
@@ -169,6 +172,73 @@ __global__ __launch_bounds__(256) void rmsnorm_kernel(RmsParams p) {
         store(i, *reinterpret_cast<const u16x8_t*>(src + i));
 }
 
+// Norm and rotation of q's and k's heads.  8 lanes hold a head: lane c the dims 8 c .. 8 c + 7 and
+// 64 + 8 c .. 64 + 8 c + 7, so that a dim and its rotation partner meet in one lane and the sum of
+// squares takes three exchanges.  A wave takes 8 heads of one side (q or k) of one token at a time.
+struct NormRopeParams {
+    RopeSide side[2];
+    const uint16_t* w[2];
+    int groups0, groups;  // 8-head groups of q, of q and k
+    const float* cos;     // [L, 128] rows, cs_b further for every request (0: the same rows)
+    const float* sin;
+    int64_t cs_b;
+    int L;
+    uint32_t units;  // tokens * groups
+    float eps;
+};
+
+__global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeParams p) {
+    const uint32_t unit = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (unit >= p.units) return;
+    const int lane = threadIdx.x & 63;
+    const int c = lane & 7;
+    const uint32_t bt = unit / p.groups;
+    const int grp = unit - bt * p.groups;
+    const bool second = grp >= p.groups0;
+    const RopeSide& sd = p.side[second ? 1 : 0];
+    const int h = (grp - (second ? p.groups0 : 0)) * 8 + (lane >> 3);
+    const bool live = h < sd.H;
+    const int b = bt / p.L;
+    const int t = bt - b * p.L;
+    const int hc = live ? h : 0;
+    const uint16_t* xr = sd.x + b * sd.xsb + (int64_t)t * sd.xst + (int64_t)hc * sd.xsh + 8 * c;
+    const u16x8_t lo = *reinterpret_cast<const u16x8_t*>(xr), hi = *reinterpret_cast<const u16x8_t*>(xr + 64);
+    const uint16_t* wr = p.w[second ? 1 : 0] + 8 * c;
+    const u16x8_t wl = *reinterpret_cast<const u16x8_t*>(wr), wh = *reinterpret_cast<const u16x8_t*>(wr + 64);
+    const int64_t at = b * p.cs_b + (int64_t)t * 128 + 8 * c;
+    const float4* cr = reinterpret_cast<const float4*>(p.cos + at);
+    const float4* sr = reinterpret_cast<const float4*>(p.sin + at);
+    float cs[16], sn[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // float4 0, 1: the low dims; 16, 17: those 64 further
+        const float4 a = cr[(i & 1) + 16 * (i >> 1)], s = sr[(i & 1) + 16 * (i >> 1)];
+        cs[4 * i] = a.x, cs[4 * i + 1] = a.y, cs[4 * i + 2] = a.z, cs[4 * i + 3] = a.w;
+        sn[4 * i] = s.x, sn[4 * i + 1] = s.y, sn[4 * i + 2] = s.z, sn[4 * i + 3] = s.w;
+    }
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float a = bf16_to_f32(lo[i]), d = bf16_to_f32(hi[i]);
+        ss = __builtin_fmaf(a, a, ss);
+        ss = __builtin_fmaf(d, d, ss);
+    }
+#pragma unroll
+    for (int o = 4; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
+    const float rstd = 1.0f / __builtin_sqrtf(ss * (1.0f / 128.0f) + p.eps);
+    u16x8_t ol, oh;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float a = bf16_to_f32(lo[i]) * rstd * bf16_to_f32(wl[i]);
+        const float d = bf16_to_f32(hi[i]) * rstd * bf16_to_f32(wh[i]);
+        ol[i] = f32_to_bf16(a * cs[i] - d * sn[i]);
+        oh[i] = f32_to_bf16(d * cs[8 + i] + a * sn[8 + i]);
+    }
+    if (!live) return;
+    uint16_t* yr = sd.y + b * sd.ysb + (int64_t)t * sd.yst + (int64_t)h * sd.ysh + 8 * c;
+    *reinterpret_cast<u16x8_t*>(yr) = ol;
+    *reinterpret_cast<u16x8_t*>(yr + 64) = oh;
+}
+
 struct SwigluParams {
     const uint16_t* g;
     const uint16_t* u;
@@ -218,6 +288,26 @@ hipError_t launch_rope(const SeqAddr& x, const SeqAddr& y, int H, const SeqAddr*
                            dim3(256), 0, stream, p);
     };
     groups1 > 0 ? launch(rope_kernel<true>) : launch(rope_kernel<false>);
+    return hipGetLastError();
+}
+
+hipError_t launch_norm_rope(const SeqAddr& q, const SeqAddr& q_out, int Hq, const uint16_t* qw, const SeqAddr& k,
+                            const SeqAddr& k_out, int Hk, const uint16_t* kw, const float* cos, const float* sin,
+                            int64_t cs_b, int B, int L, float eps, hipStream_t stream) {
+    NormRopeParams p;
+    p.side[0] = RopeSide{q.data, q.sb, q.st, q.sh, q_out.data, q_out.sb, q_out.st, q_out.sh, Hq};
+    p.side[1] = RopeSide{k.data, k.sb, k.st, k.sh, k_out.data, k_out.sb, k_out.st, k_out.sh, Hk};
+    p.w[0] = qw;
+    p.w[1] = kw;
+    p.groups0 = (Hq + 7) / 8;
+    p.groups = p.groups0 + (Hk + 7) / 8;
+    p.cos = cos;
+    p.sin = sin;
+    p.cs_b = cs_b;
+    p.L = L;
+    p.units = static_cast<uint32_t>((int64_t)B * L * p.groups);
+    p.eps = eps;
+    hipLaunchKernelGGL(norm_rope_kernel, dim3((p.units + 3) / 4), dim3(256), 0, stream, p);
     return hipGetLastError();
 }
 

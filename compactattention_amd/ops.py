@@ -8,13 +8,16 @@ a non-HIP implementation.
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 from dataclasses import dataclass
-from typing import Optional, Sequence, Tuple
+from typing import Optional, Sequence, Tuple, Union
 
+import numpy as np
 import torch
 
 from . import _hip
-from ._hip import BLOCK, HEAD_DIM, POOL_AVG, POOL_MAX, POOL_MIN, Dims, KvLayout, SelectRule, SeqLayout, check
+from ._hip import (BLOCK, HEAD_DIM, PAGE4_BYTES, POOL_AVG, POOL_MAX, POOL_MIN, Dims, Kv4Layout, KvLayout, PagePool,
+                   SelectRule, SeqLayout, check)
 
 POOL_BITS = {"max": POOL_MAX, "min": POOL_MIN, "avg": POOL_AVG}
 
@@ -98,6 +101,16 @@ def _need_cuda(name: str, t: torch.Tensor, dtype: torch.dtype) -> None:
         raise ValueError(f"{name} must be {dtype} (got {t.dtype})")
 
 
+def _on_device(first: torch.Tensor, *others: Optional[torch.Tensor]):
+    """A context in which the tensors' one device is the current one, whichever was before."""
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"all tensors of a call must be on one device (got {first.device} and {t.device})")
+    if first.device.index == torch.cuda.current_device():
+        return nullcontext()
+    return torch.cuda.device(first.device)
+
+
 def past_array(past_blocks: Sequence[int], batch: Optional[int] = None):
     """Per-request values (past blocks or kv_len) as the int32 host array the C-ABI reads
     ``batch`` entries of."""
@@ -179,6 +192,142 @@ class KV:
             if self.page_table.shape[0] < rows or self.page_table.shape[1] < blocks:
                 raise ValueError(f"{name} page_table {tuple(self.page_table.shape)} does not cover "
                                  f"[{rows}, {blocks}]")
+
+
+@dataclass
+class KV4:
+    """A K or V cache held in 4 bits: pages of 64 tokens of one KV head, E2M1 codes with a scale for every
+    32 dims (``ca_kv4_layout`` describes the bytes).  ``attn_fwd`` and ``attn_decode`` take it in the place
+    of a bf16 ``KV``; ``append_q4`` writes it, ``gather_q4`` reads it back."""
+
+    tensor: torch.Tensor
+    layout: Kv4Layout
+    page_table: torch.Tensor
+
+    @staticmethod
+    def paged(pool: torch.Tensor, page_table: torch.Tensor) -> "KV4":
+        """Page pool [num_pages, PAGE4_BYTES] uint8 and page_table [B*Hkv, blocks] int32."""
+        _need_cuda("pool", pool, torch.uint8)
+        _need_cuda("page_table", page_table, torch.int32)
+        if pool.dim() != 2 or pool.shape[1] != PAGE4_BYTES or pool.stride(1) != 1:
+            raise ValueError(f"a 4-bit page pool must be [num_pages, {PAGE4_BYTES}] with contiguous pages")
+        if page_table.dim() != 2 or page_table.stride(1) != 1:
+            raise ValueError("page_table must be [rows, blocks] with contiguous rows")
+        if pool.device != page_table.device:
+            raise ValueError(f"pool on {pool.device} and page_table on {page_table.device}")
+        return KV4(pool, Kv4Layout(pool.data_ptr(), pool.stride(0), page_table.data_ptr(), page_table.stride(0),
+                                   pool.shape[0]), page_table)
+
+    def check_blocks(self, name: str, batch: int, heads: int, blocks: int, tokens: Optional[int] = None) -> None:
+        """Raise unless the page table covers ``blocks`` blocks of each of the ``batch`` x ``heads`` rows."""
+        del tokens
+        if self.page_table.shape[0] < batch * heads or self.page_table.shape[1] < blocks:
+            raise ValueError(f"{name} page_table {tuple(self.page_table.shape)} does not cover "
+                             f"[{batch * heads}, {blocks}]")
+
+
+AnyKV = Union[KV, KV4]
+
+
+def _attn_launch(name: str, k: AnyKV, v: AnyKV, *tensors: torch.Tensor):
+    """The entry point for these caches and the context to call it in."""
+    if isinstance(k, KV4) != isinstance(v, KV4):
+        raise ValueError("K and V must both be bf16 caches or both be held in 4 bits")
+    if not isinstance(k, KV4):
+        return getattr(_hip.lib(), name), nullcontext()
+    guard = _on_device(*tensors, k.tensor, k.page_table, v.tensor, v.page_table)
+    return getattr(_hip.lib(), name + "_q4"), guard
+
+
+def _starts(start: Union[int, Sequence[int]], batch: int):
+    return past_array([start] * batch if isinstance(start, (int, np.integer)) else start, batch)
+
+
+def append_q4(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: KV4, v_cache: KV4,
+              start: Union[int, Sequence[int]], kv_cap: int) -> None:
+    """Quantise the tokens of k_new / v_new [B, L, Hkv, 128] bf16 into a 4-bit cache at positions
+    start[b] .. start[b] + L - 1 of every request's rows (one start for all, or one per request).  No page
+    may be named by two of the rows: a forked page is copied first (``copy_pages``)."""
+    B, L, Hkv, _ = k_new.shape
+    if tuple(v_new.shape) != tuple(k_new.shape):
+        raise ValueError("v_new must have k_new's shape")
+    if not isinstance(k_cache, KV4) or not isinstance(v_cache, KV4):
+        raise ValueError("append_q4 writes caches held in 4 bits (KV4)")
+    sa = _starts(start, B)
+    if L == 0:
+        return
+    kn, vn = seq_layout(k_new, "k_new"), seq_layout(v_new, "v_new")
+    for name, kv in (("k", k_cache), ("v", v_cache)):
+        kv.check_blocks(name, B, Hkv, -(-(max(sa) + L) // BLOCK))
+    d = make_dims(B, L, Hkv, Hkv, kv_cap)
+    with _on_device(k_new, v_new, k_cache.tensor, v_cache.tensor, k_cache.page_table, v_cache.page_table):
+        check(_hip.lib().ca_append_q4(ctypes.byref(d), ctypes.byref(kn), ctypes.byref(vn), ctypes.byref(k_cache.layout),
+                                      ctypes.byref(v_cache.layout), sa, _stream()))
+
+
+def gather_q4(k_cache: KV4, v_cache: Optional[KV4], batch: int, num_kv_heads: int, start: Union[int, Sequence[int]],
+              length: int) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """The values that a 4-bit cache stands for at positions start[b] .. start[b] + length - 1: K and V
+    [batch, num_kv_heads, length, 128] bf16 (exact; V None without a v_cache)."""
+    if not isinstance(k_cache, KV4) or not (v_cache is None or isinstance(v_cache, KV4)):
+        raise ValueError("gather_q4 reads caches held in 4 bits (KV4)")
+    if length < 0:
+        raise ValueError(f"length={length} < 0")
+    sa = _starts(start, batch)
+    dev = k_cache.tensor.device
+    shape = (batch, num_kv_heads, length, HEAD_DIM)
+    k_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    v_out = torch.empty(shape, dtype=torch.bfloat16, device=dev) if v_cache is not None else None
+    if length == 0:
+        return k_out, v_out
+    blocks = -(-(max(sa) + length) // BLOCK)
+    for name, kv in (("k", k_cache), ("v", v_cache)):
+        if kv is not None:
+            kv.check_blocks(name, batch, num_kv_heads, blocks)
+    d = make_dims(batch, length, num_kv_heads, num_kv_heads, blocks)
+    with _on_device(k_cache.tensor, k_cache.page_table, *(() if v_cache is None else (v_cache.tensor, v_cache.page_table))):
+        check(_hip.lib().ca_gather_q4(ctypes.byref(d), ctypes.byref(k_cache.layout),
+                                      ctypes.byref(v_cache.layout) if v_cache is not None else None, sa,
+                                      k_out.data_ptr(), _ptr(v_out), _stream()))
+    return k_out, v_out
+
+
+def _page_ids(name: str, ids) -> np.ndarray:
+    if isinstance(ids, torch.Tensor) and ids.is_cuda:
+        raise ValueError(f"{name} must be on the host (the allocator's page ids)")
+    a = np.asarray(ids)
+    if a.size == 0:
+        return np.zeros(0, np.int32)
+    if a.ndim != 1 or a.dtype.kind not in "iu":
+        raise ValueError(f"{name} must be a one-dimensional sequence of integers")
+    if int(a.min()) < 0 or int(a.max()) >= 1 << 31:
+        raise ValueError(f"{name} holds page ids outside [0, 2^31)")
+    return np.ascontiguousarray(a, np.int32)
+
+
+def copy_pages(pools: Sequence[torch.Tensor], src, dst) -> None:
+    """pool[dst[i]] = pool[src[i]] for every pool [num_pages, ...] of any type whose pages are contiguous
+    multiples of 16 bytes (bf16 pages, 4-bit pages, summaries by page).  src and dst are host integers
+    (lists, numpy arrays, CPU tensors).  No page is written twice and none that is read is written, else
+    CaError.  Nothing is uploaded and nothing waits: the ids go with the launches."""
+    if isinstance(pools, torch.Tensor):
+        pools = [pools]
+    s, d = _page_ids("src", src), _page_ids("dst", dst)
+    if s.size != d.size:
+        raise ValueError(f"{s.size} source pages and {d.size} destinations")
+    if not 1 <= len(pools) <= _hip.MAX_POOLS:
+        raise ValueError(f"between 1 and {_hip.MAX_POOLS} pools are copied in a call (got {len(pools)})")
+    descs = (PagePool * len(pools))()
+    for i, t in enumerate(pools):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise ValueError("pools must be GPU tensors")
+        if t.dim() < 2 or t.shape[0] < 1 or not t[0].is_contiguous():
+            raise ValueError("a pool must be [num_pages, ...] with contiguous pages")
+        size = t.element_size()
+        page = t[0].numel() * size
+        descs[i] = PagePool(t.data_ptr(), page, t.stride(0) * size if t.shape[0] > 1 else page, t.shape[0])
+    with _on_device(*pools):
+        check(_hip.lib().ca_copy_pages(descs, len(pools), s.ctypes.data, d.ctypes.data, s.size, _stream()))
 
 
 def cache_fill(k_new: torch.Tensor, v_new: Optional[torch.Tensor], k_cache: Optional[KV], v_cache: Optional[KV],
@@ -567,11 +716,12 @@ def attn_pick_splits(past_blocks: Sequence[int], q_len: int, num_q_heads: int, n
     return int(n)
 
 
-def attn_fwd(q: torch.Tensor, k: KV, v: KV, table: torch.Tensor, counts: torch.Tensor, past_blocks: Sequence[int],
+def attn_fwd(q: torch.Tensor, k: AnyKV, v: AnyKV, table: torch.Tensor, counts: torch.Tensor, past_blocks: Sequence[int],
              scale: float, kv_cap: int, num_kv_heads: int, out: Optional[torch.Tensor] = None, with_lse: bool = False,
              num_splits: int = 0, workspace: Optional[torch.Tensor] = None):
-    """Indexed attention prefill; q/out [B, Lq, Hq, 128] bf16.  num_splits = 0 lets the
-    library pick the split count; a positive value splits every row that many ways."""
+    """Indexed attention prefill; q/out [B, Lq, Hq, 128] bf16, K and V bf16 (KV) or held in 4 bits
+    (KV4).  num_splits = 0 lets the library pick the split count; a positive value splits every row
+    that many ways."""
     B, Lq, Hq, _ = q.shape
     ql = seq_layout(q, "q")
     if out is None:
@@ -598,10 +748,11 @@ def attn_fwd(q: torch.Tensor, k: KV, v: KV, table: torch.Tensor, counts: torch.T
     if need > 0 and (workspace is None or workspace.numel() * workspace.element_size() < need):
         workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
     lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=q.device) if with_lse else None
-    check(_hip.lib().ca_attn_fwd(ctypes.byref(d), ctypes.byref(ql), ctypes.byref(k.layout), ctypes.byref(v.layout),
-                                 table.data_ptr(), table.stride(0), counts.data_ptr(), pa, float(scale),
-                                 ctypes.byref(ol), _ptr(lse), int(num_splits), _ptr(workspace),
-                                 int(need), _stream()))
+    entry, guard = _attn_launch("ca_attn_fwd", k, v, q, out, table, counts)
+    with guard:
+        check(entry(ctypes.byref(d), ctypes.byref(ql), ctypes.byref(k.layout), ctypes.byref(v.layout),
+                    table.data_ptr(), table.stride(0), counts.data_ptr(), pa, float(scale), ctypes.byref(ol), _ptr(lse),
+                    int(num_splits), _ptr(workspace), int(need), _stream()))
     return (out, lse) if with_lse else out
 
 
@@ -614,11 +765,12 @@ def attn_decode_workspace_bytes(kv_len: Sequence[int], q_len: int, num_q_heads: 
     return int(n)
 
 
-def attn_decode(q: torch.Tensor, k: KV, v: KV, kv_len: Sequence[int], scale: float, kv_cap: int, num_kv_heads: int,
+def attn_decode(q: torch.Tensor, k: AnyKV, v: AnyKV, kv_len: Sequence[int], scale: float, kv_cap: int, num_kv_heads: int,
                 out: Optional[torch.Tensor] = None, with_lse: bool = False, num_splits: int = 0,
                 workspace: Optional[torch.Tensor] = None):
     """Dense decode attention over the whole cache: q/out [B, q_len, Hq, 128] bf16 (q_len 1..64),
-    the q_len rows being the last positions of each request's kv_len[b] tokens.
+    the q_len rows being the last positions of each request's kv_len[b] tokens.  K and V are bf16
+    (KV) or held in 4 bits (KV4).
 
     Replaces the q_len == 1 branch of LlamaSeerAttentionChunkedDense.forward
     (compact_attn/prefill_sparse/llama/modeling_llama_seerattn_chunked_dense.py:878-894)."""
@@ -644,9 +796,10 @@ def attn_decode(q: torch.Tensor, k: KV, v: KV, kv_len: Sequence[int], scale: flo
     if need > 0 and (workspace is None or workspace.numel() * workspace.element_size() < need):
         workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
     lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=q.device) if with_lse else None
-    check(_hip.lib().ca_attn_decode(ctypes.byref(d), ctypes.byref(ql), ctypes.byref(k.layout), ctypes.byref(v.layout),
-                                    ka, float(scale), ctypes.byref(ol), _ptr(lse), int(num_splits),
-                                    _ptr(workspace), int(need), _stream()))
+    entry, guard = _attn_launch("ca_attn_decode", k, v, q, out)
+    with guard:
+        check(entry(ctypes.byref(d), ctypes.byref(ql), ctypes.byref(k.layout), ctypes.byref(v.layout), ka, float(scale),
+                    ctypes.byref(ol), _ptr(lse), int(num_splits), _ptr(workspace), int(need), _stream()))
     return (out, lse) if with_lse else out
 
 
@@ -685,6 +838,36 @@ def rope_qk(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tens
     qol, kol = seq_layout(qo, "q_out"), seq_layout(ko, "k_out")
     check(_hip.lib().ca_rope_qk(ctypes.byref(ql), ctypes.byref(qol), Hq, ctypes.byref(kl), ctypes.byref(kol), Hkv, B, L,
                                 cos.data_ptr(), sin.data_ptr(), _stream()))
+    return qo, ko
+
+
+def norm_rope_qk(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, eps: float,
+                 cos: torch.Tensor, sin: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of every head of q [B, L, Hq, 128] and k [B, L, Hkv, 128] (weights [128] bf16) and the
+    rotation, in one launch: bf16(y * cos + rotate_half(y) * sin), y = x * w / sqrt(mean(x^2) + eps) in
+    fp32, rounded once.  cos / sin fp32 [L, 128], or [B, L, 128] for requests at positions of their own."""
+    B, L, Hq, _ = q.shape
+    Hkv = k.shape[2]
+    ql, kl = seq_layout(q, "q"), seq_layout(k, "k")
+    if tuple(k.shape[:2]) != (B, L):
+        raise ValueError("q and k must cover the same [B, L] tokens")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        _need_cuda(name, w, torch.bfloat16)
+        if w.shape != (HEAD_DIM,) or not w.is_contiguous():
+            raise ValueError(f"{name} must be contiguous [{HEAD_DIM}]")
+    for name, t in (("cos", cos), ("sin", sin)):
+        _need_cuda(name, t, torch.float32)
+        if t.shape not in ((L, HEAD_DIM), (B, L, HEAD_DIM)) or t.shape != cos.shape or not t.is_contiguous():
+            raise ValueError(f"cos and sin must both be contiguous fp32 [{L}, {HEAD_DIM}] or [{B}, {L}, {HEAD_DIM}]")
+    qo = torch.empty((B, L, Hq, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
+    ko = torch.empty((B, L, Hkv, HEAD_DIM), dtype=torch.bfloat16, device=k.device)
+    if B * L == 0:
+        return qo, ko
+    qol, kol = seq_layout(qo, "q_out"), seq_layout(ko, "k_out")
+    with _on_device(q, k, q_weight, k_weight, cos, sin):
+        check(_hip.lib().ca_norm_rope_qk(ctypes.byref(ql), ctypes.byref(qol), Hq, q_weight.data_ptr(), ctypes.byref(kl),
+                                         ctypes.byref(kol), Hkv, k_weight.data_ptr(), B, L, cos.data_ptr(), sin.data_ptr(),
+                                         L * HEAD_DIM if cos.dim() == 3 else 0, float(eps), _stream()))
     return qo, ko
 
 

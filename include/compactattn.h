@@ -93,6 +93,41 @@ typedef struct {
     int64_t stride_h;
 } ca_seq_layout;
 
+/*
+ * A K or V cache held in 4 bits: a pool of pages, each 64 tokens of one KV head in
+ * CA_PAGE4_BYTES bytes.  The 128 dims of a token are four groups of 32: an element is an E2M1
+ * code (0, 0.5, 1, 1.5, 2, 3, 4, 6; bit 3 the sign), a group has a scale 2^(byte - 127).
+ *   bytes 0 .. 4095, codes, two to a byte, the even dim in the low nibble:
+ *     K: dim d of token t at 64 t + d / 2
+ *     V: dim d of token t at 256 (t / 4) + 16 (d / 8) + 4 (t % 4) + d % 8 / 2
+ *   bytes 4096 .. 4351, scale bytes of group g of token t:
+ *     K: 4096 + 64 g + 4 (t % 16) + t / 16
+ *     V: 4096 + 64 g + 16 (t % 16 / 4) + 4 (t / 16) + t % 4
+ * The scale brings the group's largest magnitude into (3.5, 7] (bytes 2 .. 252; what is
+ * larger saturates at 6), codes round to nearest even; a group with an infinity or a NaN has
+ * the byte 255 and is read as NaN.
+ * Logical block kb of row (b, kv_head) is page page_table[(b*num_kv_heads + kv_head)*
+ * page_table_stride + kb] at data + page * stride_page; ids outside [0, num_pages) are clamped
+ * into it where pages are read, and nothing is written through them.
+ */
+#define CA_PAGE4_BYTES 4352
+typedef struct {
+    void* data;          /* 16-byte aligned */
+    int64_t stride_page; /* bytes from page to page, a multiple of 16 >= CA_PAGE4_BYTES */
+    const int32_t* page_table;
+    int64_t page_table_stride;
+    int64_t num_pages;
+} ca_kv4_layout;
+
+/* A pool of pages of any kind. */
+#define CA_MAX_POOLS 8
+typedef struct {
+    void* data;          /* 16-byte aligned */
+    int64_t page_bytes;  /* a multiple of 16, at most 2^22 */
+    int64_t stride_page; /* bytes from page to page, a multiple of 16 >= page_bytes */
+    int64_t num_pages;
+} ca_page_pool;
+
 typedef struct {
     int32_t flags;         /* CA_RULE_* bits                                          */
     int32_t topk;          /* blocks per (head, query block) row, over past blocks     */
@@ -415,6 +450,42 @@ int64_t ca_attn_decode_workspace_size(const ca_dims* dims, const int32_t* kv_len
                                       int32_t num_splits);
 
 /*
+ * A cache held in 4 bits (ca_kv4_layout).
+ *
+ * ca_append_q4: quantises k_new / v_new [B, q_len, Hkv, 128] bf16 (dims.batch, dims.q_len,
+ * dims.num_kv_heads; num_q_heads unused) into positions start_host[b] .. start_host[b] + q_len - 1
+ * of every request's rows; no other byte of the pages changes.  A page may be named by one row only.
+ * ca_gather_q4: the values of those positions, bf16 [B, Hkv, q_len, 128] contiguous; v_cache and
+ * v_out may both be NULL.
+ * ca_attn_fwd_q4, ca_attn_decode_q4: ca_attn_fwd and ca_attn_decode over such a cache (bf16 queries,
+ * fp32 scores and sums, the weights rounded to bf16 for the second product); workspaces as theirs
+ * (ca_attn_workspace_size, ca_attn_decode_workspace_size).  Keys that a query does not see change
+ * nothing, whatever their pages hold; a query that sees a NaN key gets NaN, one that sees a NaN
+ * value gets NaN in that group's dims.  A query that sees no key gets zeros and an lse of -inf.
+ */
+int ca_append_q4(const ca_dims* dims, const ca_seq_layout* k_new, const ca_seq_layout* v_new,
+                 const ca_kv4_layout* k_cache, const ca_kv4_layout* v_cache, const int32_t* start_host,
+                 void* stream);
+int ca_gather_q4(const ca_dims* dims, const ca_kv4_layout* k_cache, const ca_kv4_layout* v_cache,
+                 const int32_t* start_host, void* k_out, void* v_out, void* stream);
+int ca_attn_fwd_q4(const ca_dims* dims, const ca_seq_layout* q, const ca_kv4_layout* k, const ca_kv4_layout* v,
+                   const int32_t* table, int64_t table_stride, const int32_t* counts,
+                   const int32_t* past_blocks_host, float scale, const ca_seq_layout* out, float* lse,
+                   int32_t num_splits, void* workspace, int64_t workspace_bytes, void* stream);
+int ca_attn_decode_q4(const ca_dims* dims, const ca_seq_layout* q, const ca_kv4_layout* k, const ca_kv4_layout* v,
+                      const int32_t* kv_len_host, float scale, const ca_seq_layout* out, float* lse,
+                      int32_t num_splits, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Copies n pages inside each of n_pools (at most CA_MAX_POOLS) pools: page dst_host[i] becomes page
+ * src_host[i].  The ids are host arrays, read before the call returns.  Every id lies in every pool,
+ * no page is written twice and none that is read is written (CA_ERR_INVALID otherwise), so the order
+ * of the copies does not matter.  n = 0 does nothing.
+ */
+int ca_copy_pages(const ca_page_pool* pools, int32_t n_pools, const int32_t* src_host, const int32_t* dst_host,
+                  int32_t n, void* stream);
+
+/*
  * Model plumbing.  Fused element-wise kernels of the Llama integration; they have no
  * counterpart in _C_compactattn and replace chains of PyTorch element-wise kernels around
  * the compactattn layers (bf16 in and out, fp32 math).
@@ -436,6 +507,14 @@ int ca_rope_apply(const ca_seq_layout* x, const ca_seq_layout* y, int32_t batch,
 int ca_rope_qk(const ca_seq_layout* q, const ca_seq_layout* q_out, int32_t q_heads, const ca_seq_layout* k,
                const ca_seq_layout* k_out, int32_t k_heads, int32_t batch, int32_t len, const float* cos,
                const float* sin, void* stream);
+/* RMS norm of every head of q and k with its own weight ([128] bf16, one for all heads of q and one for
+ * k's), then the rotation, in one launch: y = x * w / sqrt(mean(x^2) + eps), out = bf16(y * cos +
+ * rotate_half(y) * sin), fp32 throughout and rounded once.  cos/sin as for ca_rope_apply, or with
+ * cs_stride_b (floats, a multiple of 4) from one request's len rows to the next one's (0: the same rows). */
+int ca_norm_rope_qk(const ca_seq_layout* q, const ca_seq_layout* q_out, int32_t q_heads, const uint16_t* q_weight,
+                    const ca_seq_layout* k, const ca_seq_layout* k_out, int32_t k_heads, const uint16_t* k_weight,
+                    int32_t batch, int32_t len, const float* cos, const float* sin, int64_t cs_stride_b, float eps,
+                    void* stream);
 int ca_rmsnorm(const uint16_t* x, int64_t x_stride, const uint16_t* residual, int64_t r_stride, uint16_t* sum_out,
                int64_t s_stride, const uint16_t* w, uint16_t* y, int64_t y_stride, int64_t rows, int32_t n, float eps,
                void* stream);

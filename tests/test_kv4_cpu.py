@@ -1,0 +1,190 @@
+"""The 4-bit cache, page copies and the q/k norm without a GPU: the format's oracle against its definition, the
+C-ABI's refusals (checked before any launch) and those of the tensor front end."""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from compactattention_amd import _hip, ops
+from tests import kv4_oracle as ref
+
+FAKE = 1 << 20  # aligned, never dereferenced: validation fails first
+INVALID, LIMIT, WORKSPACE = _hip.CA_ERR_INVALID, _hip.CA_ERR_LIMIT, _hip.CA_ERR_WORKSPACE
+
+
+def _dims(**kw):
+    d = dict(batch=1, q_len=4, num_q_heads=8, num_kv_heads=2, kv_cap=10)
+    d.update(kw)
+    return _hip.Dims(d["batch"], d["q_len"], d["num_q_heads"], d["num_kv_heads"], d["kv_cap"])
+
+
+def _seq(data=FAKE, sb=0, st=1024, sh=128):
+    return _hip.SeqLayout(data, sb, st, sh)
+
+
+def _kv4(data=FAKE, stride=4352, table=FAKE, pts=16, pages=100):
+    return _hip.Kv4Layout(data, stride, table, pts, pages)
+
+
+def _ints(*v):
+    return (ctypes.c_int32 * len(v))(*v)
+
+
+BAD_KV = [(dict(data=None), INVALID), (dict(data=FAKE + 8), INVALID), (dict(stride=4336), INVALID),
+          (dict(stride=4360), INVALID), (dict(table=None), INVALID), (dict(table=FAKE + 2), INVALID),
+          (dict(pts=0), INVALID), (dict(pages=0), INVALID), (dict(pages=1 << 31), INVALID)]
+
+
+def test_format_oracle():
+    """Levels, ties, the largest magnitude's bracket and the scale's limits."""
+    assert [ref.LEVELS[c] for c in range(8)] == [0, 0.5, 1, 1.5, 2, 3, 4, 6]
+    x = np.zeros((1, 128))
+    x[0, :8] = [6.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0]  # amax 6: scale 1
+    code, byte = ref.quantise(x)
+    assert byte[0, 0] == 127 and code[0, :8].tolist() == [7, 0, 2, 2, 4, 4, 6, 6]
+    assert byte[0, 1] == 2 and not code[0, 32:].any()
+    for top, want in ((7.0, 127), (7.0625, 128), (3.5, 126), (3.53125, 127), (2.0 ** -140, 2), (3.3e38, 252)):
+        y = np.zeros((1, 128))
+        y[0, 40] = -top
+        assert ref.quantise(y)[1][0, 1] == want, top
+    rng = np.random.default_rng(0)
+    z = ref.bf16(rng.standard_normal((50, 128)) * 10.0 ** rng.integers(-8, 8, (50, 1)))
+    code, byte = ref.quantise(z)
+    back = ref.values(code, byte)
+    top = np.abs(z).reshape(50, 4, 32).max(-1)
+    assert ((top / 2.0 ** (byte.astype(float) - 127) <= 7) & (top / 2.0 ** (byte.astype(float) - 127) > 3.5)).all()
+    assert (np.abs(back - z) <= 2.0 ** (byte.astype(float) - 127).repeat(32, -1)).all()
+    seen = set()
+    for of_v in (False, True):
+        at = [ref.code_at(t, d, of_v) for t in range(64) for d in range(0, 128, 2)]
+        sat = [ref.scale_at(t, g, of_v) for t in range(64) for g in range(4)]
+        assert sorted(at) == list(range(4096)) and sorted(sat) == list(range(4096, 4352))
+        seen.add(tuple(at))
+    assert len(seen) == 2
+
+
+@pytest.mark.parametrize("kw,code", BAD_KV)
+def test_4bit_layouts_are_checked(kw, code):
+    lib, d, good, bad = _hip.lib(), _dims(), _kv4(), _kv4(**kw)
+    for k, v in ((bad, good), (good, bad)):
+        p = [ctypes.byref(x) for x in (d, _seq(), k, v)]
+        assert lib.ca_append_q4(p[0], p[1], p[1], p[2], p[3], _ints(0), None) == code
+        assert lib.ca_gather_q4(p[0], p[2], p[3], _ints(0), FAKE, FAKE, None) == code
+        assert lib.ca_attn_fwd_q4(p[0], p[1], p[2], p[3], FAKE, 16, FAKE, _ints(0), 0.1, p[1], None, 1, None, 0, None) == code
+        assert lib.ca_attn_decode_q4(p[0], p[1], p[2], p[3], _ints(64), 0.1, p[1], None, 1, None, 0, None) == code
+    assert lib.ca_append_q4(ctypes.byref(d), ctypes.byref(_seq()), ctypes.byref(_seq()), None, ctypes.byref(good), _ints(0), None) == INVALID
+
+
+@pytest.mark.parametrize("dims,start,code", [
+    (dict(batch=0), (0,), INVALID), (dict(batch=65), (0,) * 65, LIMIT), (dict(q_len=0), (0,), INVALID),
+    (dict(num_kv_heads=0), (0,), INVALID), (dict(kv_cap=0), (0,), INVALID), (dict(kv_cap=(1 << 24) + 1), (0,), LIMIT),
+    (dict(), (-1,), INVALID), (dict(), (637,), INVALID), (dict(batch=2), (0, 640), INVALID),
+    (dict(), (2 ** 31 - 1,), INVALID), (dict(q_len=1 << 20, num_kv_heads=1 << 12, kv_cap=1 << 24), (0,), LIMIT),
+])
+def test_append_and_gather_rows_are_checked(dims, start, code):
+    lib, d, kv, s = _hip.lib(), _dims(**dims), _kv4(pts=1 << 25), _seq()
+    r = [ctypes.byref(x) for x in (d, s, kv)]
+    assert lib.ca_append_q4(r[0], r[1], r[1], r[2], r[2], _ints(*start), None) == code
+    assert lib.ca_gather_q4(r[0], r[2], r[2], _ints(*start), FAKE, FAKE, None) == code
+    assert lib.ca_append_q4(None, r[1], r[1], r[2], r[2], _ints(*start), None) == INVALID
+    assert lib.ca_append_q4(r[0], r[1], r[1], r[2], r[2], None, None) == INVALID
+
+
+def test_gather_outputs_are_checked():
+    lib, d, kv = _hip.lib(), _dims(), _kv4()
+    r = [ctypes.byref(x) for x in (d, kv)]
+    assert lib.ca_gather_q4(r[0], r[1], r[1], _ints(0), None, FAKE, None) == INVALID
+    assert lib.ca_gather_q4(r[0], r[1], r[1], _ints(0), FAKE, None, None) == INVALID
+    assert lib.ca_gather_q4(r[0], r[1], None, _ints(0), FAKE, FAKE, None) == INVALID
+    assert lib.ca_gather_q4(r[0], r[1], r[1], _ints(0), FAKE + 8, FAKE, None) == INVALID
+
+
+def test_attention_arguments_are_checked():
+    lib = _hip.lib()
+
+    def fwd(dims=None, q=None, table=FAKE, stride=16, counts=FAKE, past=(0,), scale=0.1, splits=1, ws=None, wsb=0):
+        r = [ctypes.byref(x) for x in (_dims(**(dims or {})), q or _seq(), _kv4())]
+        return lib.ca_attn_fwd_q4(r[0], r[1], r[2], r[2], table, stride, counts, _ints(*past), scale, ctypes.byref(_seq()),
+                                  None, splits, ws, wsb, None)
+
+    def decode(dims=None, lens=(64,), scale=0.1, splits=1, ws=None, wsb=0):
+        r = [ctypes.byref(x) for x in (_dims(**(dims or {})), _seq(), _kv4())]
+        return lib.ca_attn_decode_q4(r[0], r[1], r[2], r[2], _ints(*lens), scale, r[1], None, splits, ws, wsb, None)
+
+    assert fwd(dims=dict(num_q_heads=7)) == INVALID
+    assert fwd(dims=dict(num_q_heads=34)) == LIMIT
+    assert fwd(dims=dict(kv_cap=0)) == INVALID
+    assert fwd(past=(10,)) == INVALID and fwd(past=(-1,)) == INVALID
+    assert fwd(q=_seq(data=FAKE + 2)) == INVALID and fwd(q=_seq(st=1023)) == INVALID
+    assert fwd(table=None) == INVALID and fwd(counts=None) == INVALID and fwd(stride=9) == INVALID
+    assert fwd(table=FAKE + 2) == INVALID and fwd(counts=FAKE + 1) == INVALID
+    assert fwd(scale=0.0) == INVALID and fwd(scale=math.nan) == INVALID
+    assert fwd(splits=17) == INVALID and fwd(splits=-1) == INVALID and fwd(splits=2) == WORKSPACE
+    need = lib.ca_attn_workspace_size(ctypes.byref(_dims()), _ints(0), 2)
+    assert fwd(splits=2, ws=FAKE, wsb=need - 1) == WORKSPACE and fwd(splits=2, ws=FAKE + 4, wsb=need) == WORKSPACE
+    assert decode(dims=dict(q_len=65), lens=(65,)) == INVALID
+    assert decode(lens=(3,)) == INVALID and decode(lens=(641,)) == INVALID
+    assert decode(scale=-1.0) == INVALID and decode(splits=65) == INVALID and decode(splits=2) == WORKSPACE
+
+
+def test_copy_pages_arguments_are_checked():
+    lib = _hip.lib()
+    pool = lambda data=FAKE, page=4352, stride=4352, n=10: _hip.PagePool(data, page, stride, n)  # noqa: E731
+
+    def copy(pools, src=(0,), dst=(1,), n=None):
+        arr = (_hip.PagePool * max(1, len(pools)))(*pools)
+        return lib.ca_copy_pages(arr, len(pools), _ints(*src), _ints(*dst), len(src) if n is None else n, None)
+
+    assert copy([]) == INVALID and copy([pool()] * 9) == INVALID
+    assert lib.ca_copy_pages(None, 1, _ints(0), _ints(1), 1, None) == INVALID
+    assert copy([pool(data=None)]) == INVALID and copy([pool(data=FAKE + 8)]) == INVALID
+    assert copy([pool(page=0)]) == INVALID and copy([pool(page=4360, stride=4368)]) == INVALID
+    assert copy([pool(stride=4336)]) == INVALID and copy([pool(stride=4360)]) == INVALID
+    assert copy([pool(page=(1 << 22) + 16, stride=1 << 23)]) == LIMIT
+    assert copy([pool(n=0)]) == INVALID
+    assert copy([pool()], n=-1) == INVALID
+    assert copy([pool(), pool(n=5)], src=(0,), dst=(5,)) == INVALID  # every pool has the page
+    assert "outside" in _hip.last_error()
+    assert copy([pool()], src=(0, 1), dst=(2, 2)) == INVALID and "written twice" in _hip.last_error()
+    assert copy([pool()], src=(0, 1), dst=(2, 0)) == INVALID and "read and written" in _hip.last_error()
+    assert copy([pool()], src=(-1,), dst=(2,)) == INVALID and copy([pool()], src=(10,), dst=(2,)) == INVALID
+    assert copy([pool()], n=0) == _hip.CA_OK
+    assert lib.ca_copy_pages((_hip.PagePool * 1)(pool()), 1, None, _ints(1), 1, None) == INVALID
+
+
+def test_norm_rope_arguments_are_checked():
+    lib = _hip.lib()
+
+    def call(q=None, k=None, hq=8, hk=2, w=FAKE, batch=1, length=4, cos=FAKE, csb=0, eps=1e-5):
+        s = ctypes.byref(_seq())
+        return lib.ca_norm_rope_qk(ctypes.byref(q or _seq()), s, hq, w, ctypes.byref(k or _seq()), s, hk, w, batch, length,
+                                   cos, FAKE, csb, eps, None)
+
+    assert call(q=_seq(data=FAKE + 2)) == INVALID and call(k=_seq(st=12)) == INVALID
+    assert call(hq=0) == INVALID and call(batch=0) == INVALID and call(length=0) == INVALID
+    assert call(hq=70000) == LIMIT and call(batch=1 << 15, length=1 << 15, hq=64) == LIMIT
+    assert call(w=None) == INVALID and call(w=FAKE + 2) == INVALID and call(cos=None) == INVALID
+    assert call(csb=-4) == INVALID and call(csb=6) == INVALID
+    assert call(eps=-1.0) == INVALID and call(eps=math.nan) == INVALID
+
+
+def test_front_end_refuses_host_tensors():
+    pool, table = torch.zeros((4, 4352), dtype=torch.uint8), torch.zeros((2, 2), dtype=torch.int32)
+    with pytest.raises(ValueError, match="GPU tensor"):
+        ops.KV4.paged(pool, table)
+    x = torch.zeros((1, 1, 2, 128), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="4 bits"):
+        ops.append_q4(x, x, None, None, 0, 1)
+    with pytest.raises(ValueError, match="shape"):
+        ops.append_q4(x, x[:, :, :1], None, None, 0, 1)
+    with pytest.raises(ValueError, match="4 bits"):
+        ops.gather_q4(None, None, 1, 1, 0, 1)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.copy_pages([torch.zeros(4, 16)], [0], [1])
+    w = torch.zeros(128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="GPU tensor"):
+        ops.norm_rope_qk(x, x, w, w, 1e-5, torch.zeros(1, 128), torch.zeros(1, 128))
