@@ -753,15 +753,16 @@ int ca_gather_q4(const ca_dims* dims, const ca_kv4_layout* k_cache, const ca_kv4
     ca::Kv4Addr kc, vc;
     int blocks = 0, rc;
     if ((rc = check_rows4(dims, start_host, &blocks)) != CA_OK) return rc;
-    if ((v_cache == nullptr) != (v_out == nullptr))
-        return fail(CA_ERR_INVALID, "v_cache and v_out are given together or not at all");
-    if ((rc = check_kv4(k_cache, "k_cache", blocks, &kc)) != CA_OK) return rc;
+    if ((k_cache == nullptr) != (k_out == nullptr) || (v_cache == nullptr) != (v_out == nullptr) ||
+        (k_cache == nullptr && v_cache == nullptr))
+        return fail(CA_ERR_INVALID, "k_cache with k_out, v_cache with v_out, or both");
+    if (k_cache != nullptr && (rc = check_kv4(k_cache, "k_cache", blocks, &kc)) != CA_OK) return rc;
     if (v_cache != nullptr && (rc = check_kv4(v_cache, "v_cache", blocks, &vc)) != CA_OK) return rc;
-    if (k_out == nullptr || !aligned16(k_out) || !aligned16(v_out))
-        return fail(CA_ERR_INVALID, "k_out is required, and the outputs must be 16-byte aligned");
-    hipError_t e = ca::launch_gather4(dims->batch, dims->q_len, dims->num_kv_heads, start_host, kc,
-                                      v_cache != nullptr ? &vc : nullptr, static_cast<uint16_t*>(k_out),
-                                      static_cast<uint16_t*>(v_out), static_cast<hipStream_t>(stream));
+    if (!aligned16(k_out) || !aligned16(v_out)) return fail(CA_ERR_INVALID, "the outputs must be 16-byte aligned");
+    hipError_t e = ca::launch_gather4(dims->batch, dims->q_len, dims->num_kv_heads, start_host,
+                                      k_cache != nullptr ? &kc : nullptr, v_cache != nullptr ? &vc : nullptr,
+                                      static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out),
+                                      static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail(e, "gather_q4 launch");
     return ok();
 }

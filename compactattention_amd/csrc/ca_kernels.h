@@ -102,8 +102,8 @@ struct PagePool {
 // Quantises L tokens of every request at start[b] .. start[b] + L - 1 into its pages
 hipError_t launch_append4(int B, int L, int H, const int32_t* start, const SeqAddr& k_new, const SeqAddr& v_new,
                           const Kv4Addr& k, const Kv4Addr& v, hipStream_t stream);
-// The tokens back as bf16 [B, H, L, 128]; v and v_out nullable
-hipError_t launch_gather4(int B, int L, int H, const int32_t* start, const Kv4Addr& k, const Kv4Addr* v,
+// The tokens back as bf16 [B, H, L, 128]; k with k_out, or v with v_out, may be null
+hipError_t launch_gather4(int B, int L, int H, const int32_t* start, const Kv4Addr* k, const Kv4Addr* v,
                           uint16_t* k_out, uint16_t* v_out, hipStream_t stream);
 // pool[dst[i]] = pool[src[i]] for every pool, in launches of a few hundred pages
 hipError_t launch_copy_pages(const PagePool* pools, int n_pools, const int32_t* src, const int32_t* dst, int n,

@@ -93,8 +93,8 @@ __global__ __launch_bounds__(256) void append4_kernel(Append4Params p) {
 struct Gather4Params {
     Kv4Rows r;
     Kv4Addr k, v;
-    uint16_t* k_out;
-    uint16_t* v_out;  // nullable
+    uint16_t* k_out;  // nullable, as v_out
+    uint16_t* v_out;
 };
 
 __device__ __forceinline__ u32x4p_t decode8(const uint8_t* page, int code, int scale) {
@@ -113,9 +113,11 @@ __global__ __launch_bounds__(256) void gather4_kernel(Gather4Params p) {
     const int b = row / static_cast<uint32_t>(p.r.H);
     const int pos = p.r.start[b] + t0;
     const int kb = pos >> 6, t = pos & 63;
-    const int64_t kp = clamp_page(p.k.page_table[row * p.k.pts + kb], p.k.max_page);
-    const u32x4p_t kx = decode8(p.k.data + kp * p.k.stride, k4_code(t, 8 * m), k4_scale(t, m >> 2));
-    *reinterpret_cast<u32x4p_t*>(p.k_out + i * kD + 8 * m) = kx;
+    if (p.k_out != nullptr) {
+        const int64_t kp = clamp_page(p.k.page_table[row * p.k.pts + kb], p.k.max_page);
+        const u32x4p_t kx = decode8(p.k.data + kp * p.k.stride, k4_code(t, 8 * m), k4_scale(t, m >> 2));
+        *reinterpret_cast<u32x4p_t*>(p.k_out + i * kD + 8 * m) = kx;
+    }
     if (p.v_out != nullptr) {
         const int64_t vp = clamp_page(p.v.page_table[row * p.v.pts + kb], p.v.max_page);
         const u32x4p_t vx = decode8(p.v.data + vp * p.v.stride, v4_code(t, 8 * m), v4_scale(t, m >> 2));
@@ -179,9 +181,11 @@ hipError_t launch_append4(int B, int L, int H, const int32_t* start, const SeqAd
     return hipGetLastError();
 }
 
-hipError_t launch_gather4(int B, int L, int H, const int32_t* start, const Kv4Addr& k, const Kv4Addr* v,
+hipError_t launch_gather4(int B, int L, int H, const int32_t* start, const Kv4Addr* k, const Kv4Addr* v,
                           uint16_t* k_out, uint16_t* v_out, hipStream_t stream) {
-    Gather4Params p{rows_of(B, L, H, start), k, v != nullptr ? *v : k, k_out, v != nullptr ? v_out : nullptr};
+    const Kv4Addr none{};
+    Gather4Params p{rows_of(B, L, H, start), k != nullptr ? *k : none, v != nullptr ? *v : none,
+                    k != nullptr ? k_out : nullptr, v != nullptr ? v_out : nullptr};
     hipLaunchKernelGGL(gather4_kernel, dim3(static_cast<unsigned>((p.r.rows + 15) / 16)), dim3(256), 0, stream, p);
     return hipGetLastError();
 }

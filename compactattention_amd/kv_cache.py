@@ -10,7 +10,7 @@ Seer model (modeling_llama_seerattn_chunked_dense.py:398-478).
 
 Layout of one layer:
   - K and V pages: a pool of 64-token pages ``[num_pages, 64, 128]`` bf16 each (one 16 KiB
-    page per (request, KV head, logical block)); the pool only grows, and growing keeps every
+    page per (request, KV head, logical block)); the pool grows on demand, and growing keeps every
     page id (the contents move to the larger pool once);
   - the page table: int32 ``[B*Hkv, blocks]`` (row = b*Hkv + h), logical block -> page id,
     kept on the device for the kernels and mirrored on the host, where pages are allocated;
@@ -22,9 +22,15 @@ Layout of one layer:
     its mean-K cache when the token count disagrees, modeling_llama_flashprefill_compactattn.py:
     128-147).  Gate-K summaries come from pre-RoPE keys the cache does not hold, so a chunk that
     follows such a block raises (``require_kgate``).
+A cache of ``bits=4`` holds its pages in 4 bits (``ops.KV4``: [num_pages, 4352] uint8, a quarter of the
+bytes), quantised as tokens are appended.  The chunk summaries are still pooled from the bf16 keys; a
+mean-K that is recomputed from the cache (``refresh_kmean``) and the views are those of the stored values.
+
 Pages are reference-counted: ``fork`` lets a request share another's pages, and a decode
-append into a shared, partly filled page copies it first.  Appends write the chunk's pages
-and summaries in place through the cache-fill kernel; nothing is ever re-copied.
+append into a shared, partly filled page copies it first.  ``truncate`` gives the pages behind a
+length back, ``compact`` moves the pages in use to the front of the pool and gives the rest of its memory
+back.  Appends write the chunk's pages and summaries in place through the cache-fill kernel; nothing is
+ever re-copied.
 
 Host-side allocation happens in ``append``/``append_tokens`` before the kernels are launched
 (a small page-table upload on the current stream), so a HIP graph that captures the chunk
@@ -41,6 +47,7 @@ from . import ops
 
 BLOCK = 64
 HEAD_DIM = 128
+PAGE4_BYTES = ops.PAGE4_BYTES
 
 
 def _kernel_rows(t: torch.Tensor) -> torch.Tensor:
@@ -50,15 +57,24 @@ def _kernel_rows(t: torch.Tensor) -> torch.Tensor:
 
 
 class PagePool:
-    """Grow-only pool of 64-token K and V pages with reference counts."""
+    """Pool of 64-token K and V pages (bf16, or held in 4 bits) with reference counts; it grows on demand and
+    shrinks in ``compact`` only."""
 
-    def __init__(self, num_pages: int, device):
+    def __init__(self, num_pages: int, device, bits: int = 16):
+        if bits not in (4, 16):
+            raise ValueError(f"pages hold 16 or 4 bits a value (got {bits})")
         num_pages = max(int(num_pages), 1)
         self.device = torch.device(device)
-        self.k = torch.zeros((num_pages, BLOCK, HEAD_DIM), dtype=torch.bfloat16, device=self.device)
+        self.bits = bits
+        self.k = self._pages(num_pages)
         self.v = torch.zeros_like(self.k)
         self.refs = np.zeros(num_pages, np.int32)
         self._free: List[int] = list(range(num_pages - 1, -1, -1))  # pop() hands out ascending ids
+
+    def _pages(self, n: int) -> torch.Tensor:
+        if self.bits == 4:
+            return torch.zeros((n, PAGE4_BYTES), dtype=torch.uint8, device=self.device)
+        return torch.zeros((n, BLOCK, HEAD_DIM), dtype=torch.bfloat16, device=self.device)
 
     @property
     def num_pages(self) -> int:
@@ -91,26 +107,58 @@ class PagePool:
         old = self.num_pages
         new = max(2 * old, old + need)
         for name in ("k", "v"):
-            t = torch.zeros((new, BLOCK, HEAD_DIM), dtype=torch.bfloat16, device=self.device)
+            t = self._pages(new)
             t[:old].copy_(getattr(self, name))
             setattr(self, name, t)
         self.refs = np.concatenate([self.refs, np.zeros(new - old, np.int32)])
         self._free = list(range(new - 1, old - 1, -1)) + self._free
+
+    def copy(self, src, dst) -> None:
+        """The contents of pages src in pages dst (K and V)."""
+        if self.device.type == "cpu":
+            s, d = (torch.as_tensor(np.asarray(x, np.int64)) for x in (src, dst))
+            self.k[d] = self.k[s]
+            self.v[d] = self.v[s]
+        else:
+            ops.copy_pages([self.k, self.v], src, dst)
+
+    def compact(self, shrink: bool = True) -> np.ndarray:
+        """Move the pages in use to the lowest ids (those past the number of pages in use take the free places
+        below it, in order) and, with shrink, give the memory behind them back.  Returns the new id of every
+        old page (-1 for a free one); the holders' page tables have to follow."""
+        used = self.refs > 0
+        n = int(used.sum())
+        src = np.nonzero(used[n:])[0] + n
+        dst = np.nonzero(~used[:n])[0]
+        new_id = np.where(used, np.arange(self.num_pages), -1).astype(np.int32)
+        new_id[src] = dst
+        self.copy(src, dst)
+        self.refs[dst] = self.refs[src]
+        self.refs[src] = 0
+        size = max(n, 1) if shrink else self.num_pages
+        if size < self.num_pages:
+            self.k, self.v = self.k[:size].clone(), self.v[:size].clone()
+            self.refs = self.refs[:size].copy()
+        self._free = list(range(size - 1, n - 1, -1))
+        return new_id
 
 
 class PagedKVCache:
     """One layer's paged K/V cache for ``batch`` requests that advance together."""
 
     def __init__(self, batch: int, num_kv_heads: int, max_tokens: int, device, with_kmean: bool = True,
-                 with_kgate: bool = False, kgate_heads: Optional[int] = None, pool_pages: Optional[int] = None):
+                 with_kgate: bool = False, kgate_heads: Optional[int] = None, pool_pages: Optional[int] = None,
+                 bits: int = 16):
         """max_tokens sizes the page table and summaries (they grow on demand); pool_pages
-        sizes the initial page pool (default: every row's max_tokens)."""
+        sizes the initial page pool (default: every row's max_tokens); bits is 16 (bf16 pages) or 4."""
         self.batch = batch
         self.num_kv_heads = num_kv_heads
         self.rows = batch * num_kv_heads
         self.device = torch.device(device)
         self.cap = max(-(-int(max_tokens) // BLOCK), 1)  # blocks per row of the table and summaries
-        self.pool = PagePool(pool_pages if pool_pages is not None else self.rows * self.cap, self.device)
+        self.pool = PagePool(pool_pages if pool_pages is not None else self.rows * self.cap, self.device,
+                             bits)
+        self.bits = bits
         self._pt = np.full((self.rows, self.cap), -1, np.int32)  # host mirror; -1 = unmapped
         self.page_table = torch.full((self.rows, self.cap), -1, dtype=torch.int32, device=self.device)
         self.kgate_heads = kgate_heads or num_kv_heads
@@ -128,8 +176,10 @@ class PagedKVCache:
     def past_blocks(self) -> int:
         return self.length // BLOCK
 
-    def layouts(self) -> Tuple[ops.KV, ops.KV]:
+    def layouts(self) -> Tuple[ops.AnyKV, ops.AnyKV]:
         """K and V as (pool, page table) layouts for the kernels."""
+        if self.bits == 4:
+            return ops.KV4.paged(self.pool.k, self.page_table), ops.KV4.paged(self.pool.v, self.page_table)
         return ops.KV.paged(self.pool.k, self.page_table), ops.KV.paged(self.pool.v, self.page_table)
 
     def pages_of(self, b: int, h: int) -> List[int]:
@@ -191,10 +241,7 @@ class PagedKVCache:
             return
         old = [int(col[r]) for r in moved]
         fresh = self.pool.alloc(len(moved))
-        src = torch.as_tensor(old, device=self.device, dtype=torch.long)
-        dst = torch.as_tensor(fresh, device=self.device, dtype=torch.long)
-        self.pool.k[dst] = self.pool.k[src]
-        self.pool.v[dst] = self.pool.v[src]
+        self.pool.copy(old, fresh)
         self.pool.release(old)
         for r, p in zip(moved, fresh):
             self._pt[r, kb] = p
@@ -224,8 +271,12 @@ class PagedKVCache:
         self.refresh_kmean(past)
         self._map(past, past - (-L // BLOCK))
         K, V = self.layouts()
-        ops.cache_fill(k_new, v_new, K, V, [past] * B, self.cap, self.kmean, gate_wk=gate_wk, rope_cos=rope_cos,
-                       rope_sin=rope_sin, kgate=self.kgate if gate_wk is not None else None)
+        if self.bits == 4:
+            ops.append_q4(k_new, v_new, K, V, past * BLOCK, self.cap)
+            K = V = None  # the summaries of the bf16 keys
+        if K is not None or self.kmean is not None or gate_wk is not None:
+            ops.cache_fill(k_new, v_new, K, V, [past] * B, self.cap, self.kmean, gate_wk=gate_wk, rope_cos=rope_cos,
+                           rope_sin=rope_sin, kgate=self.kgate if gate_wk is not None else None)
         self.length += L
         if self.kmean is not None:
             self.kmean_blocks = self.past_blocks
@@ -251,7 +302,12 @@ class PagedKVCache:
         self.refresh_kmean(past)
         self._map(past, past - (-L // BLOCK))
         K, V = self.layouts()
-        qhat = ops.cache_fill_pool_query(k_new, v_new, K, V, [past] * B, self.cap, self.kmean, q)
+        if self.bits == 4:
+            ops.append_q4(k_new, v_new, K, V, past * BLOCK, self.cap)
+            ops.cache_fill(k_new, None, None, None, [past] * B, self.cap, self.kmean)
+            qhat = ops.pool_query(q, [past] * B, self.cap, num_kv_heads=Hkv)
+        else:
+            qhat = ops.cache_fill_pool_query(k_new, v_new, K, V, [past] * B, self.cap, self.kmean, q)
         self.length += L
         self.kmean_blocks = self.past_blocks
         return past, qhat
@@ -263,6 +319,12 @@ class PagedKVCache:
         if self.kmean is None or self.kmean_blocks >= upto:
             return
         b0 = self.kmean_blocks
+        if self.bits == 4:
+            n = (upto - b0) * BLOCK
+            keys, _ = ops.gather_q4(self.layouts()[0], None, self.batch, self.num_kv_heads, b0 * BLOCK, n)
+            ops.cache_fill(keys.transpose(1, 2), None, None, None, [b0] * self.batch, self.cap, self.kmean)
+            self.kmean_blocks = upto
+            return
         idx = torch.from_numpy(np.ascontiguousarray(self._pt[:, b0:upto]).astype(np.int64)).to(self.device)
         n = (upto - b0) * BLOCK
         keys = self.pool.k[idx.reshape(-1)].view(self.batch, self.num_kv_heads, n, HEAD_DIM).transpose(1, 2)
@@ -294,7 +356,12 @@ class PagedKVCache:
         self._map(start // BLOCK, -(-end // BLOCK))
         if start % BLOCK:
             self._unshare(start // BLOCK)
-        if self.device.type == "cpu":  # a cache in host memory (its kernels do not exist): plain indexing
+        if self.bits == 4:
+            if self.device.type == "cpu":
+                raise ValueError("a cache held in 4 bits is on a GPU")
+            K, V = self.layouts()
+            ops.append_q4(_kernel_rows(k_new), _kernel_rows(v_new), K, V, start, self.cap)
+        elif self.device.type == "cpu":  # a cache in host memory (its kernels do not exist): plain indexing
             pos = np.arange(start, end)
             flat = torch.from_numpy(self._pt[:, pos // BLOCK].astype(np.int64) * BLOCK + (pos % BLOCK)[None, :])
             for pool, new in ((self.pool.k, k_new), (self.pool.v, v_new)):
@@ -326,7 +393,44 @@ class PagedKVCache:
             if t is not None:
                 t[dst].copy_(t[src])
 
+    def truncate(self, tokens: int, keep_pages: bool = False) -> None:
+        """Forget what every request holds past ``tokens`` tokens (a rejected draft, a shorter prefix); the pages
+        behind them go back to the pool.  With keep_pages those that a row owns alone stay mapped, as in
+        ``reset``.  Summaries of a block that is cut are no longer valid."""
+        if not 0 <= tokens <= self.length:
+            raise ValueError(f"cannot truncate to {tokens} tokens: the cache holds {self.length}")
+        nb = -(-int(tokens) // BLOCK)
+        tail = self._pt[:, nb:]
+        drop = tail >= 0
+        if keep_pages:
+            drop &= self.pool.refs[np.where(drop, tail, 0)] > 1
+        if drop.any():
+            self.pool.release(tail[drop])
+            tail[drop] = -1
+            self._upload(nb, self.cap)
+        self.length = int(tokens)
+        self.kmean_blocks = min(self.kmean_blocks, self.length // BLOCK)
+        self.kgate_blocks = min(self.kgate_blocks, self.length // BLOCK)
+
+    def compact(self, shrink: bool = True) -> int:
+        """Move the pages in use to the front of the pool (``ops.copy_pages``) and, with shrink, give the memory
+        behind them back; returns how many pages moved.  Page ids, and with shrink the pools, change: graphs that
+        were captured on this cache are recorded again."""
+        new_id = self.pool.compact(shrink)
+        moved = int((new_id[new_id >= 0] != np.nonzero(new_id >= 0)[0]).sum())
+        if moved:
+            self._pt = np.where(self._pt >= 0, new_id[np.where(self._pt >= 0, self._pt, 0)], -1).astype(np.int32)
+            self._upload(0, self.cap)
+        return moved
+
     # -- views ----------------------------------------------------------------------------
+    def _values(self, of_v: bool) -> torch.Tensor:
+        if self.bits == 4:
+            K, V = self.layouts()
+            got = ops.gather_q4(None if of_v else K, V if of_v else None, self.batch, self.num_kv_heads, 0, self.length)
+            return got[1 if of_v else 0]
+        return self._gather(self.pool.v if of_v else self.pool.k)
+
     def _gather(self, pool: torch.Tensor) -> torch.Tensor:
         nb = -(-self.length // BLOCK)
         idx = torch.from_numpy(self._pt[:, :nb].astype(np.int64)).to(self.device)
@@ -335,10 +439,10 @@ class PagedKVCache:
 
     def k_hf(self) -> torch.Tensor:
         """The stored keys as a heads-first [B, Hkv, length, 128] tensor (a gathered copy)."""
-        return self._gather(self.pool.k)
+        return self._values(False)
 
     def v_hf(self) -> torch.Tensor:
-        return self._gather(self.pool.v)
+        return self._values(True)
 
     def reset(self, keep_pages: bool = False) -> None:
         """Empty the cache.  By default every request's pages go back to the pool (which keeps

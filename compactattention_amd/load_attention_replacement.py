@@ -200,12 +200,14 @@ def load_llama_attention_replacement_model(
     flashprefill_window_size: int = 4,
     flashprefill_last_n_block: int = 2,
     flashprefill_min_budget: int = 0,
+    kv_cache_bits: int = 16,
 ) -> nn.Module:
     """Returns the stock LlamaForCausalLM with compactattn attention in every layer.
 
     base_model: a transformers LlamaForCausalLM (moved to torch_dtype) or a local model
     directory (``from_pretrained(..., local_files_only=True)``).  model_id: optional local
-    directory or file holding the Seer gate weights (``attn_gate_weights.pth``).
+    directory or file holding the Seer gate weights (``attn_gate_weights.pth``).  kv_cache_bits: 4 for
+    a KV cache held in 4 bits (a keyword of this build).
     """
     from transformers import LlamaForCausalLM
 
@@ -223,6 +225,8 @@ def load_llama_attention_replacement_model(
         flashprefill_block_size=flashprefill_block_size, flashprefill_attention_sink=flashprefill_attention_sink,
         flashprefill_window_size=flashprefill_window_size, flashprefill_last_n_block=flashprefill_last_n_block,
         flashprefill_min_budget=flashprefill_min_budget, gate=_gate_settings(model_id))
+    seer_cfg.kv_cache_bits = int(kv_cache_bits)
+    seer_cfg.validate()
     block_rope = _BlockRope(model.model.rotary_emb, seer_cfg.max_position_embeddings)
     cls = _VARIANTS[variant]
     for layer_idx, layer in enumerate(model.model.layers):

@@ -265,19 +265,19 @@ def append_q4(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: KV4, v_cache: K
                                       ctypes.byref(v_cache.layout), sa, _stream()))
 
 
-def gather_q4(k_cache: KV4, v_cache: Optional[KV4], batch: int, num_kv_heads: int, start: Union[int, Sequence[int]],
-              length: int) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+def gather_q4(k_cache: Optional[KV4], v_cache: Optional[KV4], batch: int, num_kv_heads: int,
+              start: Union[int, Sequence[int]], length: int) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
     """The values that a 4-bit cache stands for at positions start[b] .. start[b] + length - 1: K and V
-    [batch, num_kv_heads, length, 128] bf16 (exact; V None without a v_cache)."""
-    if not isinstance(k_cache, KV4) or not (v_cache is None or isinstance(v_cache, KV4)):
+    [batch, num_kv_heads, length, 128] bf16 (exact; None for the cache that is None)."""
+    caches = [kv for kv in (k_cache, v_cache) if kv is not None]
+    if not caches or not all(isinstance(kv, KV4) for kv in caches):
         raise ValueError("gather_q4 reads caches held in 4 bits (KV4)")
     if length < 0:
         raise ValueError(f"length={length} < 0")
     sa = _starts(start, batch)
-    dev = k_cache.tensor.device
-    shape = (batch, num_kv_heads, length, HEAD_DIM)
-    k_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
-    v_out = torch.empty(shape, dtype=torch.bfloat16, device=dev) if v_cache is not None else None
+    dev = caches[0].tensor.device
+    k_out, v_out = (None if kv is None else torch.empty((batch, num_kv_heads, length, HEAD_DIM), dtype=torch.bfloat16,
+                                                        device=dev) for kv in (k_cache, v_cache))
     if length == 0:
         return k_out, v_out
     blocks = -(-(max(sa) + length) // BLOCK)
@@ -285,10 +285,9 @@ def gather_q4(k_cache: KV4, v_cache: Optional[KV4], batch: int, num_kv_heads: in
         if kv is not None:
             kv.check_blocks(name, batch, num_kv_heads, blocks)
     d = make_dims(batch, length, num_kv_heads, num_kv_heads, blocks)
-    with _on_device(k_cache.tensor, k_cache.page_table, *(() if v_cache is None else (v_cache.tensor, v_cache.page_table))):
-        check(_hip.lib().ca_gather_q4(ctypes.byref(d), ctypes.byref(k_cache.layout),
-                                      ctypes.byref(v_cache.layout) if v_cache is not None else None, sa,
-                                      k_out.data_ptr(), _ptr(v_out), _stream()))
+    kl, vl = (None if kv is None else ctypes.byref(kv.layout) for kv in (k_cache, v_cache))
+    with _on_device(*(t for kv in caches for t in (kv.tensor, kv.page_table))):
+        check(_hip.lib().ca_gather_q4(ctypes.byref(d), kl, vl, sa, _ptr(k_out), _ptr(v_out), _stream()))
     return k_out, v_out
 
 

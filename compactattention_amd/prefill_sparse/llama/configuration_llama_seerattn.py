@@ -63,6 +63,11 @@ class SeerAttnLlamaConfig:
     # this build's choice of FlashPrefill score form: "pooled" (block means, bit-reproducible)
     # or "token" (the reference's per-token exp2 mass, compute_block_score_chunked)
     seerattn_flashprefill_score_mode: str = "pooled"
+    # this build's choice of KV cache: bf16 pages (16) or pages held in 4 bits (4)
+    kv_cache_bits: int = 16
+    # RMS norm of every query and key head before the rotation (weights q_norm, k_norm [head_dim]; FlashPrefill
+    # model)
+    qk_norm: bool = False
 
     @classmethod
     def from_dict(cls, d: Dict[str, Any]) -> "SeerAttnLlamaConfig":
@@ -90,6 +95,8 @@ class SeerAttnLlamaConfig:
             raise ValueError("FlashPrefill scoring runs 64- or 128-token blocks")
         if self.seerattn_flashprefill_score_mode not in ("pooled", "token"):
             raise ValueError("seerattn_flashprefill_score_mode must be 'pooled' or 'token'")
+        if self.kv_cache_bits not in (4, 16):
+            raise ValueError("kv_cache_bits must be 16 or 4")
         from ..attn_gate import parse_gate_type
 
         parse_gate_type(self.seerattn_gate_type)

@@ -170,6 +170,24 @@ def rope_qk(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tens
     return ops.rope_qk(q, k, cos, sin)
 
 
+def make_qk_norms(attn: nn.Module, config: SeerAttnLlamaConfig, device=None) -> None:
+    """The weights q_norm and k_norm of an attention module whose config has qk_norm (None otherwise)."""
+    attn.q_norm = attn.k_norm = None
+    if config.qk_norm:
+        attn.q_norm = LlamaRMSNorm(config.head_dim, config.rms_norm_eps, device=device)
+        attn.k_norm = LlamaRMSNorm(config.head_dim, config.rms_norm_eps, device=device)
+
+
+def position_qk(attn: nn.Module, q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor
+                ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """q and k at their positions: rotated, and where the module has q_norm and k_norm normed head by head
+    before, in one launch either way."""
+    if getattr(attn, "q_norm", None) is None:
+        return rope_qk(q, k, cos, sin)
+    return ops.norm_rope_qk(q, k, attn.q_norm.weight, attn.k_norm.weight, attn.q_norm.eps, cos.float().contiguous(),
+                            sin.float().contiguous())
+
+
 def dense_decode_forward(attn: nn.Module, hidden_states: torch.Tensor, position_embeddings, cache: PagedKVCache):
     """Decode step(s) of a compactattn attention module: up to 64 new tokens per request
     attend densely to the whole cache (the reference routes q_len == 1 to dense attention,
@@ -180,7 +198,7 @@ def dense_decode_forward(attn: nn.Module, hidden_states: torch.Tensor, position_
         raise ValueError(f"decode steps take at most {BLOCK} tokens per call (got {L})")
     q, k, v = project_qkv(attn, hidden_states)
     cos, sin = position_embeddings
-    query_states, key_states = rope_qk(q, k, cos, sin)
+    query_states, key_states = position_qk(attn, q, k, cos, sin)
     cache.append_tokens(key_states, v)
     K, V = cache.layouts()
     out = ops.attn_decode(query_states.contiguous(), K, V, [cache.length] * B, attn.scaling, cache.cap,
@@ -198,7 +216,8 @@ def is_decode_step(hidden_states: torch.Tensor, cache: PagedKVCache) -> bool:
 
 
 class ChunkedPrefillCache:
-    """One PagedKVCache per layer (all layers advance together)."""
+    """One PagedKVCache per layer (all layers advance together), in bf16 or held in 4 bits
+    (``config.kv_cache_bits``)."""
 
     def __init__(self, config: SeerAttnLlamaConfig, batch: int, max_tokens: int, device, with_kmean: bool,
                  with_kgate: bool):
@@ -210,7 +229,7 @@ class ChunkedPrefillCache:
                                      config.num_key_value_heads)
         self.layers: List[PagedKVCache] = [
             PagedKVCache(batch, config.num_key_value_heads, max_tokens, device, with_kmean=with_kmean,
-                         with_kgate=with_kgate, kgate_heads=kgate_heads)
+                         with_kgate=with_kgate, kgate_heads=kgate_heads, bits=config.kv_cache_bits)
             for _ in range(config.num_hidden_layers)
         ]
         # pages for max_tokens up front, so a prefill of that length maps nothing on the way;
@@ -228,6 +247,15 @@ class ChunkedPrefillCache:
         """Start a new sequence in the same pages (pages shared by a fork are released)."""
         for c in self.layers:
             c.reset(keep_pages=True)
+
+    def truncate(self, tokens: int, keep_pages: bool = False) -> None:
+        """Forget every layer's tokens past ``tokens`` (a rejected draft)."""
+        for c in self.layers:
+            c.truncate(tokens, keep_pages)
+
+    def compact(self, shrink: bool = True) -> int:
+        """``PagedKVCache.compact`` of every layer; returns how many pages moved in all."""
+        return sum(c.compact(shrink) for c in self.layers)
 
 
 class CompactAttnLlamaDecoderLayer(nn.Module):
@@ -301,7 +329,7 @@ class CompactAttnLlamaForCausalLM(nn.Module):
         g.manual_seed(seed)
         std = self.config.initializer_range
         for name, p in self.named_parameters():
-            if name.endswith("layernorm.weight") or name == "model.norm.weight":
+            if name.endswith(("layernorm.weight", "q_norm.weight", "k_norm.weight")) or name == "model.norm.weight":
                 p.fill_(1.0)
             else:
                 p.normal_(0.0, std, generator=g)

@@ -30,7 +30,8 @@ from ...modules._core import COMPACTATTN_VERSION
 from ...modules.flashprefill_prefill import flashprefill_rule, flashprefill_tables
 from .configuration_llama_seerattn import SeerAttnLlamaConfig
 from .modeling_llama_common import (ChunkedPrefillCache, CompactAttnLlamaForCausalLM, FusedProjections,
-                                     dense_decode_forward, event_span, is_decode_step, project_qkv, rope_qk)
+                                     dense_decode_forward, event_span, is_decode_step, make_qk_norms, position_qk,
+                                     project_qkv)
 
 BLOCK = 64
 
@@ -51,6 +52,7 @@ class LlamaFlashPrefillCompactAttnAttention(nn.Module):
         self.v_proj = nn.Linear(config.hidden_size, self.num_key_value_heads * self.head_dim, **kw)
         self.o_proj = nn.Linear(self.num_heads * self.head_dim, config.hidden_size, **kw)
         self.qkv = FusedProjections(self, ("q_proj", "k_proj", "v_proj"))
+        make_qk_norms(self, config, device)
         self.attention_timer: Optional[list] = None  # a list collects timing events of the attention core
         self.table_sink: Optional[list] = None  # a list collects (counts, chunk length, past blocks) per call
         self.compactattn_version = COMPACTATTN_VERSION
@@ -79,7 +81,7 @@ class LlamaFlashPrefillCompactAttnAttention(nn.Module):
         q, k, v = project_qkv(self, hidden_states)
         cos, sin = position_embeddings
         with event_span(self.attention_timer):
-            query_states, key_states = rope_qk(q, k, cos, sin)
+            query_states, key_states = position_qk(self, q, k, cos, sin)
             cache = past_key_value.layer(self.layer_idx)
             dense = cache.past_blocks == 0 or bool(self.config.seerattn_chunked_prefill_force_dense)
             if dense:

@@ -93,6 +93,8 @@ def resolve_compactattn_threshold(schedule: Optional[dict], kv_len: int, default
 class LlamaSeerAttentionChunkedDense(nn.Module):
     def __init__(self, config: SeerAttnLlamaConfig, layer_idx: int, device=None):
         super().__init__()
+        if config.qk_norm:
+            raise ValueError("qk_norm: the AttnGate pools queries and keys before their norm; the FlashPrefill model has it")
         self.config = config
         self.layer_idx = layer_idx
         self.head_dim = config.head_dim

@@ -80,6 +80,8 @@ def test_append_writes_its_bytes_and_no_others(gpu, B, H, L, starts):
         assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(val))
     only_k, none = ops.gather_q4(K, None, B, H, starts, L)
     assert none is None and torch.equal(torch.nan_to_num(only_k), torch.nan_to_num(back[0]))
+    none, only_v = ops.gather_q4(None, V, B, H, starts, L)
+    assert none is None and torch.equal(torch.nan_to_num(only_v), torch.nan_to_num(back[1]))
 
 
 def test_append_skips_pages_outside_the_pool(gpu):

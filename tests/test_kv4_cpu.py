@@ -188,3 +188,107 @@ def test_front_end_refuses_host_tensors():
     w = torch.zeros(128, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="GPU tensor"):
         ops.norm_rope_qk(x, x, w, w, 1e-5, torch.zeros(1, 128), torch.zeros(1, 128))
+
+
+def _cpu_cache(batch=2, heads=2, pages=3):
+    from compactattention_amd.kv_cache import PagedKVCache
+
+    return PagedKVCache(batch, heads, 128, "cpu", pool_pages=pages)
+
+
+def _tokens(n, seed, batch=2, heads=2):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn((batch, n, heads, 128), generator=g).to(torch.bfloat16)
+
+
+def test_cache_truncates_and_compacts():
+    """Pages behind a length go back; compaction moves the pages in use to the lowest ids, shared ones with all
+    their holders, and gives the rest of the pool back; what is stored stays."""
+    c = _cpu_cache()
+    k = _tokens(300, 0)
+    c.append_tokens(k, -k)
+    c.truncate(130)
+    assert c.length == 130 and (c.page_table.numpy()[:, 3:] == -1).all()
+    assert c.pool.free_pages == c.pool.num_pages - 4 * 3
+    assert torch.equal(c.k_hf(), k[:, :130].transpose(1, 2))
+    c.fork(0, 1)
+    k2 = _tokens(2, 1)
+    c.append_tokens(k2, k2)  # the shared last block parts
+    want_k, want_v = c.k_hf(), c.v_hf()
+    pages = c.pool.num_pages
+    used = int((c.pool.refs > 0).sum())
+    assert used == 2 * 2 + 4 and pages > used
+    table = c.page_table.numpy().copy()
+    shared = (table[0, 0], table[2, 0])
+    assert shared[0] == shared[1]
+    c.compact(shrink=False)
+    assert c.pool.num_pages == pages and (c.pool.refs[:used] > 0).all() and (c.pool.refs[used:] == 0).all()
+    assert torch.equal(c.k_hf(), want_k) and torch.equal(c.v_hf(), want_v)
+    c.compact()
+    assert c.pool.num_pages == used and c.pool.free_pages == 0 and c.pool.k.shape[0] == used
+    assert torch.equal(c.k_hf(), want_k) and torch.equal(c.v_hf(), want_v)
+    table = c.page_table.numpy()
+    assert np.array_equal(table, c._pt) and table.max() == used - 1 and table[0, 0] == table[2, 0]
+    assert c.compact() == 0
+    k3 = _tokens(100, 2)  # the pool grows again
+    c.append_tokens(k3, k3)
+    assert torch.equal(c.k_hf()[:, :, :132], want_k) and torch.equal(c.k_hf()[:, :, 132:], k3.transpose(1, 2))
+    c.truncate(0)
+    assert c.pool.free_pages == c.pool.num_pages and c.compact() == 0 and c.pool.num_pages == 1
+    c.append_tokens(k3, k3)
+    assert torch.equal(c.v_hf(), k3.transpose(1, 2))
+
+
+def test_cache_truncate_keeps_owned_pages_and_refuses():
+    c = _cpu_cache()
+    k = _tokens(200, 3)
+    c.append_tokens(k, k)
+    owned = c.page_table.numpy().copy()
+    c.kmean_blocks = c.kgate_blocks = 4
+    c.truncate(70, keep_pages=True)
+    assert c.length == 70 and np.array_equal(c.page_table.numpy(), owned)
+    assert (c.kmean_blocks, c.kgate_blocks) == (1, 1)
+    c.append_tokens(k[:, :10], k[:, :10])
+    assert torch.equal(c.k_hf(), torch.cat([k[:, :70], k[:, :10]], 1).transpose(1, 2))
+    c.fork(0, 1)
+    c.truncate(64, keep_pages=True)  # block 1 is shared: both rows of every head give it back
+    assert (c.page_table.numpy()[:, 1] == -1).all()
+    for bad in (-1, 65):
+        with pytest.raises(ValueError, match="truncate"):
+            c.truncate(bad)
+
+
+def test_compact_moves_the_last_pages_into_the_gaps():
+    from compactattention_amd.kv_cache import PagePool
+
+    pool = PagePool(8, "cpu")
+    ids = pool.alloc(8)
+    for p in ids:
+        pool.k[p], pool.v[p] = float(p), -float(p)
+    pool.release([0, 2, 3, 6])
+    pool.retain([7])
+    new = pool.compact()
+    assert new.tolist() == [-1, 1, -1, -1, 0, 2, -1, 3]
+    assert pool.k[:, 0, 0].tolist() == [4, 1, 5, 7] and pool.v[:, 5, 9].tolist() == [-4, -1, -5, -7]
+    assert pool.refs.tolist() == [1, 1, 1, 2] and pool.free_pages == 0
+    assert sorted(pool.alloc(2)) == [4, 5]
+
+
+def test_cache_bits_are_checked():
+    from compactattention_amd.kv_cache import PagedKVCache
+    from compactattention_amd.prefill_sparse.llama import (SeerAttnLlamaChunkedDenseForCausalLM, SeerAttnLlamaConfig)
+
+    with pytest.raises(ValueError, match="bits"):
+        PagedKVCache(1, 1, 64, "cpu", bits=8)
+    c = PagedKVCache(1, 1, 64, "cpu", bits=4)
+    assert c.pool.k.shape == (1, 4352) and c.pool.k.dtype == torch.uint8
+    x = torch.zeros((1, 1, 1, 128), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="GPU"):
+        c.append_tokens(x, x)
+    assert c.length == 0
+    with pytest.raises(ValueError, match="kv_cache_bits"):
+        SeerAttnLlamaConfig(kv_cache_bits=8).validate()
+    with pytest.raises(ValueError, match="qk_norm"):
+        SeerAttnLlamaChunkedDenseForCausalLM(SeerAttnLlamaConfig(
+            vocab_size=64, hidden_size=128, intermediate_size=64, num_hidden_layers=1, num_attention_heads=1,
+            num_key_value_heads=1, max_position_embeddings=128, qk_norm=True))
