@@ -768,7 +768,7 @@ int ca_gather_q4(const ca_dims* dims, const ca_kv4_layout* k_cache, const ca_kv4
 }
 
 int ca_copy_pages(const ca_page_pool* pools, int32_t n_pools, const int32_t* src_host, const int32_t* dst_host,
-                  int32_t n, void* stream) {
+                  int32_t n, const int32_t* ids, void* stream) {
     if (pools == nullptr || n_pools < 1 || n_pools > CA_MAX_POOLS)
         return fail(CA_ERR_INVALID, "n_pools=%d outside [1, %d] or pools NULL", n_pools, CA_MAX_POOLS);
     if (n < 0) return fail(CA_ERR_INVALID, "n=%d < 0", n);
@@ -787,9 +787,13 @@ int ca_copy_pages(const ca_page_pool* pools, int32_t n_pools, const int32_t* src
     }
     if (n == 0) return ok();
     if (src_host == nullptr || dst_host == nullptr) return fail(CA_ERR_INVALID, "src_host and dst_host are required");
+    if (!aligned4(ids)) return fail(CA_ERR_INVALID, "ids misaligned");
     for (int i = 0; i < n; ++i)
         if (src_host[i] < 0 || src_host[i] >= pages || dst_host[i] < 0 || dst_host[i] >= pages)
             return fail(CA_ERR_INVALID, "copy %d: page %d to page %d outside [0, %lld)", i, src_host[i], dst_host[i], (long long)pages);
+    for (int i = 0; i < n_pools; ++i)
+        if ((int64_t)n * addr[i].bytes > (int64_t)1 << 37)  // a launch's workgroups
+            return fail(CA_ERR_LIMIT, "pool %d: more than 2^37 bytes in a call", i);
     // one bit a page: written
     const int64_t words = (pages + 63) / 64;
     uint64_t* written = static_cast<uint64_t*>(std::calloc(static_cast<size_t>(words), sizeof(uint64_t)));
@@ -806,7 +810,7 @@ int ca_copy_pages(const ca_page_pool* pools, int32_t n_pools, const int32_t* src
     std::free(written);
     if (twice >= 0) return fail(CA_ERR_INVALID, "page %d is written twice", twice);
     if (both >= 0) return fail(CA_ERR_INVALID, "page %d is read and written", both);
-    hipError_t e = ca::launch_copy_pages(addr, n_pools, src_host, dst_host, n, static_cast<hipStream_t>(stream));
+    hipError_t e = ca::launch_copy_pages(addr, n_pools, src_host, dst_host, n, ids, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail(e, "copy_pages launch");
     return ok();
 }

@@ -105,9 +105,10 @@ hipError_t launch_append4(int B, int L, int H, const int32_t* start, const SeqAd
 // The tokens back as bf16 [B, H, L, 128]; k with k_out, or v with v_out, may be null
 hipError_t launch_gather4(int B, int L, int H, const int32_t* start, const Kv4Addr* k, const Kv4Addr* v,
                           uint16_t* k_out, uint16_t* v_out, hipStream_t stream);
-// pool[dst[i]] = pool[src[i]] for every pool, in launches of a few hundred pages
+// pool[dst[i]] = pool[src[i]] for every pool: one launch where ids holds src and dst on the device, or for a
+// few hundred pages, else launches of that many
 hipError_t launch_copy_pages(const PagePool* pools, int n_pools, const int32_t* src, const int32_t* dst, int n,
-                             hipStream_t stream);
+                             const int32_t* ids, hipStream_t stream);
 
 struct AttnArgs {
     Shape s;

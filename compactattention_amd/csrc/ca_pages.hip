@@ -126,41 +126,51 @@ __global__ __launch_bounds__(256) void gather4_kernel(Gather4Params p) {
 }
 
 // ---------------------------------------------------------------------------------------
-// Copies of pages.  The ids travel in the launch's arguments: no upload, nothing to wait for, and a
-// captured graph holds them.  A thread moves 16-byte units of the launch's pages in order, four at a
-// time, a workgroup 1024 units.
+// Copies of pages.  The ids of up to kCopyPairs pages travel in the launch's arguments: no upload, nothing
+// to wait for, and a captured graph holds them.  More are read from device memory where the caller has put
+// them there (kById), else copied in several launches.  A thread moves 16-byte units of the launch's pages
+// in order, four at a time, a workgroup 1024 units.
 constexpr int kCopyPairs = 448;  // 3.5 KB of the 4 KB of arguments
 constexpr int kCopyUnits = 4;
 
 struct CopyParams {
     PagePool pool[CA_MAX_POOLS];
-    int units;  // 16-byte units of a page of this launch's pool
+    const int32_t* ids;  // kById: n sources, then n destinations
     int n;
     int32_t src[kCopyPairs];
     int32_t dst[kCopyPairs];
 };
 static_assert(sizeof(CopyParams) <= 4096, "the arguments of a launch");
 
+template <bool kById>
 __global__ __launch_bounds__(256) void copy_pages_kernel(CopyParams p) {
     const PagePool pool = p.pool[blockIdx.y];
     const uint32_t units = static_cast<uint32_t>(pool.bytes >> 4);
-    const uint32_t total = units * p.n;
-    const uint32_t u0 = blockIdx.x * (256 * kCopyUnits) + threadIdx.x;
+    const uint64_t total = (uint64_t)units * p.n;
+    const uint64_t first = (uint64_t)blockIdx.x * (256 * kCopyUnits);
+    if (first >= total) return;  // a pool of smaller pages than the largest
+    const uint32_t pair0 = static_cast<uint32_t>(first / units);
+    const uint32_t off0 = static_cast<uint32_t>(first - (uint64_t)pair0 * units) + threadIdx.x;
     u32x4p_t v[kCopyUnits];
     uint8_t* to[kCopyUnits];
+    bool live[kCopyUnits];
 #pragma unroll
     for (int i = 0; i < kCopyUnits; ++i) {
-        const uint32_t u = u0 + 256 * i;
-        if (u < total) {
-            const uint32_t pair = u / units;
-            const int64_t off = (int64_t)(u - pair * units) * 16;
-            v[i] = *reinterpret_cast<const u32x4p_t*>(pool.data + p.src[pair] * pool.stride + off);
-            to[i] = pool.data + p.dst[pair] * pool.stride + off;
+        const uint32_t u = off0 + 256 * i;  // from the first unit of page pair0
+        const uint32_t k = u / units;
+        const uint32_t pair = pair0 + k;
+        live[i] = pair < (uint32_t)p.n;
+        if (live[i]) {
+            const int64_t off = (int64_t)(u - k * units) * 16;
+            const int32_t src = kById ? p.ids[pair] : p.src[pair];
+            const int32_t dst = kById ? p.ids[p.n + pair] : p.dst[pair];
+            v[i] = *reinterpret_cast<const u32x4p_t*>(pool.data + src * pool.stride + off);
+            to[i] = pool.data + dst * pool.stride + off;
         }
     }
 #pragma unroll
     for (int i = 0; i < kCopyUnits; ++i)
-        if (u0 + 256 * i < total) *reinterpret_cast<u32x4p_t*>(to[i]) = v[i];
+        if (live[i]) *reinterpret_cast<u32x4p_t*>(to[i]) = v[i];
 }
 
 Kv4Rows rows_of(int B, int L, int H, const int32_t* start) {
@@ -191,23 +201,28 @@ hipError_t launch_gather4(int B, int L, int H, const int32_t* start, const Kv4Ad
 }
 
 hipError_t launch_copy_pages(const PagePool* pools, int n_pools, const int32_t* src, const int32_t* dst, int n,
-                             hipStream_t stream) {
+                             const int32_t* ids, hipStream_t stream) {
     CopyParams p;
     int64_t most = 0;
     for (int i = 0; i < n_pools; ++i) {
         p.pool[i] = pools[i];
         most = max(most, pools[i].bytes);
     }
-    p.units = static_cast<int>(most >> 4);
+    auto launch = [&](auto kernel, int count) {
+        p.n = count;
+        const int64_t blocks = ((most >> 4) * count + 256 * kCopyUnits - 1) / (256 * kCopyUnits);
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks), n_pools), dim3(256), 0, stream, p);
+        return hipGetLastError();
+    };
+    p.ids = ids;
+    if (ids != nullptr && n > kCopyPairs) return launch(copy_pages_kernel<true>, n);
     for (int at = 0; at < n; at += kCopyPairs) {
-        p.n = min(kCopyPairs, n - at);
-        for (int i = 0; i < p.n; ++i) {
+        const int count = min(kCopyPairs, n - at);
+        for (int i = 0; i < count; ++i) {
             p.src[i] = src[at + i];
             p.dst[i] = dst[at + i];
         }
-        const int64_t blocks = ((int64_t)p.units * p.n + 256 * kCopyUnits - 1) / (256 * kCopyUnits);
-        hipLaunchKernelGGL(copy_pages_kernel, dim3(static_cast<unsigned>(blocks), n_pools), dim3(256), 0, stream, p);
-        const hipError_t e = hipGetLastError();
+        const hipError_t e = launch(copy_pages_kernel<false>, count);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;

@@ -84,8 +84,9 @@ class Rule:
         )
 
 
-def _stream() -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+def _stream() -> int:
+    """The current stream of the current device (its handle alone: building torch's Stream object takes 2.7 us)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -101,14 +102,16 @@ def _need_cuda(name: str, t: torch.Tensor, dtype: torch.dtype) -> None:
         raise ValueError(f"{name} must be {dtype} (got {t.dtype})")
 
 
+_HERE = nullcontext()
+
+
 def _on_device(first: torch.Tensor, *others: Optional[torch.Tensor]):
     """A context in which the tensors' one device is the current one, whichever was before."""
+    dev = first.get_device()
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"all tensors of a call must be on one device (got {first.device} and {t.device})")
-    if first.device.index == torch.cuda.current_device():
-        return nullcontext()
-    return torch.cuda.device(first.device)
+    return _HERE if dev == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def past_array(past_blocks: Sequence[int], batch: Optional[int] = None):
@@ -129,9 +132,16 @@ def make_dims(batch: int, q_len: int, num_q_heads: int, num_kv_heads: int, kv_ca
 def seq_layout(t: torch.Tensor, name: str = "tensor") -> SeqLayout:
     """[B, T, H, 128] bf16 with a contiguous head dim."""
     _need_cuda(name, t, torch.bfloat16)
-    if t.dim() != 4 or t.shape[-1] != HEAD_DIM or t.stride(-1) != 1:
+    st = t.stride()
+    if len(st) != 4 or t.shape[3] != HEAD_DIM or st[3] != 1:
         raise ValueError(f"{name} must be [B, T, H, {HEAD_DIM}] with a contiguous last dim")
-    return SeqLayout(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+    return SeqLayout(t.data_ptr(), st[0], st[1], st[2])
+
+
+def _new_seq(like: torch.Tensor, B: int, T: int, H: int) -> Tuple[torch.Tensor, SeqLayout]:
+    """A contiguous [B, T, H, 128] tensor of like's type and device, and its layout."""
+    t = like.new_empty((B, T, H, HEAD_DIM))
+    return t, SeqLayout(t.data_ptr(), T * H * HEAD_DIM, H * HEAD_DIM, HEAD_DIM)
 
 
 @dataclass
@@ -209,19 +219,18 @@ class KV4:
         """Page pool [num_pages, PAGE4_BYTES] uint8 and page_table [B*Hkv, blocks] int32."""
         _need_cuda("pool", pool, torch.uint8)
         _need_cuda("page_table", page_table, torch.int32)
-        if pool.dim() != 2 or pool.shape[1] != PAGE4_BYTES or pool.stride(1) != 1:
+        shape, st, pt = pool.shape, pool.stride(), page_table.stride()
+        if len(shape) != 2 or shape[1] != PAGE4_BYTES or st[1] != 1:
             raise ValueError(f"a 4-bit page pool must be [num_pages, {PAGE4_BYTES}] with contiguous pages")
-        if page_table.dim() != 2 or page_table.stride(1) != 1:
+        if len(pt) != 2 or pt[1] != 1:
             raise ValueError("page_table must be [rows, blocks] with contiguous rows")
-        if pool.device != page_table.device:
-            raise ValueError(f"pool on {pool.device} and page_table on {page_table.device}")
-        return KV4(pool, Kv4Layout(pool.data_ptr(), pool.stride(0), page_table.data_ptr(), page_table.stride(0),
-                                   pool.shape[0]), page_table)
+        return KV4(pool, Kv4Layout(pool.data_ptr(), st[0], page_table.data_ptr(), pt[0], shape[0]), page_table)
 
     def check_blocks(self, name: str, batch: int, heads: int, blocks: int, tokens: Optional[int] = None) -> None:
         """Raise unless the page table covers ``blocks`` blocks of each of the ``batch`` x ``heads`` rows."""
         del tokens
-        if self.page_table.shape[0] < batch * heads or self.page_table.shape[1] < blocks:
+        rows, cols = self.page_table.shape
+        if rows < batch * heads or cols < blocks:
             raise ValueError(f"{name} page_table {tuple(self.page_table.shape)} does not cover "
                              f"[{batch * heads}, {blocks}]")
 
@@ -229,12 +238,12 @@ class KV4:
 AnyKV = Union[KV, KV4]
 
 
-def _attn_launch(name: str, k: AnyKV, v: AnyKV, *tensors: torch.Tensor):
+def _attn_launch(name: str, k: AnyKV, v: AnyKV, *tensors: Optional[torch.Tensor]):
     """The entry point for these caches and the context to call it in."""
     if isinstance(k, KV4) != isinstance(v, KV4):
         raise ValueError("K and V must both be bf16 caches or both be held in 4 bits")
     if not isinstance(k, KV4):
-        return getattr(_hip.lib(), name), nullcontext()
+        return getattr(_hip.lib(), name), _HERE
     guard = _on_device(*tensors, k.tensor, k.page_table, v.tensor, v.page_table)
     return getattr(_hip.lib(), name + "_q4"), guard
 
@@ -299,34 +308,52 @@ def _page_ids(name: str, ids) -> np.ndarray:
         return np.zeros(0, np.int32)
     if a.ndim != 1 or a.dtype.kind not in "iu":
         raise ValueError(f"{name} must be a one-dimensional sequence of integers")
+    if a.dtype == np.int32:
+        return np.ascontiguousarray(a)
     if int(a.min()) < 0 or int(a.max()) >= 1 << 31:
         raise ValueError(f"{name} holds page ids outside [0, 2^31)")
     return np.ascontiguousarray(a, np.int32)
+
+
+# From this many pages on the ids are uploaded and one launch copies them all: 9001 4-bit pages of two pools 98 us
+# in the 21 launches that carry their ids, 43 us so; the upload takes the host 12 us more than a launch.
+_COPY_UPLOAD = 4 * 448
 
 
 def copy_pages(pools: Sequence[torch.Tensor], src, dst) -> None:
     """pool[dst[i]] = pool[src[i]] for every pool [num_pages, ...] of any type whose pages are contiguous
     multiples of 16 bytes (bf16 pages, 4-bit pages, summaries by page).  src and dst are host integers
     (lists, numpy arrays, CPU tensors).  No page is written twice and none that is read is written, else
-    CaError.  Nothing is uploaded and nothing waits: the ids go with the launches."""
+    CaError.  Nothing waits: the ids go with the launches, or through pinned memory where there are many
+    (not while a graph is captured, which keeps the ids itself)."""
     if isinstance(pools, torch.Tensor):
         pools = [pools]
     s, d = _page_ids("src", src), _page_ids("dst", dst)
-    if s.size != d.size:
-        raise ValueError(f"{s.size} source pages and {d.size} destinations")
+    n = s.size
+    if n != d.size:
+        raise ValueError(f"{n} source pages and {d.size} destinations")
     if not 1 <= len(pools) <= _hip.MAX_POOLS:
         raise ValueError(f"between 1 and {_hip.MAX_POOLS} pools are copied in a call (got {len(pools)})")
     descs = (PagePool * len(pools))()
     for i, t in enumerate(pools):
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise ValueError("pools must be GPU tensors")
-        if t.dim() < 2 or t.shape[0] < 1 or not t[0].is_contiguous():
+        shape, strides, page = t.shape, t.stride(), 1
+        for dim in range(len(shape) - 1, 0, -1):
+            if shape[dim] != 1 and strides[dim] != page:
+                page = 0
+            page *= shape[dim]
+        if len(shape) < 2 or shape[0] < 1 or page < 1:
             raise ValueError("a pool must be [num_pages, ...] with contiguous pages")
         size = t.element_size()
-        page = t[0].numel() * size
-        descs[i] = PagePool(t.data_ptr(), page, t.stride(0) * size if t.shape[0] > 1 else page, t.shape[0])
+        descs[i] = PagePool(t.data_ptr(), page * size, (strides[0] if shape[0] > 1 else page) * size, shape[0])
     with _on_device(*pools):
-        check(_hip.lib().ca_copy_pages(descs, len(pools), s.ctypes.data, d.ctypes.data, s.size, _stream()))
+        ids = None
+        if n >= _COPY_UPLOAD and not torch.cuda.is_current_stream_capturing():
+            host = torch.empty((2, n), dtype=torch.int32, pin_memory=True)
+            host.numpy()[0], host.numpy()[1] = s, d
+            ids = host.to(pools[0].device, non_blocking=True)
+        check(_hip.lib().ca_copy_pages(descs, len(pools), s.ctypes.data, d.ctypes.data, n, _ptr(ids), _stream()))
 
 
 def cache_fill(k_new: torch.Tensor, v_new: Optional[torch.Tensor], k_cache: Optional[KV], v_cache: Optional[KV],
@@ -747,7 +774,7 @@ def attn_fwd(q: torch.Tensor, k: AnyKV, v: AnyKV, table: torch.Tensor, counts: t
     if need > 0 and (workspace is None or workspace.numel() * workspace.element_size() < need):
         workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
     lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=q.device) if with_lse else None
-    entry, guard = _attn_launch("ca_attn_fwd", k, v, q, out, table, counts)
+    entry, guard = _attn_launch("ca_attn_fwd", k, v, q, out, table, counts, workspace)
     with guard:
         check(entry(ctypes.byref(d), ctypes.byref(ql), ctypes.byref(k.layout), ctypes.byref(v.layout),
                     table.data_ptr(), table.stride(0), counts.data_ptr(), pa, float(scale), ctypes.byref(ol), _ptr(lse),
@@ -784,18 +811,18 @@ def attn_decode(q: torch.Tensor, k: AnyKV, v: AnyKV, kv_len: Sequence[int], scal
     ol = seq_layout(out, "out")
     # the kernel's buffer ranges end at each request's kv_len: a contiguous cache needs those
     # tokens only, a paged one a page for every block they touch
-    max_len = max(int(x) for x in kv_len)
+    ka = past_array(kv_len, B)
+    max_len = max(ka)
     for name, kv in (("k", k), ("v", v)):
         kv.check_blocks(name, B, num_kv_heads, (max_len + BLOCK - 1) // BLOCK, tokens=max_len)
     d = make_dims(B, Lq, Hq, num_kv_heads, kv_cap)
-    ka = past_array(kv_len, d.batch)
     need = _hip.lib().ca_attn_decode_workspace_size(ctypes.byref(d), ka, int(num_splits))
     if need < 0:
         raise _hip.CaError(int(need), _hip.last_error())
     if need > 0 and (workspace is None or workspace.numel() * workspace.element_size() < need):
         workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
     lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=q.device) if with_lse else None
-    entry, guard = _attn_launch("ca_attn_decode", k, v, q, out)
+    entry, guard = _attn_launch("ca_attn_decode", k, v, q, out, workspace)
     with guard:
         check(entry(ctypes.byref(d), ctypes.byref(ql), ctypes.byref(k.layout), ctypes.byref(v.layout), ka, float(scale),
                     ctypes.byref(ol), _ptr(lse), int(num_splits), _ptr(workspace), int(need), _stream()))
@@ -846,27 +873,30 @@ def norm_rope_qk(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     rotation, in one launch: bf16(y * cos + rotate_half(y) * sin), y = x * w / sqrt(mean(x^2) + eps) in
     fp32, rounded once.  cos / sin fp32 [L, 128], or [B, L, 128] for requests at positions of their own."""
     B, L, Hq, _ = q.shape
-    Hkv = k.shape[2]
+    Bk, Lk, Hkv, _ = k.shape
     ql, kl = seq_layout(q, "q"), seq_layout(k, "k")
-    if tuple(k.shape[:2]) != (B, L):
+    if Bk != B or Lk != L:
         raise ValueError("q and k must cover the same [B, L] tokens")
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         _need_cuda(name, w, torch.bfloat16)
-        if w.shape != (HEAD_DIM,) or not w.is_contiguous():
+        if w.dim() != 1 or w.numel() != HEAD_DIM or not w.is_contiguous():
             raise ValueError(f"{name} must be contiguous [{HEAD_DIM}]")
+    per_request = cos.dim() == 3
+    shape = (B, L, HEAD_DIM) if per_request else (L, HEAD_DIM)
     for name, t in (("cos", cos), ("sin", sin)):
         _need_cuda(name, t, torch.float32)
-        if t.shape not in ((L, HEAD_DIM), (B, L, HEAD_DIM)) or t.shape != cos.shape or not t.is_contiguous():
+        if t.shape != shape or not t.is_contiguous():
             raise ValueError(f"cos and sin must both be contiguous fp32 [{L}, {HEAD_DIM}] or [{B}, {L}, {HEAD_DIM}]")
-    qo = torch.empty((B, L, Hq, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
-    ko = torch.empty((B, L, Hkv, HEAD_DIM), dtype=torch.bfloat16, device=k.device)
+    guard = _on_device(q, k, q_weight, k_weight, cos, sin)
+    qo, qol = _new_seq(q, B, L, Hq)
+    ko, kol = _new_seq(k, B, L, Hkv)
     if B * L == 0:
         return qo, ko
-    qol, kol = seq_layout(qo, "q_out"), seq_layout(ko, "k_out")
-    with _on_device(q, k, q_weight, k_weight, cos, sin):
-        check(_hip.lib().ca_norm_rope_qk(ctypes.byref(ql), ctypes.byref(qol), Hq, q_weight.data_ptr(), ctypes.byref(kl),
-                                         ctypes.byref(kol), Hkv, k_weight.data_ptr(), B, L, cos.data_ptr(), sin.data_ptr(),
-                                         L * HEAD_DIM if cos.dim() == 3 else 0, float(eps), _stream()))
+    byref = ctypes.byref
+    with guard:
+        check(_hip.lib().ca_norm_rope_qk(byref(ql), byref(qol), Hq, q_weight.data_ptr(), byref(kl), byref(kol), Hkv,
+                                         k_weight.data_ptr(), B, L, cos.data_ptr(), sin.data_ptr(),
+                                         L * HEAD_DIM if per_request else 0, eps, _stream()))
     return qo, ko
 
 

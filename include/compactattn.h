@@ -481,9 +481,11 @@ int ca_attn_decode_q4(const ca_dims* dims, const ca_seq_layout* q, const ca_kv4_
  * src_host[i].  The ids are host arrays, read before the call returns.  Every id lies in every pool,
  * no page is written twice and none that is read is written (CA_ERR_INVALID otherwise), so the order
  * of the copies does not matter.  n = 0 does nothing.
+ * ids is NULL, or device memory that holds src_host and then dst_host (2 n int32) by the time the
+ * launch runs: one launch then copies any n, where the ids of 448 pages go with a launch's arguments.
  */
 int ca_copy_pages(const ca_page_pool* pools, int32_t n_pools, const int32_t* src_host, const int32_t* dst_host,
-                  int32_t n, void* stream);
+                  int32_t n, const int32_t* ids, void* stream);
 
 /*
  * Model plumbing.  Fused element-wise kernels of the Llama integration; they have no

@@ -16,7 +16,7 @@ def _pairs(n, total, seed):
     return perm[:n], perm[n:2 * n]
 
 
-@pytest.mark.parametrize("n", [0, 1, 2, 447, 448, 449, 1000])
+@pytest.mark.parametrize("n", [0, 1, 2, 447, 448, 449, 1000, 1791, 1792, 2500])
 def test_copy_pages(gpu, n):
     """Several pools of different pages in one call; all other pages stay."""
     print(f"case: copy_pages n={n}", flush=True)
@@ -46,6 +46,16 @@ def test_copy_pages_of_a_strided_pool_and_from_a_graph(gpu):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         ops.copy_pages([pool], np.arange(10), np.arange(10, 20))  # the ids live in the graph
+    big = torch.randint(0, 256, (5000, 16), dtype=torch.uint8, device=gpu)
+    many = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(many):
+        ops.copy_pages([big], np.arange(2500), np.arange(2500, 5000))
+    for _ in range(3):
+        big[:2500] = torch.randint(0, 256, (2500, 16), dtype=torch.uint8, device=gpu)
+        many.replay()
+        ops.copy_pages([big[:, :16].clone()], np.arange(2400), np.arange(2500, 4900))  # its ids take the pinned memory's place
+        torch.cuda.synchronize()
+        assert torch.equal(big[2500:], big[:2500])
     for _ in range(3):
         pool[:10] = torch.randint(0, 256, (10, 4352), dtype=torch.uint8, device=gpu)
         graph.replay()
@@ -109,9 +119,8 @@ class _Elsewhere(torch.Tensor):
     def __new__(cls, t):
         return torch.Tensor._make_subclass(cls, t)
 
-    @property
-    def device(self):
-        return torch.device("cuda", 1)
+    def get_device(self):
+        return 1
 
 
 def _norm_rope64(x, w, eps, cos, sin):

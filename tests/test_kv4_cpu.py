@@ -135,12 +135,12 @@ def test_copy_pages_arguments_are_checked():
     lib = _hip.lib()
     pool = lambda data=FAKE, page=4352, stride=4352, n=10: _hip.PagePool(data, page, stride, n)  # noqa: E731
 
-    def copy(pools, src=(0,), dst=(1,), n=None):
+    def copy(pools, src=(0,), dst=(1,), n=None, ids=None):
         arr = (_hip.PagePool * max(1, len(pools)))(*pools)
-        return lib.ca_copy_pages(arr, len(pools), _ints(*src), _ints(*dst), len(src) if n is None else n, None)
+        return lib.ca_copy_pages(arr, len(pools), _ints(*src), _ints(*dst), len(src) if n is None else n, ids, None)
 
     assert copy([]) == INVALID and copy([pool()] * 9) == INVALID
-    assert lib.ca_copy_pages(None, 1, _ints(0), _ints(1), 1, None) == INVALID
+    assert lib.ca_copy_pages(None, 1, _ints(0), _ints(1), 1, None, None) == INVALID
     assert copy([pool(data=None)]) == INVALID and copy([pool(data=FAKE + 8)]) == INVALID
     assert copy([pool(page=0)]) == INVALID and copy([pool(page=4360, stride=4368)]) == INVALID
     assert copy([pool(stride=4336)]) == INVALID and copy([pool(stride=4360)]) == INVALID
@@ -153,7 +153,9 @@ def test_copy_pages_arguments_are_checked():
     assert copy([pool()], src=(0, 1), dst=(2, 0)) == INVALID and "read and written" in _hip.last_error()
     assert copy([pool()], src=(-1,), dst=(2,)) == INVALID and copy([pool()], src=(10,), dst=(2,)) == INVALID
     assert copy([pool()], n=0) == _hip.CA_OK
-    assert lib.ca_copy_pages((_hip.PagePool * 1)(pool()), 1, None, _ints(1), 1, None) == INVALID
+    assert copy([pool()], ids=FAKE + 2) == INVALID
+    assert copy([pool(page=1 << 22, stride=1 << 22, n=1 << 17)], src=[0] * 40000, dst=list(range(1, 40001))) == LIMIT
+    assert lib.ca_copy_pages((_hip.PagePool * 1)(pool()), 1, None, _ints(1), 1, None, None) == INVALID
 
 
 def test_norm_rope_arguments_are_checked():
