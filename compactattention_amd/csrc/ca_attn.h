@@ -173,7 +173,7 @@ __device__ __forceinline__ int32_t sload(const int32_t* p) {
 }
 
 // Fills a launch's parameters and its plan.
-void attn_fill(const AttnArgs& a, AttnParams* p, SplitPlan* plan);
+void attn_fill(const AttnArgs& a, const AttnTiling& tiling, AttnParams* p, SplitPlan* plan);
 // Merges the partial results of a launch whose plan has more than one split.  nan_lse: a row whose
 // partial sums are NaN gets NaN as its lse (else -inf).
 hipError_t launch_attn_merge(const AttnParams& p, bool nan_lse, hipStream_t stream);

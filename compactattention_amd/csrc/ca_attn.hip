@@ -1023,7 +1023,12 @@ bool attn_uses_decode_kernel(const Shape& s, bool dense) {
     return dense && s.Lq * s.G <= kDecRows;
 }
 
-void attn_plan(const Shape& s, const int32_t* nkb, int forced, bool dense, SplitPlan* plan) {
+AttnTiling attn_tiling(const Shape& s, bool dense, bool decode) {
+    if (decode && attn_uses_decode_kernel(s, dense)) return AttnTiling{kDecRows, true, false, 4, 32};
+    return AttnTiling{kBM, false, false, 16, dense ? kMaxDecodeSplits : kMaxPrefillSplits};
+}
+
+void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling& tiling, SplitPlan* plan) {
     // One workgroup is resident per CU (128 KB of LDS).  Without a forced count, the
     // decode kernel splits each request's block list so its work items carry about the
     // same number of blocks as everyone else's (total work / slots); attn_fwd_kernel uses
@@ -1041,13 +1046,13 @@ void attn_plan(const Shape& s, const int32_t* nkb, int forced, bool dense, Split
     //    per split; 4 blocks per split at 1K tokens: 9.9 us, 9.0 and 9.5 us for 8 and 16 splits).
     //  - dense decode with more rows runs attn_fwd_kernel with the prefill sizing and up to
     //    64 splits.
-    const bool dec = attn_uses_decode_kernel(s, dense);
+    const bool dec = tiling.streams;
     plan->may_unsplit = 0;
     const int slots = dec ? 256 : 512;
-    const int min_blocks = dec ? 4 : 16;
-    const int max_splits = dec ? 32 : dense ? kMaxDecodeSplits : kMaxPrefillSplits;
+    const int min_blocks = tiling.min_blocks;
+    const int max_splits = tiling.max_splits;
     const int rows_total = s.Lq * s.G;
-    const int ntiles = dec ? 1 : (rows_total + kBM - 1) / kBM;
+    const int ntiles = (rows_total + tiling.tile_rows - 1) / tiling.tile_rows;
     double total = 0.0;
     int nkb_max = 1;
     for (int b = 0; b < s.B; ++b) {
@@ -1082,12 +1087,41 @@ void attn_plan(const Shape& s, const int32_t* nkb, int forced, bool dense, Split
         // 293-295 us split, while its dense tables need the split, 2.1 vs 3.2 ms)
         plan->may_unsplit = !same_len && units * 4 >= 3 * 256 && forced > 1;
     }
+    // Pages of 4 bits: a page takes a wave 1.65 us however many CUs work, so the launch takes as long as the
+    // most pages that a wave has in turn (a split of n blocks: ceil(n / 8)), and what a merge adds is 2 to 3
+    // pages' time.  The fewest pages in turn with which the items still fit one round, and no splits where
+    // these save fewer than three (32 Q / 8 KV heads, one token: 1024 tokens 7.8 us whole, 8.4 in 4 splits;
+    // 2048 tokens 10.9, 8.7).
+    int turns = 0;
+    if (tiling.steps && forced <= 0) {
+        auto splits = [&](int nb, int t) { return max(1, (nb + kNW * t - 1) / (kNW * t)); };
+        auto fits = [&](int t) {
+            int items = 0;
+            for (int b = 0; b < s.B; ++b) {
+                if (splits(nkb[b], t) > max_splits) return false;
+                items += s.Hkv * ntiles * splits(nkb[b], t);
+            }
+            return items <= slots;
+        };
+        const int whole = (nkb_max + kNW - 1) / kNW;
+        int lo = 1, hi = whole;  // fits() holds from some count on, or only without splits
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (fits(mid))
+                hi = mid;
+            else
+                lo = mid + 1;
+        }
+        turns = whole - lo < 3 ? whole : lo;
+    }
     plan->max = 1;
     plan->off[0] = 0;
     for (int b = 0; b < s.B; ++b) {
         const int nb = nkb[b];
         int sb = forced;
-        if (forced <= 0) {
+        if (turns > 0) {
+            sb = max(1, (nb + kNW * turns - 1) / (kNW * turns));
+        } else if (forced <= 0) {
             sb = static_cast<int>(nb / item_blocks + 0.5);
             sb = min(sb, max(1, nb / min_blocks));
             sb = max(1, min(sb, max_splits));
@@ -1214,10 +1248,14 @@ void attn_positions(const Shape& s, const PastBlocks& pb, const int32_t* kv_len,
 }
 
 int attn_pick_splits(const Shape& s, const PastBlocks& pb, const int32_t* kv_len) {
+    return attn_pick_splits(s, pb, kv_len, attn_tiling(s, kv_len != nullptr));
+}
+
+int attn_pick_splits(const Shape& s, const PastBlocks& pb, const int32_t* kv_len, const AttnTiling& tiling) {
     int32_t qpos0[CA_MAX_BATCH], nkb[CA_MAX_BATCH];
     attn_positions(s, pb, kv_len, qpos0, nkb);
     SplitPlan plan;
-    attn_plan(s, nkb, 0, kv_len != nullptr, &plan);
+    attn_plan(s, nkb, 0, tiling, &plan);
     return plan.max;
 }
 
@@ -1228,7 +1266,7 @@ int64_t attn_workspace_bytes(const Shape& s, int num_splits) {
     return (int64_t)num_splits * rows_all * (128 + 1) * (int64_t)sizeof(float) + 16;
 }
 
-void attn_fill(const AttnArgs& a, AttnParams* p, SplitPlan* plan) {
+void attn_fill(const AttnArgs& a, const AttnTiling& tiling, AttnParams* p, SplitPlan* plan) {
     p->s = a.s;
     p->q = a.q;
     p->k = a.k;
@@ -1241,12 +1279,12 @@ void attn_fill(const AttnArgs& a, AttnParams* p, SplitPlan* plan) {
     p->out = a.out;
     p->lse = a.lse;
     p->rows_total = a.s.Lq * a.s.G;
-    p->ntiles = (p->rows_total + kBM - 1) / kBM;
+    p->ntiles = (p->rows_total + tiling.tile_rows - 1) / tiling.tile_rows;
     int32_t nkb[CA_MAX_BATCH];
     attn_positions(a.s, a.pb, a.kv_len, p->qpos0, nkb);
     for (int b = 0; b < CA_MAX_BATCH; ++b) p->nkb[b] = b < a.s.B ? nkb[b] : 0;
     for (int b = a.s.B; b < CA_MAX_BATCH; ++b) p->qpos0[b] = 0;
-    attn_plan(a.s, nkb, a.num_splits, a.kv_len != nullptr, plan);
+    attn_plan(a.s, nkb, a.num_splits, tiling, plan);
     for (int b = 0; b < CA_MAX_BATCH; ++b) p->sp[b] = b < a.s.B ? plan->s[b] : 1;
     for (int b = 0; b <= CA_MAX_BATCH; ++b) p->ioff[b] = b <= a.s.B ? plan->off[b] : plan->off[a.s.B];
     p->total_items = plan->off[a.s.B];
@@ -1278,7 +1316,7 @@ hipError_t launch_attn_merge(const AttnParams& p, bool nan_lse, hipStream_t stre
 hipError_t launch_attn(const AttnArgs& a, hipStream_t stream) {
     AttnParams p;
     SplitPlan plan;
-    attn_fill(a, &p, &plan);
+    attn_fill(a, attn_tiling(a.s, a.kv_len != nullptr), &p, &plan);
     bool row_res;
     {
         int max_tokens = 0;

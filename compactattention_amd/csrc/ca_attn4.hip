@@ -32,10 +32,11 @@ __device__ __forceinline__ u32x4_t decode_row(uint32_t w, float s) {
 }
 
 // ---------------------------------------------------------------------------------------
-// Single tokens: at most 16 packed query rows per KV row.  Bound by memory: every cached byte is read
-// once (68 bytes a token of K and of V).  16x16x32 MFMAs, S^T = K Q^T and O^T += V^T P^T, with the
-// packed rows as the N dimension.  Eight waves, each with pages of its own (e0 + w, e0 + w + 8, ...) and
-// its own softmax; their results meet in LDS at the end.
+// Single tokens and short drafts, the whole cache: kN tiles of 16 packed query rows a workgroup (1 for at
+// most 16 rows, 2 for more, in several workgroups).  Bound by memory for 16 rows: every cached byte is read
+// once (68 bytes a token of K and of V).  16x16x32 MFMAs, S^T = K Q^T and O^T += V^T P^T, with the packed
+// rows as the N dimension.  Eight waves, each with pages of its own (e0 + w, e0 + w + 8, ...) and its own
+// softmax; their results meet in LDS at the end.
 //  - The contraction order of a product is free as long as both operands share it, so the page's layout
 //    decides it and nothing crosses lanes: lane (n = l % 16, g = l / 16) has token 16 kt + n's group g
 //    (16 bytes) as its share of K, and takes the dims 32 g + 8 s .. + 7 in step s; the scores then lie
@@ -43,7 +44,6 @@ __device__ __forceinline__ u32x4_t decode_row(uint32_t w, float s) {
 //  - V's words are tokens, the MFMA wants tokens side by side: v_perm_b32 pairs them.  Output tile j
 //    holds the dims 8 m + j, so a lane ends with 8 consecutive dims of its row.
 constexpr int kWaves4 = 8;
-constexpr int kRows4 = 16;
 constexpr int kOStride4 = 132;  // floats per row of a wave's partial O in LDS (padded)
 
 struct Page4 {
@@ -51,16 +51,18 @@ struct Page4 {
     uint32_t ks;             // K's scale bytes (byte: tile)
 };
 
-__global__ __launch_bounds__(kWaves4 * 64) void attn4_decode_kernel(Attn4Params p4) {
-    __shared__ __attribute__((aligned(16))) float mo[kWaves4 * kRows4 * kOStride4];
-    __shared__ float ml[kWaves4 * kRows4 * 2];
+template <int kN>
+__global__ __launch_bounds__(kWaves4 * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn4_decode_kernel(Attn4Params p4) {
+    __shared__ __attribute__((aligned(16))) float mo[kWaves4 * 16 * kOStride4];
+    __shared__ float ml[kWaves4 * 16 * 2];
     const AttnParams& p = p4.a;
     Item it;
-    if (!find_item(p, 1, &it)) return;
+    if (!find_item(p, kN == 1 ? 1 : p.ntiles, &it)) return;
     const Shape& s = p.s;
     const int row = __builtin_amdgcn_readfirstlane(it.row);
     const int b = __builtin_amdgcn_readfirstlane(it.b);
     const int split = __builtin_amdgcn_readfirstlane(it.split);
+    const int r0 = kN == 1 ? 0 : 16 * kN * __builtin_amdgcn_readfirstlane(it.tile);
     const int hk = row - b * s.Hkv;
     const int nsplit = p.sp[b];
     const int G = s.G;
@@ -78,20 +80,6 @@ __global__ __launch_bounds__(kWaves4 * 64) void attn4_decode_kernel(Attn4Params 
     const int l = tid & 63;
     const int n = l & 15;
     const int g = l >> 4;
-
-    const bool qvalid = n < R;
-    const int qt = qvalid ? n / G : 0;
-    const int qg = qvalid ? n - qt * G : 0;
-    bf16x8_t qf[4];
-    {
-        const uint16_t* qp = p.q.data + b * p.q.sb + (int64_t)qt * p.q.st + (int64_t)(hk * G + qg) * p.q.sh + 32 * g;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const u32x4_t z = {0u, 0u, 0u, 0u};
-            qf[j] = qvalid ? *reinterpret_cast<const bf16x8_t*>(qp + 8 * j) : __builtin_bit_cast(bf16x8_t, z);
-        }
-    }
-    const int qpos = qpos0 + qt;
 
     const int32_t* kpt = p4.k.page_table + (int64_t)row * p4.k.pts;
     const int32_t* vpt = p4.v.page_table + (int64_t)row * p4.v.pts;
@@ -123,27 +111,53 @@ __global__ __launch_bounds__(kWaves4 * 64) void attn4_decode_kernel(Attn4Params 
         for (int kt = 0; kt < 4; ++kt) x.v[kt] = load16(vp + v_off + 1024 * kt);
         return x;
     };
+    Page4 xa, xb;
+    if (nb_w > 0) xa = load_page(0);
+
+    bf16x8_t qf[kN][4];
+    int qpos[kN];
+#pragma unroll
+    for (int u = 0; u < kN; ++u) {
+        const int r = r0 + 16 * u + n;
+        const bool valid = r < R;
+        const int qt = valid ? r / G : 0;
+        const int qg = valid ? r - qt * G : 0;
+        const uint16_t* qp = p.q.data + b * p.q.sb + (int64_t)qt * p.q.st + (int64_t)(hk * G + qg) * p.q.sh + 32 * g;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const u32x4_t z = {0u, 0u, 0u, 0u};
+            qf[u][j] = valid ? *reinterpret_cast<const bf16x8_t*>(qp + 8 * j) : __builtin_bit_cast(bf16x8_t, z);
+        }
+        qpos[u] = qpos0 + qt;
+    }
 
     const float sl2 = p.scale_log2;
-    f32x4_t oacc[8];
+    f32x4_t oacc[kN][8];
+    float m_run[kN], l_run[kN];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) oacc[j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    float m_run = kNegInf;
-    float l_run = 0.0f;
+    for (int u = 0; u < kN; ++u) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) oacc[u][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        m_run[u] = kNegInf;
+        l_run[u] = 0.0f;
+    }
     const bf16x2_t ones = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
 
-    auto k_scale = [&](const Page4& x, int kt) { return __uint_as_float(((x.ks >> (8 * kt)) & 0xffu) << 23); };
     auto compute = [&](Page4& x, int i) {
         const int kb = e0 + w + kWaves4 * i;
-        f32x4_t sc[4];
+        f32x4_t sc[kN][4];
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
-            sc[kt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            const float ks = k_scale(x, kt);
+            const float ks = scale_of(x.ks, kt);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                sc[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, decode_row(x.k[kt][j], ks)),
-                                                                 qf[j], sc[kt], 0, 0, 0);
+            for (int u = 0; u < kN; ++u) sc[u][kt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bf16x8_t kf = __builtin_bit_cast(bf16x8_t, decode_row(x.k[kt][j], ks));
+#pragma unroll
+                for (int u = 0; u < kN; ++u)
+                    sc[u][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[u][j], sc[u][kt], 0, 0, 0);
+            }
         }
         int nan_at = kNoKey;  // the first position with a NaN value in this lane's output dims
         if (kb >= e_mask) {
@@ -154,7 +168,9 @@ __global__ __launch_bounds__(kWaves4 * 64) void attn4_decode_kernel(Attn4Params 
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int key = first + 16 * kt + e;
-                    if (key > qpos) sc[kt][e] = kNegInf;
+#pragma unroll
+                    for (int u = 0; u < kN; ++u)
+                        if (key > qpos[u]) sc[u][kt][e] = kNegInf;
                     const bool bad = ((x.vs[kt] >> (8 * e)) & 0xffu) == kScaleNan;
                     if (bad && key < kv_tokens) nan_at = min(nan_at, key);
                     if (bad || key >= kv_tokens) {
@@ -172,39 +188,47 @@ __global__ __launch_bounds__(kWaves4 * 64) void attn4_decode_kernel(Attn4Params 
                 nan_at = __shfl(nan_at, 4 * g, 64);
             }
         }
-        float mx = kNegInf;
+        bf16x8_t pf[kN][2];
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
+        for (int u = 0; u < kN; ++u) {
+            float mx = kNegInf;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[kt][e]);
-        mx = xor32_max(xor16_max(mx)) * sl2;
-        float alpha = 1.0f;
-        if (mx > m_run + kRescale) {
-            alpha = __builtin_amdgcn_exp2f(m_run - mx);
-            m_run = mx;
-            l_run *= alpha;
+            for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[u][kt][e]);
+            mx = xor32_max(xor16_max(mx)) * sl2;
+            float alpha = 1.0f;
+            if (mx > m_run[u] + kRescale) {
+                alpha = __builtin_amdgcn_exp2f(m_run[u] - mx);
+                m_run[u] = mx;
+                l_run[u] *= alpha;
+            }
+            if (__ballot(alpha != 1.0f)) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) oacc[u][j] *= alpha;
+            }
+            const float m_use = m_run[u] == kNegInf ? 0.0f : m_run[u];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                f32x8_t pv8;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    pv8[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][2 * half + (e >> 2)][e & 3], sl2, -m_use));
+                const bf16x8_t pw = __builtin_convertvector(pv8, bf16x8_t);
+                l_run[u] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pw, pw, 0, 1), ones, l_run[u], false);
+                l_run[u] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pw, pw, 2, 3), ones, l_run[u], false);
+                l_run[u] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pw, pw, 4, 5), ones, l_run[u], false);
+                l_run[u] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pw, pw, 6, 7), ones, l_run[u], false);
+                pf[u][half] = pw;
+            }
         }
-        if (__ballot(alpha != 1.0f)) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) oacc[j] *= alpha;
-        }
-        const float m_use = m_run == kNegInf ? 0.0f : m_run;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            f32x8_t pv8;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                pv8[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * half + (e >> 2)][e & 3], sl2, -m_use));
-            const bf16x8_t pf = __builtin_convertvector(pv8, bf16x8_t);
-            l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pf, pf, 0, 1), ones, l_run, false);
-            l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pf, pf, 2, 3), ones, l_run, false);
-            l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pf, pf, 4, 5), ones, l_run, false);
-            l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pf, pf, 6, 7), ones, l_run, false);
             u32x4_t t[8];  // the 8 tokens' rows of 8 dims
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int kt = 2 * half + (e >> 2);
-                t[e] = decode_row(x.v[kt][e & 3], __uint_as_float(((x.vs[kt] >> (8 * (e & 3))) & 0xffu) << 23));
+                t[e] = decode_row(x.v[kt][e & 3], scale_of(x.vs[kt], e & 3));
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -213,17 +237,22 @@ __global__ __launch_bounds__(kWaves4 * 64) void attn4_decode_kernel(Attn4Params 
                                    __builtin_amdgcn_perm(t[3][j >> 1], t[2][j >> 1], sel),
                                    __builtin_amdgcn_perm(t[5][j >> 1], t[4][j >> 1], sel),
                                    __builtin_amdgcn_perm(t[7][j >> 1], t[6][j >> 1], sel)};
-                oacc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), pf, oacc[j], 0, 0, 0);
+#pragma unroll
+                for (int u = 0; u < kN; ++u)
+                    oacc[u][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), pf[u][half],
+                                                                         oacc[u][j], 0, 0, 0);
             }
         }
-        if (nan_at <= qpos) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) oacc[j] = f32x4_t{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
-        }
+        for (int u = 0; u < kN; ++u)
+            if (nan_at <= qpos[u]) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) oacc[u][j][e] = __builtin_nanf("");
+            }
     };
 
-    Page4 xa, xb;
-    if (nb_w > 0) xa = load_page(0);
     for (int i = 0; i < nb_w; i += 2) {
         if (i + 1 < nb_w) xb = load_page(i + 1);
         compute(xa, i);
@@ -231,51 +260,57 @@ __global__ __launch_bounds__(kWaves4 * 64) void attn4_decode_kernel(Attn4Params 
         if (i + 1 < nb_w) compute(xb, i + 1);
     }
 
-    // ---- the eight waves' results through LDS ----
-    l_run += __shfl_xor(l_run, 16, 64);
-    l_run += __shfl_xor(l_run, 32, 64);
-    // tile j, value i: dim 8 (4 g + i) + j of row n
+    // ---- the eight waves' results through LDS, 16 rows at a time ----
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float* to = mo + (w * kRows4 + n) * kOStride4 + 8 * (4 * g + i);
-        *reinterpret_cast<f32x4_t*>(to) = f32x4_t{oacc[0][i], oacc[1][i], oacc[2][i], oacc[3][i]};
-        *reinterpret_cast<f32x4_t*>(to + 4) = f32x4_t{oacc[4][i], oacc[5][i], oacc[6][i], oacc[7][i]};
-    }
-    if (g == 0) {
-        ml[(w * kRows4 + n) * 2 + 0] = m_run;
-        ml[(w * kRows4 + n) * 2 + 1] = l_run;
-    }
-    __syncthreads();
-    const int orow = tid >> 5;  // 16 rows x 32 threads, 4 dims each
-    const int d4 = (tid & 31) * 4;
-    if (orow >= R) return;
-    float mx = kNegInf;
+    for (int u = 0; u < kN; ++u) {
+        float ls = l_run[u];
+        ls += __shfl_xor(ls, 16, 64);
+        ls += __shfl_xor(ls, 32, 64);
+        if (u > 0) __syncthreads();
+        // tile j, value i: dim 8 (4 g + i) + j of row n
 #pragma unroll
-    for (int v = 0; v < kWaves4; ++v) mx = fmaxf(mx, ml[(v * kRows4 + orow) * 2]);
-    const float m_use = mx == kNegInf ? 0.0f : mx;
-    f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    float wsum = 0.0f;
+        for (int i = 0; i < 4; ++i) {
+            float* to = mo + (w * 16 + n) * kOStride4 + 8 * (4 * g + i);
+            *reinterpret_cast<f32x4_t*>(to) = f32x4_t{oacc[u][0][i], oacc[u][1][i], oacc[u][2][i], oacc[u][3][i]};
+            *reinterpret_cast<f32x4_t*>(to + 4) = f32x4_t{oacc[u][4][i], oacc[u][5][i], oacc[u][6][i], oacc[u][7][i]};
+        }
+        if (g == 0) {
+            ml[(w * 16 + n) * 2 + 0] = m_run[u];
+            ml[(w * 16 + n) * 2 + 1] = ls;
+        }
+        __syncthreads();
+        const int lrow = tid >> 5;  // 16 rows x 32 threads, 4 dims each
+        const int orow = r0 + 16 * u + lrow;
+        const int d4 = (tid & 31) * 4;
+        if (orow < R) {
+            float mx = kNegInf;
 #pragma unroll
-    for (int v = 0; v < kWaves4; ++v) {
-        const float wv = __builtin_amdgcn_exp2f(ml[(v * kRows4 + orow) * 2] - m_use);
-        wsum += wv * ml[(v * kRows4 + orow) * 2 + 1];
-        acc += wv * *reinterpret_cast<const f32x4_t*>(mo + (v * kRows4 + orow) * kOStride4 + d4);
-    }
-    // no key: zeros and -inf; a NaN sum stays
-    const float inv = wsum == 0.0f ? 0.0f : 1.0f / wsum;
-    const float lse2 = wsum == 0.0f ? kNegInf : mx + __log2f(wsum);
-    acc *= inv;
-    const int ot = orow / G;
-    const int og = orow - ot * G;
-    if (nsplit == 1) {
-        const int hq = hk * G + og;
-        uint16_t* op = p.out.data + b * p.out.sb + (int64_t)ot * p.out.st + (int64_t)hq * p.out.sh + d4;
-        *reinterpret_cast<bf16x4_t*>(op) = __builtin_convertvector(acc, bf16x4_t);
-        if (p.lse && (tid & 31) == 0) p.lse[((int64_t)b * s.Hq + hq) * s.Lq + ot] = lse2 * 0.69314718055994531f;
-    } else {
-        const int64_t prow = ((int64_t)split * (s.B * s.Hkv) + row) * R + orow;
-        *reinterpret_cast<f32x4_t*>(p.ws_o + prow * 128 + d4) = acc;
-        if ((tid & 31) == 0) p.ws_lse[prow] = lse2;
+            for (int v = 0; v < kWaves4; ++v) mx = fmaxf(mx, ml[(v * 16 + lrow) * 2]);
+            const float m_use = mx == kNegInf ? 0.0f : mx;
+            f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+            float wsum = 0.0f;
+#pragma unroll
+            for (int v = 0; v < kWaves4; ++v) {
+                const float wv = __builtin_amdgcn_exp2f(ml[(v * 16 + lrow) * 2] - m_use);
+                wsum += wv * ml[(v * 16 + lrow) * 2 + 1];
+                acc += wv * *reinterpret_cast<const f32x4_t*>(mo + (v * 16 + lrow) * kOStride4 + d4);
+            }
+            // no key: zeros and -inf; a NaN sum stays
+            const float inv = wsum == 0.0f ? 0.0f : 1.0f / wsum;
+            const float lse2 = wsum == 0.0f ? kNegInf : m_use + __log2f(wsum);
+            acc *= inv;
+            const int ot = orow / G;
+            const int hq = hk * G + orow - ot * G;
+            if (nsplit == 1) {
+                uint16_t* op = p.out.data + b * p.out.sb + (int64_t)ot * p.out.st + (int64_t)hq * p.out.sh + d4;
+                *reinterpret_cast<bf16x4_t*>(op) = __builtin_convertvector(acc, bf16x4_t);
+                if (p.lse && (tid & 31) == 0) p.lse[((int64_t)b * s.Hq + hq) * s.Lq + ot] = lse2 * 0.69314718055994531f;
+            } else {
+                const int64_t prow = ((int64_t)split * (s.B * s.Hkv) + row) * R + orow;
+                *reinterpret_cast<f32x4_t*>(p.ws_o + prow * 128 + d4) = acc;
+                if ((tid & 31) == 0) p.ws_lse[prow] = lse2;
+            }
+        }
     }
 }
 
@@ -394,7 +429,7 @@ __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) v
     auto stage = [&](int j) {
         uint8_t* to = smem + (j & 1) * 2 * kKv4Bytes;
         if (!is_v) {
-            const float sc = __uint_as_float(scale_w << 23);
+            const float sc = scale_of<0>(scale_w);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 *reinterpret_cast<u32x4_t*>(to + st_t * 256 + ((st_c + i) ^ (st_t & 15)) * 16) = decode_row(code[i], sc);
@@ -414,7 +449,7 @@ __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) v
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 *reinterpret_cast<u32x4_t*>(to + kKv4Bytes + (st_t + i) * 256 + (st_c ^ (4 * i)) * 16) =
-                    decode_row(code[i], __uint_as_float(((scale_w >> (8 * i)) & 0xffu) << 23));
+                    decode_row(code[i], scale_of(scale_w, i));
         }
     };
 
@@ -562,10 +597,20 @@ __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) v
 
 }  // namespace
 
+// Rows up to which the decode kernel's pairs of tiles are used (measured beside attn4_tiling)
+constexpr int kDraftRows4 = 128;
+
+AttnTiling attn4_tiling(const Shape& s, bool dense) {
+    const int rows = s.Lq * s.G;
+    if (!dense || rows > kDraftRows4) return attn_tiling(s, dense, false);
+    return AttnTiling{rows <= 16 ? 16 : 32, true, true, 0, 32};
+}
+
 hipError_t launch_attn4(const AttnArgs& a, const Kv4Addr& k, const Kv4Addr& v, hipStream_t stream) {
     Attn4Params p;
     SplitPlan plan;
-    attn_fill(a, &p.a, &plan);
+    const AttnTiling tiling = attn4_tiling(a.s, a.kv_len != nullptr);
+    attn_fill(a, tiling, &p.a, &plan);
     p.a.ws_unsplit = nullptr;  // a launch with splits keeps them
     p.k = k;
     p.v = v;
@@ -573,8 +618,10 @@ hipError_t launch_attn4(const AttnArgs& a, const Kv4Addr& k, const Kv4Addr& v, h
     static_assert(kNW == kWaves4, "one workgroup size");
     if (a.table)
         launch(attn4_fwd_kernel<true>);
-    else if (attn_uses_decode_kernel(a.s, true))
-        launch(attn4_decode_kernel);
+    else if (tiling.tile_rows == 16)
+        launch(attn4_decode_kernel<1>);
+    else if (tiling.tile_rows == 32)
+        launch(attn4_decode_kernel<2>);
     else
         launch(attn4_fwd_kernel<false>);
     const hipError_t e = hipGetLastError();

@@ -159,11 +159,23 @@ struct SplitPlan {
     int32_t xoff[9];
 };
 
-// dense = identity block lists over kv_len tokens (decode); otherwise per-row tables
-void attn_plan(const Shape& s, const int32_t* nkb, int forced, bool dense, SplitPlan* plan);
+// How a launch cuts its packed rows and block lists.
+struct AttnTiling {
+    int tile_rows;     // packed rows of a workgroup
+    bool streams;      // its waves take blocks on their own (decode kernels)
+    bool steps;        // splits chosen by the blocks that a wave takes in turn (attn_plan)
+    int min_blocks;    // least blocks of a split
+    int max_splits;
+};
+// dense = identity block lists over kv_len tokens (decode); otherwise per-row tables.  decode: whether few
+// rows may take the decode kernel.
+AttnTiling attn_tiling(const Shape& s, bool dense, bool decode = true);
+AttnTiling attn4_tiling(const Shape& s, bool dense);
+void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling& tiling, SplitPlan* plan);
 bool attn_uses_decode_kernel(const Shape& s, bool dense);
 void attn_positions(const Shape& s, const PastBlocks& pb, const int32_t* kv_len, int32_t* qpos0, int32_t* nkb);
 int attn_pick_splits(const Shape& s, const PastBlocks& pb, const int32_t* kv_len);
+int attn_pick_splits(const Shape& s, const PastBlocks& pb, const int32_t* kv_len, const AttnTiling& tiling);
 int64_t attn_workspace_bytes(const Shape& s, int num_splits);
 hipError_t launch_attn(const AttnArgs& a, hipStream_t stream);
 // The same over pages held in 4 bits (a.k and a.v unused; ca_attn4.hip)

@@ -816,7 +816,9 @@ def attn_decode(q: torch.Tensor, k: AnyKV, v: AnyKV, kv_len: Sequence[int], scal
     for name, kv in (("k", k), ("v", v)):
         kv.check_blocks(name, B, num_kv_heads, (max_len + BLOCK - 1) // BLOCK, tokens=max_len)
     d = make_dims(B, Lq, Hq, num_kv_heads, kv_cap)
-    need = _hip.lib().ca_attn_decode_workspace_size(ctypes.byref(d), ka, int(num_splits))
+    lib = _hip.lib()
+    size = lib.ca_attn_decode_q4_workspace_size if isinstance(k, KV4) else lib.ca_attn_decode_workspace_size
+    need = size(ctypes.byref(d), ka, int(num_splits))
     if need < 0:
         raise _hip.CaError(int(need), _hip.last_error())
     if need > 0 and (workspace is None or workspace.numel() * workspace.element_size() < need):
