@@ -315,18 +315,29 @@ __global__ __launch_bounds__(kWaves4 * 64) __attribute__((amdgpu_waves_per_eu(2)
 }
 
 // ---------------------------------------------------------------------------------------
-// Chunks, and drafts with more than 16 packed rows: 256 packed rows a workgroup, 32 a wave, the
-// 32x32x16 products of the bf16 kernel.  A block's codes go from memory to registers (16 bytes a thread:
-// waves 0-3 a group of a token of K, waves 4-7 8 dims of four tokens of V), through 16 conversions to
-// bf16 and into LDS in the bf16 kernel's places, two blocks deep, while the block before is multiplied.
+// Chunks, and drafts with many packed rows: 256 packed rows a workgroup, 32 a wave, with the products and
+// the software pipeline of the bf16 kernel: the scores of the next block run beside the softmax of this one,
+// then its PV product beside the next block's row max, instruction by instruction (fused).
+// A block's codes go from memory to registers (16 bytes a thread: waves 0-3 a group of a token of K, waves
+// 4-7 8 dims of four tokens of V), through 16 conversions to bf16 and into LDS in the bf16 kernel's places,
+// between the MFMAs of the PV product.  Rings of four K and four V blocks in LDS, K of block j in place
+// j & 3 and V in place (j + 1) & 3; slot j writes K of j + 3 and V of j + 2 (one place for all waves)
+// and loads the codes of the blocks after those.
 // kTab: block lists come from the per-row table; otherwise they are the identity (drafts).
-constexpr int kKv4Bytes = 64 * 256;  // K or V rows of one block in LDS
+constexpr int kPlace4 = 64 * 256;     // K or V rows of one block in LDS
+constexpr int kVRing4 = 4 * kPlace4;  // LDS byte offset of the V ring
+
+template <int N>
+struct Int4C {
+    static constexpr int value = N;
+};
 
 template <bool kTab>
 __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn4_fwd_kernel(Attn4Params p4) {
-    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * 2 * kKv4Bytes];  // K and V of two blocks
+    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * kVRing4];
     // by block modulo 4 and group of dims: the first key in the block with a NaN value (masked blocks)
     __shared__ int vnan[4][4];
+    __shared__ int late[kNW];
     const AttnParams& p = p4.a;
     const Shape& s = p.s;
     Item it;
@@ -347,18 +358,21 @@ __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) v
     const int32_t* tab = kTab ? p.table + (int64_t)row * p.table_stride : nullptr;
     const int lim = (qpos0 + t_last) >> 6;  // last block the tile can see
     const int kv_tokens = qpos0 + s.Lq;
+    const int first_q = qpos0 + t_first;  // blocks that reach past it are masked
     const int tid = threadIdx.x;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l = tid & 63;
     const int h = l >> 5;
     const int n = l & 31;
 
-    const int qrow = r0 + 32 * w + n;
-    const bool qvalid = qrow < rows_total;
-    const int qt = qvalid ? qrow / G : 0;
-    const int qg = qvalid ? qrow - qt * G : 0;
+    int qpos;
     bf16x8_t qf[8];
     {
+        const int qrow = r0 + 32 * w + n;
+        const bool qvalid = qrow < rows_total;
+        const int qt = qvalid ? qrow / G : 0;
+        const int qg = qvalid ? qrow - qt * G : 0;
+        qpos = qpos0 + qt;
         const uint16_t* qp = p.q.data + b * p.q.sb + (int64_t)qt * p.q.st + (int64_t)(hk * G + qg) * p.q.sh + 8 * h;
 #pragma unroll
         for (int ds = 0; ds < 8; ++ds) {
@@ -366,6 +380,7 @@ __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) v
             qf[ds] = qvalid ? *reinterpret_cast<const bf16x8_t*>(qp + 16 * ds) : __builtin_bit_cast(bf16x8_t, z);
         }
     }
+    if (tid < 16) vnan[tid >> 2][tid & 3] = 64;
     // entries up to the last one that the tile can see
     int n_vis = kTab ? 0 : min(nkb, lim + 1);
     if (kTab) {
@@ -381,8 +396,21 @@ __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) v
     const int chunk = (n_vis + nsplit - 1) / nsplit;
     const int e0 = min(n_vis, split * chunk);
     const int nblk = min(n_vis, e0 + chunk) - e0;
-    const int qpos = qpos0 + qt;
-    const int first_q = qpos0 + t_first;  // blocks that reach past it are masked
+    // blocks before the first masked one; a list's order is not relied on: every wave looks through an eighth
+    const int whole = (first_q + 1) >> 6;  // blocks [0, whole) hold no key past the tile's first query
+    int n_un = min(max(whole - e0, 0), nblk);
+    if (kTab) {
+        int first = nblk;
+        for (int at = 64 * w; at < nblk; at += 64 * kNW) {
+            const int id = at + l < nblk ? tab[e0 + at + l] : 0;
+            const uint64_t hit = __ballot(at + l < nblk && min(max(id, 0), nkb - 1) >= whole);
+            if (hit != 0) {
+                first = at + __ffsll(static_cast<unsigned long long>(hit)) - 1;
+                break;
+            }
+        }
+        if (l == 0) late[w] = first;
+    }
 
     f32x16_t oacc[4];
 #pragma unroll
@@ -393,64 +421,73 @@ __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) v
     float l_run = 0.0f;
     float m_neg = 0.0f;  // -m_run, 0 while a row has seen no key
 
-    // ---- the list's blocks, 64 entries at a time, one per lane ----
-    // (logical id and this wave's page: K's for waves 0-3, V's for the others)
+    // ---- the pages of the list's blocks, 64 entries at a time, one per lane (past its end: the last entry) ----
     const bool is_v = w >= 4;
     const Kv4Addr& kv = is_v ? p4.v : p4.k;
     const int32_t* pt = kv.page_table + (int64_t)row * kv.pts;
-    int ids = 0, pages = 0;
-    auto load_ids = [&](int c) {
-        const int e = 64 * c + l;
-        if (e < nblk) {
-            ids = kTab ? min(max(tab[e0 + e], 0), nkb - 1) : e0 + e;
-            pages = static_cast<int>(clamp_page(pt[ids], kv.max_page));
-        }
+    int cur_page = 0, next_page = 0;
+    auto load_pages = [&](int c) {
+        const int e = e0 + min(64 * c + l, nblk - 1);
+        const int id = kTab ? min(max(tab[e], 0), nkb - 1) : e;
+        next_page = static_cast<int>(clamp_page(pt[id], kv.max_page));
     };
-    // ---- a block's codes: memory -> registers ----
+    auto id_of = [&](int i) { return kTab ? min(max(sload(tab + e0 + i), 0), nkb - 1) : e0 + i; };
+    // ---- a block's codes: memory -> registers (of this wave's cache; i asked for in ascending order) ----
     const int u = tid & 255;
     const int st_t = is_v ? 4 * (u >> 4) : u >> 2;  // token (of V: the first of four)
     const int st_c = is_v ? u & 15 : 4 * (u & 3);   // 16-byte chunk of the row in LDS (of K: the first of four)
-    const int sc_off = is_v ? v4_scale(st_t, st_c >> 2) : k4_scale(st_t, u & 3);
-    u32x4_t code;
-    uint32_t scale_w = 0;
-    int next_id = 0;  // of the block in the registers
-    auto fetch = [&](int j) {
-        if ((j & 63) == 0) load_ids(j >> 6);
-        next_id = __builtin_amdgcn_readlane(ids, j & 63);
-        const uint8_t* page = kv.data + (int64_t)__builtin_amdgcn_readlane(pages, j & 63) * kv.stride;
-        code = load16(page + 16 * u);
-        if (is_v)
-            scale_w = *reinterpret_cast<const uint32_t*>(page + sc_off);
-        else
-            scale_w = page[sc_off];
+    const int sc_off = is_v ? v4_scale(st_t, st_c >> 2) : k4_scale(st_t, u & 3) & ~3;  // the word with the byte(s)
+    struct Codes {
+        u32x4_t code;
+        uint32_t scale;
     };
-    // ---- registers -> bf16 rows in LDS, block j in place j & 1 ----
+    auto fetch = [&](int i) {
+        if ((i & 63) == 0) {
+            cur_page = next_page;
+            load_pages((i >> 6) + 1);
+        }
+        Codes x;
+        const uint8_t* page = kv.data + (int64_t)__builtin_amdgcn_readlane(cur_page, i & 63) * kv.stride;
+        x.code = load16(page + 16 * u);
+        x.scale = *reinterpret_cast<const uint32_t*>(page + sc_off);
+        return x;
+    };
+    // ---- registers -> bf16 rows in LDS ----
     //   K: 16-byte chunk c of row r sits at chunk c ^ (r & 15), V: at chunk c ^ 4 (r & 3)
-    auto stage = [&](int j) {
-        uint8_t* to = smem + (j & 1) * 2 * kKv4Bytes;
+    // (chunk or row i of a thread's four: bits flipped and bytes added to the first one's address)
+    const int to = is_v ? kVRing4 + st_t * 256 + st_c * 16 : st_t * 256 + (st_c ^ (st_t & 15)) * 16;
+    const int to_flip = is_v ? 64 : 16, to_add = is_v ? 256 : 0;
+    // Before a block's conversions: K's one scale byte to all four words' places; of V's blocks from the first
+    // masked one on the values that no query may see become zero, and NaN, which goes to the rows that see it
+    // after the product.
+    auto settle = [&](Codes& x, int block) {
         if (!is_v) {
-            const float sc = scale_of<0>(scale_w);
+            x.scale = ((x.scale >> (8 * w)) & 0xffu) * 0x01010101u;  // K's token 16 w + l / 4
+        } else if (block >= n_un) {
+            const int first = 64 * id_of(min(block, nblk - 1)) + st_t;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<u32x4_t*>(to + st_t * 256 + ((st_c + i) ^ (st_t & 15)) * 16) = decode_row(code[i], sc);
-        } else {
-            if (64 * next_id + 63 > first_q) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool bad = ((scale_w >> (8 * i)) & 0xffu) == kScaleNan;
-                    const bool there = 64 * next_id + st_t + i < kv_tokens;
-                    if (bad && there) atomicMin(&vnan[j & 3][st_c >> 2], st_t + i);
-                    if (bad || !there) {
-                        code[i] = 0;
-                        scale_w &= ~(0xffu << (8 * i));
-                    }
+            for (int i = 0; i < 4; ++i) {
+                const bool bad = ((x.scale >> (8 * i)) & 0xffu) == kScaleNan;
+                const bool there = first + i < kv_tokens;
+                if (bad && there) atomicMin(&vnan[block & 3][st_c >> 2], st_t + i);
+                if (bad || !there) {
+                    x.code[i] = 0;
+                    x.scale &= ~(0xffu << (8 * i));
                 }
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<u32x4_t*>(to + kKv4Bytes + (st_t + i) * 256 + (st_c ^ (4 * i)) * 16) =
-                    decode_row(code[i], scale_of(scale_w, i));
         }
+    };
+    auto put = [&](const Codes& x, int place, int i) {
+        *reinterpret_cast<u32x4_t*>(smem + ((to ^ (to_flip * i)) + to_add * i) + place * kPlace4) = decode_row(x.code[i], scale_of(x.scale, i));
+    };
+    // slot j writes this wave's block j + lead (K: j + 3, V: j + 2) to place (j + 3) & 3
+    const int lead = is_v ? 2 : 3;
+    Codes held;  // the codes that the next slot writes
+    auto stage = [&](int j) {
+        settle(held, j + lead);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) put(held, (j + 3) & 3, i);
+        held = fetch(j + lead + 1);
     };
 
     const float sl2 = p.scale_log2;
@@ -464,54 +501,64 @@ __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) v
     const int v_x = 2 * ((l >> 4) & 1) + ((l & 3) >> 1);
     int v_off[4];
 #pragma unroll
-    for (int dt = 0; dt < 4; ++dt) v_off[dt] = kKv4Bytes + (8 * h + v_rq) * 256 + (4 * (dt ^ v_rq) + v_x) * 16 + (l & 1) * 8;
+    for (int dt = 0; dt < 4; ++dt) v_off[dt] = kVRing4 + (8 * h + v_rq) * 256 + (4 * (dt ^ v_rq) + v_x) * 16 + (l & 1) * 8;
     const i16x4_t ones = {0x3f80, 0x3f80, 0x3f80, 0x3f80};
     auto add_weights = [&](uint32_t w0, uint32_t w1, f32x4_t acc) {
         const u32x2_t ww = {w0, w1};
         return __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(ones, __builtin_bit_cast(i16x4_t, ww), acc, 0, 0, 0);
     };
-    auto compute = [&](int j, int kb) {
-        const uint8_t* at = smem + (j & 1) * 2 * kKv4Bytes;
-        f32x16_t sc[2];
+    f32x16_t sc[2];  // scores of the block whose softmax comes next (32 keys each)
+    auto k_frag = [&](int base, int i) {
+        return *reinterpret_cast<const bf16x8_t*>(smem + base + k_off[i >> 1] + (i & 1) * 8192);
+    };
+    auto v_frag = [&](int base, int i) {  // A operand of PV MFMA i: 16-key step i / 4, 32-d tile i % 4
+        const uint8_t* vp = smem + base + v_off[i & 3] + (i >> 2) * 4096;
+        const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(to_lds_v4(vp));
+        const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(to_lds_v4(vp + 1024));
+        return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    auto scores = [&](int kbase) {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) sc[kt][e] = 0.0f;
+            for (int j = 0; j < 16; ++j) sc[kt][j] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(at + k_off[i >> 1] + (i & 1) * 8192);
-            sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[i >> 1], sc[i & 1], 0, 0, 0);
+        for (int i = 0; i < 16; ++i)
+            sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(kbase, i), qf[i >> 1], sc[i & 1], 0, 0, 0);
+    };
+    auto mask = [&](int kb) {
+        const int vis = qpos - 64 * kb - 8 * h;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int key = kt * 32 + 16 * (e >> 3) + 4 * ((e >> 2) & 1) + (e & 3);
+                if (key > vis) sc[kt][e] = kNegInf;
+            }
+    };
+    auto rise = [&](float mx) {
+        float alpha = 1.0f;
+        if (mx > m_run + kRescale) {
+            alpha = __builtin_amdgcn_exp2f(m_run - mx);  // 0 when m_run = -inf
+            m_run = mx;
+            m_neg = -mx;
+            l_run *= alpha;
         }
-        const bool masked = 64 * kb + 63 > first_q;
-        if (masked) {
-            const int vis = qpos - 64 * kb - 8 * h;
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+        for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int key = kt * 32 + 16 * (e >> 3) + 4 * ((e >> 2) & 1) + (e & 3);
-                    if (key > vis) sc[kt][e] = kNegInf;
-                }
-        }
+            for (int e = 0; e < 16; ++e) oacc[dt][e] *= alpha;
+    };
+    auto block_max = [&]() {
         float mx = kNegInf;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[kt][e]);
         mx = xor32_max(mx) * sl2;
-        if (__ballot(mx > m_run + kRescale)) {
-            float alpha = 1.0f;
-            if (mx > m_run + kRescale) {
-                alpha = __builtin_amdgcn_exp2f(m_run - mx);
-                m_run = mx;
-                m_neg = -mx;
-                l_run *= alpha;
-            }
-#pragma unroll
-            for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) oacc[dt][e] *= alpha;
-        }
+        if (__ballot(mx > m_run + kRescale)) rise(mx);
+    };
+    auto finish = [&](int j, int kb) {
         bf16x8_t pf[4];
         f32x4_t rs = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -526,47 +573,164 @@ __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) v
             rs = add_weights(w4[2], w4[3], rs);
         }
         l_run += rs[0];
+        const int vbase = ((j + 1) & 3) * kPlace4;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const uint8_t* vp = at + v_off[i & 3] + (i >> 2) * 4096;
-            const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(to_lds_v4(vp));
-            const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(to_lds_v4(vp + 1024));
-            const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-            oacc[i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[i >> 2], oacc[i & 3], 0, 0, 0);
-        }
-        if (masked) {
+        for (int i = 0; i < 16; ++i)
+            oacc[i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_frag(vbase, i), pf[i >> 2], oacc[i & 3], 0, 0, 0);
+        if (j >= n_un) {
 #pragma unroll
-            for (int dt = 0; dt < 4; ++dt)
-                if (64 * kb + vnan[j & 3][dt] <= qpos && vnan[j & 3][dt] < 64)
+            for (int dt = 0; dt < 4; ++dt) {
+                const int at = vnan[j & 3][dt];
+                if (at < 64 && 64 * kb + at <= qpos)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) oacc[dt][e] = __builtin_nanf("");
+            }
         }
     };
-
-    if (tid < 16) vnan[tid >> 2][tid & 3] = 64;
-    if (nblk > 0) {
-        fetch(0);
-        __syncthreads();
-        stage(0);
-        int kb = next_id;
-        if (nblk > 1) fetch(1);
-        for (int j = 0; j < nblk; ++j) {
-            // block j has been written, and place (j + 1) & 1 has been read
-            __syncthreads();
-            const int kb_next = next_id;
-            if (tid < 4) vnan[(j + 3) & 3][tid] = 64;  // read last for block j - 1, written next for j + 3
-            if (j + 1 < nblk) {
-                stage(j + 1);
-                if (j + 2 < nblk) fetch(j + 2);
+    // ---- KV loop ----
+    // Slot j computes the scores of block j + 1 and the PV product of block j.  The barrier of slot j stands
+    // for: K of block j + 2 and V of block j + 1 are in LDS, and every wave has read K of block j + 1 and V
+    // of block j - 1.
+    auto mid_slot = [&]() {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's writes
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    constexpr int kAhead = 4;   // K fragments in flight ahead of their MFMA
+    constexpr int kVAhead = 3;  // V fragments
+    bf16x8_t kf[16];
+    // As in the bf16 kernel: the pins fix the order of the instructions in groups of one MFMA, a fragment read
+    // and the stages of one weight, so no instruction of a group waits for another.
+    auto fused = [&](f32x16_t(&sc)[2], f32x16_t(&sn)[2], auto place, int j) {
+        constexpr int R = decltype(place)::value;
+        constexpr int kK = ((R + 1) & 3) * kPlace4, kV = ((R + 1) & 3) * kPlace4, kN = ((R + 2) & 3) * kPlace4;
+        bf16x8_t vf[16];
+        uint32_t pw[16];  // packed weights, two per word
+        float y[33], x[34];
+        f32x4_t rs = {0.0f, 0.0f, 0.0f, 0.0f};
+        auto weight = [&](int e) {  // e = 0 .. 34
+            if (e >= 6 && (e & 3) == 2) rs = add_weights(pw[(e - 6) >> 1], pw[((e - 6) >> 1) + 1], rs);
+            if (e >= 3 && (e & 1) && e < 34) {
+                const f32x2_t pr = {x[e - 3], x[e - 2]};
+                pw[(e - 3) >> 1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(pr, bf16x2_t));
             }
-            compute(j, kb);
-            kb = kb_next;
+            if (e >= 1 && e <= 32) x[e - 1] = __builtin_amdgcn_exp2f(y[e - 1]);
+            if (e < 32) y[e] = __builtin_fmaf(sc[e >> 4][e & 15], sl2, m_neg);
+        };
+        auto pf = [&](int s4) {
+            const u32x4_t v = {pw[4 * s4], pw[4 * s4 + 1], pw[4 * s4 + 2], pw[4 * s4 + 3]};
+            return __builtin_bit_cast(bf16x8_t, v);
+        };
+        const f32x16_t zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+        constexpr int kEarly = 6;  // groups with two stages
+        int e = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (i + kAhead < 16) kf[i + kAhead] = k_frag(kK, i + kAhead);
+            if (i >= 16 - kVAhead) vf[i - 16 + kVAhead] = v_frag(kV, i - 16 + kVAhead);
+            sn[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i], qf[i >> 1], i < 2 ? zero : sn[i & 1], 0, 0, 0);
+            weight(e++);
+            if (i < kEarly) weight(e++);
+            asm volatile("" : "+v"(sn[i & 1]), "+v"(y[e - 1]), "+v"(x[e - 2]), "+v"(rs), "+v"(sc[e >> 4]) : : "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        mid_slot();
+        __builtin_amdgcn_s_setprio(1);
+        settle(held, j + lead);
+        float mx = kNegInf;
+        bool up = false;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (i + kVAhead < 16) vf[i + kVAhead] = v_frag(kV, i + kVAhead);
+            if (i >= 16 - kAhead) kf[i - 16 + kAhead] = k_frag(kN, i - 16 + kAhead);
+            oacc[i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[i], pf(i >> 2), oacc[i & 3], 0, 0, 0);
+            if (e < 35) {
+                weight(e++);
+                if (e < 33) asm volatile("" : "+v"(y[e - 1]) : : "memory");
+                if (e < 34) asm volatile("" : "+v"(x[e - 2]) : : "memory");
+                asm volatile("" : "+v"(rs), "+v"(sc[1]) : : "memory");
+            }
+            if (i >= 4 && i < 12) {  // the row max of the next block's 32 scores
+                const int v = i - 4;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) mx = fmaxf(mx, sn[v >> 2][4 * (v & 3) + q]);
+            }
+            if (i == 12) mx = xor32_max(mx) * sl2;
+            if (i == 13) up = __ballot(mx > m_run + kRescale) != 0;
+            if (i == 14) l_run += rs[0];
+            asm volatile("" : "+v"(oacc[i & 3]), "+v"(mx), "+v"(l_run) : : "memory");
+            if (i >= 1 && i <= 10 && (i - 1) % 3 == 0) put(held, (R + 3) & 3, (i - 1) / 3);
+            if (i == 11) held = fetch(j + lead + 1);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        if (up) rise(mx);
+    };
+
+    if (nblk > 0) {
+        load_pages(0);
+        Codes c0 = fetch(0), c1 = fetch(1);
+        __syncthreads();  // vnan, late
+        if (kTab) {
+            n_un = nblk;
+#pragma unroll
+            for (int i = 0; i < kNW; ++i) n_un = min(n_un, late[i]);
+            n_un = __builtin_amdgcn_readfirstlane(n_un);
+        }
+        settle(c0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) put(c0, is_v ? 1 : 0, i);
+        if (!is_v) {
+            settle(c1, 1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) put(c1, 1, i);
+            c1 = fetch(2);
+        }
+        held = c1;
+        mid_slot();  // K of blocks 0 and 1, V of block 0
+        scores(0);
+        if (n_un == 0) mask(id_of(0));
+        block_max();
+        stage(-1);
+        int j = 0;
+        f32x16_t sn[2];
+        if (j + 2 < n_un) {
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) kf[i] = k_frag(kPlace4, i);
+        }
+        // four slots a round: the ring places are constants and the scores change places without copies
+        for (; j + 4 < n_un; j += 4) {
+            fused(sc, sn, Int4C<0>{}, j);
+            fused(sn, sc, Int4C<1>{}, j + 1);
+            fused(sc, sn, Int4C<2>{}, j + 2);
+            fused(sn, sc, Int4C<3>{}, j + 3);
+        }
+        if (j + 2 < n_un) {
+            fused(sc, sn, Int4C<0>{}, j);
+            fused(sn, sc, Int4C<1>{}, j + 1);
+            j += 2;
+        }
+        for (; j < nblk; ++j) {  // the next block is masked, or there is none
+            finish(j, id_of(j));
+            if (j + 1 < nblk) {
+                scores(((j + 1) & 3) * kPlace4);
+                const int kb = id_of(j + 1);
+                if (64 * kb + 63 > first_q) mask(kb);
+                block_max();
+                mid_slot();
+                if (tid < 4) vnan[(j + 3) & 3][tid] = 64;  // read last for block j - 1, written next for j + 3
+                stage(j);
+            }
         }
     }
 
-    // ---- epilogue ----
+    // ---- epilogue (the row's place computed again: kept, it would take registers from the loop) ----
     l_run += __shfl_xor(l_run, 32, 64);
-    if (qvalid) {
+    int tid2 = threadIdx.x;
+    asm volatile("" : "+v"(tid2));
+    const int qrow = r0 + 32 * (tid2 >> 6) + (tid2 & 31);
+    if (qrow < rows_total) {
+        const int qt = qrow / G, qg = qrow - qt * G, h = (tid2 >> 5) & 1;
         // no key: zeros and -inf; a NaN sum stays
         const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
         const float lse2 = l_run == 0.0f ? kNegInf : (m_run == kNegInf ? 0.0f : m_run) + __log2f(l_run);
