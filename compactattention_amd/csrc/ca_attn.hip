@@ -1087,14 +1087,15 @@ void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling&
         // 293-295 us split, while its dense tables need the split, 2.1 vs 3.2 ms)
         plan->may_unsplit = !same_len && units * 4 >= 3 * 256 && forced > 1;
     }
-    // Pages of 4 bits: a page takes a wave 1.65 us however many CUs work, so the launch takes as long as the
-    // most pages that a wave has in turn (a split of n blocks: ceil(n / 8)), and what a merge adds is 2 to 3
-    // pages' time.  The fewest pages in turn with which the items still fit one round, and no splits where
-    // these save fewer than three (32 Q / 8 KV heads, one token: 1024 tokens 7.8 us whole, 8.4 in 4 splits;
-    // 2048 tokens 10.9, 8.7).
+    // Pages of 4 bits: a workgroup takes 0.8 us for four blocks (one on each SIMD) however many CUs work, so
+    // the launch takes as long as the most fours of blocks that an item has (turns), and what a merge adds is
+    // three turns' time.  The fewest turns with which the items still fit one round, and no splits where
+    // these save fewer than four (32 Q / 8 KV heads, one token: 1024 tokens 7.8 us whole, 8.1 in 8 splits;
+    // 2048 tokens 10.8, 8.5; 8192 tokens 9.9 in 16 splits of eight blocks, 9.2 in 32 of four).
+    constexpr int kTurn = 4;
     int turns = 0;
     if (tiling.steps && forced <= 0) {
-        auto splits = [&](int nb, int t) { return max(1, (nb + kNW * t - 1) / (kNW * t)); };
+        auto splits = [&](int nb, int t) { return max(1, (nb + kTurn * t - 1) / (kTurn * t)); };
         auto fits = [&](int t) {
             int items = 0;
             for (int b = 0; b < s.B; ++b) {
@@ -1103,7 +1104,7 @@ void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling&
             }
             return items <= slots;
         };
-        const int whole = (nkb_max + kNW - 1) / kNW;
+        const int whole = (nkb_max + kTurn - 1) / kTurn;
         int lo = 1, hi = whole;  // fits() holds from some count on, or only without splits
         while (lo < hi) {
             const int mid = (lo + hi) / 2;
@@ -1112,7 +1113,7 @@ void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling&
             else
                 lo = mid + 1;
         }
-        turns = whole - lo < 3 ? whole : lo;
+        turns = whole - lo < 4 ? whole : lo;
     }
     plan->max = 1;
     plan->off[0] = 0;
@@ -1120,7 +1121,7 @@ void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling&
         const int nb = nkb[b];
         int sb = forced;
         if (turns > 0) {
-            sb = max(1, (nb + kNW * turns - 1) / (kNW * turns));
+            sb = max(1, (nb + kTurn * turns - 1) / (kTurn * turns));
         } else if (forced <= 0) {
             sb = static_cast<int>(nb / item_blocks + 0.5);
             sb = min(sb, max(1, nb / min_blocks));

@@ -759,6 +759,71 @@ __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) v
     }
 }
 
+// Merge of many splits of few rows: four groups of 32 threads share a row, each a quarter of its splits, so
+// that the partials' loads go out in one or two rounds where 32 threads take them in up to eight.
+__global__ __launch_bounds__(128) void attn4_merge_kernel(AttnParams p) {
+    __shared__ f32x4_t part[3][32];
+    const Shape& s = p.s;
+    const int64_t rows_all = (int64_t)s.B * s.Hkv * p.rows_total;
+    const int64_t gid = blockIdx.x;
+    const int row = static_cast<int>(gid / p.rows_total);
+    const int r = static_cast<int>(gid - (int64_t)row * p.rows_total);
+    const int b = row / s.Hkv;
+    const int hk = row - b * s.Hkv;
+    const int nsplit = p.sp[b];
+    if (nsplit == 1) return;  // the attention kernel wrote this request's rows
+    const int lane = threadIdx.x & 31;
+    const int grp = threadIdx.x >> 5;
+    constexpr int kAtOnce = 8;
+    // group grp's splits: grp, grp + 4, ...; their partials are loaded before the weights are known
+    const float* wo = p.ws_o + gid * 128 + 4 * lane;
+    f32x4_t o[kAtOnce];
+    auto load = [&](int sp0) {
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int sp = sp0 + grp + 4 * i;
+            o[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            if (sp < nsplit) o[i] = *reinterpret_cast<const f32x4_t*>(wo + (int64_t)sp * rows_all * 128);
+        }
+    };
+    const float ls0 = lane < nsplit ? p.ws_lse[(int64_t)lane * rows_all + gid] : kNegInf;
+    const float ls1 = lane + 32 < nsplit ? p.ws_lse[(int64_t)(lane + 32) * rows_all + gid] : kNegInf;
+    load(0);
+    float mx = fmaxf(ls0, ls1);
+#pragma unroll
+    for (int i = 16; i >= 1; i >>= 1) mx = fmaxf(mx, __shfl_xor(mx, i, 32));
+    const float m_use = mx == kNegInf ? 0.0f : mx;
+    const float w0 = __builtin_amdgcn_exp2f(ls0 - m_use), w1 = __builtin_amdgcn_exp2f(ls1 - m_use);
+    float wsum = w0 + w1;
+#pragma unroll
+    for (int i = 16; i >= 1; i >>= 1) wsum += __shfl_xor(wsum, i, 32);
+    f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int sp0 = 0;;) {
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int sp = sp0 + grp + 4 * i;  // the same in all 32 threads
+            const float wa = __shfl(w0, sp & 31, 32), wb = __shfl(w1, sp & 31, 32);
+            const float wt = sp >= nsplit ? 0.0f : sp < 32 ? wa : wb;
+            if (wt != 0.0f) acc += wt * o[i];
+        }
+        sp0 += 4 * kAtOnce;
+        if (sp0 >= nsplit) break;
+        load(sp0);
+    }
+    if (grp > 0) part[grp - 1][lane] = acc;
+    __syncthreads();
+    if (grp > 0) return;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) acc += part[i][lane];
+    acc *= wsum == 0.0f ? 0.0f : 1.0f / wsum;  // no key: zeros and -inf; a NaN sum stays
+    const int t = r / s.G;
+    const int hq = hk * s.G + r - t * s.G;
+    uint16_t* op = p.out.data + b * p.out.sb + (int64_t)t * p.out.st + (int64_t)hq * p.out.sh + 4 * lane;
+    *reinterpret_cast<bf16x4_t*>(op) = __builtin_convertvector(acc, bf16x4_t);
+    if (p.lse && lane == 0)
+        p.lse[((int64_t)b * s.Hq + hq) * s.Lq + t] = wsum == 0.0f ? kNegInf : (m_use + __log2f(wsum)) * 0.69314718055994531f;
+}
+
 }  // namespace
 
 // Rows up to which the decode kernel's pairs of tiles are used (measured beside attn4_tiling)
@@ -790,7 +855,10 @@ hipError_t launch_attn4(const AttnArgs& a, const Kv4Addr& k, const Kv4Addr& v, h
         launch(attn4_fwd_kernel<false>);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || plan.max <= 1) return e;
-    return launch_attn_merge(p.a, true, stream);
+    const int64_t rows_all = (int64_t)a.s.B * a.s.Hkv * p.a.rows_total;
+    if (!tiling.streams || rows_all >= int64_t{1} << 31) return launch_attn_merge(p.a, true, stream);
+    hipLaunchKernelGGL(attn4_merge_kernel, dim3(static_cast<unsigned>(rows_all)), dim3(128), 0, stream, p.a);
+    return hipGetLastError();
 }
 
 }  // namespace ca

@@ -163,7 +163,7 @@ struct SplitPlan {
 struct AttnTiling {
     int tile_rows;     // packed rows of a workgroup
     bool streams;      // its waves take blocks on their own (decode kernels)
-    bool steps;        // splits chosen by the blocks that a wave takes in turn (attn_plan)
+    bool steps;        // splits chosen by the blocks that a workgroup takes in turn (attn_plan)
     int min_blocks;    // least blocks of a split
     int max_splits;
 };
