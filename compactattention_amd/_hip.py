@@ -66,6 +66,7 @@ EXPORTED = (
     "ca_gather_q4",
     "ca_attn_fwd_q4",
     "ca_attn_decode_q4",
+    "ca_attn_fwd_q4_workspace_size",
     "ca_attn_decode_q4_workspace_size",
     "ca_copy_pages",
     "ca_rope_apply",
@@ -197,6 +198,7 @@ _SIGNATURES = {
                                       _f32, _P(SeqLayout), _vp, _i32, _vp, _i64, _vp]),
     "ca_attn_decode_q4": (ctypes.c_int, [_P(Dims), _P(SeqLayout), _P(Kv4Layout), _P(Kv4Layout), _vp, _f32,
                                          _P(SeqLayout), _vp, _i32, _vp, _i64, _vp]),
+    "ca_attn_fwd_q4_workspace_size": (ctypes.c_int64, [_P(Dims), _vp, _i32]),
     "ca_attn_decode_q4_workspace_size": (ctypes.c_int64, [_P(Dims), _vp, _i32]),
     "ca_copy_pages": (ctypes.c_int, [_P(PagePool), _i32, _vp, _vp, _i32, _vp, _vp]),
     "ca_rmsnorm": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i32, _f32, _vp]),

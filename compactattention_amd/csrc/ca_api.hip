@@ -692,6 +692,17 @@ int ca_attn_fwd(const ca_dims* dims, const ca_seq_layout* q, const ca_kv_layout*
     return ok();
 }
 
+int64_t ca_attn_fwd_q4_workspace_size(const ca_dims* dims, const int32_t* past_blocks_host, int32_t num_splits) {
+    ca::Shape s;
+    ca::PastBlocks pb;
+    int max_nkb = 0;
+    if (check_dims(dims, past_blocks_host, &s, &pb, &max_nkb) != CA_OK) return -1;
+    if (num_splits == 0) num_splits = ca::attn_pick_splits(s, pb, nullptr, ca::attn4_tiling(s, false));
+    if (num_splits < 1 || num_splits > ca::kMaxPrefillSplits)
+        return fail(CA_ERR_INVALID, "num_splits=%d outside [0, %d]", num_splits, ca::kMaxPrefillSplits);
+    return ca::attn_workspace_bytes(s, num_splits);
+}
+
 int ca_attn_fwd_q4(const ca_dims* dims, const ca_seq_layout* q, const ca_kv4_layout* k, const ca_kv4_layout* v,
                    const int32_t* table, int64_t table_stride, const int32_t* counts,
                    const int32_t* past_blocks_host, float scale, const ca_seq_layout* out, float* lse,
@@ -711,7 +722,7 @@ int ca_attn_fwd_q4(const ca_dims* dims, const ca_seq_layout* q, const ca_kv4_lay
     a.table = table;
     a.table_stride = table_stride;
     a.counts = counts;
-    const int max_splits = num_splits == 0 ? ca::attn_pick_splits(a.s, a.pb, nullptr) : num_splits;
+    const int max_splits = num_splits == 0 ? ca::attn_pick_splits(a.s, a.pb, nullptr, ca::attn4_tiling(a.s, false)) : num_splits;
     return attn4(a, ka, va, scale, lse, num_splits, max_splits, ca::kMaxPrefillSplits, workspace, workspace_bytes, stream);
 }
 

@@ -1047,6 +1047,7 @@ void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling&
     //  - dense decode with more rows runs attn_fwd_kernel with the prefill sizing and up to
     //    64 splits.
     const bool dec = tiling.streams;
+    const bool dense_lists = tiling.max_splits > kMaxPrefillSplits;
     plan->may_unsplit = 0;
     const int slots = dec ? 256 : 512;
     const int min_blocks = tiling.min_blocks;
@@ -1082,6 +1083,26 @@ void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling&
         forced = min(forced, max(1, nkb_max / min_blocks));
         forced = max(1, min(forced, max_splits));
         if (same_len && units * 4 >= 3 * 256) forced = 1;
+        if (tiling.steps && forced >= 1) {
+            // Pages of 4 bits: of the counts that fit the rounds the one with the least time by what was measured:
+            // 1.3 us a block in turn (half of a row's blocks, as selections keep a part), 4 us and 0.15 ns a partial
+            // row (516 bytes written and read) for the merge.  64 queries over 32 + 1 blocks (32 Q / 8 KV heads)
+            // 37.4 us in the 2 splits of the rule above, 24.7 in 8; 256 over 24 + 4 49.5 whole, 33.7 in 5; but 256
+            // over 64 + 4, half kept, 36.2 in 4 and 48.3 in 16.
+            const int cap = min(min(max_splits, max(1, nkb_max / 2)),
+                                max(1, same_len ? 256 / units : static_cast<int>(slots / (double)units + 0.5)));
+            const double n = dense_lists ? nkb_max : 0.5 * nkb_max;
+            const double part_us = 1.5e-4 * s.B * s.Hkv * rows_total;
+            double best = 0.0;
+            forced = 1;
+            for (int c = 1; c <= cap; ++c) {
+                const double us = 1.3 * ceil(n / c) + (c > 1 ? 4.0 + part_us * c : 0.0);
+                if (c == 1 || us < best) {
+                    best = us;
+                    forced = c;
+                }
+            }
+        }
         // ragged batches with that many row tiles: the kernel decides from the selected
         // counts (even counts: one round of unsplit tiles; config 4 at 20 % keep 278-281 vs
         // 293-295 us split, while its dense tables need the split, 2.1 vs 3.2 ms)

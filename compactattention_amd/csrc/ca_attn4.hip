@@ -831,7 +831,11 @@ constexpr int kDraftRows4 = 128;
 
 AttnTiling attn4_tiling(const Shape& s, bool dense) {
     const int rows = s.Lq * s.G;
-    if (!dense || rows > kDraftRows4) return attn_tiling(s, dense, false);
+    if (!dense || rows > kDraftRows4) {
+        AttnTiling t = attn_tiling(s, dense, false);
+        t.steps = true;
+        return t;
+    }
     return AttnTiling{rows <= 16 ? 16 : 32, true, true, 0, 32};
 }
 

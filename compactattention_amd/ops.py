@@ -768,7 +768,9 @@ def attn_fwd(q: torch.Tensor, k: AnyKV, v: AnyKV, table: torch.Tensor, counts: t
     d = make_dims(B, Lq, Hq, num_kv_heads, kv_cap)
     pa = past_array(past_blocks, d.batch)
     # num_splits = 0 hands the choice to the library
-    need = _hip.lib().ca_attn_workspace_size(ctypes.byref(d), pa, int(num_splits))
+    lib = _hip.lib()
+    size = lib.ca_attn_fwd_q4_workspace_size if isinstance(k, KV4) else lib.ca_attn_workspace_size
+    need = size(ctypes.byref(d), pa, int(num_splits))
     if need < 0:
         raise _hip.CaError(int(need), _hip.last_error())
     if need > 0 and (workspace is None or workspace.numel() * workspace.element_size() < need):

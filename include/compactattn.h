@@ -458,8 +458,8 @@ int64_t ca_attn_decode_workspace_size(const ca_dims* dims, const int32_t* kv_len
  * ca_gather_q4: the values of those positions, bf16 [B, Hkv, q_len, 128] contiguous; k_cache and
  * k_out, or v_cache and v_out, may both be NULL.
  * ca_attn_fwd_q4, ca_attn_decode_q4: ca_attn_fwd and ca_attn_decode over such a cache (bf16 queries,
- * fp32 scores and sums, the weights rounded to bf16 for the second product); ca_attn_workspace_size
- * and ca_attn_decode_q4_workspace_size give their workspaces.  Keys that a query does not see change
+ * fp32 scores and sums, the weights rounded to bf16 for the second product); the two
+ * ..._q4_workspace_size functions give the bytes of their workspaces.  Keys that a query does not see change
  * nothing, whatever their pages hold; a query that sees a NaN key gets NaN, one that sees a NaN
  * value gets NaN in that group's dims.  A query that sees no key gets zeros and an lse of -inf.
  */
@@ -475,6 +475,7 @@ int ca_attn_fwd_q4(const ca_dims* dims, const ca_seq_layout* q, const ca_kv4_lay
 int ca_attn_decode_q4(const ca_dims* dims, const ca_seq_layout* q, const ca_kv4_layout* k, const ca_kv4_layout* v,
                       const int32_t* kv_len_host, float scale, const ca_seq_layout* out, float* lse,
                       int32_t num_splits, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t ca_attn_fwd_q4_workspace_size(const ca_dims* dims, const int32_t* past_blocks_host, int32_t num_splits);
 int64_t ca_attn_decode_q4_workspace_size(const ca_dims* dims, const int32_t* kv_len_host, int32_t num_splits);
 
 /*

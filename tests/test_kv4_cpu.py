@@ -124,7 +124,11 @@ def test_attention_arguments_are_checked():
     assert fwd(table=FAKE + 2) == INVALID and fwd(counts=FAKE + 1) == INVALID
     assert fwd(scale=0.0) == INVALID and fwd(scale=math.nan) == INVALID
     assert fwd(splits=17) == INVALID and fwd(splits=-1) == INVALID and fwd(splits=2) == WORKSPACE
-    need = lib.ca_attn_workspace_size(ctypes.byref(_dims()), _ints(0), 2)
+    need = lib.ca_attn_fwd_q4_workspace_size(ctypes.byref(_dims()), _ints(0), 2)
+    assert need == 2 * 2 * 4 * 4 * 129 * 4 + 16
+    assert lib.ca_attn_fwd_q4_workspace_size(ctypes.byref(_dims()), _ints(0), 17) < 0
+    assert lib.ca_attn_decode_q4_workspace_size(ctypes.byref(_dims()), _ints(64), 65) < 0
+    assert lib.ca_attn_decode_q4_workspace_size(ctypes.byref(_dims()), _ints(3), 0) < 0
     assert fwd(splits=2, ws=FAKE, wsb=need - 1) == WORKSPACE and fwd(splits=2, ws=FAKE + 4, wsb=need) == WORKSPACE
     assert decode(dims=dict(q_len=65), lens=(65,)) == INVALID
     assert decode(lens=(3,)) == INVALID and decode(lens=(641,)) == INVALID
@@ -294,3 +298,30 @@ def test_cache_bits_are_checked():
         SeerAttnLlamaChunkedDenseForCausalLM(SeerAttnLlamaConfig(
             vocab_size=64, hidden_size=128, intermediate_size=64, num_hidden_layers=1, num_attention_heads=1,
             num_key_value_heads=1, max_position_embeddings=128, qk_norm=True))
+
+
+@pytest.mark.parametrize("heads,q_len,kv,expect", [
+    ((32, 8), 1, [64], 1), ((32, 8), 1, [1024], 1),  # up to four fours of blocks: whole
+    ((32, 8), 1, [2048], 8), ((32, 8), 1, [8192], 32), ((32, 8), 1, [131072], 32),
+    ((32, 8), 1, [4096] * 16, 2),    # 128 rows: two splits fill one round of 256 items
+    ((32, 8), 1, [1024] * 32, 1),    # as many rows as places
+    ((32, 8), 16, [20011], 16),      # 64 rows: two tiles of 32
+    ((64, 64), 1, [131072] * 8, 1),  # more rows than places
+])
+def test_4bit_decode_split_counts(heads, q_len, kv, expect):
+    """Read back from the workspace that the plan asks for."""
+    d = _dims(batch=len(kv), q_len=q_len, num_q_heads=heads[0], num_kv_heads=heads[1], kv_cap=-(-max(kv) // 64))
+    need = _hip.lib().ca_attn_decode_q4_workspace_size(ctypes.byref(d), _ints(*kv), 0)
+    rows = len(kv) * heads[0] * q_len
+    assert need == (0 if expect == 1 else expect * rows * 129 * 4 + 16)
+
+
+@pytest.mark.parametrize("heads,chunk,past,expect", [
+    ((32, 8), 1024, [1024], 2), ((32, 8), 2048, [512], 1), ((28, 4), 500, [16, 48, 96, 128], 2),
+    ((32, 8), 64, [4], 1), ((32, 8), 256, [24], 5), ((8, 8), 64, [0], 1), ((1, 1), 1, [0], 1),
+])
+def test_4bit_chunk_split_counts(heads, chunk, past, expect):
+    d = _dims(batch=len(past), q_len=chunk, num_q_heads=heads[0], num_kv_heads=heads[1], kv_cap=max(past) + -(-chunk // 64))
+    need = _hip.lib().ca_attn_fwd_q4_workspace_size(ctypes.byref(d), _ints(*past), 0)
+    rows = len(past) * heads[0] * chunk
+    assert need == (0 if expect == 1 else expect * rows * 129 * 4 + 16)
