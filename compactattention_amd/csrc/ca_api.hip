@@ -967,9 +967,8 @@ int ca_norm_rope_qk(const ca_seq_layout* q, const ca_seq_layout* q_out, int32_t 
     if ((rc = check_seq(k_out, "k_out", &ko)) != CA_OK) return rc;
     if (batch < 1 || len < 1 || q_heads < 1 || k_heads < 1)
         return fail(CA_ERR_INVALID, "batch, len and heads must be positive");
-    if (q_heads > 65535 || k_heads > 65535 ||
-        (int64_t)batch * len >= ((int64_t)1 << 31) / ((q_heads + 7) / 8 + (k_heads + 7) / 8))
-        return fail(CA_ERR_LIMIT, "too many heads");
+    if (q_heads > 65535 || k_heads > 65535) return fail(CA_ERR_LIMIT, "too many heads");
+    if (batch > 65535 || len > 1 << 22) return fail(CA_ERR_LIMIT, "batch=%d above 65535 or len=%d above 2^22", batch, len);
     if (q_weight == nullptr || k_weight == nullptr || cos == nullptr || sin == nullptr)
         return fail(CA_ERR_INVALID, "the weights, cos and sin are required");
     if (!aligned16(q_weight) || !aligned16(k_weight) || !aligned16(cos) || !aligned16(sin))

@@ -174,7 +174,9 @@ __global__ __launch_bounds__(256) void rmsnorm_kernel(RmsParams p) {
 
 // Norm and rotation of q's and k's heads.  8 lanes hold a head: lane c the dims 8 c .. 8 c + 7 and
 // 64 + 8 c .. 64 + 8 c + 7, so that a dim and its rotation partner meet in one lane and the sum of
-// squares takes three exchanges.  A wave takes 8 heads of one side (q or k) of one token at a time.
+// squares takes three exchanges.  A workgroup is a token (blockIdx.x) of a request (blockIdx.y), a wave
+// 8 heads of q or of k at a time, so nothing is divided and a wave's side is uniform.  Bound by memory, and
+// below some hundred tokens by the launch.
 struct NormRopeParams {
     RopeSide side[2];
     const uint16_t* w[2];
@@ -182,29 +184,19 @@ struct NormRopeParams {
     const float* cos;     // [L, 128] rows, cs_b further for every request (0: the same rows)
     const float* sin;
     int64_t cs_b;
-    int L;
-    uint32_t units;  // tokens * groups
     float eps;
 };
 
-__global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeParams p) {
-    const uint32_t unit = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (unit >= p.units) return;
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x8_t __attribute__((ext_vector_type(8)));
+
+constexpr int kNormWaves = 8;  // at most
+
+__global__ __launch_bounds__(64 * kNormWaves) void norm_rope_kernel(NormRopeParams p) {
     const int lane = threadIdx.x & 63;
     const int c = lane & 7;
-    const uint32_t bt = unit / p.groups;
-    const int grp = unit - bt * p.groups;
-    const bool second = grp >= p.groups0;
-    const RopeSide& sd = p.side[second ? 1 : 0];
-    const int h = (grp - (second ? p.groups0 : 0)) * 8 + (lane >> 3);
-    const bool live = h < sd.H;
-    const int b = bt / p.L;
-    const int t = bt - b * p.L;
-    const int hc = live ? h : 0;
-    const uint16_t* xr = sd.x + b * sd.xsb + (int64_t)t * sd.xst + (int64_t)hc * sd.xsh + 8 * c;
-    const u16x8_t lo = *reinterpret_cast<const u16x8_t*>(xr), hi = *reinterpret_cast<const u16x8_t*>(xr + 64);
-    const uint16_t* wr = p.w[second ? 1 : 0] + 8 * c;
-    const u16x8_t wl = *reinterpret_cast<const u16x8_t*>(wr), wh = *reinterpret_cast<const u16x8_t*>(wr + 64);
+    const int t = blockIdx.x;
+    const int b = blockIdx.y;
     const int64_t at = b * p.cs_b + (int64_t)t * 128 + 8 * c;
     const float4* cr = reinterpret_cast<const float4*>(p.cos + at);
     const float4* sr = reinterpret_cast<const float4*>(p.sin + at);
@@ -215,28 +207,40 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeParams p) {
         cs[4 * i] = a.x, cs[4 * i + 1] = a.y, cs[4 * i + 2] = a.z, cs[4 * i + 3] = a.w;
         sn[4 * i] = s.x, sn[4 * i + 1] = s.y, sn[4 * i + 2] = s.z, sn[4 * i + 3] = s.w;
     }
-    float ss = 0.0f;
+    for (int grp = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); grp < p.groups; grp += kNormWaves) {
+        const bool second = grp >= p.groups0;
+        const RopeSide& sd = p.side[second ? 1 : 0];
+        const int h = (grp - (second ? p.groups0 : 0)) * 8 + (lane >> 3);
+        const bool live = h < sd.H;
+        const int hc = live ? h : 0;
+        const uint16_t* xr = sd.x + b * sd.xsb + t * sd.xst + hc * sd.xsh + 8 * c;
+        const u16x8_t lo = *reinterpret_cast<const u16x8_t*>(xr), hi = *reinterpret_cast<const u16x8_t*>(xr + 64);
+        const uint16_t* wr = p.w[second ? 1 : 0] + 8 * c;
+        const u16x8_t wl = *reinterpret_cast<const u16x8_t*>(wr), wh = *reinterpret_cast<const u16x8_t*>(wr + 64);
+        float ss = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float a = bf16_to_f32(lo[i]), d = bf16_to_f32(hi[i]);
-        ss = __builtin_fmaf(a, a, ss);
-        ss = __builtin_fmaf(d, d, ss);
+        for (int i = 0; i < 8; ++i) {
+            const float a = bf16_to_f32(lo[i]), d = bf16_to_f32(hi[i]);
+            ss = __builtin_fmaf(a, a, ss);
+            ss = __builtin_fmaf(d, d, ss);
+        }
+#pragma unroll
+        for (int o = 4; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
+        const float rstd = 1.0f / __builtin_sqrtf(ss * (1.0f / 128.0f) + p.eps);
+        f32x8_t ol, oh;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float a = bf16_to_f32(lo[i]) * rstd * bf16_to_f32(wl[i]);
+            const float d = bf16_to_f32(hi[i]) * rstd * bf16_to_f32(wh[i]);
+            ol[i] = a * cs[i] - d * sn[i];
+            oh[i] = d * cs[8 + i] + a * sn[8 + i];
+        }
+        if (live) {
+            uint16_t* yr = sd.y + b * sd.ysb + t * sd.yst + h * sd.ysh + 8 * c;
+            *reinterpret_cast<bf16x8_t*>(yr) = __builtin_convertvector(ol, bf16x8_t);
+            *reinterpret_cast<bf16x8_t*>(yr + 64) = __builtin_convertvector(oh, bf16x8_t);
+        }
     }
-#pragma unroll
-    for (int o = 4; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
-    const float rstd = 1.0f / __builtin_sqrtf(ss * (1.0f / 128.0f) + p.eps);
-    u16x8_t ol, oh;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float a = bf16_to_f32(lo[i]) * rstd * bf16_to_f32(wl[i]);
-        const float d = bf16_to_f32(hi[i]) * rstd * bf16_to_f32(wh[i]);
-        ol[i] = f32_to_bf16(a * cs[i] - d * sn[i]);
-        oh[i] = f32_to_bf16(d * cs[8 + i] + a * sn[8 + i]);
-    }
-    if (!live) return;
-    uint16_t* yr = sd.y + b * sd.ysb + (int64_t)t * sd.yst + (int64_t)h * sd.ysh + 8 * c;
-    *reinterpret_cast<u16x8_t*>(yr) = ol;
-    *reinterpret_cast<u16x8_t*>(yr + 64) = oh;
 }
 
 struct SwigluParams {
@@ -304,10 +308,9 @@ hipError_t launch_norm_rope(const SeqAddr& q, const SeqAddr& q_out, int Hq, cons
     p.cos = cos;
     p.sin = sin;
     p.cs_b = cs_b;
-    p.L = L;
-    p.units = static_cast<uint32_t>((int64_t)B * L * p.groups);
     p.eps = eps;
-    hipLaunchKernelGGL(norm_rope_kernel, dim3((p.units + 3) / 4), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL(norm_rope_kernel, dim3(static_cast<unsigned>(L), static_cast<unsigned>(B)),
+                       dim3(64 * min(p.groups, kNormWaves)), 0, stream, p);
     return hipGetLastError();
 }
 

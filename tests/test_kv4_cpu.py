@@ -172,7 +172,7 @@ def test_norm_rope_arguments_are_checked():
 
     assert call(q=_seq(data=FAKE + 2)) == INVALID and call(k=_seq(st=12)) == INVALID
     assert call(hq=0) == INVALID and call(batch=0) == INVALID and call(length=0) == INVALID
-    assert call(hq=70000) == LIMIT and call(batch=1 << 15, length=1 << 15, hq=64) == LIMIT
+    assert call(hq=70000) == LIMIT and call(batch=1 << 16) == LIMIT and call(length=(1 << 22) + 1) == LIMIT
     assert call(w=None) == INVALID and call(w=FAKE + 2) == INVALID and call(cos=None) == INVALID
     assert call(csb=-4) == INVALID and call(csb=6) == INVALID
     assert call(eps=-1.0) == INVALID and call(eps=math.nan) == INVALID
