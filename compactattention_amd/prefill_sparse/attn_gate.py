@@ -46,6 +46,10 @@ class MultiHeadLinear(nn.Module):
         self.hidden_size = hidden_size
         self.num_head = num_head
         self.weight = nn.Parameter(torch.empty(num_head, in_channel_size, hidden_size, dtype=torch.float32))
+        # weights that nothing loads or draws are the same in every process, and leave torch's generator alone
+        with torch.no_grad():
+            self.weight.copy_(0.02 * torch.randn(self.weight.shape, generator=torch.Generator().manual_seed(0),
+                                                 device="cpu"))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.shape[2] < self.num_head:
