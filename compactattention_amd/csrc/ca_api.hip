@@ -810,26 +810,33 @@ int ca_copy_pages(const ca_page_pool* pools, int32_t n_pools, const int32_t* src
     if (n == 0) return ok();
     if (src_host == nullptr || dst_host == nullptr) return fail(CA_ERR_INVALID, "src_host and dst_host are required");
     if (!aligned4(ids)) return fail(CA_ERR_INVALID, "ids misaligned");
-    for (int i = 0; i < n; ++i)
-        if (src_host[i] < 0 || src_host[i] >= pages || dst_host[i] < 0 || dst_host[i] >= pages)
-            return fail(CA_ERR_INVALID, "copy %d: page %d to page %d outside [0, %lld)", i, src_host[i], dst_host[i], (long long)pages);
     for (int i = 0; i < n_pools; ++i)
-        if ((int64_t)n * addr[i].bytes > (int64_t)1 << 37)  // a launch's workgroups
-            return fail(CA_ERR_LIMIT, "pool %d: more than 2^37 bytes in a call", i);
+        if (n >= ((int64_t)1 << 36) / addr[i].bytes)  // a launch's threads
+            return fail(CA_ERR_LIMIT, "pool %d: 2^36 bytes or more in a call", i);
     // one bit a page: written
     const int64_t words = (pages + 63) / 64;
     uint64_t* written = static_cast<uint64_t*>(std::calloc(static_cast<size_t>(words), sizeof(uint64_t)));
     if (written == nullptr) return fail(CA_ERR_LIMIT, "no host memory to check %lld pages", (long long)pages);
-    auto bit = [](int32_t page) { return uint64_t{1} << (page & 63); };
-    int twice = -1, both = -1;
-    for (int i = 0; i < n && twice < 0; ++i) {
-        uint64_t& w = written[dst_host[i] >> 6];
-        if (w & bit(dst_host[i])) twice = dst_host[i];
-        w |= bit(dst_host[i]);
+    const uint64_t limit = static_cast<uint64_t>(pages <= INT32_MAX ? pages : (int64_t)INT32_MAX + 1);
+    int outside = -1, twice = -1, both = -1;
+    for (int i = 0; i < n; ++i) {
+        const uint32_t d = static_cast<uint32_t>(dst_host[i]), s = static_cast<uint32_t>(src_host[i]);
+        if (d >= limit || s >= limit) {
+            outside = i;
+            break;
+        }
+        const uint64_t bit = uint64_t{1} << (d & 63);
+        if (written[d >> 6] & bit) twice = static_cast<int>(d);
+        written[d >> 6] |= bit;
     }
-    for (int i = 0; i < n && both < 0; ++i)
-        if (written[src_host[i] >> 6] & bit(src_host[i])) both = src_host[i];
+    for (int i = 0; outside < 0 && i < n; ++i) {
+        const uint32_t s = static_cast<uint32_t>(src_host[i]);
+        if ((written[s >> 6] >> (s & 63)) & 1) both = static_cast<int>(s);
+    }
     std::free(written);
+    if (outside >= 0)
+        return fail(CA_ERR_INVALID, "copy %d: page %d to page %d outside [0, %lld)", outside, src_host[outside],
+                    dst_host[outside], (long long)pages);
     if (twice >= 0) return fail(CA_ERR_INVALID, "page %d is written twice", twice);
     if (both >= 0) return fail(CA_ERR_INVALID, "page %d is read and written", both);
     hipError_t e = ca::launch_copy_pages(addr, n_pools, src_host, dst_host, n, ids, static_cast<hipStream_t>(stream));

@@ -128,10 +128,12 @@ __global__ __launch_bounds__(256) void gather4_kernel(Gather4Params p) {
 // ---------------------------------------------------------------------------------------
 // Copies of pages.  The ids of up to kCopyPairs pages travel in the launch's arguments: no upload, nothing
 // to wait for, and a captured graph holds them.  More are read from device memory where the caller has put
-// them there (kById), else copied in several launches.  A thread moves 16-byte units of the launch's pages
-// in order, four at a time, a workgroup 1024 units.
+// them there (kById), else copied in several launches.  A thread moves 16 bytes.  Bound by memory: 9001
+// 4-bit pages (157 MB read and written) of two pools 36.4 us with four such pieces a thread, 30.2 with one and
+// stores past the caches (5.2 TB/s); 2300 bf16 pages (151 MB) 34.9 and 26.1.  Few pages, such as those that a
+// decode step is about to read, are stored to stay in the caches.
 constexpr int kCopyPairs = 448;  // 3.5 KB of the 4 KB of arguments
-constexpr int kCopyUnits = 4;
+constexpr int kCopyThreads = 256;
 
 struct CopyParams {
     PagePool pool[CA_MAX_POOLS];
@@ -143,34 +145,25 @@ struct CopyParams {
 static_assert(sizeof(CopyParams) <= 4096, "the arguments of a launch");
 
 template <bool kById>
-__global__ __launch_bounds__(256) void copy_pages_kernel(CopyParams p) {
+__global__ __launch_bounds__(kCopyThreads) void copy_pages_kernel(CopyParams p) {
     const PagePool pool = p.pool[blockIdx.y];
     const uint32_t units = static_cast<uint32_t>(pool.bytes >> 4);
-    const uint64_t total = (uint64_t)units * p.n;
-    const uint64_t first = (uint64_t)blockIdx.x * (256 * kCopyUnits);
-    if (first >= total) return;  // a pool of smaller pages than the largest
-    const uint32_t pair0 = static_cast<uint32_t>(first / units);
-    const uint32_t off0 = static_cast<uint32_t>(first - (uint64_t)pair0 * units) + threadIdx.x;
-    u32x4p_t v[kCopyUnits];
-    uint8_t* to[kCopyUnits];
-    bool live[kCopyUnits];
-#pragma unroll
-    for (int i = 0; i < kCopyUnits; ++i) {
-        const uint32_t u = off0 + 256 * i;  // from the first unit of page pair0
-        const uint32_t k = u / units;
-        const uint32_t pair = pair0 + k;
-        live[i] = pair < (uint32_t)p.n;
-        if (live[i]) {
-            const int64_t off = (int64_t)(u - k * units) * 16;
-            const int32_t src = kById ? p.ids[pair] : p.src[pair];
-            const int32_t dst = kById ? p.ids[p.n + pair] : p.dst[pair];
-            v[i] = *reinterpret_cast<const u32x4p_t*>(pool.data + src * pool.stride + off);
-            to[i] = pool.data + dst * pool.stride + off;
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < kCopyUnits; ++i)
-        if (live[i]) *reinterpret_cast<u32x4p_t*>(to[i]) = v[i];
+    // the workgroup's first unit (64 bits) by uniform arithmetic, the thread's from there
+    const uint64_t first = (uint64_t)blockIdx.x * kCopyThreads;
+    const uint64_t pair0 = first / units;
+    const uint32_t u = static_cast<uint32_t>(first - pair0 * units) + threadIdx.x;
+    const uint32_t k = u / units;
+    const uint64_t pair = pair0 + k;
+    if (pair >= (uint64_t)p.n) return;
+    const int64_t off = (int64_t)(u - k * units) * 16;
+    const int32_t src = kById ? p.ids[pair] : p.src[pair];
+    const int32_t dst = kById ? p.ids[p.n + pair] : p.dst[pair];
+    const u32x4p_t v = *reinterpret_cast<const u32x4p_t*>(pool.data + src * pool.stride + off);
+    u32x4p_t* to = reinterpret_cast<u32x4p_t*>(pool.data + dst * pool.stride + off);
+    if (kById)
+        __builtin_nontemporal_store(v, to);
+    else
+        *to = v;
 }
 
 Kv4Rows rows_of(int B, int L, int H, const int32_t* start) {
@@ -206,12 +199,12 @@ hipError_t launch_copy_pages(const PagePool* pools, int n_pools, const int32_t* 
     int64_t most = 0;
     for (int i = 0; i < n_pools; ++i) {
         p.pool[i] = pools[i];
-        most = max(most, pools[i].bytes);
+        if (pools[i].bytes > most) most = pools[i].bytes;
     }
     auto launch = [&](auto kernel, int count) {
         p.n = count;
-        const int64_t blocks = ((most >> 4) * count + 256 * kCopyUnits - 1) / (256 * kCopyUnits);
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks), n_pools), dim3(256), 0, stream, p);
+        const int64_t blocks = ((most >> 4) * count + kCopyThreads - 1) / kCopyThreads;
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks), n_pools), dim3(kCopyThreads), 0, stream, p);
         return hipGetLastError();
     };
     p.ids = ids;

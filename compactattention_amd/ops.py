@@ -315,8 +315,8 @@ def _page_ids(name: str, ids) -> np.ndarray:
     return np.ascontiguousarray(a, np.int32)
 
 
-# From this many pages on the ids are uploaded and one launch copies them all: 9001 4-bit pages of two pools 98 us
-# in the 21 launches that carry their ids, 43 us so; the upload takes the host 12 us more than a launch.
+# From this many pages on the ids are uploaded and one launch copies them all: 9001 4-bit pages of two pools 68 us
+# in the 21 launches that carry their ids, 43 us so; the upload takes the host 10 us, a launch 4.
 _COPY_UPLOAD = 4 * 448
 
 

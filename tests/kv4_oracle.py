@@ -23,9 +23,8 @@ def quantise(x: np.ndarray):
     bad = ~np.isfinite(g).all(-1)
     g = np.where(np.isfinite(g), g, 0.0)
     amax = np.abs(g).max(-1)
-    byte = np.full(amax.shape, 2, np.int64)
-    for k in range(2, 252):
-        byte = np.where(amax > 7.0 * 2.0 ** (k - 127), k + 1, byte)
+    m, e = np.frexp(amax)  # amax = m 2^e, m in [1/2, 1): at most 7 * 2^(e - 3) exactly where m <= 7/8
+    byte = np.where(amax == 0.0, 2, np.clip(np.where(m <= 0.875, e - 3, e - 2) + 127, 2, 252))
     y = g / 2.0 ** (byte[..., None].astype(np.float64) - 127)
     d = np.abs(np.abs(y)[..., None] - LEVELS)
     # the nearest level; of two equally near the even code (codes order as levels)

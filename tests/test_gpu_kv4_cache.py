@@ -4,7 +4,6 @@ from __future__ import annotations
 
 import math
 
-import numpy as np
 import pytest
 import torch
 import torch.nn.functional as F
@@ -14,9 +13,9 @@ from compactattention_amd.chunked_prefill import run_chunked_prefill_once, synth
 from compactattention_amd.kv_cache import PagedKVCache
 from compactattention_amd.prefill_sparse.llama import (SeerAttnLlamaChunkedDenseForCausalLM,
                                                        SeerAttnLlamaFlashPrefillCompactAttnForCausalLM)
-from compactattention_amd.prefill_sparse.llama.modeling_llama_common import apply_rotary_pos_emb
 from tests import kv4_oracle as ref
 from tests.test_gpu_model import CHUNK, T, tiny_config
+from tests.test_gpu_pages_norm import _norm_rope64
 
 pytestmark = pytest.mark.gpu
 SCALE = 1.0 / math.sqrt(128)
@@ -186,9 +185,8 @@ def test_four_bits_agree_with_bf16_on_the_same_values(gpu, L, past):
     assert ((a.double() - want).abs() <= tol).all() and ((b.double() - want).abs() <= tol).all()
 
 
-def _logits64(model, ids, bits):
-    """The model's last logits in 64 bits over the whole prompt, dense, with q/k norms where it has them, and K and V
-    as a cache of these bits stores them."""
+def _logits64(model, ids):
+    """The model's last logits in 64 bits over the whole prompt, dense, with the q/k norms where it has them."""
     c = model.config
     sd = {k: v.detach().double().cpu() for k, v in model.state_dict().items()}
     L = ids.shape[1]
@@ -203,8 +201,6 @@ def _logits64(model, ids, bits):
             q, k = rms(q, sd[p + "self_attn.q_norm.weight"]), rms(k, sd[p + "self_attn.k_norm.weight"])
         rot = lambda y: y * cos[None, :, None] + torch.cat([-y[..., 64:], y[..., :64]], -1) * sin[None, :, None]  # noqa: E731
         q, k = rot(q), rot(k)
-        if bits == 4:
-            k, v = (torch.from_numpy(ref.values(*ref.quantise(ref.bf16(y.numpy())))) for y in (k, v))
         G = c.num_key_value_groups
         k, v = k.repeat_interleave(G, 2), v.repeat_interleave(G, 2)
         s = torch.einsum("bqhd,bkhd->bhqk", q, k) * SCALE
@@ -216,40 +212,105 @@ def _logits64(model, ids, bits):
     return rms(h, sd["model.norm.weight"])[:, -1:] @ sd["lm_head.weight"].T
 
 
-@pytest.mark.parametrize("cls,bits,qk_norm", [
-    (SeerAttnLlamaChunkedDenseForCausalLM, 4, False), (SeerAttnLlamaFlashPrefillCompactAttnForCausalLM, 4, True),
-    (SeerAttnLlamaFlashPrefillCompactAttnForCausalLM, 16, True),
-])
-def test_models_on_a_4_bit_cache_and_with_qk_norms(gpu, cls, bits, qk_norm):
-    """Dense chunks, a decode step, a draft that is rejected, another step: each step's logits against 64 bits with the
-    cache's values.  (0.999 and 5 % are what the bf16 models are held to; a key next to a rounding border may fall on
-    the other side of it, a change of one level in one of a thousand keys.)"""
-    print(f"case: model kv4 {cls.__name__} bits={bits} qk_norm={qk_norm}", flush=True)
-    m = cls(tiny_config(seerattn_chunked_prefill_force_dense=True, kv_cache_bits=bits, qk_norm=qk_norm), device=gpu)
+def _build(cls, gpu, **kw):
+    m = cls(tiny_config(**kw), device=gpu)
     m.init_weights(seed=11)
-    if qk_norm:
+    if kw.get("qk_norm"):
+        g = torch.Generator(device=gpu).manual_seed(3)
         with torch.no_grad():
             for layer in m.model.layers:
-                assert (layer.self_attn.q_norm.weight == 1).all()
-                layer.self_attn.q_norm.weight.uniform_(0.5, 1.5)
-                layer.self_attn.k_norm.weight.uniform_(0.5, 1.5)
+                for n in (layer.self_attn.q_norm, layer.self_attn.k_norm):
+                    assert (n.weight == 1).all()
+                    n.weight.uniform_(0.5, 1.5, generator=g)
+    return m
+
+
+def test_model_with_qk_norms(gpu):
+    """Dense chunks, a decode step, a draft that is rejected, another step, on a bf16 cache: each step's logits against
+    64 bits, as near as the models without norms are held to."""
+    print("case: model qk_norm", flush=True)
+    m = _build(SeerAttnLlamaFlashPrefillCompactAttnForCausalLM, gpu, seerattn_chunked_prefill_force_dense=True, qk_norm=True)
     ids = synthetic_prompt(1, T + 2, m.config.vocab_size, 4321, gpu)
     cache = m.new_cache(1, T + 64)
-    assert cache.layer(0).bits == bits
-    logits, _ = run_chunked_prefill_once(m, ids[:, :T], CHUNK, cache)
 
     def near(got, n):
-        want = _logits64(m, ids[:, :n], bits).float()
+        want = _logits64(m, ids[:, :n]).float()
         got = got.float().cpu()
         assert F.cosine_similarity(got.flatten(), want.flatten(), dim=0).item() > 0.999
         assert (got - want).abs().max().item() <= 0.05 * want.abs().max().item()
 
-    near(logits, T)
+    near(run_chunked_prefill_once(m, ids[:, :T], CHUNK, cache)[0], T)
     near(m(ids[:, T:T + 1], cache), T + 1)
     m(torch.flip(ids[:, :17], [1]), cache)
     cache.truncate(T + 1)
     cache.compact()
     near(m(ids[:, T + 1:], cache), T + 2)
+
+
+@pytest.mark.parametrize("cls,qk_norm", [(SeerAttnLlamaChunkedDenseForCausalLM, False),
+                                         (SeerAttnLlamaFlashPrefillCompactAttnForCausalLM, True)])
+def test_models_on_a_4_bit_cache(gpu, cls, qk_norm, monkeypatch):
+    """Every call that a model makes of the operators, against 64 bits on the call's own inputs: what is appended is what
+    the format says, and every layer's attention is that of the values in its cache.  (Logits of the two caches are not
+    compared: a key next to a rounding border falls on either side of it.)"""
+    print(f"case: model kv4 {cls.__name__} qk_norm={qk_norm}", flush=True)
+    m = _build(cls, gpu, seerattn_chunked_prefill_force_dense=True, kv_cache_bits=4, qk_norm=qk_norm)
+    ids = synthetic_prompt(1, T + 2, m.config.vocab_size, 4321, gpu)
+    cache = m.new_cache(1, T + 64)
+    assert cache.layer(0).bits == 4
+    seen = {"append": 0, "chunk": 0, "decode": 0, "norm": 0}
+    real = {n: getattr(ops, n) for n in ("append_q4", "attn_fwd", "attn_decode", "norm_rope_qk")}
+
+    def append(k, v, K, V, start, cap):
+        real["append_q4"](k, v, K, V, start, cap)
+        back = ops.gather_q4(K, V, k.shape[0], k.shape[2], start, k.shape[1])
+        for new, got in zip((k, v), back):
+            assert torch.equal(got.double().cpu(), _stored(new, 4))
+        seen["append"] += 1
+
+    def holder(K):
+        return next(c for c in cache.layers if c.pool.k.data_ptr() == K.tensor.data_ptr())
+
+    def check(out, q, K, length):
+        c = holder(K)
+        c_len, c.length = c.length, length
+        want, tol = _attend(c, q, length)
+        c.length = c_len
+        assert ((out.double() - want).abs() <= tol).all()
+
+    def chunk(q, K, V, table, counts, past, *a, **kw):
+        out = real["attn_fwd"](q, K, V, table, counts, past, *a, **kw)
+        check(out, q, K, 64 * past[0] + q.shape[1])
+        seen["chunk"] += 1
+        return out
+
+    def decode(q, K, V, kv_len, *a, **kw):
+        out = real["attn_decode"](q, K, V, kv_len, *a, **kw)
+        check(out, q, K, kv_len[0])
+        seen["decode"] += 1
+        return out
+
+    def norm(q, k, qw, kw, eps, cos, sin):
+        got = real["norm_rope_qk"](q, k, qw, kw, eps, cos, sin)
+        for x, w, y in ((q, qw, got[0]), (k, kw, got[1])):
+            want, terms = _norm_rope64(x, w, eps, cos, sin)
+            assert ((y.double() - want).abs() <= 1.01 * (75 * 2.0 ** -24 * terms + 2.0 ** -8 * want.abs()) + 2.0 ** -126).all()
+        seen["norm"] += 1
+        return got
+
+    for n, f in (("append_q4", append), ("attn_fwd", chunk), ("attn_decode", decode), ("norm_rope_qk", norm)):
+        monkeypatch.setattr(ops, n, f)
+    logits, _ = run_chunked_prefill_once(m, ids[:, :T], CHUNK, cache)
+    first = m(ids[:, T:T + 1], cache)
+    m(torch.flip(ids[:, :17], [1]), cache)
+    cache.truncate(T + 1)
+    cache.compact()
+    last = m(ids[:, T + 1:], cache)
+    for x in (logits, first, last):
+        assert torch.isfinite(x).all()
+    layers = m.config.num_hidden_layers
+    assert seen == {"append": layers * (T // CHUNK + 3), "chunk": layers * (T // CHUNK), "decode": layers * 3,
+                    "norm": layers * (T // CHUNK + 3) if qk_norm else 0}
 
 
 @pytest.mark.parametrize("cls", [SeerAttnLlamaChunkedDenseForCausalLM, SeerAttnLlamaFlashPrefillCompactAttnForCausalLM])
