@@ -697,7 +697,7 @@ int64_t ca_attn_fwd_q4_workspace_size(const ca_dims* dims, const int32_t* past_b
     ca::PastBlocks pb;
     int max_nkb = 0;
     if (check_dims(dims, past_blocks_host, &s, &pb, &max_nkb) != CA_OK) return -1;
-    if (num_splits == 0) num_splits = ca::attn_pick_splits(s, pb, nullptr, ca::attn4_tiling(s, false));
+    if (num_splits == 0) num_splits = ca::attn_pick_splits(s, pb, nullptr, ca::attn4_tiling(s, pb, nullptr));
     if (num_splits < 1 || num_splits > ca::kMaxPrefillSplits)
         return fail(CA_ERR_INVALID, "num_splits=%d outside [0, %d]", num_splits, ca::kMaxPrefillSplits);
     return ca::attn_workspace_bytes(s, num_splits);
@@ -722,7 +722,7 @@ int ca_attn_fwd_q4(const ca_dims* dims, const ca_seq_layout* q, const ca_kv4_lay
     a.table = table;
     a.table_stride = table_stride;
     a.counts = counts;
-    const int max_splits = num_splits == 0 ? ca::attn_pick_splits(a.s, a.pb, nullptr, ca::attn4_tiling(a.s, false)) : num_splits;
+    const int max_splits = num_splits == 0 ? ca::attn_pick_splits(a.s, a.pb, nullptr, ca::attn4_tiling(a.s, a.pb, nullptr)) : num_splits;
     return attn4(a, ka, va, scale, lse, num_splits, max_splits, ca::kMaxPrefillSplits, workspace, workspace_bytes, stream);
 }
 
@@ -731,7 +731,7 @@ int64_t ca_attn_decode_q4_workspace_size(const ca_dims* dims, const int32_t* kv_
     ca::PastBlocks pb;
     int max_nkb = 0;
     if (check_decode_dims(dims, kv_len_host, &s, &pb, &max_nkb) != CA_OK) return -1;
-    if (num_splits == 0) num_splits = ca::attn_pick_splits(s, pb, kv_len_host, ca::attn4_tiling(s, true));
+    if (num_splits == 0) num_splits = ca::attn_pick_splits(s, pb, kv_len_host, ca::attn4_tiling(s, pb, kv_len_host));
     if (num_splits < 1 || num_splits > ca::kMaxDecodeSplits)
         return fail(CA_ERR_INVALID, "num_splits=%d outside [0, %d]", num_splits, ca::kMaxDecodeSplits);
     return ca::attn_workspace_bytes(s, num_splits);
@@ -749,7 +749,7 @@ int ca_attn_decode_q4(const ca_dims* dims, const ca_seq_layout* q, const ca_kv4_
     if ((rc = check_kv4(k, "k", max_nkb, &ka)) != CA_OK) return rc;
     if ((rc = check_kv4(v, "v", max_nkb, &va)) != CA_OK) return rc;
     a.kv_len = kv_len_host;
-    const int max_splits = num_splits == 0 ? ca::attn_pick_splits(a.s, a.pb, kv_len_host, ca::attn4_tiling(a.s, true)) : num_splits;
+    const int max_splits = num_splits == 0 ? ca::attn_pick_splits(a.s, a.pb, kv_len_host, ca::attn4_tiling(a.s, a.pb, kv_len_host)) : num_splits;
     return attn4(a, ka, va, scale, lse, num_splits, max_splits, ca::kMaxDecodeSplits, workspace, workspace_bytes, stream);
 }
 

@@ -1024,8 +1024,8 @@ bool attn_uses_decode_kernel(const Shape& s, bool dense) {
 }
 
 AttnTiling attn_tiling(const Shape& s, bool dense, bool decode) {
-    if (decode && attn_uses_decode_kernel(s, dense)) return AttnTiling{kDecRows, true, false, 4, 32};
-    return AttnTiling{kBM, false, false, 16, dense ? kMaxDecodeSplits : kMaxPrefillSplits};
+    if (decode && attn_uses_decode_kernel(s, dense)) return AttnTiling{kDecRows, true, false, false, 4, 32};
+    return AttnTiling{kBM, false, false, !dense, 16, dense ? kMaxDecodeSplits : kMaxPrefillSplits};
 }
 
 void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling& tiling, SplitPlan* plan) {
@@ -1047,7 +1047,8 @@ void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling&
     //  - dense decode with more rows runs attn_fwd_kernel with the prefill sizing and up to
     //    64 splits.
     const bool dec = tiling.streams;
-    const bool dense_lists = tiling.max_splits > kMaxPrefillSplits;
+    // blocks of a request as planned for: of lists half, as selections keep a part
+    auto expected = [&](int nb) { return tiling.lists ? (nb + 1) / 2 : nb; };
     plan->may_unsplit = 0;
     const int slots = dec ? 256 : 512;
     const int min_blocks = tiling.min_blocks;
@@ -1085,13 +1086,13 @@ void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling&
         if (same_len && units * 4 >= 3 * 256) forced = 1;
         if (tiling.steps && forced >= 1) {
             // Pages of 4 bits: of the counts that fit the rounds the one with the least time by what was measured:
-            // 1.3 us a block in turn (half of a row's blocks, as selections keep a part), 4 us and 0.15 ns a partial
+            // 1.3 us a block in turn, 4 us and 0.15 ns a partial
             // row (516 bytes written and read) for the merge.  64 queries over 32 + 1 blocks (32 Q / 8 KV heads)
             // 37.4 us in the 2 splits of the rule above, 24.7 in 8; 256 over 24 + 4 49.5 whole, 33.7 in 5; but 256
             // over 64 + 4, half kept, 36.2 in 4 and 48.3 in 16.
             const int cap = min(min(max_splits, max(1, nkb_max / 2)),
                                 max(1, same_len ? 256 / units : static_cast<int>(slots / (double)units + 0.5)));
-            const double n = dense_lists ? nkb_max : 0.5 * nkb_max;
+            const double n = expected(nkb_max);
             const double part_us = 1.5e-4 * s.B * s.Hkv * rows_total;
             double best = 0.0;
             forced = 1;
@@ -1120,12 +1121,12 @@ void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling&
         auto fits = [&](int t) {
             int items = 0;
             for (int b = 0; b < s.B; ++b) {
-                if (splits(nkb[b], t) > max_splits) return false;
-                items += s.Hkv * ntiles * splits(nkb[b], t);
+                if (splits(expected(nkb[b]), t) > max_splits) return false;
+                items += s.Hkv * ntiles * splits(expected(nkb[b]), t);
             }
             return items <= slots;
         };
-        const int whole = (nkb_max + kTurn - 1) / kTurn;
+        const int whole = (expected(nkb_max) + kTurn - 1) / kTurn;
         int lo = 1, hi = whole;  // fits() holds from some count on, or only without splits
         while (lo < hi) {
             const int mid = (lo + hi) / 2;
@@ -1142,7 +1143,7 @@ void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling&
         const int nb = nkb[b];
         int sb = forced;
         if (turns > 0) {
-            sb = max(1, (nb + kTurn * turns - 1) / (kTurn * turns));
+            sb = max(1, (expected(nb) + kTurn * turns - 1) / (kTurn * turns));
         } else if (forced <= 0) {
             sb = static_cast<int>(nb / item_blocks + 0.5);
             sb = min(sb, max(1, nb / min_blocks));
@@ -1171,6 +1172,9 @@ void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling&
     //    be (the host only knows their past lengths); each XCD runs its units longest first.
     bool same_len = true;
     for (int b = 1; b < s.B; ++b) same_len = same_len && nkb[b] == nkb[0];
+    //  - Several row tiles of items that the turns made alike: dealt in order, an eighth to every XCD (a unit's
+    //    tiles share an XCD, and two rows' units in one split each would leave six of them idle).
+    if (tiling.steps && tiling.streams && ntiles > 1 && !(same_len && rows % 8 == 0)) return;
     int nunits = 0;
     for (int r = 0; r < rows; ++r) nunits += plan->s[r / s.Hkv];
     // (a launch that may run unsplit keeps whole rows: each XCD's tiles then fit one round)

@@ -32,8 +32,8 @@ __device__ __forceinline__ u32x4_t decode_row(uint32_t w, float s) {
 }
 
 // ---------------------------------------------------------------------------------------
-// Single tokens and short drafts, the whole cache: kN tiles of 16 packed query rows a workgroup (1 for at
-// most 16 rows, 2 for more, in several workgroups).  Bound by memory for 16 rows: every cached byte is read
+// Single tokens, drafts and small chunks: kN tiles of 16 packed query rows a workgroup (1 for at most 16
+// rows, 2 for more, in several workgroups), over the whole cache or (kTab) the blocks of the per-row lists.  Bound by memory for 16 rows: every cached byte is read
 // once (68 bytes a token of K and of V).  16x16x32 MFMAs, S^T = K Q^T and O^T += V^T P^T, with the packed
 // rows as the N dimension.  Eight waves, each with pages of its own (e0 + w, e0 + w + 8, ...) and its own
 // softmax; their results meet in LDS at the end.
@@ -49,9 +49,10 @@ constexpr int kOStride4 = 132;  // floats per row of a wave's partial O in LDS (
 struct Page4 {
     u32x4_t k[4], v[4], vs;  // by tile of 16 tokens: K, V; V's scale bytes (word: tile)
     uint32_t ks;             // K's scale bytes (byte: tile)
+    int kb;                  // logical block
 };
 
-template <int kN>
+template <int kN, bool kTab>
 __global__ __launch_bounds__(kWaves4 * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn4_decode_kernel(Attn4Params p4) {
     __shared__ __attribute__((aligned(16))) float mo[kWaves4 * 16 * kOStride4];
     __shared__ float ml[kWaves4 * 16 * 2];
@@ -69,17 +70,31 @@ __global__ __launch_bounds__(kWaves4 * 64) __attribute__((amdgpu_waves_per_eu(2)
     const int R = p.rows_total;
     const int qpos0 = p.qpos0[b];
     const int nkb = p.nkb[b];
-    const int chunk = (nkb + nsplit - 1) / nsplit;
-    const int e0 = min(nkb, split * chunk);
-    const int e1 = min(nkb, e0 + chunk);
-    const int e_mask = (qpos0 + 1) >> 6;  // blocks from here on hold keys past query row 0
     const int kv_tokens = qpos0 + s.Lq;
-
     const int tid = threadIdx.x;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l = tid & 63;
     const int n = l & 15;
     const int g = l >> 4;
+    // blocks from here on hold keys past the tile's first query
+    const int mask_from = (qpos0 + (kN == 1 ? 0 : r0 / G) + 1) >> 6;
+    const int32_t* tab = kTab ? p.table + (int64_t)row * p.table_stride : nullptr;
+    int n_vis = nkb;
+    if (kTab) {  // entries up to the last one that the tile can see
+        const int lim = (qpos0 + min(r0 + 16 * kN - 1, R - 1) / G) >> 6;
+        n_vis = 0;
+        for (int end = min(max(sload(p.counts + row), 0), s.cap); end > 0; end -= 64) {
+            const int e = end - 1 - l;
+            const uint64_t seen = __ballot(e >= 0 && max(tab[max(e, 0)], 0) <= lim);
+            if (seen != 0) {
+                n_vis = end - (__ffsll(static_cast<unsigned long long>(seen)) - 1);
+                break;
+            }
+        }
+    }
+    const int chunk = (n_vis + nsplit - 1) / nsplit;
+    const int e0 = min(n_vis, split * chunk);
+    const int e1 = min(n_vis, e0 + chunk);
 
     const int32_t* kpt = p4.k.page_table + (int64_t)row * p4.k.pts;
     const int32_t* vpt = p4.v.page_table + (int64_t)row * p4.v.pts;
@@ -94,8 +109,9 @@ __global__ __launch_bounds__(kWaves4 * 64) __attribute__((amdgpu_waves_per_eu(2)
     auto load_ids = [&](int c) {
         const int e = e0 + w + kWaves4 * (64 * c + l);
         if (e < e1) {
-            kid = static_cast<int>(clamp_page(kpt[e], p4.k.max_page));
-            vid = static_cast<int>(clamp_page(vpt[e], p4.v.max_page));
+            const int kb = kTab ? min(max(tab[e], 0), nkb - 1) : e;
+            kid = static_cast<int>(clamp_page(kpt[kb], p4.k.max_page));
+            vid = static_cast<int>(clamp_page(vpt[kb], p4.v.max_page));
         }
     };
     auto load_page = [&](int i) {
@@ -103,6 +119,8 @@ __global__ __launch_bounds__(kWaves4 * 64) __attribute__((amdgpu_waves_per_eu(2)
         const uint8_t* kp = p4.k.data + (int64_t)__builtin_amdgcn_readlane(kid, i & 63) * p4.k.stride;
         const uint8_t* vp = p4.v.data + (int64_t)__builtin_amdgcn_readlane(vid, i & 63) * p4.v.stride;
         Page4 x;
+        const int e = e0 + w + kWaves4 * i;
+        x.kb = kTab ? min(max(sload(tab + e), 0), nkb - 1) : e;
         x.ks = *reinterpret_cast<const uint32_t*>(kp + ks_off);
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) x.k[kt] = load16(kp + k_off + 1024 * kt);
@@ -143,8 +161,7 @@ __global__ __launch_bounds__(kWaves4 * 64) __attribute__((amdgpu_waves_per_eu(2)
     }
     const bf16x2_t ones = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
 
-    auto compute = [&](Page4& x, int i) {
-        const int kb = e0 + w + kWaves4 * i;
+    auto compute = [&](Page4& x) {
         f32x4_t sc[kN][4];
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
@@ -160,9 +177,9 @@ __global__ __launch_bounds__(kWaves4 * 64) __attribute__((amdgpu_waves_per_eu(2)
             }
         }
         int nan_at = kNoKey;  // the first position with a NaN value in this lane's output dims
-        if (kb >= e_mask) {
+        if (x.kb >= mask_from) {
             // value i of tile kt is key 64 kb + 16 kt + 4 g + i
-            const int first = 64 * kb + 4 * g;
+            const int first = 64 * x.kb + 4 * g;
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
@@ -255,9 +272,9 @@ __global__ __launch_bounds__(kWaves4 * 64) __attribute__((amdgpu_waves_per_eu(2)
 
     for (int i = 0; i < nb_w; i += 2) {
         if (i + 1 < nb_w) xb = load_page(i + 1);
-        compute(xa, i);
+        compute(xa);
         if (i + 2 < nb_w) xa = load_page(i + 2);
-        if (i + 1 < nb_w) compute(xb, i + 1);
+        if (i + 1 < nb_w) compute(xb);
     }
 
     // ---- the eight waves' results through LDS, 16 rows at a time ----
@@ -826,23 +843,31 @@ __global__ __launch_bounds__(128) void attn4_merge_kernel(AttnParams p) {
 
 }  // namespace
 
-// Rows up to which the decode kernel's pairs of tiles are used (measured beside attn4_tiling)
-constexpr int kDraftRows4 = 128;
-
-AttnTiling attn4_tiling(const Shape& s, bool dense) {
+// Which kernel: tiles of 16 or 32 rows whose waves take blocks on their own, or of 256 rows whose waves share
+// them.  A workgroup takes 0.9 us for 32 rows x four blocks and 1.3 us for 256 x one, so the small tiles do
+// less up to 160 rows, and beyond do 1.4 times the work but start and end 6 to 12 us earlier, need no merge
+// where their tiles alone fill the CUs, and waste fewer rows.  They win up to 12 blocks of 256 rows for every
+// CU (all blocks counted; 32 Q / 8 KV heads, small tiles and large): 64 queries over 16 + 1 blocks 15.1, 22.4 us;
+// 256 over 8 + 4 13.7, 28.0; 256 over 64 + 4 (8.5 blocks a CU) 32.5, 46.3; 256 over 256 + 4 (32.5) 96.2, 82.2,
+// with 30 % kept 38.8, 46.0; 512 over 128 + 8 (34) 105.6, 86.2, with 30 % kept 55.0, 50.4.
+AttnTiling attn4_tiling(const Shape& s, const PastBlocks& pb, const int32_t* kv_len) {
+    const bool dense = kv_len != nullptr;
     const int rows = s.Lq * s.G;
-    if (!dense || rows > kDraftRows4) {
-        AttnTiling t = attn_tiling(s, dense, false);
-        t.steps = true;
-        return t;
-    }
-    return AttnTiling{rows <= 16 ? 16 : 32, true, true, 0, 32};
+    int32_t qpos0[CA_MAX_BATCH], nkb[CA_MAX_BATCH];
+    attn_positions(s, pb, kv_len, qpos0, nkb);
+    double blocks = 0.0;  // of 256 rows
+    for (int b = 0; b < s.B; ++b) blocks += (double)s.Hkv * ((rows + kBM - 1) / kBM) * nkb[b];
+    if (rows <= 160 || blocks <= 12.0 * 256)
+        return AttnTiling{dense && rows <= 16 ? 16 : 32, true, true, !dense, 0, dense ? 32 : kMaxPrefillSplits};
+    AttnTiling t = attn_tiling(s, dense, false);
+    t.steps = true;
+    return t;
 }
 
 hipError_t launch_attn4(const AttnArgs& a, const Kv4Addr& k, const Kv4Addr& v, hipStream_t stream) {
     Attn4Params p;
     SplitPlan plan;
-    const AttnTiling tiling = attn4_tiling(a.s, a.kv_len != nullptr);
+    const AttnTiling tiling = attn4_tiling(a.s, a.pb, a.kv_len);
     attn_fill(a, tiling, &p.a, &plan);
     p.a.ws_unsplit = nullptr;  // a launch with splits keeps them
     p.k = k;
@@ -850,11 +875,11 @@ hipError_t launch_attn4(const AttnArgs& a, const Kv4Addr& k, const Kv4Addr& v, h
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(plan.per_xcd * 8), dim3(kNW * 64), 0, stream, p); };
     static_assert(kNW == kWaves4, "one workgroup size");
     if (a.table)
-        launch(attn4_fwd_kernel<true>);
+        tiling.streams ? launch(attn4_decode_kernel<2, true>) : launch(attn4_fwd_kernel<true>);
     else if (tiling.tile_rows == 16)
-        launch(attn4_decode_kernel<1>);
+        launch(attn4_decode_kernel<1, false>);
     else if (tiling.tile_rows == 32)
-        launch(attn4_decode_kernel<2>);
+        launch(attn4_decode_kernel<2, false>);
     else
         launch(attn4_fwd_kernel<false>);
     const hipError_t e = hipGetLastError();

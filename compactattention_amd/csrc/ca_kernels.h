@@ -164,13 +164,14 @@ struct AttnTiling {
     int tile_rows;     // packed rows of a workgroup
     bool streams;      // its waves take blocks on their own (decode kernels)
     bool steps;        // splits chosen by the blocks that a workgroup takes in turn (attn_plan)
+    bool lists;        // block lists of the device's choosing (else every block)
     int min_blocks;    // least blocks of a split
     int max_splits;
 };
 // dense = identity block lists over kv_len tokens (decode); otherwise per-row tables.  decode: whether few
 // rows may take the decode kernel.
 AttnTiling attn_tiling(const Shape& s, bool dense, bool decode = true);
-AttnTiling attn4_tiling(const Shape& s, bool dense);
+AttnTiling attn4_tiling(const Shape& s, const PastBlocks& pb, const int32_t* kv_len);
 void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling& tiling, SplitPlan* plan);
 bool attn_uses_decode_kernel(const Shape& s, bool dense);
 void attn_positions(const Shape& s, const PastBlocks& pb, const int32_t* kv_len, int32_t* qpos0, int32_t* nkb);

@@ -10,7 +10,7 @@ import torch
 
 from compactattention_amd import ops
 from tests import kv4_oracle as ref
-from tests.test_gpu_kv4 import SCALE, _cache, _check, _lists, _tables
+from tests.test_gpu_kv4 import SCALE, _cache, _check, _lists, _poison, _tables
 
 pytestmark = pytest.mark.gpu
 
@@ -142,6 +142,76 @@ def test_chunk_of_2048_over_32768(gpu):
             o, ls, A, S = ref.attention(rows, k, v, kpos, torch.full((2,), 64 * past + t, device=gpu), SCALE)
             assert ((out[0, t, 2 * h:2 * h + 2].double() - o).abs() <= ref.tolerance(o, A, S)).all(), (h, t)
             assert ((lse[0, 2 * h:2 * h + 2, t].double() - ls).abs() <= ref.lse_tolerance(S)).all(), (h, t)
+
+
+# launches of more than 12 blocks of 256 rows for every CU take the kernel with tiles of 256 rows
+LARGE = [
+    # (Hq, Hkv, chunk, past blocks, kept share, splits)
+    (16, 16, 300, [100], 1.0, 0), (16, 16, 300, [100], 0.4, 1), (8, 8, 161, [200, 230], 0.7, 2), (28, 4, 150, [300, 20, 150], 0.8, 0),
+    (24, 6, 400, [130], 1.0, 3), (32, 8, 512, [60, 61], 0.5, 0), (16, 1, 1000, [100], 0.3, 16), (12, 12, 257, [120, 3], 0.05, 4),
+]
+
+
+@pytest.mark.parametrize("Hq,H,L,past,keep,splits", LARGE)
+def test_chunks_in_large_tiles(gpu, Hq, H, L, past, keep, splits):
+    print(f"case: chunk4 large heads={Hq}/{H} chunk={L} past={past} keep={keep} splits={splits}", flush=True)
+    B, qb = len(past), -(-L // 64)
+    cap = max(past) + qb
+    assert H * -(-L * (Hq // H) // 256) * sum(p + qb for p in past) > 12 * 256 and L * (Hq // H) > 160
+    K, V, kt, vt = _big_cache(B * H, cap, gpu, seed=L)
+    q = _q(gpu, B, L, Hq, 128, seed=L)
+    lists = _lists(B, H, past, qb, keep, seed=L)
+    table, counts = _tables(lists, cap, gpu)
+    out, lse = ops.attn_fwd(q, K, V, table, counts, past, SCALE, cap, H, with_lse=True, num_splits=splits)
+    _check(out, lse, q, K, V, kt, vt, H, lists, [64 * p for p in past], [64 * p + L for p in past], every=3)
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+def test_large_tiles_with_odd_lists_and_nan(gpu, splits):
+    """Empty lists, unordered ones, and NaN in hidden and in seen places, in tiles of 256 rows."""
+    print(f"case: chunk4 large odd lists splits={splits}", flush=True)
+    H, Hq, L, past = 16, 16, 300, [100]
+    cap = 105
+    K, V, kt, vt = _big_cache(H, cap, gpu, seed=1)
+    rng = np.random.default_rng(2)
+    own = list(range(100, 105))
+    lists = [[[] if h == 0 else [104] if h == 1 else own + rng.permutation(100)[:40].tolist() if h == 2 else
+              sorted(rng.permutation(100)[:int(rng.integers(1, 100))].tolist()) + own for h in range(H)]]
+    lists[0][3] = [7, 7, 9] + own[::-1]
+    for h in range(H):  # behind the last token, and in a block that no list names
+        for pos in range(6400 + L, 64 * cap):
+            _poison(K, V, kt, vt, h, pos, {"k": range(4), "v": range(4)})
+        free = min(set(range(100)) - set(lists[0][h]))
+        _poison(K, V, kt, vt, h, 64 * free + 3, {"k": range(4), "v": range(4)})
+    q = _q(gpu, 1, L, Hq, 128, seed=3)
+    table, counts = _tables(lists, cap, gpu)
+    args = (q, K, V, table, counts, past, SCALE, cap, H)
+    out, lse = ops.attn_fwd(*args, with_lse=True, num_splits=splits)
+    assert torch.isfinite(out).all() and (out[0, :, 0] == 0).all() and torch.isneginf(lse[0, 0]).all()
+    assert (out[0, :256, 1] == 0).all() and torch.isneginf(lse[0, 1, :256]).all()
+    _check(out, lse, q, K, V, kt, vt, H, lists, [6400], [6400 + L])
+    _poison(K, V, kt, vt, 2, 6400 + 130, {"v": [2]})
+    _poison(K, V, kt, vt, 3, 6400 + 290, {"v": [0], "k": [1]})
+    _poison(K, V, kt, vt, 4, 64 * lists[0][4][0] + 9, {"v": [3]})  # seen by all, in a block that is not masked
+    out, lse = ops.attn_fwd(*args, with_lse=True, num_splits=splits)
+    _check(out, lse, q, K, V, kt, vt, H, lists, [6400], [6400 + L])
+    assert torch.isfinite(out[0, :130, 2]).all() and torch.isnan(out[0, 130:, 2, 64:96]).all()
+    assert torch.isfinite(out[0, :290, 3]).all() and torch.isnan(out[0, 290:, 3]).all()
+    assert torch.isnan(out[0, :, 4, 96:]).all() and torch.isfinite(out[0, :, 4, :96]).all()
+
+
+def test_drafts_in_large_tiles(gpu):
+    """More than 160 packed rows over the whole cache."""
+    print("case: decode4 large tiles", flush=True)
+    B, H, Hq, L = 2, 4, 64, 64
+    lens = [64 * 100 + 5, 64 * 120]
+    K, V, kt, vt = _big_cache(B * H, 120, gpu, seed=4)
+    assert H * 4 * (101 + 120) > 12 * 256
+    q = _q(gpu, B, L, Hq, 128, seed=5)
+    lists = [[list(range(-(-n // 64)))] * H for n in lens]
+    for splits in (0, 1, 5):
+        out, lse = ops.attn_decode(q, K, V, lens, SCALE, 120, H, with_lse=True, num_splits=splits)
+        _check(out, lse, q, K, V, kt, vt, H, lists, [n - L for n in lens], lens)
 
 
 def test_two_streams_at_once(gpu):
