@@ -33,10 +33,13 @@ __device__ __forceinline__ u32x4_t decode_row(uint32_t w, float s) {
 
 // ---------------------------------------------------------------------------------------
 // Single tokens, drafts and small chunks: kN tiles of 16 packed query rows a workgroup (1 for at most 16
-// rows, 2 for more, in several workgroups), over the whole cache or (kTab) the blocks of the per-row lists.  Bound by memory for 16 rows: every cached byte is read
-// once (68 bytes a token of K and of V).  16x16x32 MFMAs, S^T = K Q^T and O^T += V^T P^T, with the packed
-// rows as the N dimension.  Eight waves, each with pages of its own (e0 + w, e0 + w + 8, ...) and its own
-// softmax; their results meet in LDS at the end.
+// rows, 2 for more, in several workgroups), over the whole cache or (kTab) the blocks of the per-row lists.
+// 16x16x32 MFMAs, S^T = K Q^T and O^T += V^T P^T, with the packed rows as the N dimension.  Eight waves, each
+// with pages of its own (e0 + w, e0 + w + 8, ...) and its own softmax; their results meet in LDS at the end.
+// Every cached byte is read once for 16 rows (68 bytes a token of K and of V).  One token over 131072 (8 KV
+// heads, 143 MB) takes 28 us, 5.1 TB/s; 6 us of every launch are its start, a first page's way from memory and
+// the end in LDS, and what follows comes at 6.6 TB/s.  Short lists are bound by the conversions: a page is some
+// 500 vector instructions, 0.8 us for the four SIMDs' pages of a turn.
 //  - The contraction order of a product is free as long as both operands share it, so the page's layout
 //    decides it and nothing crosses lanes: lane (n = l % 16, g = l / 16) has token 16 kt + n's group g
 //    (16 bytes) as its share of K, and takes the dims 32 g + 8 s .. + 7 in step s; the scores then lie
@@ -340,6 +343,8 @@ __global__ __launch_bounds__(kWaves4 * 64) __attribute__((amdgpu_waves_per_eu(2)
 // between the MFMAs of the PV product.  Rings of four K and four V blocks in LDS, K of block j in place
 // j & 3 and V in place (j + 1) & 3; slot j writes K of j + 3 and V of j + 2 (one place for all waves)
 // and loads the codes of the blocks after those.
+// Bound by the matrix cores and their power, as the bf16 kernel: 2048 queries over 34816 dense keys (32 Q / 8 KV
+// heads) 913-950 us where bf16 pages take 876-909, 1.2 PFLOP/s.  A loop without the pipeline took 1095.
 // kTab: block lists come from the per-row table; otherwise they are the identity (drafts).
 constexpr int kPlace4 = 64 * 256;     // K or V rows of one block in LDS
 constexpr int kVRing4 = 4 * kPlace4;  // LDS byte offset of the V ring
@@ -841,6 +846,67 @@ __global__ __launch_bounds__(128) void attn4_merge_kernel(AttnParams p) {
         p.lse[((int64_t)b * s.Hq + hq) * s.Lq + t] = wsum == 0.0f ? kNegInf : (m_use + __log2f(wsum)) * 0.69314718055994531f;
 }
 
+// Merge of few splits of many rows: 16 threads a row, 8 dims each.  Bound by memory (a row of a split is 516
+// bytes, read once): 2 splits of 32768 rows (42 MB) 9.8 us, 12.1 in the bf16 kernels' merge.
+__global__ __launch_bounds__(256) void attn4_merge_rows_kernel(AttnParams p) {
+    const Shape& s = p.s;
+    const int64_t rows_all = (int64_t)s.B * s.Hkv * p.rows_total;
+    const int64_t gid = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (gid >= rows_all) return;
+    const int row = static_cast<int>(gid / p.rows_total);
+    const int r = static_cast<int>(gid - (int64_t)row * p.rows_total);
+    const int b = row / s.Hkv;
+    const int hk = row - b * s.Hkv;
+    const int nsplit = p.sp[b];
+    if (nsplit == 1) return;  // the attention kernel wrote this request's rows
+    const int d = 8 * (threadIdx.x & 15);
+    const float* wo = p.ws_o + gid * 128 + d;
+    constexpr int kAtOnce = 2;
+    f32x4_t o[kAtOnce][2];
+    auto load = [&](int sp0) {
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            if (sp0 + i < nsplit) {
+                const f32x4_t* at = reinterpret_cast<const f32x4_t*>(wo + (int64_t)(sp0 + i) * rows_all * 128);
+                o[i][0] = __builtin_nontemporal_load(at);
+                o[i][1] = __builtin_nontemporal_load(at + 1);
+            }
+        }
+    };
+    load(0);
+    float mx = kNegInf;
+    for (int sp = 0; sp < nsplit; ++sp) mx = fmaxf(mx, p.ws_lse[(int64_t)sp * rows_all + gid]);
+    const float m_use = mx == kNegInf ? 0.0f : mx;
+    f32x4_t acc[2] = {f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}};
+    float wsum = 0.0f;
+    for (int sp0 = 0;;) {
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            if (sp0 + i < nsplit) {
+                const float wt = __builtin_amdgcn_exp2f(p.ws_lse[(int64_t)(sp0 + i) * rows_all + gid] - m_use);
+                wsum += wt;
+                if (wt != 0.0f) {
+                    acc[0] += wt * o[i][0];
+                    acc[1] += wt * o[i][1];
+                }
+            }
+        }
+        sp0 += kAtOnce;
+        if (sp0 >= nsplit) break;
+        load(sp0);
+    }
+    const float inv = wsum == 0.0f ? 0.0f : 1.0f / wsum;  // no key: zeros and -inf; a NaN sum stays
+    const int t = r / s.G;
+    const int hq = hk * s.G + r - t * s.G;
+    uint16_t* op = p.out.data + b * p.out.sb + (int64_t)t * p.out.st + (int64_t)hq * p.out.sh + d;
+    f32x8_t v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = acc[i >> 2][i & 3] * inv;
+    *reinterpret_cast<bf16x8_t*>(op) = __builtin_convertvector(v, bf16x8_t);
+    if (p.lse && d == 0)
+        p.lse[((int64_t)b * s.Hq + hq) * s.Lq + t] = wsum == 0.0f ? kNegInf : (m_use + __log2f(wsum)) * 0.69314718055994531f;
+}
+
 }  // namespace
 
 // Which kernel: tiles of 16 or 32 rows whose waves take blocks on their own, or of 256 rows whose waves share
@@ -885,8 +951,14 @@ hipError_t launch_attn4(const AttnArgs& a, const Kv4Addr& k, const Kv4Addr& v, h
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || plan.max <= 1) return e;
     const int64_t rows_all = (int64_t)a.s.B * a.s.Hkv * p.a.rows_total;
-    if (!tiling.streams || rows_all >= int64_t{1} << 31) return launch_attn_merge(p.a, true, stream);
-    hipLaunchKernelGGL(attn4_merge_kernel, dim3(static_cast<unsigned>(rows_all)), dim3(128), 0, stream, p.a);
+    // By rows and splits, with 128, 16 and (the bf16 kernels' merge) 32 threads a row: 32 splits of 32 rows 4.0,
+    // 22.1 us, 16 of 2048 5.4, 10.8; 2 of 32768 32.9, 10.0, 12.1; 12 of 4800 in a launch of 68.5 us with 32 74.1
+    // with 16.
+    if (rows_all > 4096 && plan.max > 4) return launch_attn_merge(p.a, true, stream);
+    if (rows_all <= 4096)
+        hipLaunchKernelGGL(attn4_merge_kernel, dim3(static_cast<unsigned>(rows_all)), dim3(128), 0, stream, p.a);
+    else
+        hipLaunchKernelGGL(attn4_merge_rows_kernel, dim3(static_cast<unsigned>((rows_all + 15) / 16)), dim3(256), 0, stream, p.a);
     return hipGetLastError();
 }
 
