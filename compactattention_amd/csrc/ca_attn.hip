@@ -1028,7 +1028,8 @@ AttnTiling attn_tiling(const Shape& s, bool dense, bool decode) {
     return AttnTiling{kBM, false, false, !dense, 16, dense ? kMaxDecodeSplits : kMaxPrefillSplits};
 }
 
-void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling& tiling, SplitPlan* plan) {
+// The plan's split counts (its placement: attn_plan).
+static void attn_plan_counts(const Shape& s, const int32_t* nkb, int forced, const AttnTiling& tiling, SplitPlan* plan) {
     // One workgroup is resident per CU (128 KB of LDS).  Without a forced count, the
     // decode kernel splits each request's block list so its work items carry about the
     // same number of blocks as everyone else's (total work / slots); attn_fwd_kernel uses
@@ -1153,6 +1154,11 @@ void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling&
         plan->max = max(plan->max, sb);
         plan->off[b + 1] = plan->off[b] + s.Hkv * ntiles * sb;
     }
+}
+
+void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling& tiling, SplitPlan* plan) {
+    attn_plan_counts(s, nkb, forced, tiling, plan);
+    const int ntiles = (s.Lq * s.G + tiling.tile_rows - 1) / tiling.tile_rows;
     const int rows = s.B * s.Hkv;
     plan->sp0 = plan->s[0];
     plan->placement = kPlaceLinear;
@@ -1281,7 +1287,7 @@ int attn_pick_splits(const Shape& s, const PastBlocks& pb, const int32_t* kv_len
     int32_t qpos0[CA_MAX_BATCH], nkb[CA_MAX_BATCH];
     attn_positions(s, pb, kv_len, qpos0, nkb);
     SplitPlan plan;
-    attn_plan(s, nkb, 0, tiling, &plan);
+    attn_plan_counts(s, nkb, 0, tiling, &plan);
     return plan.max;
 }
 
