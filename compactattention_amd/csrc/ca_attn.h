@@ -172,6 +172,19 @@ __device__ __forceinline__ int32_t sload(const int32_t* p) {
     return *(const_i32_t*)p;
 }
 
+// The pages of the item's first block that another request reads too (requests that share a prefix
+// share its leading blocks at the same places; entries past a request's last block are not read).
+__device__ __forceinline__ bool shares_pages(const AttnParams& p, const Item& it, const int32_t* page_table, int64_t pts) {
+    const int hk = it.row - it.b * p.s.Hkv;
+    const int e0 = it.split * ((p.nkb[it.b] + p.sp[it.b] - 1) / p.sp[it.b]);
+    if (e0 >= p.nkb[it.b]) return false;
+    const int o = threadIdx.x & 63;  // another request (there are at most 64)
+    const bool other = o < p.s.B && o != it.b && p.nkb[o] > e0;
+    const int64_t at = (int64_t)((other ? o : it.b) * p.s.Hkv + hk) * pts + e0;
+    const int id = page_table[at];
+    return __ballot(other && id == sload(page_table + (int64_t)it.row * pts + e0)) != 0;
+}
+
 // Fills a launch's parameters and its plan.
 void attn_fill(const AttnArgs& a, const AttnTiling& tiling, AttnParams* p, SplitPlan* plan);
 // Merges the partial results of a launch whose plan has more than one split.  nan_lse: a row whose

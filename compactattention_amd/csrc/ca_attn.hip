@@ -987,19 +987,6 @@ __device__ __forceinline__ void decode_item(const AttnParams& p, const Item& it,
     }
 }
 
-// The pages of the item's first block that another request reads too (requests that share a prefix
-// share its leading blocks at the same places; entries past a request's last block are not read).
-__device__ __forceinline__ bool shares_pages(const AttnParams& p, const Item& it) {
-    const int hk = it.row - it.b * p.s.Hkv;
-    const int e0 = it.split * ((p.nkb[it.b] + p.sp[it.b] - 1) / p.sp[it.b]);
-    if (e0 >= p.nkb[it.b]) return false;
-    const int o = threadIdx.x & 63;  // another request (there are at most 64)
-    const bool other = o < p.s.B && o != it.b && p.nkb[o] > e0;
-    const int64_t at = (int64_t)((other ? o : it.b) * p.s.Hkv + hk) * p.k.pts + e0;
-    const int id = p.k.page_table[at];
-    return __ballot(other && id == sload(p.k.page_table + (int64_t)it.row * p.k.pts + e0)) != 0;
-}
-
 // How K and V are loaded (launch_attn): to stay in the caches, past them, or past them where no other
 // request reads the item's pages.
 enum { kLoadsKept, kLoadsStreamed, kLoadsStreamedUnshared };
@@ -1011,7 +998,7 @@ __global__ __launch_bounds__(kDecWaves * 64) void attn_decode_kernel(AttnParams 
     it.row = __builtin_amdgcn_readfirstlane(it.row);
     it.b = __builtin_amdgcn_readfirstlane(it.b);
     it.split = __builtin_amdgcn_readfirstlane(it.split);
-    if (kLoads == kLoadsStreamed || (kLoads == kLoadsStreamedUnshared && !shares_pages(p, it)))
+    if (kLoads == kLoadsStreamed || (kLoads == kLoadsStreamedUnshared && !shares_pages(p, it, p.k.page_table, p.k.pts)))
         decode_item<true>(p, it, smem);
     else
         decode_item<false>(p, it, smem);

@@ -55,18 +55,16 @@ struct Page4 {
     int kb;                  // logical block
 };
 
-template <int kN, bool kTab>
-__global__ __launch_bounds__(kWaves4 * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn4_decode_kernel(Attn4Params p4) {
-    __shared__ __attribute__((aligned(16))) float mo[kWaves4 * 16 * kOStride4];
-    __shared__ float ml[kWaves4 * 16 * 2];
+// One work item.  kStream: K and V are loaded with the non-temporal hint.
+template <int kN, bool kTab, bool kStream>
+__device__ __forceinline__ void decode4_item(const Attn4Params& p4, const Item& it, float* mo, float* ml) {
+    constexpr int kCache = kStream ? 2 : 0;  // cache policy of the loads: nt
     const AttnParams& p = p4.a;
-    Item it;
-    if (!find_item(p, kN == 1 ? 1 : p.ntiles, &it)) return;
     const Shape& s = p.s;
-    const int row = __builtin_amdgcn_readfirstlane(it.row);
-    const int b = __builtin_amdgcn_readfirstlane(it.b);
-    const int split = __builtin_amdgcn_readfirstlane(it.split);
-    const int r0 = kN == 1 ? 0 : 16 * kN * __builtin_amdgcn_readfirstlane(it.tile);
+    const int row = it.row;
+    const int b = it.b;
+    const int split = it.split;
+    const int r0 = kN == 1 ? 0 : 16 * kN * it.tile;
     const int hk = row - b * s.Hkv;
     const int nsplit = p.sp[b];
     const int G = s.G;
@@ -128,13 +126,13 @@ __global__ __launch_bounds__(kWaves4 * 64) __attribute__((amdgpu_waves_per_eu(2)
             const_cast<uint8_t*>(p4.v.data) + (int64_t)__builtin_amdgcn_readlane(vid, i & 63) * p4.v.stride, 0, size, 0x00020000);
         Page4 x;
         x.kb = __builtin_amdgcn_readlane(kbid, i & 63);
-        x.ks = __builtin_amdgcn_raw_buffer_load_b32(kr, ks_off, 0, 0);
+        x.ks = __builtin_amdgcn_raw_buffer_load_b32(kr, ks_off, 0, kCache);
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) x.k[kt] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_off + 1024 * kt, 0, 0);
+        for (int kt = 0; kt < 4; ++kt) x.k[kt] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_off + 1024 * kt, 0, kCache);
         __builtin_amdgcn_sched_barrier(0);
-        x.vs = __builtin_amdgcn_raw_buffer_load_b128(vr, vs_off, 0, 0);
+        x.vs = __builtin_amdgcn_raw_buffer_load_b128(vr, vs_off, 0, kCache);
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) x.v[kt] = __builtin_amdgcn_raw_buffer_load_b128(vr, v_off + 1024 * kt, 0, 0);
+        for (int kt = 0; kt < 4; ++kt) x.v[kt] = __builtin_amdgcn_raw_buffer_load_b128(vr, v_off + 1024 * kt, 0, kCache);
         return x;
     };
     load_ids(0);
@@ -339,6 +337,30 @@ __global__ __launch_bounds__(kWaves4 * 64) __attribute__((amdgpu_waves_per_eu(2)
             }
         }
     }
+}
+
+// How K and V are loaded: to stay in the caches (chunks and drafts of several tiles read them again), past them,
+// or past them where no other request reads the item's pages.  Past them is faster even for small caches, as a
+// model's layers take turns in what the last-level cache (256 MB) holds: one token over 4096 tokens, 80 caches
+// in turn, 10.9 us kept, 9.4 past them; one cache again and again 9.1, 9.1; 131072 tokens, 4 caches in turn 33.3,
+// 29.1, 64 requests of 4096 54.8, 49.5.  Slower only for one cache near that size again and again (214 MB 40.9,
+// 43.2).
+enum { kLoadsKept, kLoadsStreamed, kLoadsStreamedUnshared };
+template <int kN, bool kTab, int kLoads>
+__global__ __launch_bounds__(kWaves4 * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn4_decode_kernel(Attn4Params p4) {
+    __shared__ __attribute__((aligned(16))) float mo[kWaves4 * 16 * kOStride4];
+    __shared__ float ml[kWaves4 * 16 * 2];
+    Item it;
+    if (!find_item(p4.a, kN == 1 ? 1 : p4.a.ntiles, &it)) return;
+    it.row = __builtin_amdgcn_readfirstlane(it.row);
+    it.b = __builtin_amdgcn_readfirstlane(it.b);
+    it.split = __builtin_amdgcn_readfirstlane(it.split);
+    it.tile = __builtin_amdgcn_readfirstlane(it.tile);
+    if (kLoads == kLoadsStreamed ||
+        (kLoads == kLoadsStreamedUnshared && !shares_pages(p4.a, it, p4.k.page_table, p4.k.pts)))
+        decode4_item<kN, kTab, true>(p4, it, mo, ml);
+    else
+        decode4_item<kN, kTab, false>(p4, it, mo, ml);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -948,11 +970,12 @@ hipError_t launch_attn4(const AttnArgs& a, const Kv4Addr& k, const Kv4Addr& v, h
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(plan.per_xcd * 8), dim3(kNW * 64), 0, stream, p); };
     static_assert(kNW == kWaves4, "one workgroup size");
     if (a.table)
-        tiling.streams ? launch(attn4_decode_kernel<2, true>) : launch(attn4_fwd_kernel<true>);
+        tiling.streams ? launch(attn4_decode_kernel<2, true, kLoadsKept>) : launch(attn4_fwd_kernel<true>);
     else if (tiling.tile_rows == 16)
-        launch(attn4_decode_kernel<1, false>);
+        a.s.B > 1 ? launch(attn4_decode_kernel<1, false, kLoadsStreamedUnshared>)
+                  : launch(attn4_decode_kernel<1, false, kLoadsStreamed>);
     else if (tiling.tile_rows == 32)
-        launch(attn4_decode_kernel<2, false>);
+        launch(attn4_decode_kernel<2, false, kLoadsKept>);
     else
         launch(attn4_fwd_kernel<false>);
     const hipError_t e = hipGetLastError();

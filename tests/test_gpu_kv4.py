@@ -342,6 +342,31 @@ def test_pages_past_32_bits(gpu):
     _check(out, lse, qc, K, V, kt, kt, 2, lists, [128], [190])
 
 
+def test_requests_that_share_pages_read_the_same(gpu):
+    """Decode of forked requests (the same pages at the same places, then pages of their own, of different lengths)
+    gives bit for bit what the same values on separate pages give: where an item's pages are shared, another copy of
+    its code runs."""
+    print("case: forks", flush=True)
+    B, H, G, blocks = 5, 2, 4, 40
+    lens = [64 * 40, 64 * 40 - 13, 64 * 17 + 1, 5, 64 * 33]
+    first_own = [0, 30, 12, 0, 20]  # request 0's pages up to here (request 3 shares nothing)
+    K, V, kt, vt = _cache(B, H, blocks, gpu, 77)
+    shared = []
+    for kv, own in ((K, kt), (V, vt)):
+        forked = own.clone()
+        for b in range(B):
+            forked[b * H:(b + 1) * H, :first_own[b]] = own[:H, :first_own[b]]
+        shared.append(ops.KV4.paged(kv.tensor, forked.to(gpu)))
+        moved = forked != own
+        ops.copy_pages(kv.tensor, forked[moved], own[moved])
+    torch.manual_seed(5)
+    q = torch.randn((B, 1, H * G, 128), device=gpu, dtype=torch.bfloat16)
+    for splits in (0, 1, 3):
+        a = ops.attn_decode(q, *shared, lens, SCALE, blocks, H, with_lse=True, num_splits=splits)
+        b = ops.attn_decode(q, K, V, lens, SCALE, blocks, H, with_lse=True, num_splits=splits)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 def test_pools_with_a_page_stride(gpu):
     """Pages that are a part of larger records, one pool for K and V."""
     print("case: decode4 strided pages", flush=True)
