@@ -873,7 +873,9 @@ int ca_copy_pages(const ca_page_pool* pools, int32_t n_pools, const int32_t* src
     rc = pages <= 1 << 17 ? check_copies<ByteMap>(src_host, dst_host, n, pages)
                           : check_copies<BitMap>(src_host, dst_host, n, pages);
     if (rc != CA_OK) return rc;
-    hipError_t e = ca::launch_copy_pages(addr, n_pools, src_host, dst_host, n, ids, static_cast<hipStream_t>(stream));
+    hipError_t e = ca::launch_copy_pages(addr, n_pools, src_host, dst_host, n, ids,
+                                         static_cast<uint32_t>(pages <= INT32_MAX ? pages : (int64_t)INT32_MAX + 1),
+                                         static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail(e, "copy_pages launch");
     return ok();
 }

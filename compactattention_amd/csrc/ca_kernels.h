@@ -108,7 +108,7 @@ hipError_t launch_gather4(int B, int L, int H, const int32_t* start, const Kv4Ad
 // pool[dst[i]] = pool[src[i]] for every pool: one launch where ids holds src and dst on the device, or for a
 // few hundred pages, else launches of that many
 hipError_t launch_copy_pages(const PagePool* pools, int n_pools, const int32_t* src, const int32_t* dst, int n,
-                             const int32_t* ids, hipStream_t stream);
+                             const int32_t* ids, uint32_t pages, hipStream_t stream);
 
 struct AttnArgs {
     Shape s;

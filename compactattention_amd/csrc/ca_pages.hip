@@ -138,6 +138,7 @@ constexpr int kCopyThreads = 256;
 struct CopyParams {
     PagePool pool[CA_MAX_POOLS];
     const int32_t* ids;  // kById: n sources, then n destinations
+    uint32_t pages;      // kById: nothing is copied from or to an id that is not below
     int n;
     int32_t src[kCopyPairs];
     int32_t dst[kCopyPairs];
@@ -158,6 +159,7 @@ __global__ __launch_bounds__(kCopyThreads) void copy_pages_kernel(CopyParams p) 
     const int64_t off = (int64_t)(u - k * units) * 16;
     const int32_t src = kById ? p.ids[pair] : p.src[pair];
     const int32_t dst = kById ? p.ids[p.n + pair] : p.dst[pair];
+    if (kById && (static_cast<uint32_t>(src) >= p.pages || static_cast<uint32_t>(dst) >= p.pages)) return;
     const u32x4p_t v = *reinterpret_cast<const u32x4p_t*>(pool.data + src * pool.stride + off);
     u32x4p_t* to = reinterpret_cast<u32x4p_t*>(pool.data + dst * pool.stride + off);
     if (kById)
@@ -194,8 +196,9 @@ hipError_t launch_gather4(int B, int L, int H, const int32_t* start, const Kv4Ad
 }
 
 hipError_t launch_copy_pages(const PagePool* pools, int n_pools, const int32_t* src, const int32_t* dst, int n,
-                             const int32_t* ids, hipStream_t stream) {
+                             const int32_t* ids, uint32_t pages, hipStream_t stream) {
     CopyParams p;
+    p.pages = pages;
     int64_t most = 0;
     for (int i = 0; i < n_pools; ++i) {
         p.pool[i] = pools[i];

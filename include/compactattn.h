@@ -484,7 +484,8 @@ int64_t ca_attn_decode_q4_workspace_size(const ca_dims* dims, const int32_t* kv_
  * no page is written twice and none that is read is written (CA_ERR_INVALID otherwise), so the order
  * of the copies does not matter.  n = 0 does nothing.
  * ids is NULL, or device memory that holds src_host and then dst_host (2 n int32) by the time the
- * launch runs: one launch then copies any n, where the ids of 448 pages go with a launch's arguments.
+ * launch runs (ids outside the pools are passed over): one launch then copies any n, where the ids of 448
+ * pages go with a launch's arguments.
  */
 int ca_copy_pages(const ca_page_pool* pools, int32_t n_pools, const int32_t* src_host, const int32_t* dst_host,
                   int32_t n, const int32_t* ids, void* stream);

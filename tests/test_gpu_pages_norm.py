@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from compactattention_amd import ops
+from compactattention_amd import _hip, ops
 from compactattention_amd._hip import CaError
 
 pytestmark = pytest.mark.gpu
@@ -61,6 +61,25 @@ def test_copy_pages_of_a_strided_pool_and_from_a_graph(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(pool[10:20], pool[:10])
+
+
+def test_copy_pages_passes_over_ids_outside_the_pools(gpu):
+    """Ids in device memory that do not name a page of every pool are bounds-checked by the kernel."""
+    print("case: copy_pages, ids in device memory", flush=True)
+    n, total = 1000, 2100
+    pools = [torch.randint(0, 256, (total + i, 48), dtype=torch.uint8, device=gpu) for i in (0, 9)]
+    src, dst = (np.ascontiguousarray(x, np.int32) for x in _pairs(n, total, 3))
+    want = [p.clone() for p in pools]
+    ids = np.stack([src, dst])
+    ids[0, 5], ids[0, 6], ids[1, 900], ids[1, 901], ids[0, 999] = -1, total, total + 3, -2 ** 31, 2 ** 31 - 1
+    kept = np.array([i for i in range(n) if i not in (5, 6, 900, 901, 999)])
+    for p in want:
+        p[torch.as_tensor(dst[kept], device=gpu, dtype=torch.long)] = p[torch.as_tensor(src[kept], device=gpu, dtype=torch.long)]
+    descs = (_hip.PagePool * 2)(*(_hip.PagePool(p.data_ptr(), 48, 48, p.shape[0]) for p in pools))
+    dev = torch.from_numpy(ids).to(gpu)
+    _hip.check(_hip.lib().ca_copy_pages(descs, 2, src.ctypes.data, dst.ctypes.data, n, dev.data_ptr(), ops._stream()))
+    for got, w in zip(pools, want):
+        assert torch.equal(got, w)
 
 
 def test_copy_pages_past_32_bits(gpu):

@@ -162,6 +162,32 @@ def test_copy_pages_arguments_are_checked():
     assert lib.ca_copy_pages((_hip.PagePool * 1)(pool()), 1, None, _ints(1), 1, None, None) == INVALID
 
 
+@pytest.mark.parametrize("pages", [5000, 1 << 17, (1 << 17) + 1, 1 << 24])
+def test_copies_of_many_pages_are_checked(pages):
+    """The page that is named twice is found wherever it stands, with a byte and with a bit a page."""
+    lib = _hip.lib()
+    pool = (_hip.PagePool * 1)(_hip.PagePool(FAKE, 16, 16, pages))
+    ids = np.random.default_rng(pages).permutation(np.arange(pages - 2, pages - 5000, -1))[:4000].astype(np.int32)
+    ids[7] = pages - 1  # the last page there is
+
+    def copy(src, dst):
+        src, dst = np.ascontiguousarray(src, np.int32), np.ascontiguousarray(dst, np.int32)
+        return lib.ca_copy_pages(pool, 1, src.ctypes.data, dst.ctypes.data, len(src), None, None), _hip.last_error()
+
+    src, dst = ids[:2000], ids[2000:]
+    for at, other in ((1999, 0), (3, 1234), (1234, 1233)):
+        d = dst.copy()
+        d[at] = d[other]
+        assert copy(src, d) == (INVALID, f"page {d[at]} is written twice")
+        d = dst.copy()
+        d[at] = src[other]
+        assert copy(src, d) == (INVALID, f"page {src[other]} is read and written")
+    for bad in (pages, -1):
+        s = src.copy()
+        s[1500] = bad
+        assert copy(s, dst) == (INVALID, f"copy 1500: page {bad} to page {dst[1500]} outside [0, {pages})")
+
+
 def test_norm_rope_arguments_are_checked():
     lib = _hip.lib()
 
