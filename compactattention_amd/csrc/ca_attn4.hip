@@ -37,8 +37,8 @@ __device__ __forceinline__ u32x4_t decode_row(uint32_t w, float s) {
 // 16x16x32 MFMAs, S^T = K Q^T and O^T += V^T P^T, with the packed rows as the N dimension.  Eight waves, each
 // with pages of its own (e0 + w, e0 + w + 8, ...) and its own softmax; their results meet in LDS at the end.
 // Every cached byte is read once for 16 rows (68 bytes a token of K and of V).  One token over 131072 (8 KV
-// heads, 143 MB) takes 26.5 us, 5.4 TB/s; 6 us of every launch are its start, a first page's way from memory and
-// the end in LDS, and what follows comes at 7 TB/s.  Short lists are bound by the conversions: a page is some
+// heads, 143 MB) takes 27 us, 5.3 TB/s; 6 us of every launch are its start, a first page's way from memory and
+// the end in LDS, and what follows comes at 6.8 TB/s.  Short lists are bound by the conversions: a page is some
 // 500 vector instructions, 0.8 us for the four SIMDs' pages of a turn.
 //  - The contraction order of a product is free as long as both operands share it, so the page's layout
 //    decides it and nothing crosses lanes: lane (n = l % 16, g = l / 16) has token 16 kt + n's group g
