@@ -1074,10 +1074,9 @@ static void attn_plan_counts(const Shape& s, const int32_t* nkb, int forced, con
         if (same_len && units * 4 >= 3 * 256) forced = 1;
         if (tiling.steps && forced >= 1) {
             // Pages of 4 bits: of the counts that fit the rounds the one with the least time by what was measured:
-            // 1.3 us a block in turn, 4 us and 0.15 ns a partial
-            // row (516 bytes written and read) for the merge.  64 queries over 32 + 1 blocks (32 Q / 8 KV heads)
-            // 37.4 us in the 2 splits of the rule above, 24.7 in 8; 256 over 24 + 4 49.5 whole, 33.7 in 5; but 256
-            // over 64 + 4, half kept, 36.2 in 4 and 48.3 in 16.
+            // 1.3 us a block in turn, and for the merge 4 us and 0.15 ns a partial row (516 bytes written and read).
+            // 64 queries over 32 + 1 blocks (32 Q / 8 KV heads) 37.4 us in the 2 splits of the rule above, 24.7 in
+            // 8; 256 over 24 + 4 49.5 whole, 33.7 in 5; but 256 over 64 + 4, half kept, 36.2 in 4 and 48.3 in 16.
             const int cap = min(min(max_splits, max(1, nkb_max / 2)),
                                 max(1, same_len ? 256 / units : static_cast<int>(slots / (double)units + 0.5)));
             const double n = expected(nkb_max);

@@ -115,8 +115,8 @@ __device__ __forceinline__ void decode4_item(const Attn4Params& p4, const Item& 
         vid = static_cast<int>(clamp_page(vp, p4.v.max_page));
     };
     // Loads stand outside any branch: behind one, the page in use would wait for those ahead of it too (131072
-    // tokens 30.6 us with the merge, 29.4 so; 32 requests of 1024 12.2, 10.8).  Past the
-    // last page their range is empty and nothing is read.
+    // tokens 30.6 us with the merge, 29.4 so; 32 requests of 1024 12.2, 10.8).  Past the last page their range is
+    // empty and nothing is read.
     auto load_page = [&](int i) {
         if (i > 0 && (i & 63) == 0) load_ids(i >> 6);
         const int size = i < nb_w ? kPage4 : 0;

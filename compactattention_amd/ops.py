@@ -114,15 +114,18 @@ def _on_device(first: torch.Tensor, *others: Optional[torch.Tensor]):
     return _HERE if dev == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
+_INT32_ARRAYS = [ctypes.c_int32 * n for n in range(_hip.MAX_BATCH + 1)]
+
+
 def past_array(past_blocks: Sequence[int], batch: Optional[int] = None):
     """Per-request values (past blocks or kv_len) as the int32 host array the C-ABI reads
     ``batch`` entries of."""
-    vals = [int(x) for x in past_blocks]
+    vals = list(map(int, past_blocks))
     if not 1 <= len(vals) <= _hip.MAX_BATCH:
         raise ValueError(f"batch must be in [1, {_hip.MAX_BATCH}]")
     if batch is not None and len(vals) != batch:
         raise ValueError(f"{len(vals)} per-request values for a batch of {batch}")
-    return (ctypes.c_int32 * len(vals))(*vals)
+    return _INT32_ARRAYS[len(vals)](*vals)
 
 
 def make_dims(batch: int, q_len: int, num_q_heads: int, num_kv_heads: int, kv_cap: int) -> Dims:
@@ -248,8 +251,12 @@ def _attn_launch(name: str, k: AnyKV, v: AnyKV, *tensors: Optional[torch.Tensor]
     return getattr(_hip.lib(), name + "_q4"), guard
 
 
-def _starts(start: Union[int, Sequence[int]], batch: int):
-    return past_array([start] * batch if isinstance(start, (int, np.integer)) else start, batch)
+def _starts(start: Union[int, Sequence[int]], batch: int, length: int):
+    """The first positions of every request's tokens as a host array, and the blocks a row needs for ``length``."""
+    if isinstance(start, (int, np.integer)):
+        start = [start] * batch
+    array = past_array(start, batch)
+    return array, -(-(max(map(int, start)) + length) // BLOCK)
 
 
 def append_q4(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: KV4, v_cache: KV4,
@@ -262,12 +269,12 @@ def append_q4(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: KV4, v_cache: K
         raise ValueError("v_new must have k_new's shape")
     if not isinstance(k_cache, KV4) or not isinstance(v_cache, KV4):
         raise ValueError("append_q4 writes caches held in 4 bits (KV4)")
-    sa = _starts(start, B)
+    sa, blocks = _starts(start, B, L)
     if L == 0:
         return
     kn, vn = seq_layout(k_new, "k_new"), seq_layout(v_new, "v_new")
-    for name, kv in (("k", k_cache), ("v", v_cache)):
-        kv.check_blocks(name, B, Hkv, -(-(max(sa) + L) // BLOCK))
+    k_cache.check_blocks("k", B, Hkv, blocks)
+    v_cache.check_blocks("v", B, Hkv, blocks)
     d = make_dims(B, L, Hkv, Hkv, kv_cap)
     with _on_device(k_new, v_new, k_cache.tensor, v_cache.tensor, k_cache.page_table, v_cache.page_table):
         check(_hip.lib().ca_append_q4(ctypes.byref(d), ctypes.byref(kn), ctypes.byref(vn), ctypes.byref(k_cache.layout),
@@ -283,13 +290,12 @@ def gather_q4(k_cache: Optional[KV4], v_cache: Optional[KV4], batch: int, num_kv
         raise ValueError("gather_q4 reads caches held in 4 bits (KV4)")
     if length < 0:
         raise ValueError(f"length={length} < 0")
-    sa = _starts(start, batch)
+    sa, blocks = _starts(start, batch, length)
     dev = caches[0].tensor.device
     k_out, v_out = (None if kv is None else torch.empty((batch, num_kv_heads, length, HEAD_DIM), dtype=torch.bfloat16,
                                                         device=dev) for kv in (k_cache, v_cache))
     if length == 0:
         return k_out, v_out
-    blocks = -(-(max(sa) + length) // BLOCK)
     for name, kv in (("k", k_cache), ("v", v_cache)):
         if kv is not None:
             kv.check_blocks(name, batch, num_kv_heads, blocks)
