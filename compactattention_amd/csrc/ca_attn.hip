@@ -1050,6 +1050,7 @@ static void attn_plan_counts(const Shape& s, const int32_t* nkb, int forced, con
         nkb_max = max(nkb_max, nkb[b]);
     }
     const double item_blocks = total / slots;
+    int chunk = 0;  // blocks of a split, where the requests have counts of their own
     if (!dec && forced <= 0) {
         // attn_fwd_kernel: one split count for every request.  Splitting in proportion to
         // each request's blocks measured slower on ragged batches (config 4: 380 vs 319 us
@@ -1094,7 +1095,35 @@ static void attn_plan_counts(const Shape& s, const int32_t* nkb, int forced, con
         // ragged batches with that many row tiles: the kernel decides from the selected
         // counts (even counts: one round of unsplit tiles; config 4 at 20 % keep 278-281 vs
         // 293-295 us split, while its dense tables need the split, 2.1 vs 3.2 ms)
-        plan->may_unsplit = !same_len && units * 4 >= 3 * 256 && forced > 1;
+        plan->may_unsplit = !tiling.steps && !same_len && units * 4 >= 3 * 256 && forced > 1;
+        // Pages of 4 bits: where the longest request's items would take a third more than an even share of all
+        // blocks, every request gets splits of about one length instead, as many as fit two rounds, or one round
+        // more than there are tiles (512 queries over 2000 blocks and seven times 10, 32 Q / 8 KV heads, 2733 ->
+        // 1250 us, 30 % kept 882 -> 417; 1024 over 500 and three times 10 715 -> 570; 256 over 5, 20 and 400 155
+        // -> 141).  Nearer to even one count for all is faster (500 over 16 to 128, 28 / 4, 176 against 191).
+        double share = 0.0;
+        for (int b = 0; b < s.B; ++b) share += (double)s.Hkv * ntiles * expected(nkb[b]) / 256;
+        if (tiling.steps && !same_len && expected(nkb_max) > 1.35 * share * forced) {
+            const int most = max(slots, units + 256);
+            auto items = [&](int t) {
+                int n = 0;
+                for (int b = 0; b < s.B; ++b) {
+                    const int sb = (expected(nkb[b]) + t - 1) / t;
+                    if (sb > max_splits) return most + 1;
+                    n += s.Hkv * ntiles * sb;
+                }
+                return n;
+            };
+            int lo = 1, hi = expected(nkb_max);
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                if (items(mid) <= most)
+                    hi = mid;
+                else
+                    lo = mid + 1;
+            }
+            chunk = lo;
+        }
     }
     // Pages of 4 bits: a workgroup takes 0.8 us for four blocks (one on each SIMD) however many CUs work, so
     // the launch takes as long as the most fours of blocks that an item has (turns), and what a merge adds is
@@ -1129,7 +1158,9 @@ static void attn_plan_counts(const Shape& s, const int32_t* nkb, int forced, con
     for (int b = 0; b < s.B; ++b) {
         const int nb = nkb[b];
         int sb = forced;
-        if (turns > 0) {
+        if (chunk > 0) {
+            sb = max(1, (expected(nb) + chunk - 1) / chunk);
+        } else if (turns > 0) {
             sb = max(1, (expected(nb) + kTurn * turns - 1) / (kTurn * turns));
         } else if (forced <= 0) {
             sb = static_cast<int>(nb / item_blocks + 0.5);
@@ -1202,7 +1233,7 @@ void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling&
     int xcd_of[kPlanRows];
     double load[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     int items[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (split_units) {
+    if (split_units && !(tiling.steps && !tiling.streams && units <= 128)) {
         for (int u = 0; u < units; ++u) xcd_of[u] = u % 8;  // request-major unit order
     } else {
         int order[kPlanRows];

@@ -200,6 +200,21 @@ def test_large_tiles_with_odd_lists_and_nan(gpu, splits):
     assert torch.isnan(out[0, :, 4, 96:]).all() and torch.isfinite(out[0, :, 4, :96]).all()
 
 
+@pytest.mark.parametrize("keep", [1.0, 0.4])
+def test_chunks_of_very_unequal_requests(gpu, keep):
+    """Split counts of their own for every request (3 or 4 and 1), units dealt by their blocks."""
+    B, H, Hq, L, past = 3, 8, 32, 300, [3, 420, 17]
+    print(f"case: kv4 chunks of unequal requests keep={keep}", flush=True)
+    qb = -(-L // 64)
+    cap = max(past) + qb
+    K, V, kt, vt = _big_cache(B * H, cap, gpu, seed=21)
+    q = _q(gpu, B, L, Hq, 128, seed=22)
+    lists = _lists(B, H, past, qb, keep, seed=23)
+    table, counts = _tables(lists, cap, gpu)
+    out, lse = ops.attn_fwd(q, K, V, table, counts, past, SCALE, cap, H, with_lse=True)
+    _check(out, lse, q, K, V, kt, vt, H, lists, [64 * p for p in past], [64 * p + L for p in past], every=3)
+
+
 def test_drafts_in_large_tiles(gpu):
     """More than 160 packed rows over the whole cache."""
     print("case: decode4 large tiles", flush=True)

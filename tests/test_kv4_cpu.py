@@ -345,6 +345,8 @@ def test_4bit_decode_split_counts(heads, q_len, kv, expect):
 @pytest.mark.parametrize("heads,chunk,past,expect", [
     ((32, 8), 1024, [1024], 2), ((32, 8), 2048, [512], 1), ((28, 4), 500, [16, 48, 96, 128], 2),
     ((32, 8), 64, [4], 1), ((32, 8), 256, [24], 1), ((32, 8), 256, [256], 8), ((32, 8), 64, [64], 3), ((8, 8), 64, [0], 1), ((1, 1), 1, [0], 1),
+    # one request much longer than the rest: splits of one length, one round more than there are tiles
+    ((32, 8), 512, [2000] + [10] * 7, 5), ((32, 8), 1024, [500, 10, 10, 10], 3), ((32, 8), 256, [5, 20, 400], 14),
 ])
 def test_4bit_chunk_split_counts(heads, chunk, past, expect):
     d = _dims(batch=len(past), q_len=chunk, num_q_heads=heads[0], num_kv_heads=heads[1], kv_cap=max(past) + -(-chunk // 64))
