@@ -215,6 +215,21 @@ def test_chunks_of_very_unequal_requests(gpu, keep):
     _check(out, lse, q, K, V, kt, vt, H, lists, [64 * p for p in past], [64 * p + L for p in past], every=3)
 
 
+def test_one_long_request_among_many(gpu):
+    """480 KV rows whose splits are more than the plan places one by one: whole rows with counts that differ."""
+    B, H, Hq, L = 60, 8, 8, 300
+    past = [300] + [b % 3 for b in range(1, B)]
+    print("case: kv4 one long request among 60", flush=True)
+    qb = -(-L // 64)
+    cap = max(past) + qb
+    K, V, kt, vt = _big_cache(B * H, cap, gpu, seed=31)
+    q = _q(gpu, B, L, Hq, 128, seed=32)
+    lists = _lists(B, H, past, qb, 0.8, seed=33)
+    table, counts = _tables(lists, cap, gpu)
+    out, lse = ops.attn_fwd(q, K, V, table, counts, past, SCALE, cap, H, with_lse=True)
+    _check(out, lse, q, K, V, kt, vt, H, lists, [64 * p for p in past], [64 * p + L for p in past], every=7)
+
+
 def test_drafts_in_large_tiles(gpu):
     """More than 160 packed rows over the whole cache."""
     print("case: decode4 large tiles", flush=True)
