@@ -127,26 +127,30 @@ __global__ __launch_bounds__(256) void gather4_kernel(Gather4Params p) {
 
 // ---------------------------------------------------------------------------------------
 // Copies of pages.  The ids of up to kCopyPairs pages travel in the launch's arguments: no upload, nothing
-// to wait for, and a captured graph holds them.  More are read from device memory where the caller has put
-// them there (kById), else copied in several launches.  A thread moves 16 bytes.  Bound by memory: 9001
+// to wait for, and a captured graph holds them.  (Up to kFewPairs in fewer arguments: a call for 32 pages 9.5 us
+// with 3.8 KB of them, 9.2 so.)  More are read from device memory where the caller has put them there, else copied in
+// several launches.  A thread moves 16 bytes.  Bound by memory: 9001
 // 4-bit pages (157 MB read and written) of two pools 36.4 us with four such pieces a thread, 30.2 with one and
 // stores past the caches (5.2 TB/s); 2300 bf16 pages (151 MB) 34.9 and 26.1.  Few pages, such as those that a
 // decode step is about to read, are stored to stay in the caches.
 constexpr int kCopyPairs = 448;  // 3.5 KB of the 4 KB of arguments
+constexpr int kFewPairs = 64;
 constexpr int kCopyThreads = 256;
 
+template <int kPairs>  // 0: by id
 struct CopyParams {
     PagePool pool[CA_MAX_POOLS];
-    const int32_t* ids;  // kById: n sources, then n destinations
-    uint32_t pages;      // kById: nothing is copied from or to an id that is not below
+    const int32_t* ids;  // by id: n sources, then n destinations
+    uint32_t pages;      // by id: nothing is copied from or to an id that is not below
     int n;
-    int32_t src[kCopyPairs];
-    int32_t dst[kCopyPairs];
+    int32_t src[kPairs > 0 ? kPairs : 1];
+    int32_t dst[kPairs > 0 ? kPairs : 1];
 };
-static_assert(sizeof(CopyParams) <= 4096, "the arguments of a launch");
+static_assert(sizeof(CopyParams<kCopyPairs>) <= 4096, "the arguments of a launch");
 
-template <bool kById>
-__global__ __launch_bounds__(kCopyThreads) void copy_pages_kernel(CopyParams p) {
+template <int kPairs>
+__global__ __launch_bounds__(kCopyThreads) void copy_pages_kernel(CopyParams<kPairs> p) {
+    constexpr bool kById = kPairs == 0;
     const PagePool pool = p.pool[blockIdx.y];
     const uint32_t units = static_cast<uint32_t>(pool.bytes >> 4);
     // the workgroup's first unit (64 bits) by uniform arithmetic, the thread's from there
@@ -197,28 +201,28 @@ hipError_t launch_gather4(int B, int L, int H, const int32_t* start, const Kv4Ad
 
 hipError_t launch_copy_pages(const PagePool* pools, int n_pools, const int32_t* src, const int32_t* dst, int n,
                              const int32_t* ids, uint32_t pages, hipStream_t stream) {
-    CopyParams p;
-    p.pages = pages;
     int64_t most = 0;
-    for (int i = 0; i < n_pools; ++i) {
-        p.pool[i] = pools[i];
+    for (int i = 0; i < n_pools; ++i)
         if (pools[i].bytes > most) most = pools[i].bytes;
-    }
-    auto launch = [&](auto kernel, int count) {
-        p.n = count;
+    auto launch = [&](auto params, auto kernel, int at, int count) {
+        for (int i = 0; i < n_pools; ++i) params.pool[i] = pools[i];
+        params.ids = ids;
+        params.pages = pages;
+        params.n = count;
+        if (sizeof(params.src) > sizeof(int32_t)) {
+            for (int i = 0; i < count; ++i) {
+                params.src[i] = src[at + i];
+                params.dst[i] = dst[at + i];
+            }
+        }
         const int64_t blocks = ((most >> 4) * count + kCopyThreads - 1) / kCopyThreads;
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks), n_pools), dim3(kCopyThreads), 0, stream, p);
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks), n_pools), dim3(kCopyThreads), 0, stream, params);
         return hipGetLastError();
     };
-    p.ids = ids;
-    if (ids != nullptr && n > kCopyPairs) return launch(copy_pages_kernel<true>, n);
+    if (n <= kFewPairs) return launch(CopyParams<kFewPairs>(), copy_pages_kernel<kFewPairs>, 0, n);
+    if (ids != nullptr && n > kCopyPairs) return launch(CopyParams<0>(), copy_pages_kernel<0>, 0, n);
     for (int at = 0; at < n; at += kCopyPairs) {
-        const int count = min(kCopyPairs, n - at);
-        for (int i = 0; i < count; ++i) {
-            p.src[i] = src[at + i];
-            p.dst[i] = dst[at + i];
-        }
-        const hipError_t e = launch(copy_pages_kernel<false>, count);
+        const hipError_t e = launch(CopyParams<kCopyPairs>(), copy_pages_kernel<kCopyPairs>, at, min(kCopyPairs, n - at));
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
