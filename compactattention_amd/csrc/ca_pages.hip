@@ -127,12 +127,12 @@ __global__ __launch_bounds__(256) void gather4_kernel(Gather4Params p) {
 
 // ---------------------------------------------------------------------------------------
 // Copies of pages.  The ids of up to kCopyPairs pages travel in the launch's arguments: no upload, nothing
-// to wait for, and a captured graph holds them.  (Up to kFewPairs in fewer arguments: a call for 32 pages 9.5 us
-// with 3.8 KB of them, 9.2 so.)  More are read from device memory where the caller has put them there, else copied in
-// several launches.  A thread moves 16 bytes.  Bound by memory: 9001
-// 4-bit pages (157 MB read and written) of two pools 36.4 us with four such pieces a thread, 30.2 with one and
-// stores past the caches (5.2 TB/s); 2300 bf16 pages (151 MB) 34.9 and 26.1.  Few pages, such as those that a
-// decode step is about to read, are stored to stay in the caches.
+// to wait for, and a captured graph holds them.  (Up to kFewPairs in fewer arguments: a call for 32 pages 9.5
+// us with 3.8 KB of them, 9.2 so.)  More are read from device memory where the caller has put them there,
+// else copied in several launches.  A thread moves 16 bytes.  Bound by memory: 9001 4-bit pages (157 MB read
+// and written) of two pools 36.4 us with four such pieces a thread, 30.2 with one and stores past the caches
+// (5.2 TB/s); 2300 bf16 pages (151 MB) 34.9 and 26.1.  Few pages, such as those that a decode step is about
+// to read, are stored to stay in the caches.
 constexpr int kCopyPairs = 448;  // 3.5 KB of the 4 KB of arguments
 constexpr int kFewPairs = 64;
 constexpr int kCopyThreads = 256;
