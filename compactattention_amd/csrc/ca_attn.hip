@@ -663,7 +663,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
 // the max and the weights take two loads per thread, then add the partial outputs eight
 // splits at a time with the loads issued together.
 static_assert(kMaxPrefillSplits <= 64 && kMaxDecodeSplits <= 64, "the merge holds two splits per lane");
-// kNan: a row whose sum is NaN keeps it as its lse (else -inf); its output is NaN either way.
+// kNan (pages of 4 bits): a split with a NaN score has a NaN lse, which makes the row's output and lse NaN.  The bf16
+// kernels give such a split an lse of -inf, and it is left out like one without keys.
 template <bool kNan>
 __global__ __launch_bounds__(256) void attn_merge_kernel(AttnParams p) {
     const Shape& s = p.s;
@@ -687,8 +688,9 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(AttnParams p) {
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 32));
     const bool any = mx != -__builtin_inff();
-    const float w0 = any ? __builtin_amdgcn_exp2f(ls0 - mx) : 0.0f;  // 0 for absent or empty splits
-    const float w1 = any ? __builtin_amdgcn_exp2f(ls1 - mx) : 0.0f;
+    if (kNan && !any) mx = 0.0f;  // fmaxf drops NaN: no key at all, or NaN lses alone
+    const float w0 = kNan || any ? __builtin_amdgcn_exp2f(ls0 - mx) : 0.0f;  // 0 for absent or empty splits
+    const float w1 = kNan || any ? __builtin_amdgcn_exp2f(ls1 - mx) : 0.0f;
     float wsum = w0 + w1;
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) wsum += __shfl_xor(wsum, o, 32);
@@ -721,14 +723,15 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(AttnParams p) {
             acc.w += use ? wgt[u] * o[u].w : 0.0f;
         }
     }
-    const float inv = wsum > 0.0f ? 1.0f / wsum : 0.0f;
+    const bool some = kNan ? wsum != 0.0f : wsum > 0.0f;
+    const float inv = some ? 1.0f / wsum : 0.0f;
     const int hq = hk * s.G + g;
     uint16_t* op = p.out.data + b * p.out.sb + (int64_t)t * p.out.st + (int64_t)hq * p.out.sh + 4 * lane;
     f32x4_t o4 = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
     *reinterpret_cast<bf16x4_t*>(op) = __builtin_convertvector(o4, bf16x4_t);
     if (p.lse && lane == 0)
         p.lse[((int64_t)b * s.Hq + hq) * s.Lq + t] =
-            (kNan ? wsum != 0.0f : wsum > 0.0f) ? (mx + __log2f(wsum)) * 0.69314718055994531f : -__builtin_inff();
+            some ? (mx + __log2f(wsum)) * 0.69314718055994531f : -__builtin_inff();
 }
 
 // ---------------------------------------------------------------------------------------

@@ -380,6 +380,8 @@ int ca_dense_table(const ca_dims* dims, const int32_t* past_blocks_host, int32_t
  * the trailing blocks past a query tile's causal edge and applies the causal mask only to
  * the trailing run of blocks that reach past the tile's first query, so an out-of-order
  * row could let a query see later keys.
+ * Scores are taken to be finite: a row with a NaN score gets an lse of -inf, and where splits
+ * are joined a split with a NaN score is left out like one without keys.
  * num_splits >= 1 splits every row's block list that many ways; num_splits = 0 picks one
  * count for the launch (ca_attn_pick_splits) with at least ~16 blocks per split: at most 256
  * work items (row tiles x splits, one per CU) when all requests have one length, 1 when
