@@ -700,7 +700,8 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(AttnParams p) {
         float4 o[8];
         float wgt[8];
         // the partials' loads do not wait for the weights; a split with weight 0 (no keys)
-        // is dropped by a select, so whatever its slot holds never reaches the sum
+        // is dropped by a select, so whatever its slot holds never reaches the sum (kNan: such a
+        // slot holds zeros, or a NaN that is kept)
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const int sp = sp0 + u;
@@ -716,7 +717,7 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(AttnParams p) {
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            const bool use = wgt[u] != 0.0f;
+            const bool use = kNan ? sp0 + u < nsplit : wgt[u] != 0.0f;
             acc.x += use ? wgt[u] * o[u].x : 0.0f;
             acc.y += use ? wgt[u] * o[u].y : 0.0f;
             acc.z += use ? wgt[u] * o[u].z : 0.0f;

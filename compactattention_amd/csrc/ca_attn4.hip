@@ -821,6 +821,9 @@ struct Merge4Params {
     int32_t sp[CA_MAX_BATCH];
 };
 
+// The joins weigh every split, those of weight 0 too: one without keys holds zeros, and a NaN sum stays NaN however
+// little its split weighs, as it does within a split.
+
 // Merge of many splits of few rows: four groups of 32 threads share a row, each a quarter of its splits, so
 // that the partials' loads go out in one or two rounds where 32 threads take them in up to eight.
 __global__ __launch_bounds__(128) void attn4_merge_kernel(Merge4Params p) {
@@ -866,7 +869,7 @@ __global__ __launch_bounds__(128) void attn4_merge_kernel(Merge4Params p) {
             const int sp = sp0 + grp + 4 * i;  // the same in all 32 threads
             const float wa = __shfl(w0, sp & 31, 32), wb = __shfl(w1, sp & 31, 32);
             const float wt = sp >= nsplit ? 0.0f : sp < 32 ? wa : wb;
-            if (wt != 0.0f) acc += wt * o[i];
+            acc += wt * o[i];
         }
         sp0 += 4 * kAtOnce;
         if (sp0 >= nsplit) break;
@@ -925,10 +928,8 @@ __global__ __launch_bounds__(256) void attn4_merge_rows_kernel(Merge4Params p) {
             if (sp0 + i < nsplit) {
                 const float wt = __builtin_amdgcn_exp2f(p.ws_lse[(int64_t)(sp0 + i) * rows_all + gid] - m_use);
                 wsum += wt;
-                if (wt != 0.0f) {
-                    acc[0] += wt * o[i][0];
-                    acc[1] += wt * o[i][1];
-                }
+                acc[0] += wt * o[i][0];
+                acc[1] += wt * o[i][1];
             }
         }
         sp0 += kAtOnce;

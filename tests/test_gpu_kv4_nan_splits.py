@@ -1,5 +1,5 @@
 """NaN in queries, keys and values of a 4-bit cache comes through every way in which splits are joined: few rows, many
-rows of few splits, many rows of many splits."""
+rows of few splits, many rows of many splits, whatever the split that holds it weighs."""
 from __future__ import annotations
 
 import pytest
@@ -55,3 +55,35 @@ def test_tokens_and_drafts(gpu, Hq, H, L, lens, splits):
     assert torch.isnan(out[0, L - 1, G:2 * G]).all() and torch.isfinite(out[0, :L - 1]).all()
     lists = [[list(range(-(-n // 64)))] * H for n in lens]
     _check(out, lse, q, K, V, kt, vt, H, lists, [n - L for n in lens], lens)
+
+
+@pytest.mark.parametrize("Hq,H,L,past,splits", [(8, 8, 1, 12, 3), (16, 2, 300, 100, 2), (16, 2, 300, 100, 6), (8, 2, 64, 100, 7),
+                                                (16, 16, 300, 100, 6)])
+def test_values_in_a_split_of_no_weight(gpu, Hq, H, L, past, splits):
+    """Scores of -181 in the first blocks and 181 in the rest: the first split's weight is 0 in fp32, and a NaN value in
+    it is a NaN sum all the same, as it is without splits."""
+    print(f"case: kv4 nan value of no weight heads={Hq}/{H} q_len={L} past={past} splits={splits}", flush=True)
+    qb = -(-L // 64)
+    cap = past + qb
+    K, V, kt, vt = _big_cache(H, cap, gpu, seed=5)
+    cut = -(-cap // splits)  # the first split's blocks
+    plus, minus = 0x66, 0xEE  # two codes of 4 and of -4, under a scale of 1
+    K.tensor[:, :4096] = plus
+    K.tensor[:, 4096:] = 127
+    low = kt[:, :cut].reshape(-1).long().to(gpu)
+    K.tensor[low, :4096] = minus
+    q = torch.full((1, L, Hq, 128), 4.0, dtype=torch.bfloat16, device=gpu)
+    for h in range(H):
+        _poison(K, V, kt, vt, h, 7, {"v": [h % 4]})
+    n = 64 * past + L
+    lists = [[list(range(cap))] * H]
+    if L == 1:
+        out, lse = ops.attn_decode(q, K, V, [n], SCALE, cap, H, with_lse=True, num_splits=splits)
+    else:
+        table, counts = _tables(lists, cap, gpu)
+        out, lse = ops.attn_fwd(q, K, V, table, counts, [past], SCALE, cap, H, with_lse=True, num_splits=splits)
+    G = Hq // H
+    for h in range(H):
+        o = out[0, :, h * G:(h + 1) * G].unflatten(-1, (4, 32))
+        assert torch.isnan(o[..., h % 4, :]).all() and torch.isfinite(o[..., (h + 1) % 4, :]).all()
+    assert torch.isfinite(lse).all()
