@@ -86,7 +86,7 @@ __device__ __forceinline__ void decode4_item(const Attn4Params& p4, const Item& 
         n_vis = 0;
         for (int end = min(max(sload(p.counts + row), 0), s.cap); end > 0; end -= 64) {
             const int e = end - 1 - l;
-            const uint64_t seen = __ballot(e >= 0 && max(tab[max(e, 0)], 0) <= lim);
+            const uint64_t seen = __ballot(e >= 0 && min(max(tab[max(e, 0)], 0), nkb - 1) <= lim);
             if (seen != 0) {
                 n_vis = end - (__ffsll(static_cast<unsigned long long>(seen)) - 1);
                 break;
@@ -437,7 +437,7 @@ __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) v
     if (kTab) {
         for (int end = min(max(sload(p.counts + row), 0), s.cap); end > 0; end -= 64) {
             const int e = end - 1 - l;
-            const uint64_t seen = __ballot(e >= 0 && max(tab[max(e, 0)], 0) <= lim);
+            const uint64_t seen = __ballot(e >= 0 && min(max(tab[max(e, 0)], 0), nkb - 1) <= lim);
             if (seen != 0) {
                 n_vis = end - (__ffsll(static_cast<unsigned long long>(seen)) - 1);
                 break;

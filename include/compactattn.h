@@ -461,7 +461,8 @@ int64_t ca_attn_decode_workspace_size(const ca_dims* dims, const int32_t* kv_len
  * k_out, or v_cache and v_out, may both be NULL.
  * ca_attn_fwd_q4, ca_attn_decode_q4: ca_attn_fwd and ca_attn_decode over such a cache (bf16 queries,
  * fp32 scores and sums, the weights rounded to bf16 for the second product); the two
- * ..._q4_workspace_size functions give the bytes of their workspaces.  Keys that a query does not see change
+ * ..._q4_workspace_size functions give the bytes of their workspaces.  A block table's entries may
+ * stand in any order, and one outside the request's blocks is its first or last block.  Keys that a query does not see change
  * nothing, whatever their pages hold; a query that sees a NaN key gets NaN, one that sees a NaN
  * value gets NaN in that group's dims.  A query that sees no key gets zeros and an lse of -inf.
  */
