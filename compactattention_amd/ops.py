@@ -125,6 +125,8 @@ def past_array(past_blocks: Sequence[int], batch: Optional[int] = None):
         raise ValueError(f"batch must be in [1, {_hip.MAX_BATCH}]")
     if batch is not None and len(vals) != batch:
         raise ValueError(f"{len(vals)} per-request values for a batch of {batch}")
+    if min(vals) < -(1 << 31) or max(vals) >= 1 << 31:  # a ctypes array would take them modulo 2^32
+        raise ValueError(f"per-request values must fit 32 bits (got {min(vals)} .. {max(vals)})")
     return _INT32_ARRAYS[len(vals)](*vals)
 
 
