@@ -260,7 +260,10 @@ int check_rows4(const ca_dims* d, const int32_t* start, int* blocks) {
         return fail(CA_ERR_INVALID, "q_len=%d and num_kv_heads=%d must be positive", d->q_len, d->num_kv_heads);
     if (d->kv_cap < 1 || (int64_t)d->kv_cap * CA_BLOCK > (int64_t)1 << 30)
         return fail(d->kv_cap < 1 ? CA_ERR_INVALID : CA_ERR_LIMIT, "kv_cap=%d blocks outside [1, 2^24]", d->kv_cap);
-    if ((int64_t)d->batch * d->num_kv_heads > INT32_MAX / d->q_len) return fail(CA_ERR_LIMIT, "too many rows");
+    constexpr int64_t kMostRows = ((int64_t)1 << 28) - 16;  // 16 threads a row, fewer than 2^32 in a launch
+    if ((int64_t)d->batch * d->num_kv_heads > kMostRows / d->q_len)
+        return fail(CA_ERR_LIMIT, "batch=%d x num_kv_heads=%d x q_len=%d are more than %lld rows", d->batch, d->num_kv_heads,
+                    d->q_len, (long long)kMostRows);
     *blocks = 0;
     for (int b = 0; b < d->batch; ++b) {
         const int64_t end = (int64_t)start[b] + d->q_len;

@@ -457,6 +457,7 @@ int64_t ca_attn_decode_workspace_size(const ca_dims* dims, const int32_t* kv_len
  * ca_append_q4: quantises k_new / v_new [B, q_len, Hkv, 128] bf16 (dims.batch, dims.q_len,
  * dims.num_kv_heads; num_q_heads unused) into positions start_host[b] .. start_host[b] + q_len - 1
  * of every request's rows; no other byte of the pages changes.  A page may be named by one row only.
+ * B * Hkv * q_len is at most 2^28 - 16 here and in ca_gather_q4 (CA_ERR_LIMIT).
  * ca_gather_q4: the values of those positions, bf16 [B, Hkv, q_len, 128] contiguous; k_cache and
  * k_out, or v_cache and v_out, may both be NULL.
  * ca_attn_fwd_q4, ca_attn_decode_q4: ca_attn_fwd and ca_attn_decode over such a cache (bf16 queries,

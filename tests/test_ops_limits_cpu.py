@@ -1,9 +1,12 @@
-"""Host arguments beyond what the C interface holds are refused, not taken modulo 2^32."""
+"""Arguments beyond what the C interface or a launch holds are refused before anything is launched."""
 from __future__ import annotations
+
+import ctypes
 
 import pytest
 
-from compactattention_amd import ops
+from compactattention_amd import _hip, ops
+from tests.test_kv4_cpu import FAKE, INVALID, LIMIT, _dims, _ints, _kv4, _seq
 
 
 @pytest.mark.parametrize("value", [1 << 31, (1 << 32) + 5, -(1 << 31) - 1, 1 << 70])
@@ -22,3 +25,16 @@ def test_per_request_values_fit_32_bits(value):
 def test_per_request_values_at_the_edges():
     vals = [-(1 << 31), 0, (1 << 31) - 1]
     assert list(ops.past_array(vals, 3)) == vals
+
+
+@pytest.mark.parametrize("batch,heads,length,code", [
+    (1, 1 << 10, 1 << 18, LIMIT), (64, 1 << 4, 1 << 18, LIMIT), (1, 1, 1 << 28, LIMIT), (1, 1, (1 << 28) - 15, LIMIT),
+    (64, (1 << 31) - 1, (1 << 31) - 1, LIMIT), (1, 1, (1 << 28) - 16, INVALID), (3, 5, 17895696, INVALID),
+])
+def test_rows_of_a_launch(batch, heads, length, code):
+    """16 threads a row: 2^28 rows would be 2^32 threads.  (INVALID: the start, which is looked at after the rows.)"""
+    lib, d, kv, s = _hip.lib(), _dims(batch=batch, q_len=length, num_kv_heads=heads, kv_cap=1 << 24), _kv4(pts=1 << 25), _seq()
+    r = [ctypes.byref(x) for x in (d, s, kv)]
+    start = _ints(*([-1] * batch))
+    assert lib.ca_append_q4(r[0], r[1], r[1], r[2], r[2], start, None) == code
+    assert lib.ca_gather_q4(r[0], r[2], r[2], start, FAKE, FAKE, None) == code
