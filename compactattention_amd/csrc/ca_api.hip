@@ -869,9 +869,11 @@ int ca_copy_pages(const ca_page_pool* pools, int32_t n_pools, const int32_t* src
     if (n == 0) return ok();
     if (src_host == nullptr || dst_host == nullptr) return fail(CA_ERR_INVALID, "src_host and dst_host are required");
     if (!aligned4(ids)) return fail(CA_ERR_INVALID, "ids misaligned");
+    // 16 bytes a thread in workgroups of 256, fewer than 2^32 threads in a launch
+    constexpr int64_t kMostBytes = ((int64_t)1 << 36) - 4096;
     for (int i = 0; i < n_pools; ++i)
-        if (n >= ((int64_t)1 << 36) / addr[i].bytes)  // a launch's threads
-            return fail(CA_ERR_LIMIT, "pool %d: 2^36 bytes or more in a call", i);
+        if (n > kMostBytes / addr[i].bytes)
+            return fail(CA_ERR_LIMIT, "pool %d: more than %lld bytes in a call", i, (long long)kMostBytes);
     // 9001 ids of 18007 pages: bytes 10 us, bits 12 to 22; of a million pages bytes 25 to 35, bits 20
     rc = pages <= 1 << 17 ? check_copies<ByteMap>(src_host, dst_host, n, pages)
                           : check_copies<BitMap>(src_host, dst_host, n, pages);

@@ -3,6 +3,7 @@ from __future__ import annotations
 
 import ctypes
 
+import numpy as np
 import pytest
 
 from compactattention_amd import _hip, ops
@@ -38,3 +39,12 @@ def test_rows_of_a_launch(batch, heads, length, code):
     start = _ints(*([-1] * batch))
     assert lib.ca_append_q4(r[0], r[1], r[1], r[2], r[2], start, None) == code
     assert lib.ca_gather_q4(r[0], r[2], r[2], start, FAKE, FAKE, None) == code
+
+
+@pytest.mark.parametrize("page_bytes,pages,code", [(2048, (1 << 25) - 1, LIMIT), (2048, (1 << 25) - 2, INVALID), (1 << 22, 1 << 14, LIMIT),
+                                                   (1 << 22, (1 << 14) - 1, INVALID)])
+def test_bytes_of_a_copy(page_bytes, pages, code):
+    """16 bytes a thread, rounded up to workgroups of 256.  (INVALID: every id is 0, which is looked at afterwards.)"""
+    pool = (_hip.PagePool * 1)(_hip.PagePool(FAKE, page_bytes, page_bytes, 1 << 26))
+    ids = np.zeros(pages, np.int32)
+    assert _hip.lib().ca_copy_pages(pool, 1, ids.ctypes.data, ids.ctypes.data, pages, None, None) == code
