@@ -9,6 +9,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <numeric>
 #include <string>
 
 #include "../../include/compactattn.h"
@@ -291,6 +292,22 @@ int attn4(ca::AttnArgs& a, const ca::Kv4Addr& k, const ca::Kv4Addr& v, float sca
     hipError_t e = ca::launch_attn4(a, k, v, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail(e, "4-bit attn launch");
     return ok();
+}
+
+// Whether pages of two pools may share memory other than by being the same page (two descriptions of one pool
+// do no harm: the same bytes are written twice).  With g the strides' greatest common divisor, page starts of the two
+// lie any multiple of g apart from their first ones' distance, so pages that fit side by side in g bytes never meet.
+bool pools_overlap(const ca_page_pool& a, const ca_page_pool& b) {
+    const int64_t x = reinterpret_cast<intptr_t>(a.data), y = reinterpret_cast<intptr_t>(b.data);
+    if (x == y && a.page_bytes == b.page_bytes && a.stride_page == b.stride_page) return false;
+    auto behind = [](int64_t at, const ca_page_pool& p) {  // 2^63 at most
+        const int64_t left = INT64_MAX - at - p.page_bytes;
+        return p.num_pages - 1 > left / p.stride_page ? INT64_MAX : at + (p.num_pages - 1) * p.stride_page + p.page_bytes;
+    };
+    if (behind(x, a) <= y || behind(y, b) <= x) return false;
+    const int64_t g = std::gcd(a.stride_page, b.stride_page);
+    const int64_t off = ((y - x) % g + g) % g;  // b's pages start so far behind multiples of g from a's first
+    return off < a.page_bytes || g - off < b.page_bytes;
 }
 
 // Which pages a copy writes.  A byte each is set without reading what is there; a bit each keeps the map of a
@@ -866,6 +883,9 @@ int ca_copy_pages(const ca_page_pool* pools, int32_t n_pools, const int32_t* src
         addr[i] = ca::PagePool{static_cast<uint8_t*>(p.data), p.page_bytes, p.stride_page};
         if (p.num_pages < pages) pages = p.num_pages;
     }
+    for (int i = 1; i < n_pools; ++i)
+        for (int j = 0; j < i; ++j)
+            if (pools_overlap(pools[j], pools[i])) return fail(CA_ERR_INVALID, "pools %d and %d overlap", j, i);
     if (n == 0) return ok();
     if (src_host == nullptr || dst_host == nullptr) return fail(CA_ERR_INVALID, "src_host and dst_host are required");
     if (!aligned4(ids)) return fail(CA_ERR_INVALID, "ids misaligned");

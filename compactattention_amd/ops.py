@@ -331,8 +331,8 @@ _COPY_UPLOAD = 4 * 448
 def copy_pages(pools: Sequence[torch.Tensor], src, dst) -> None:
     """pool[dst[i]] = pool[src[i]] for every pool [num_pages, ...] of any type whose pages are contiguous
     multiples of 16 bytes (bf16 pages, 4-bit pages, summaries by page).  src and dst are host integers
-    (lists, numpy arrays, CPU tensors).  No page is written twice and none that is read is written, else
-    CaError.  Nothing waits: the ids go with the launches, or through pinned memory where there are many
+    (lists, numpy arrays, CPU tensors).  No page is written twice, none that is read is written and pools do
+    not overlap, else CaError.  Nothing waits: the ids go with the launches, or through pinned memory where there are many
     (not while a graph is captured, which keeps the ids itself)."""
     if isinstance(pools, torch.Tensor):
         pools = [pools]

@@ -485,7 +485,8 @@ int64_t ca_attn_decode_q4_workspace_size(const ca_dims* dims, const int32_t* kv_
 /*
  * Copies n pages inside each of n_pools (at most CA_MAX_POOLS) pools: page dst_host[i] becomes page
  * src_host[i].  The ids are host arrays, read before the call returns.  Every id lies in every pool,
- * no page is written twice and none that is read is written (CA_ERR_INVALID otherwise), so the order
+ * no page is written twice and none that is read is written, pools do not overlap but for a pool
+ * that is named twice (CA_ERR_INVALID otherwise), so the order
  * of the copies does not matter.  n = 0 does nothing, more than 2^36 - 4096 bytes of a pool are refused.
  * ids is NULL, or device memory that holds src_host and then dst_host (2 n int32) by the time the
  * launch runs (ids outside the pools are passed over): one launch then copies any n, where the ids of 448

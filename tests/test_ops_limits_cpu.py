@@ -48,3 +48,25 @@ def test_bytes_of_a_copy(page_bytes, pages, code):
     pool = (_hip.PagePool * 1)(_hip.PagePool(FAKE, page_bytes, page_bytes, 1 << 26))
     ids = np.zeros(pages, np.int32)
     assert _hip.lib().ca_copy_pages(pool, 1, ids.ctypes.data, ids.ctypes.data, pages, None, None) == code
+
+
+@pytest.mark.parametrize("a,b,fine", [
+    # (offset, page bytes, stride, pages) twice
+    ((0, 4352, 4352, 100), (435200, 4352, 4352, 100), True), ((0, 4352, 4352, 100), (435184, 4352, 4352, 100), False),
+    ((0, 4352, 4352, 100), (0, 4352, 4352, 100), True),    # one pool, named twice
+    ((0, 4352, 4352, 100), (0, 4352, 4352, 50), True),
+    ((0, 4352, 4352, 100), (4352, 4352, 4352, 100), False),  # the same pages under other ids
+    ((0, 4352, 8704, 100), (4352, 4352, 8704, 100), True),   # K and V in turn
+    ((4352, 4352, 8704, 100), (0, 4352, 8704, 100), True), ((0, 4352, 8704, 100), (4336, 4352, 8704, 100), False),
+    ((0, 4352, 8704, 100), (4368, 4352, 8704, 100), False), ((0, 1024, 4096, 10), (2048, 1024, 8192, 10), True),
+    ((0, 1024, 4096, 10), (8192, 1024, 8192, 10), False), ((0, 1024, 1024, 100), (0, 2048, 2048, 50), False),
+    ((0, 1024, 1024, 1 << 40), (1 << 50, 1024, 1024, 1 << 60), True), ((0, 1024, 1024, 1 << 60), (1 << 50, 1024, 2048, 8), False),
+])
+def test_pools_of_a_copy_do_not_overlap(a, b, fine):
+    """A page of one pool that another pool knows by another id could be read and written in one call."""
+    pools = (_hip.PagePool * 3)(*(_hip.PagePool(FAKE + p[0], *p[1:]) for p in (a, b, (16 - FAKE, 16, 16, 1))))
+    lib = _hip.lib()
+    assert lib.ca_copy_pages(pools, 3, None, None, 0, None, None) == (0 if fine else INVALID)
+    swapped = (_hip.PagePool * 2)(pools[1], pools[0])
+    assert lib.ca_copy_pages(swapped, 2, None, None, 0, None, None) == (0 if fine else INVALID)
+    assert fine or "overlap" in _hip.last_error()
