@@ -1042,6 +1042,7 @@ static void attn_plan_counts(const Shape& s, const int32_t* nkb, int forced, con
     // blocks of a request as planned for: of lists half, as selections keep a part
     auto expected = [&](int nb) { return tiling.lists ? (nb + 1) / 2 : nb; };
     plan->may_unsplit = 0;
+    plan->uneven = 0;
     const int slots = dec ? 256 : 512;
     const int min_blocks = tiling.min_blocks;
     const int max_splits = tiling.max_splits;
@@ -1162,6 +1163,50 @@ static void attn_plan_counts(const Shape& s, const int32_t* nkb, int forced, con
                 lo = mid + 1;
         }
         turns = whole - lo < 4 ? whole : lo;
+        // One round leaves a long request no splits where the others' rows (and tiles) take the CUs' places, though
+        // those end soon.  Then the count that the longest request is cut into is the one that ends first by this
+        // estimate, in turns: an item is its turns and three for its start and end; those longer than half the longest
+        // take whole rounds of an XCD's 32 CUs, dealt in units of a row's tiles; the rest fill them; three for a merge
+        // and what it reads (0.15 ns a partial row); and no less than the reads from memory, 1.7 turns' time for a turn
+        // of pages on every CU.  It has to be a fifth and four turns shorter.  (32 Q / 8 KV heads, one token, 131072
+        // tokens beside 23 requests of 640 57 -> 37 us, beside 31 387 -> 37; four of 31001 in 32 requests 110 -> 80;
+        // drafts of 40 tokens, 131072 beside four of 640 306 -> 121; 40 queries over 700 blocks and five times 10
+        // 211 -> 65.)
+        bool same_len = true;
+        for (int b = 1; b < s.B; ++b) same_len = same_len && nkb[b] == nkb[0];
+        if (!same_len) {
+            double work = 0.0;  // turns of all items
+            for (int b = 0; b < s.B; ++b) work += (double)s.Hkv * ntiles * ((expected(nkb[b]) + kTurn - 1) / kTurn);
+            const double reads = 1.7 * work / (256.0 * ntiles);
+            auto estimate = [&](int t, bool dealt) {
+                int longest = 0;
+                double units = 0.0, large = 0.0, parts = 0.0;  // units: of ntiles items
+                for (int b = 0; b < s.B; ++b) longest = max(longest, min(t, (expected(nkb[b]) + kTurn - 1) / kTurn));
+                for (int b = 0; b < s.B; ++b) {
+                    const int sb = splits(expected(nkb[b]), t);
+                    const int len = (expected(nkb[b]) + kTurn * sb - 1) / (kTurn * sb);
+                    units += (double)s.Hkv * sb;
+                    if (2 * len > longest) large += (double)s.Hkv * sb;
+                    if (sb > 1) parts += (double)s.Hkv * rows_total * sb;
+                }
+                const double filled = (work + 3.0 * units * ntiles) / 256;
+                const double rounds = ceil((dealt ? ceil(large / 8) : large / 8) * ntiles / 32) * (longest + 3);
+                return fmax(fmax(filled, rounds), reads) + (parts > 0.0 ? 3.0 + 1.9e-4 * parts : 0.0);
+            };
+            const double now = estimate(turns, false);
+            if (now > 1.25 * fmax((work + 3.0 * s.B * s.Hkv * ntiles) / 256, reads)) {
+                double best = fmin(0.8 * now, now - 4.0);
+                for (int c = 2; c <= max_splits; c += max(1, c / 3)) {
+                    const int t = max(1, (whole + c - 1) / c);
+                    const double then = t < turns ? estimate(t, true) : now;
+                    if (then < (plan->uneven ? 0.98 : 1.0) * best) {
+                        best = then;
+                        plan->uneven = t;
+                    }
+                }
+                if (plan->uneven) turns = plan->uneven;
+            }
+        }
     }
     plan->max = 1;
     plan->off[0] = 0;
@@ -1208,8 +1253,9 @@ void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling&
     bool same_len = true;
     for (int b = 1; b < s.B; ++b) same_len = same_len && nkb[b] == nkb[0];
     //  - Several row tiles of items that the turns made alike: dealt in order, an eighth to every XCD (a unit's
-    //    tiles share an XCD, and two rows' units in one split each would leave six of them idle).
-    if (tiling.steps && tiling.streams && ntiles > 1 && !(same_len && rows % 8 == 0)) return;
+    //    tiles share an XCD, and two rows' units in one split each would leave six of them idle).  Not where the
+    //    longest request has splits beyond one round: its items are most of the work and lie side by side.
+    if (tiling.steps && tiling.streams && ntiles > 1 && !plan->uneven && !(same_len && rows % 8 == 0)) return;
     int nunits = 0;
     for (int r = 0; r < rows; ++r) nunits += plan->s[r / s.Hkv];
     // (a launch that may run unsplit keeps whole rows: each XCD's tiles then fit one round)

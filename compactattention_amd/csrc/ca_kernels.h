@@ -155,6 +155,7 @@ struct SplitPlan {
     int unit_splits;  // kPlaceRows, kPlaceTable: the splits of every unit, 0 when they differ
     int per_xcd;      // work items per XCD (grid = 8 * per_xcd)
     int may_unsplit;  // the kernel drops the splits when the rows' selected counts are even
+    int uneven;       // pages of 4 bits, small tiles: more than a round of items for a long request's sake
     uint32_t unit[kPlanRows];
     int32_t xoff[9];
 };
