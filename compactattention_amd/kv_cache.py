@@ -167,6 +167,7 @@ class PagedKVCache:
         self.length = 0  # tokens stored per request
         self.kmean_blocks = 0  # leading blocks with a valid kmean
         self.kgate_blocks = 0  # leading blocks with a valid kgate
+        self.kgate_tokens = 0  # tokens that those pooled (the last block's may end inside it); 0: not known
 
     # -- layout ---------------------------------------------------------------------------
     def _summary(self, heads: int) -> torch.Tensor:
@@ -281,7 +282,7 @@ class PagedKVCache:
         if self.kmean is not None:
             self.kmean_blocks = self.past_blocks
         if gate_wk is not None:
-            self.kgate_blocks = -(-self.length // BLOCK)
+            self.set_kgate(self.length)
         return past
 
     def append_with_query_means(self, k_new: torch.Tensor, v_new: torch.Tensor,
@@ -330,6 +331,11 @@ class PagedKVCache:
         keys = self.pool.k[idx.reshape(-1)].view(self.batch, self.num_kv_heads, n, HEAD_DIM).transpose(1, 2)
         ops.cache_fill(keys, None, None, None, [b0] * self.batch, self.cap, self.kmean)
         self.kmean_blocks = upto
+
+    def set_kgate(self, tokens: int) -> None:
+        """The gate-K summaries now pool the first ``tokens`` tokens (a partial last block's counts as valid)."""
+        self.kgate_tokens = int(tokens)
+        self.kgate_blocks = -(-self.kgate_tokens // BLOCK)
 
     def require_kgate(self, past: int) -> None:
         """A selecting chunk at ``past`` blocks needs gate-K summaries for every past block."""
@@ -396,7 +402,8 @@ class PagedKVCache:
     def truncate(self, tokens: int, keep_pages: bool = False) -> None:
         """Forget what every request holds past ``tokens`` tokens (a rejected draft, a shorter prefix); the pages
         behind them go back to the pool.  With keep_pages those that a row owns alone stay mapped, as in
-        ``reset``.  Summaries of a block that is cut are no longer valid."""
+        ``reset``.  Summaries that pooled a token that goes are no longer valid: a rejected draft after a chunk that
+        ended inside a block leaves that block's gate-K summary as it is."""
         if not 0 <= tokens <= self.length:
             raise ValueError(f"cannot truncate to {tokens} tokens: the cache holds {self.length}")
         nb = -(-int(tokens) // BLOCK)
@@ -410,7 +417,9 @@ class PagedKVCache:
             self._upload(nb, self.cap)
         self.length = int(tokens)
         self.kmean_blocks = min(self.kmean_blocks, self.length // BLOCK)
-        self.kgate_blocks = min(self.kgate_blocks, self.length // BLOCK)
+        if not 0 < self.kgate_tokens <= self.length:
+            self.kgate_blocks = min(self.kgate_blocks, self.length // BLOCK)
+            self.kgate_tokens = min(self.kgate_tokens, BLOCK * self.kgate_blocks)
 
     def compact(self, shrink: bool = True) -> int:
         """Move the pages in use to the front of the pool (``ops.copy_pages``) and, with shrink, give the memory
@@ -464,4 +473,4 @@ class PagedKVCache:
             self.page_table.fill_(-1)
         self.length = 0
         self.kmean_blocks = 0
-        self.kgate_blocks = 0
+        self.set_kgate(0)

@@ -142,7 +142,7 @@ class LlamaSeerAttentionChunkedDense(nn.Module):
         self.attn_gate.compress_key_blocks(key_states_nope, out=cache.kgate, first_block=past,
                                            position_embeddings=block_position_embeddings)
         if cache.kgate_blocks == past:  # a gap left by decode-completed blocks stays a gap
-            cache.kgate_blocks = past - (-key_states_nope.shape[1] // BLOCK)  # a partial block's summary counts
+            cache.set_kgate(BLOCK * past + key_states_nope.shape[1])  # a partial block's summary counts
 
     def _select_tables(self, query_states_nope: torch.Tensor, cache, past: int, block_position_embeddings
                        ) -> Tuple[torch.Tensor, torch.Tensor]:
