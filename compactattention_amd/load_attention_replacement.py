@@ -22,6 +22,7 @@ causal mask; the compactattn modules apply causality themselves.
 from __future__ import annotations
 
 import os
+import warnings
 from types import MethodType
 from typing import Optional, Union
 
@@ -180,9 +181,11 @@ def _load_gate_weights(model: nn.Module, model_id: str) -> None:
         raise ValueError(f"gate weights not found at {path} (local files only; there is no hub download)")
     state = torch.load(path, map_location="cpu", weights_only=True)
     missing, unexpected = model.load_state_dict(state, strict=False)
-    del missing
     if unexpected:
         raise ValueError(f"gate weight keys not in the model: {sorted(unexpected)[:4]} ...")
+    gates = sorted(k for k in missing if ".attn_gate." in k)  # (the rest of the model comes from base_model)
+    if gates:
+        warnings.warn(f"{path} lacks {len(gates)} gate weights ({gates[0]} ...): they stay as they were drawn", stacklevel=3)
 
 
 def load_llama_attention_replacement_model(
@@ -206,8 +209,9 @@ def load_llama_attention_replacement_model(
 
     base_model: a transformers LlamaForCausalLM (moved to torch_dtype) or a local model
     directory (``from_pretrained(..., local_files_only=True)``).  model_id: optional local
-    directory or file holding the Seer gate weights (``attn_gate_weights.pth``).  kv_cache_bits: 4 for
-    a KV cache held in 4 bits (a keyword of this build).
+    directory or file holding the Seer gate weights (``attn_gate_weights.pth``); a Seer variant whose
+    gate weights are not all there warns.  kv_cache_bits: 4 for a KV cache held in 4 bits (a keyword of
+    this build).
     """
     from transformers import LlamaForCausalLM
 
@@ -240,8 +244,12 @@ def load_llama_attention_replacement_model(
         _adapt_to_transformers(impl, block_rope)
         layer.self_attn = impl
     model.eval()
-    if variant != "flashprefill_compactattn" and model_id is not None:
-        _load_gate_weights(model, model_id)
+    if variant != "flashprefill_compactattn":
+        if model_id is not None:
+            _load_gate_weights(model, model_id)
+        else:
+            warnings.warn(f"{variant} without gate weights (model_id): its gates select by weights drawn at random, the "
+                          "same in every layer, until others are loaded", stacklevel=2)
     _register_attention_implementation()
     model.config._attn_implementation = ATTN_IMPLEMENTATION
     model.config.seerattn_attention_harness = "replacement"
