@@ -65,8 +65,9 @@ struct Item {
 // Workgroup L runs on XCD L % 8 and is that XCD's (L / 8)-th; false when the XCD has no such
 // item.  Where all units hold the same number of splits the unit's place is computed: equal
 // requests need no table (kPlaceRows, kPlaceSplits), a ragged launch reads one entry.  The units
-// of a ragged launch differ only when a decode has more than kPlanRows splits in all; those are
-// read 64 at a time, one per lane, and found by a prefix sum over their items.
+// of a ragged launch differ where its requests have split counts of their own (decodes, and pages
+// of 4 bits) and all splits are more than kPlanRows, so that units are whole rows; those are read
+// 64 at a time, one per lane, and found by a prefix sum over their items.
 // Every workgroup starts with this, so its latency shows in short launches (decode, from graph
 // replays: a scalar scan over the units, the prefix sum in all ragged launches, this): 5 requests
 // of 254-23110 tokens, 8 / 8 heads 33.6, 34.6, 33.9 us; 4 of 460-42073, 16 / 2 heads 26.1, 26.5,

@@ -1058,7 +1058,8 @@ static void attn_plan_counts(const Shape& s, const int32_t* nkb, int forced, con
     int chunk = 0;     // blocks of a split, where the requests have counts of their own
     // Pages of 4 bits: requests of at most so many blocks, a quarter of the longest one's items, are not split
     // and need no merge (1000 queries over 33, 300 and 2 blocks, 16 Q / 2 KV heads, 30 % kept, 131 -> 112 us;
-    // from half on, 500 over 16 to 128, 28 / 4, 174 -> 183: fewer units balance the XCDs less).
+    // from half on, 500 over 16 to 128, 28 / 4, 174 -> 183: fewer units balance the XCDs less).  Of 100 drawn launches
+    // 16 are slower without, by 6 % on the average, none faster.
     int whole_if = 0;
     if (!dec && forced <= 0) {
         // attn_fwd_kernel: one split count for every request.  Splitting in proportion to
@@ -1084,7 +1085,8 @@ static void attn_plan_counts(const Shape& s, const int32_t* nkb, int forced, con
         if (same_len && units * 4 >= 3 * 256) forced = 1;
         if (tiling.steps && forced >= 1) {
             // Pages of 4 bits: of the counts that fit the rounds the one with the least time by what was measured:
-            // 1.3 us a block in turn, and for the merge 4 us and 0.15 ns a partial row (516 bytes written and read).
+            // 1.3 us a block in turn (in short lists; long ones take up to 2 us a block at the clock that the power
+            // limit sets), and for the merge 4 us and 0.15 ns a partial row (516 bytes written and read).
             // 64 queries over 32 + 1 blocks (32 Q / 8 KV heads) 37.4 us in the 2 splits of the rule above, 24.7 in
             // 8; 256 over 24 + 4 49.5 whole, 33.7 in 5; but 256 over 64 + 4, half kept, 36.2 in 4 and 48.3 in 16.
             const int cap = min(min(max_splits, max(1, nkb_max / 2)),
@@ -1109,7 +1111,9 @@ static void attn_plan_counts(const Shape& s, const int32_t* nkb, int forced, con
         // blocks, every request gets splits of about one length instead, as many as fit two rounds, or one round
         // more than there are tiles (512 queries over 2000 blocks and seven times 10, 32 Q / 8 KV heads, 2733 ->
         // 1250 us, 30 % kept 882 -> 417; 1024 over 500 and three times 10 715 -> 570; 256 over 5, 20 and 400 155
-        // -> 141).  Nearer to even one count for all is faster (500 over 16 to 128, 28 / 4, 176 against 191).
+        // -> 141).  Nearer to even one count for all is faster (500 over 16 to 128, 28 / 4, 176 against 191).  In 100
+        // drawn launches without this rule 31 are slower, to 1.8 times, and 12 faster, to 0.7 times (7 % in the mean);
+        // from an even share on 30 slower and 2 faster (2 %), from 1.8 even shares on 15 and 9 (none in the mean).
         double share = 0.0;
         for (int b = 0; b < s.B; ++b) share += (double)s.Hkv * ntiles * expected(nkb[b]) / 256;
         if (tiling.steps && !same_len && expected(nkb_max) > 1.35 * share * forced) {
@@ -1250,6 +1254,10 @@ void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling&
     //    splits, dealt round-robin over the XCDs request by request, so every XCD gets an
     //    equal share of every request's work whatever the rows' selected counts turn out to
     //    be (the host only knows their past lengths); each XCD runs its units longest first.
+    //    Chunks over pages of 4 bits have few units there, as their requests' split counts
+    //    differ: up to 128 go one by one, longest first, to the XCD with the least blocks
+    //    (100 drawn launches: dealt in turn 17 differ, on the average by 10 %, at most 38 %
+    //    slower; so placed above 128 too no faster, and the sort takes the host longer).
     bool same_len = true;
     for (int b = 1; b < s.B; ++b) same_len = same_len && nkb[b] == nkb[0];
     //  - Several row tiles of items that the turns made alike: dealt in order, an eighth to every XCD (a unit's

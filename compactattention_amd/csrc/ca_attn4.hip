@@ -342,9 +342,9 @@ __device__ __forceinline__ void decode4_item(const Attn4Params& p4, const Item& 
 // How K and V are loaded: to stay in the caches (chunks and drafts of several tiles read them again), past them,
 // or past them where no other request reads the item's pages.  Past them is faster even for small caches, as a
 // model's layers take turns in what the last-level cache (256 MB) holds: one token over 4096 tokens, 80 caches
-// in turn, 10.9 us kept, 9.4 past them; one cache again and again 9.1, 9.1; 131072 tokens, 4 caches in turn 33.3,
-// 29.1, 64 requests of 4096 54.8, 49.5.  Slower only for one cache near that size again and again (214 MB 40.9,
-// 43.2).
+// in turn, 10.0 us kept, 9.0 past them; one cache again and again 8.6, 8.6; 131072 tokens, 4 caches in turn 34.8,
+// 30.5, 64 requests of 4096, 3 caches 55.5, 50.5.  Slower only for one cache near that size again and again (64
+// requests of 4096, 285 MB, 47.2, 48.9).
 enum { kLoadsKept, kLoadsStreamed, kLoadsStreamedUnshared };
 template <int kN, bool kTab, int kLoads>
 __global__ __launch_bounds__(kWaves4 * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn4_decode_kernel(Attn4Params p4) {
@@ -954,9 +954,10 @@ __global__ __launch_bounds__(256) void attn4_merge_rows_kernel(Merge4Params p) {
 // them.  A workgroup takes 0.9 us for 32 rows x four blocks and 1.3 us for 256 x one, so the small tiles do
 // less up to 160 rows, and beyond do 1.4 times the work but start and end 6 to 12 us earlier, need no merge
 // where their tiles alone fill the CUs, and waste fewer rows.  They win up to 12 blocks of 256 rows for every
-// CU (all blocks counted; 32 Q / 8 KV heads, small tiles and large): 64 queries over 16 + 1 blocks 15.1, 22.4 us;
-// 256 over 8 + 4 13.7, 28.0; 256 over 64 + 4 (8.5 blocks a CU) 32.5, 46.3; 256 over 256 + 4 (32.5) 96.2, 82.2,
-// with 30 % kept 38.8, 46.0; 512 over 128 + 8 (34) 105.6, 86.2, with 30 % kept 55.0, 50.4.
+// CU (all blocks counted; 32 Q / 8 KV heads, small tiles and large): 64 queries over 16 + 1 blocks 13.4, 21.3 us;
+// 256 over 8 + 4 11.7, 26.8; 256 over 64 + 4 (8.5 blocks a CU) 26.5, 41; 256 over 256 + 4 (32.5) 78.4, 75.3,
+// with 30 % kept 32.7, 42.5; 512 over 128 + 8 (34) 87.5, 77.2, with 30 % kept 43.6, 43.0.  (Not always: 300 over
+// 40 + 5 with 28 / 4 heads, 6.3 blocks a CU, 39.3, 33.3.)
 AttnTiling attn4_tiling(const Shape& s, const PastBlocks& pb, const int32_t* kv_len) {
     const bool dense = kv_len != nullptr;
     const int rows = s.Lq * s.G;
