@@ -134,6 +134,8 @@ RAGGED = [
     # (Hq, Hkv, q_len, lens): one or two long requests among many short ones, rows and tiles near and past 256 and 512
     (32, 8, 1, [20000] + [640 + 7 * b for b in range(31)]), (32, 8, 1, [900] * 20 + [16383] + [64] * 12),
     (8, 8, 1, [30000] + [70 + b for b in range(63)]), (9, 9, 1, [25000] + [64 + b for b in range(62)] + [10000]),
+    # several tiles a row: single splits, whole rows (512, with the splits more than are placed one by one) and 513 rows
+    (8, 8, 40, [9000] + [64 + b for b in range(63)]), (9, 9, 40, [9000] + [64 + b for b in range(56)]),
     (32, 8, 40, [20000] + [640] * 4), (28, 4, 16, [300, 12000, 64, 65, 9000, 16, 400, 500, 600, 20]),
 ]
 
