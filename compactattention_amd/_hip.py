@@ -69,6 +69,16 @@ EXPORTED = (
     "ca_attn_fwd_q4_workspace_size",
     "ca_attn_decode_q4_workspace_size",
     "ca_copy_pages",
+    "ca_attn_window",
+    "ca_attn_window_q4",
+    "ca_attn_window_workspace_size",
+    "ca_attn_window_q4_workspace_size",
+    "ca_key_mass",
+    "ca_key_mass_q4",
+    "ca_heavy_tokens",
+    "ca_heavy_tokens_workspace_size",
+    "ca_move_tokens",
+    "ca_move_tokens_q4",
     "ca_rope_apply",
     "ca_rope_qk",
     "ca_norm_rope_qk",
@@ -201,6 +211,22 @@ _SIGNATURES = {
     "ca_attn_fwd_q4_workspace_size": (ctypes.c_int64, [_P(Dims), _vp, _i32]),
     "ca_attn_decode_q4_workspace_size": (ctypes.c_int64, [_P(Dims), _vp, _i32]),
     "ca_copy_pages": (ctypes.c_int, [_P(PagePool), _i32, _vp, _vp, _i32, _vp, _vp]),
+    "ca_attn_window": (ctypes.c_int, [_P(Dims), _P(SeqLayout), _P(KvLayout), _P(KvLayout), _vp, _i32, _i32, _f32,
+                                      _P(SeqLayout), _vp, _i32, _vp, _i64, _vp]),
+    "ca_attn_window_workspace_size": (ctypes.c_int64, [_P(Dims), _vp, _i32, _i32, _i32]),
+    "ca_key_mass": (ctypes.c_int, [_P(Dims), _P(SeqLayout), _P(KvLayout), _vp, _i64, _i64, _vp, _i32, _i32, _vp, _i64,
+                                   _vp, _f32, _vp, _i64, _vp, _i64, _vp]),
+    "ca_move_tokens": (ctypes.c_int, [_P(KvLayout), _P(KvLayout), _P(KvLayout), _P(KvLayout), _vp, _i64, _i32, _i32, _vp,
+                                      _i32, _vp, _i64, _vp, _i64, _vp]),
+    "ca_attn_window_q4": (ctypes.c_int, [_P(Dims), _P(SeqLayout), _P(Kv4Layout), _P(Kv4Layout), _vp, _i32, _i32, _f32,
+                                      _P(SeqLayout), _vp, _i32, _vp, _i64, _vp]),
+    "ca_attn_window_q4_workspace_size": (ctypes.c_int64, [_P(Dims), _vp, _i32, _i32, _i32]),
+    "ca_key_mass_q4": (ctypes.c_int, [_P(Dims), _P(SeqLayout), _P(Kv4Layout), _vp, _i64, _i64, _vp, _i32, _i32, _vp, _i64,
+                                   _vp, _f32, _vp, _i64, _vp, _i64, _vp]),
+    "ca_move_tokens_q4": (ctypes.c_int, [_P(Kv4Layout), _P(Kv4Layout), _P(Kv4Layout), _P(Kv4Layout), _vp, _i64, _i32, _i32, _vp,
+                                      _i32, _vp, _i64, _vp, _i64, _vp]),
+    "ca_heavy_tokens": (ctypes.c_int, [_vp, _i64, _i32, _i32, _vp, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp]),
+    "ca_heavy_tokens_workspace_size": (ctypes.c_int64, [_i32, _i32, _vp, _i32]),
     "ca_rmsnorm": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i32, _f32, _vp]),
     "ca_swiglu": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _vp]),
 }

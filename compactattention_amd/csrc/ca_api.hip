@@ -864,6 +864,329 @@ int ca_gather_q4(const ca_dims* dims, const ca_kv4_layout* k_cache, const ca_kv4
     return ok();
 }
 
+// ---- caches of bounded size ----
+}  // extern "C"
+
+namespace {
+
+// The dims of q_len query rows at start[b] .. start[b] + q_len - 1; kv_len: the tokens of every request.
+int check_start_dims(const ca_dims* d, const int32_t* start, ca::Shape* s, int32_t* kv_len, int* max_nkb) {
+    if (d == nullptr || start == nullptr) return fail(CA_ERR_INVALID, "dims or start_host is NULL");
+    if (d->batch < 1 || d->batch > CA_MAX_BATCH)
+        return fail(d->batch < 1 ? CA_ERR_INVALID : CA_ERR_LIMIT, "batch=%d outside [1, %d]", d->batch, CA_MAX_BATCH);
+    if (d->q_len < 1) return fail(CA_ERR_INVALID, "q_len=%d must be positive", d->q_len);
+    if (d->num_q_heads <= 0 || d->num_kv_heads <= 0 || d->num_q_heads % d->num_kv_heads != 0)
+        return fail(CA_ERR_INVALID, "num_q_heads=%d must be a positive multiple of num_kv_heads=%d",
+                    d->num_q_heads, d->num_kv_heads);
+    const int G = d->num_q_heads / d->num_kv_heads;
+    if (G > 16) return fail(CA_ERR_LIMIT, "GQA group size %d > 16", G);
+    if ((int64_t)d->q_len * G > (int64_t)1 << 24) return fail(CA_ERR_LIMIT, "q_len * group too large");
+    if (d->kv_cap < 1 || (int64_t)d->kv_cap * CA_BLOCK > (int64_t)1 << 30)
+        return fail(d->kv_cap < 1 ? CA_ERR_INVALID : CA_ERR_LIMIT, "kv_cap=%d blocks outside [1, 2^24]", d->kv_cap);
+    *max_nkb = 0;
+    for (int b = 0; b < d->batch; ++b) {
+        const int64_t end = (int64_t)start[b] + d->q_len;
+        if (start[b] < 0 || end > (int64_t)d->kv_cap * CA_BLOCK)
+            return fail(CA_ERR_INVALID, "tokens [%d, %lld) of request %d outside a cache of %d blocks", start[b],
+                        (long long)end, b, d->kv_cap);
+        kv_len[b] = static_cast<int32_t>(end);
+        *max_nkb = max(*max_nkb, static_cast<int>((end + CA_BLOCK - 1) / CA_BLOCK));
+    }
+    *s = ca::Shape{d->batch, d->q_len, d->num_q_heads, d->num_kv_heads, G, 0, d->kv_cap, (d->kv_cap + 31) / 32};
+    return CA_OK;
+}
+
+// A window and sinks past every position are as good as that many tokens (the kernels add positions to them).
+int check_window(int least, int max_nkb, int32_t* window, int32_t* sinks) {
+    if (*window < least) return fail(CA_ERR_INVALID, "window=%d must be at least %d", *window, least);
+    if (*sinks < 0) return fail(CA_ERR_INVALID, "sinks=%d < 0", *sinks);
+    *window = min(*window, max_nkb * CA_BLOCK);
+    *sinks = min(*sinks, max_nkb * CA_BLOCK);
+    return CA_OK;
+}
+
+int64_t window_workspace(const ca_dims* dims, const int32_t* start, int32_t window, int32_t sinks, int num_splits, bool bits4) {
+    ca::Shape s;
+    int32_t kv_len[CA_MAX_BATCH];
+    int max_nkb = 0;
+    if (check_start_dims(dims, start, &s, kv_len, &max_nkb) != CA_OK || check_window(1, max_nkb, &window, &sinks) != CA_OK) return -1;
+    if (num_splits < 0 || num_splits > ca::kMaxDecodeSplits)
+        return fail(CA_ERR_INVALID, "num_splits=%d outside [0, %d]", num_splits, ca::kMaxDecodeSplits);
+    if (num_splits == 0) num_splits = ca::attn_window_splits(s, kv_len, window, sinks, bits4);
+    return ca::attn_workspace_bytes(s, num_splits);
+}
+
+// The arguments of ca_attn_window and its 4-bit form but for the cache, and the launch.
+template <typename Launch>
+int attn_window(const ca_dims* dims, const ca_seq_layout* q, const int32_t* start, int32_t window, int32_t sinks, float scale,
+                const ca_seq_layout* out, float* lse, int num_splits, void* workspace, int64_t workspace_bytes, bool bits4,
+                const Launch& launch) {
+    ca::AttnArgs a{};
+    int32_t kv_len[CA_MAX_BATCH];
+    int max_nkb = 0, rc;
+    if ((rc = check_start_dims(dims, start, &a.s, kv_len, &max_nkb)) != CA_OK) return rc;
+    if ((rc = check_window(1, max_nkb, &window, &sinks)) != CA_OK) return rc;
+    if ((rc = check_seq(q, "q", &a.q)) != CA_OK) return rc;
+    if ((rc = check_seq(out, "out", &a.out)) != CA_OK) return rc;
+    if (!aligned4(lse)) return fail(CA_ERR_INVALID, "lse must be 4-byte aligned");
+    if (!(scale > 0.0f) || scale > 3.0e38f) return fail(CA_ERR_INVALID, "scale must be positive and finite");
+    if (num_splits < 0 || num_splits > ca::kMaxDecodeSplits)
+        return fail(CA_ERR_INVALID, "num_splits=%d outside [0, %d]", num_splits, ca::kMaxDecodeSplits);
+    // a launch has less than 2^32 threads: 512 for a split of at least 32 rows (or of all there are)
+    if ((int64_t)a.s.B * a.s.Hkv * (((int64_t)a.s.Lq * a.s.G + 31) / 32) * max(num_splits, 1) >= (int64_t)1 << 23)
+        return fail(CA_ERR_LIMIT, "%d rows of %d queries in %d splits are too many", a.s.B * a.s.Hkv, a.s.Lq * a.s.G, num_splits);
+    const int splits = num_splits == 0 ? ca::attn_window_splits(a.s, kv_len, window, sinks, bits4) : num_splits;
+    const int64_t need = ca::attn_workspace_bytes(a.s, splits);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
+        return fail(CA_ERR_WORKSPACE, "num_splits=%d needs a 16-byte aligned workspace of %lld bytes (got %lld)",
+                    num_splits, (long long)need, (long long)workspace_bytes);
+    a.scale = scale;
+    a.lse = lse;
+    a.num_splits = num_splits;
+    a.workspace = workspace;
+    a.kv_len = kv_len;
+    a.window = window;
+    a.sinks = sinks;
+    hipError_t e = hipSuccess;
+    if ((rc = launch(a, max_nkb, &e)) != CA_OK) return rc;
+    if (e != hipSuccess) return hip_fail(e, "attn_window launch");
+    return ok();
+}
+
+// The arguments of ca_key_mass and its 4-bit form but for the keys, and the launch.
+template <typename Keys>
+int key_mass(const ca_dims* dims, const ca_seq_layout* q, const float* lse, int64_t lse_sb, int64_t lse_sh, const int32_t* start,
+             int32_t window, int32_t sinks, const int32_t* table, int64_t table_stride, const int32_t* counts, float scale,
+             const float* mass, int64_t mass_stride, float* out, int64_t out_stride, void* stream, const Keys& keys) {
+    ca::MassArgs a{};
+    int32_t kv_len[CA_MAX_BATCH];
+    int max_nkb = 0, rc;
+    if ((rc = check_start_dims(dims, start, &a.s, kv_len, &max_nkb)) != CA_OK) return rc;
+    if ((rc = check_window(0, max_nkb, &window, &sinks)) != CA_OK) return rc;
+    if ((rc = check_seq(q, "q", &a.q)) != CA_OK) return rc;
+    if ((rc = keys(max_nkb, &a)) != CA_OK) return rc;
+    if (lse == nullptr || mass == nullptr || out == nullptr) return fail(CA_ERR_INVALID, "lse, mass and out are required");
+    if (!aligned4(lse) || !aligned4(mass) || !aligned4(out)) return fail(CA_ERR_INVALID, "lse, mass and out must be 4-byte aligned");
+    if (lse_sb < 0 || lse_sh < 0) return fail(CA_ERR_INVALID, "negative lse stride");
+    if ((table == nullptr) != (counts == nullptr)) return fail(CA_ERR_INVALID, "table and counts must both be given or both be NULL");
+    if (table != nullptr && (!aligned4(table) || !aligned4(counts))) return fail(CA_ERR_INVALID, "table and counts must be 4-byte aligned");
+    if (table != nullptr && table_stride < a.s.cap)
+        return fail(CA_ERR_INVALID, "table_stride=%lld < kv_cap=%d", (long long)table_stride, a.s.cap);
+    if (!(scale > 0.0f) || scale > 3.0e38f) return fail(CA_ERR_INVALID, "scale must be positive and finite");
+    int tokens = 0;
+    for (int b = 0; b < a.s.B; ++b) tokens = max(tokens, kv_len[b]);
+    if (mass_stride < tokens || out_stride < tokens)
+        return fail(CA_ERR_INVALID, "rows of mass (%lld) and out (%lld) do not hold %d tokens", (long long)mass_stride,
+                    (long long)out_stride, tokens);
+    if (mass == out && mass_stride != out_stride) return fail(CA_ERR_INVALID, "mass in place has one stride");
+    if (mass != out) {  // rows of one may not be read after the other's were written
+        const int64_t rows = (int64_t)a.s.B * a.s.Hkv;
+        const float *m1 = mass + (rows - 1) * mass_stride + tokens, *o1 = out + (rows - 1) * out_stride + tokens;
+        if (mass < o1 && out < m1) return fail(CA_ERR_INVALID, "mass and out overlap");
+    }
+    // eight blocks a workgroup of 512 threads, fewer only in launches of few blocks; a launch has less than 2^32 threads
+    if ((int64_t)(max_nkb / 8 + 2) * a.s.B * a.s.Hkv >= (int64_t)1 << 23)
+        return fail(CA_ERR_LIMIT, "%d rows of up to %d blocks are too many", a.s.B * a.s.Hkv, max_nkb);
+    a.start = start;
+    a.lse = lse;
+    a.lse_sb = lse_sb;
+    a.lse_sh = lse_sh;
+    a.mass = mass;
+    a.mass_stride = mass_stride;
+    a.out = out;
+    a.out_stride = out_stride;
+    a.table = table;
+    a.table_stride = table_stride;
+    a.counts = counts;
+    a.scale = scale;
+    a.window = window;
+    a.sinks = sinks;
+    hipError_t e = ca::launch_key_mass(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "key_mass launch");
+    return ok();
+}
+
+int check_rows(int32_t batch, int32_t hkv, const int32_t* len, int32_t n, const char* what, int* longest) {
+    if (batch < 1 || batch > CA_MAX_BATCH)
+        return fail(batch < 1 ? CA_ERR_INVALID : CA_ERR_LIMIT, "batch=%d outside [1, %d]", batch, CA_MAX_BATCH);
+    if (hkv < 1 || len == nullptr) return fail(CA_ERR_INVALID, "num_kv_heads=%d must be positive and len_host given", hkv);
+    if (n < 1) return fail(CA_ERR_INVALID, "%s=%d must be positive", what, n);
+    if (n > 1 << 30) return fail(CA_ERR_LIMIT, "%s=%d beyond 2^30", what, n);
+    *longest = 0;
+    for (int b = 0; b < batch; ++b) {
+        if (len[b] < 0) return fail(CA_ERR_INVALID, "len[%d]=%d < 0", b, len[b]);
+        if (len[b] > 1 << 30) return fail(CA_ERR_LIMIT, "len[%d]=%d beyond 2^30", b, len[b]);
+        *longest = max(*longest, len[b]);
+    }
+    // a workgroup a block of 64 tokens
+    if ((int64_t)batch * hkv * ((max(n, *longest) + 63) / 64) >= (int64_t)1 << 24)
+        return fail(CA_ERR_LIMIT, "batch=%d x num_kv_heads=%d rows of %d tokens are too many", batch, hkv, max(n, *longest));
+    return CA_OK;
+}
+
+template <typename Caches>
+int move_tokens(const int32_t* keep, int64_t keep_stride, int32_t batch, int32_t hkv, const int32_t* len, int32_t n,
+                const float* mass, int64_t mass_stride, float* mass_out, int64_t mass_out_stride, void* stream, const Caches& caches) {
+    ca::MoveArgs a{};
+    int longest = 0, rc;
+    if ((rc = check_rows(batch, hkv, len, n, "n", &longest)) != CA_OK) return rc;
+    if (keep == nullptr || !aligned4(keep)) return fail(CA_ERR_INVALID, "keep is NULL or misaligned");
+    if (keep_stride < n) return fail(CA_ERR_INVALID, "keep_stride=%lld < n=%d", (long long)keep_stride, n);
+    if ((mass == nullptr) != (mass_out == nullptr)) return fail(CA_ERR_INVALID, "mass and mass_out must both be given or both be NULL");
+    if (mass != nullptr && (mass_stride < longest || mass_out_stride < n || !aligned4(mass) || !aligned4(mass_out)))
+        return fail(CA_ERR_INVALID, "rows of mass (%lld) and mass_out (%lld) do not hold %d and %d tokens, or are misaligned",
+                    (long long)mass_stride, (long long)mass_out_stride, longest, n);
+    if (mass != nullptr) {
+        const int64_t rows = (int64_t)batch * hkv;
+        const float *m1 = mass + (rows - 1) * mass_stride + longest, *o1 = mass_out + (rows - 1) * mass_out_stride + n;
+        if (mass < o1 && mass_out < m1) return fail(CA_ERR_INVALID, "mass and mass_out overlap");
+    }
+    if ((rc = caches((longest + 63) / 64, (min(n, longest) + 63) / 64, &a)) != CA_OK) return rc;
+    a.B = batch;
+    a.Hkv = hkv;
+    a.n = n;
+    a.len = len;
+    a.keep = keep;
+    a.keep_stride = keep_stride;
+    a.mass = mass;
+    a.mass_stride = mass_stride;
+    a.mass_out = mass_out;
+    a.mass_out_stride = mass_out_stride;
+    hipError_t e = ca::launch_move_tokens(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "move_tokens launch");
+    return ok();
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t ca_attn_window_workspace_size(const ca_dims* dims, const int32_t* start_host, int32_t window, int32_t sinks,
+                                      int32_t num_splits) {
+    return window_workspace(dims, start_host, window, sinks, num_splits, false);
+}
+
+int64_t ca_attn_window_q4_workspace_size(const ca_dims* dims, const int32_t* start_host, int32_t window, int32_t sinks,
+                                         int32_t num_splits) {
+    return window_workspace(dims, start_host, window, sinks, num_splits, true);
+}
+
+int ca_attn_window(const ca_dims* dims, const ca_seq_layout* q, const ca_kv_layout* k, const ca_kv_layout* v,
+                   const int32_t* start_host, int32_t window, int32_t sinks, float scale, const ca_seq_layout* out,
+                   float* lse, int32_t num_splits, void* workspace, int64_t workspace_bytes, void* stream) {
+    return attn_window(dims, q, start_host, window, sinks, scale, out, lse, num_splits, workspace, workspace_bytes, false,
+                       [&](ca::AttnArgs& a, int max_nkb, hipError_t* e) {
+                           int rc;
+                           if ((rc = check_kv(k, "k", max_nkb, &a.k)) != CA_OK) return rc;
+                           if ((rc = check_kv(v, "v", max_nkb, &a.v)) != CA_OK) return rc;
+                           *e = ca::launch_attn(a, static_cast<hipStream_t>(stream));
+                           return static_cast<int>(CA_OK);
+                       });
+}
+
+int ca_attn_window_q4(const ca_dims* dims, const ca_seq_layout* q, const ca_kv4_layout* k, const ca_kv4_layout* v,
+                      const int32_t* start_host, int32_t window, int32_t sinks, float scale, const ca_seq_layout* out,
+                      float* lse, int32_t num_splits, void* workspace, int64_t workspace_bytes, void* stream) {
+    return attn_window(dims, q, start_host, window, sinks, scale, out, lse, num_splits, workspace, workspace_bytes, true,
+                       [&](ca::AttnArgs& a, int max_nkb, hipError_t* e) {
+                           ca::Kv4Addr ka, va;
+                           int rc;
+                           if ((rc = check_kv4(k, "k", max_nkb, &ka)) != CA_OK) return rc;
+                           if ((rc = check_kv4(v, "v", max_nkb, &va)) != CA_OK) return rc;
+                           *e = ca::launch_attn4(a, ka, va, static_cast<hipStream_t>(stream));
+                           return static_cast<int>(CA_OK);
+                       });
+}
+
+int ca_key_mass(const ca_dims* dims, const ca_seq_layout* q, const ca_kv_layout* k, const float* lse, int64_t lse_stride_b,
+                int64_t lse_stride_h, const int32_t* start_host, int32_t window, int32_t sinks, const int32_t* table,
+                int64_t table_stride, const int32_t* counts, float scale, const float* mass, int64_t mass_stride,
+                float* out, int64_t out_stride, void* stream) {
+    ca::KvAddr ka;
+    return key_mass(dims, q, lse, lse_stride_b, lse_stride_h, start_host, window, sinks, table, table_stride, counts, scale, mass,
+                    mass_stride, out, out_stride, stream, [&](int max_nkb, ca::MassArgs* a) {
+                        a->k = &ka;
+                        return check_kv(k, "k", max_nkb, &ka);
+                    });
+}
+
+int ca_key_mass_q4(const ca_dims* dims, const ca_seq_layout* q, const ca_kv4_layout* k, const float* lse,
+                   int64_t lse_stride_b, int64_t lse_stride_h, const int32_t* start_host, int32_t window, int32_t sinks,
+                   const int32_t* table, int64_t table_stride, const int32_t* counts, float scale, const float* mass,
+                   int64_t mass_stride, float* out, int64_t out_stride, void* stream) {
+    ca::Kv4Addr ka;
+    return key_mass(dims, q, lse, lse_stride_b, lse_stride_h, start_host, window, sinks, table, table_stride, counts, scale, mass,
+                    mass_stride, out, out_stride, stream, [&](int max_nkb, ca::MassArgs* a) {
+                        a->k4 = &ka;
+                        return check_kv4(k, "k", max_nkb, &ka);
+                    });
+}
+
+int64_t ca_heavy_tokens_workspace_size(int32_t batch, int32_t num_kv_heads, const int32_t* len_host, int32_t budget) {
+    int longest = 0;
+    if (check_rows(batch, num_kv_heads, len_host, budget, "budget", &longest) != CA_OK) return -1;
+    return 0;
+}
+
+int ca_heavy_tokens(const float* mass, int64_t mass_stride, int32_t batch, int32_t num_kv_heads, const int32_t* len_host,
+                    int32_t budget, int32_t sinks, int32_t recent, int32_t* keep, int64_t keep_stride, void* workspace,
+                    int64_t workspace_bytes, void* stream) {
+    int longest = 0, rc;
+    if ((rc = check_rows(batch, num_kv_heads, len_host, budget, "budget", &longest)) != CA_OK) return rc;
+    if (mass == nullptr || keep == nullptr || !aligned4(mass) || !aligned4(keep))
+        return fail(CA_ERR_INVALID, "mass or keep is NULL or misaligned");
+    if (sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget)
+        return fail(CA_ERR_INVALID, "sinks=%d and recent=%d must not be negative nor more than budget=%d together", sinks, recent,
+                    budget);
+    if (mass_stride < longest || keep_stride < budget)
+        return fail(CA_ERR_INVALID, "rows of mass (%lld) and keep (%lld) do not hold %d tokens and %d places",
+                    (long long)mass_stride, (long long)keep_stride, longest, budget);
+    (void)workspace;
+    (void)workspace_bytes;
+    hipError_t e = ca::launch_heavy_tokens(mass, mass_stride, batch, num_kv_heads, len_host, budget, sinks, recent, keep,
+                                           keep_stride, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "heavy_tokens launch");
+    return ok();
+}
+
+int ca_move_tokens(const ca_kv_layout* k, const ca_kv_layout* v, const ca_kv_layout* k_dst, const ca_kv_layout* v_dst,
+                   const int32_t* keep, int64_t keep_stride, int32_t batch, int32_t num_kv_heads, const int32_t* len_host,
+                   int32_t n, const float* mass, int64_t mass_stride, float* mass_out, int64_t mass_out_stride, void* stream) {
+    ca::KvAddr t[4];
+    return move_tokens(keep, keep_stride, batch, num_kv_heads, len_host, n, mass, mass_stride, mass_out, mass_out_stride, stream,
+                       [&](int from, int to, ca::MoveArgs* a) {
+                           int rc;
+                           if ((rc = check_kv(k, "k", from, &t[0])) != CA_OK) return rc;
+                           if ((rc = check_kv(v, "v", from, &t[1])) != CA_OK) return rc;
+                           if ((rc = check_kv(k_dst, "k_dst", to, &t[2])) != CA_OK) return rc;
+                           if ((rc = check_kv(v_dst, "v_dst", to, &t[3])) != CA_OK) return rc;
+                           a->k = &t[0];
+                           a->v = &t[1];
+                           a->k_dst = &t[2];
+                           a->v_dst = &t[3];
+                           return static_cast<int>(CA_OK);
+                       });
+}
+
+int ca_move_tokens_q4(const ca_kv4_layout* k, const ca_kv4_layout* v, const ca_kv4_layout* k_dst, const ca_kv4_layout* v_dst,
+                      const int32_t* keep, int64_t keep_stride, int32_t batch, int32_t num_kv_heads, const int32_t* len_host,
+                      int32_t n, const float* mass, int64_t mass_stride, float* mass_out, int64_t mass_out_stride, void* stream) {
+    ca::Kv4Addr t[4];
+    return move_tokens(keep, keep_stride, batch, num_kv_heads, len_host, n, mass, mass_stride, mass_out, mass_out_stride, stream,
+                       [&](int from, int to, ca::MoveArgs* a) {
+                           int rc;
+                           if ((rc = check_kv4(k, "k", from, &t[0])) != CA_OK) return rc;
+                           if ((rc = check_kv4(v, "v", from, &t[1])) != CA_OK) return rc;
+                           if ((rc = check_kv4(k_dst, "k_dst", to, &t[2])) != CA_OK) return rc;
+                           if ((rc = check_kv4(v_dst, "v_dst", to, &t[3])) != CA_OK) return rc;
+                           a->k4 = &t[0];
+                           a->v4 = &t[1];
+                           a->k4_dst = &t[2];
+                           a->v4_dst = &t[3];
+                           return static_cast<int>(CA_OK);
+                       });
+}
+
 int ca_copy_pages(const ca_page_pool* pools, int32_t n_pools, const int32_t* src_host, const int32_t* dst_host,
                   int32_t n, const int32_t* ids, void* stream) {
     if (pools == nullptr || n_pools < 1 || n_pools > CA_MAX_POOLS)

@@ -16,6 +16,7 @@ typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void_t;
 typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
@@ -55,6 +56,48 @@ struct AttnParams {
     int unit_splits;                 // kPlaceRows, kPlaceTable: the splits of every unit, 0 when they differ
     int32_t xoff[9];                 // kPlaceTable
     uint32_t unit[kPlanRows];
+    int window, sinks;               // the window kernels: tokens (WindowList)
+};
+
+// The blocks that a tile of queries at positions first .. last sees under a window: a query at p sees key j <= p
+// where p - j < window or j < sinks.  Entries [0, full) are the blocks that every query of the tile sees whole (sinks,
+// then the window's), [full, total) those where the mask cuts (the block in which the sinks end, the window's first
+// blocks, the queries' own), so that the loops run their unmasked part first and masked blocks after it: the order of
+// blocks is free in an online softmax.  All from six values, without a list in memory.
+struct WindowList {
+    int s1, c1;          // sinks: blocks [0, s1) whole, [s1, c1) in part
+    int d0, b0, b1, e1;  // the window: [d0, b0) in part, [b0, b1) whole, [b1, e1) in part
+    int full, total;
+
+    __host__ __device__ __forceinline__ WindowList(int first, int last, int window, int sinks) {
+        const int lo = first - window + 1;  // the first key that the window shows to the tile
+        const int out = last - window;      // the last key that it hides from some query
+        const int whole = (first + 1) >> 6;  // blocks [0, whole) hold no key past the first query
+        d0 = lo > 0 ? lo >> 6 : 0;
+        e1 = (last >> 6) + 1;
+        c1 = (sinks >> 6) + ((sinks & 63) != 0);
+        c1 = c1 < d0 ? c1 : d0;  // (d0 <= whole)
+        s1 = (sinks >> 6) < c1 ? sinks >> 6 : c1;
+        b0 = out < 0 ? 0 : (out >> 6) + 1;  // >= d0, <= e1
+        b1 = whole > b0 ? whole : b0;
+        full = s1 + b1 - b0;
+        total = full + (c1 - s1) + (b0 - d0) + (e1 - b1);
+    }
+    __host__ __device__ __forceinline__ int block(int e) const {
+        int at = 0, off = 0;
+        auto part = [&](int from, int to) {  // entries from `at` on stand for blocks from `from` on
+            off = e >= at ? from - at : off;
+            at += to - from;
+        };
+        part(0, s1);
+        part(b0, b1);
+        part(s1, c1);
+        part(d0, b0);
+        part(b1, e1);
+        return e + off;
+    }
+    // whether the mask cuts in block kb of the list
+    __device__ __forceinline__ bool cut(int kb) const { return kb >= s1 && (kb < b0 || kb >= b1); }
 };
 
 // The work item of a workgroup: KV row, request, split of the row's list (of p.sp[b]) and, for

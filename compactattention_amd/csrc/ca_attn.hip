@@ -92,8 +92,9 @@ __device__ __forceinline__ void wait_dma() {
 // share a SIMD: one wave's softmax overlaps the other's MFMAs.  One 8-wave workgroup per
 // CU (128 KB of LDS).
 // kTab: block lists come from the per-row table (prefill); otherwise they are the identity
-// 0 .. nkb-1 (dense decode).
-template <int NW, bool kTab, bool kRow>
+// 0 .. nkb-1 (dense decode), or kWin the blocks of a window (WindowList).  Under a window what is hidden has no
+// effect, whatever it holds (finish).
+template <int NW, bool kTab, bool kRow, bool kWin = false>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_fwd_kernel(AttnParams p) {
     constexpr int BM = 32 * NW;
     __shared__ __attribute__((aligned(16))) uint8_t smem[kStages * (kKBytes + kVBytes)];  // K ring, then V ring
@@ -171,7 +172,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     // Table entries are clamped into [0, nkb) so a corrupt table cannot address outside the
     // KV tensors.
     const int32_t* tab = kTab ? p.table + (int64_t)row * p.table_stride : nullptr;
-    auto block_id = [&](int e) { return kTab ? min(max(sload(tab + e), 0), nkb - 1) : e; };
+    static_assert(!kWin || (!kTab && !kRow), "windows have lists of their own and a resource for each block");
+    const WindowList win(qpos0 + t_first, qpos0 + t_last, p.window, p.sinks);
+    auto block_id = [&](int e) { return kTab ? min(max(sload(tab + e), 0), nkb - 1) : kWin ? win.block(e) : e; };
     const int lim = (qpos0 + t_last) >> 6;  // last block the tile can see
     const int tid = threadIdx.x;
     const int w = tid >> 6;
@@ -222,6 +225,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
                 break;
             }
         }
+    } else if (kWin) {
+        n_vis = win.total;
+        n_whole = win.full;
     } else {
         n_vis = min(nkb, lim + 1);
         n_whole = whole;
@@ -304,7 +310,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     auto load_blks = [&](int c) {
         const int e = e0 + 64 * c + l;
         if (e >= e1) return Blk{nkb, 0, 0};
-        const int id = kTab ? min(max(tab[e], 0), nkb - 1) : e;
+        const int id = kTab ? min(max(tab[e], 0), nkb - 1) : kWin ? win.block(e) : e;
         if (kRow) return Blk{id, 0, 0};
         return Blk{id, kpt ? static_cast<int>(clamp_page(kpt[id], p.k.max_page)) : id,
                    vpt ? static_cast<int>(clamp_page(vpt[id], p.v.max_page)) : id};
@@ -392,12 +398,13 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
         // value j of half kt holds key kt*32 + swap23(8*(j/4) + 4*h + j%4)
         // = kt*32 + 8*h + key_off(j); visible iff kb*64 + key <= qpos0 + t
         const int vis = qpos0 + qtok - kb * 64 - 8 * h;
+        const int past = kWin ? vis - p.window : 0, sink = kWin ? p.sinks - kb * 64 - 8 * h : 0;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
                 const int key = kt * 32 + 16 * (j >> 3) + 4 * ((j >> 2) & 1) + (j & 3);
-                if (key > vis) sc[kt][j] = -__builtin_inff();
+                if (key > vis || (kWin && key <= past && key >= sink)) sc[kt][j] = -__builtin_inff();
             }
     };
     // The running max of each row rises to mx (both lane halves' row max, scaled) where mx
@@ -425,8 +432,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
         mx = xor32_max(mx) * sl2;
         if (__ballot(mx > m_run + kRescale)) rise(mx);
     };
-    // softmax of sc and O^T += V^T P^T
-    auto finish = [&](int vbase) {
+    // softmax of sc and O^T += V^T P^T.  cut (windows): the mask cuts in the block, kb
+    auto finish = [&](int vbase, bool cut = false, int kb = 0) {
         bf16x8_t pf[4];
         f32x4_t rs = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -441,6 +448,47 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
             rs = add_weights(w4[2], w4[3], rs);
         }
         l_run += rs[0];  // this lane's half of the row; combined across lanes n, n+32 at the end
+        if (kWin && cut) {
+            // A hidden key's weight of 0 times a value that is not finite would be NaN: where the block holds such a
+            // value its keys are taken one by one, those that a row does not see left out.
+            u16x2_t top = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const u32x4_t x = __builtin_bit_cast(u32x4_t, v_frag(vbase, i));
+#pragma unroll
+                for (int c = 0; c < 4; ++c) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, x[c] & 0x7f807f80u));
+            }
+            if (__ballot(top[0] == 0x7f80 || top[1] == 0x7f80)) {
+                const int vis = qpos0 + qtok - kb * 64;
+#pragma unroll 1
+                for (int key = 0; key < 64; ++key) {
+                    const int word = 4 * (key >> 4) + ((key & 7) >> 1);  // of the lane half (key / 8) % 2
+                    uint32_t mine = 0;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const u32x4_t w4 = __builtin_bit_cast(u32x4_t, pf[i >> 2]);
+                        mine = i == word ? w4[i & 3] : mine;
+                    }
+                    const uint32_t other = __shfl_xor(mine, 32, 64);
+                    const uint32_t both = ((key >> 3) & 1) == h ? mine : other;
+                    const float wt = __uint_as_float((key & 1) ? both & 0xffff0000u : both << 16);
+                    const bool seen = key <= vis && (key > vis - p.window || key < p.sinks - kb * 64);
+                    const uint8_t* vr = smem + kVRing + vbase + key * 256 + 8 * h;
+#pragma unroll
+                    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                        for (int jq = 0; jq < 4; ++jq) {
+                            const u32x2_t x = *reinterpret_cast<const u32x2_t*>(vr + ((4 * dt + jq) ^ (4 * (key & 3))) * 16);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float val = __uint_as_float((i & 1) ? x[i >> 1] & 0xffff0000u : x[i >> 1] << 16);
+                                oacc[dt][4 * jq + i] += seen ? wt * val : 0.0f;
+                            }
+                        }
+                }
+                return;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             oacc[i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_frag(vbase, i), pf[i >> 2], oacc[i & 3], 0, 0, 0);
@@ -604,7 +652,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
             j += 2;
         }
         for (; j < nblk; ++j) {  // the next block is masked, or there is none
-            finish((j & 3) * 16384);
+            if (kWin)
+                finish((j & 3) * 16384, j >= n_un, block_id(e0 + j));
+            else
+                finish((j & 3) * 16384);
             if (j + 1 < nblk) {
                 scores(((j + 1) & 3) * 16384);
                 if (j + 1 >= n_un) mask(block_id(e0 + j + 1));
@@ -621,8 +672,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     // here (both were rescaled by the same factors)
     l_run += __shfl_xor(l_run, 32, 64);
     if (qvalid) {
-        const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
-        const float lse2 = l_run > 0.0f ? m_run + __log2f(l_run) : -__builtin_inff();
+        const bool some = kWin ? l_run != 0.0f : l_run > 0.0f;  // (windows: a NaN sum stays)
+        const float inv = some ? 1.0f / l_run : 0.0f;
+        const float lse2 = some ? m_run + __log2f(l_run) : -__builtin_inff();
         if (nsplit == 1) {
             const int hq = hk * G + qg;
             uint16_t* op = p.out.data + b * p.out.sb + (int64_t)qt * p.out.st + (int64_t)hq * p.out.sh;
@@ -755,8 +807,8 @@ constexpr int kDecRows = 16;
 constexpr int kDecVBytes = 64 * 256;
 constexpr int kDecOStride = 132;  // floats per row of a wave's partial O in LDS (padded)
 
-// One work item.  kStream: K and V are loaded with the non-temporal hint.
-template <bool kStream>
+// One work item.  kStream: K and V are loaded with the non-temporal hint.  kWin: the blocks of a window (WindowList).
+template <bool kStream, bool kWin = false>
 __device__ __forceinline__ void decode_item(const AttnParams& p, const Item& it, uint8_t* smem) {
     constexpr int kCache = kStream ? 2 : 0;  // cache policy of the loads: nt
     const Shape& s = p.s;
@@ -768,7 +820,8 @@ __device__ __forceinline__ void decode_item(const AttnParams& p, const Item& it,
     const int G = s.G;
     const int R = p.rows_total;
     const int qpos0 = p.qpos0[b];
-    const int nkb = p.nkb[b];  // the last query row sees every block
+    const WindowList win(qpos0, qpos0 + s.Lq - 1, p.window, p.sinks);
+    const int nkb = kWin ? win.total : p.nkb[b];  // the last query row sees every block
     const int chunk = (nkb + nsplit - 1) / nsplit;
     const int e0 = min(nkb, split * chunk);
     const int e1 = min(nkb, e0 + chunk);
@@ -844,7 +897,10 @@ __device__ __forceinline__ void decode_item(const AttnParams& p, const Item& it,
     };
     const int nb_w = e0 + w < e1 ? (e1 - 1 - (e0 + w)) / kDecWaves + 1 : 0;  // this wave's blocks
     const int nsteps = 2 * nb_w;
-    auto step_block = [&](int st) { return e0 + w + kDecWaves * (st >> 1); };
+    auto step_block = [&](int st) {
+        const int e = e0 + w + kDecWaves * (st >> 1);
+        return kWin ? win.block(e) : e;
+    };
     auto issue = [&](int st, int set) {
         const int kb = step_block(st);
         const int half = st & 1;
@@ -883,14 +939,18 @@ __device__ __forceinline__ void decode_item(const AttnParams& p, const Item& it,
             for (int kt = 0; kt < 2; ++kt)
                 sacc[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kf[set][kt][j]), qf[j],
                                                                   sacc[kt], 0, 0, 0);
-        if (kb >= e_mask) {
+        const bool cut = kWin ? win.cut(kb) : kb >= e_mask;
+        if (cut) {
             // value i of tile kt is key 64 kb + 32 half + 16 kt + 4 g + i
             const int vis = qpos - kb * 64 - 32 * half - 4 * g;
+            const int past = kWin ? vis - p.window : 0, sink = kWin ? p.sinks - kb * 64 - 32 * half - 4 * g : 0;
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (16 * kt + i > vis) sacc[kt][i] = -__builtin_inff();
+                for (int i = 0; i < 4; ++i) {
+                    const int key = 16 * kt + i;
+                    if (key > vis || (kWin && key <= past && key >= sink)) sacc[kt][i] = -__builtin_inff();
+                }
         }
         float mx = -__builtin_inff();
 #pragma unroll
@@ -918,6 +978,39 @@ __device__ __forceinline__ void decode_item(const AttnParams& p, const Item& it,
         l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pf, pf, 2, 3), ones, l_run, false);
         l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pf, pf, 4, 5), ones, l_run, false);
         l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pf, pf, 6, 7), ones, l_run, false);
+        if (kWin && cut) {
+            // as in attn_fwd_kernel: keys one by one where the half block holds a value that is not finite
+            u16x2_t top = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const u32x4_t x = *reinterpret_cast<const u32x4_t*>(vhalf[set] + 16 * l + 1024 * i);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, x[c] & 0x7f807f80u));
+            }
+            if (__ballot(top[0] == 0x7f80 || top[1] == 0x7f80)) {
+                const int vis = qpos - kb * 64 - 32 * half;
+#pragma unroll 1
+                for (int key = 0; key < 32; ++key) {
+                    const u32x4_t w4 = __builtin_bit_cast(u32x4_t, pf);
+                    const int word = 2 * (key >> 4) + ((key & 3) >> 1);  // of lane group (key / 4) % 4
+                    const uint32_t mine = word == 0 ? w4[0] : word == 1 ? w4[1] : word == 2 ? w4[2] : w4[3];
+                    const uint32_t both = __shfl(mine, n + 16 * ((key >> 2) & 3), 64);
+                    const float wt = __uint_as_float((key & 1) ? both & 0xffff0000u : both << 16);
+                    const bool seen = key <= vis && (key > vis - p.window || key < p.sinks - kb * 64 - 32 * half);
+                    const uint8_t* vr = vhalf[set] + key * 256 + 8 * (g & 1);
+#pragma unroll
+                    for (int dt = 0; dt < 8; ++dt) {
+                        const u32x2_t x = *reinterpret_cast<const u32x2_t*>(vr + ((2 * dt + (g >> 1)) ^ (2 * (key & 7))) * 16);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float val = __uint_as_float((i & 1) ? x[i >> 1] & 0xffff0000u : x[i >> 1] << 16);
+                            oacc[dt][i] += seen ? wt * val : 0.0f;
+                        }
+                    }
+                }
+                return;
+            }
+        }
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) {
             const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(to_lds_v4(vhalf[set] + v_off[dt]));
@@ -966,7 +1059,8 @@ __device__ __forceinline__ void decode_item(const AttnParams& p, const Item& it,
     for (int v = 0; v < kDecWaves; ++v) mx = fmaxf(mx, ml[(v * kDecRows + orow) * 2]);
     f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
     float wsum = 0.0f;
-    if (mx != -__builtin_inff()) {
+    if (kWin && mx == -__builtin_inff()) mx = 0.0f;  // (fmaxf drops NaN: a NaN sum stays)
+    if (kWin || mx != -__builtin_inff()) {
 #pragma unroll
         for (int v = 0; v < kDecWaves; ++v) {
             const float wv = __builtin_amdgcn_exp2f(ml[(v * kDecRows + orow) * 2] - mx);
@@ -974,8 +1068,9 @@ __device__ __forceinline__ void decode_item(const AttnParams& p, const Item& it,
             acc += wv * *reinterpret_cast<const f32x4_t*>(mo + (v * kDecRows + orow) * kDecOStride + d4);
         }
     }
-    const float inv = wsum > 0.0f ? 1.0f / wsum : 0.0f;
-    const float lse2 = wsum > 0.0f ? mx + __log2f(wsum) : -__builtin_inff();
+    const bool some = kWin ? wsum != 0.0f : wsum > 0.0f;
+    const float inv = some ? 1.0f / wsum : 0.0f;
+    const float lse2 = some ? mx + __log2f(wsum) : -__builtin_inff();
     acc *= inv;
     const int ot = orow / G;
     const int og = orow - ot * G;
@@ -1006,6 +1101,16 @@ __global__ __launch_bounds__(kDecWaves * 64) void attn_decode_kernel(AttnParams 
         decode_item<true>(p, it, smem);
     else
         decode_item<false>(p, it, smem);
+}
+
+__global__ __launch_bounds__(kDecWaves * 64) void attn_window_decode_kernel(AttnParams p) {
+    __shared__ __attribute__((aligned(16))) uint8_t smem[kDecWaves * kDecVBytes];
+    Item it;
+    if (!find_item(p, 1, &it)) return;
+    it.row = __builtin_amdgcn_readfirstlane(it.row);
+    it.b = __builtin_amdgcn_readfirstlane(it.b);
+    it.split = __builtin_amdgcn_readfirstlane(it.split);
+    decode_item<false, true>(p, it, smem);
 }
 
 }  // namespace
@@ -1374,6 +1479,29 @@ int attn_pick_splits(const Shape& s, const PastBlocks& pb, const int32_t* kv_len
     return plan.max;
 }
 
+int attn_window_blocks(const Shape& s, int tile_rows, int qpos0, int window, int sinks) {
+    // the lists grow until the window has passed position 0, so the last full tile's or the last one's is the longest
+    const int rows = s.Lq * s.G;
+    int most = 1;
+    for (int back = 1; back <= 2; ++back) {
+        const int r0 = ((rows + tile_rows - 1) / tile_rows - back) * tile_rows;
+        if (r0 < 0) break;
+        const WindowList list(qpos0 + r0 / s.G, qpos0 + min(r0 + tile_rows - 1, rows - 1) / s.G, window, sinks);
+        most = max(most, list.total);
+    }
+    return most;
+}
+
+int attn_window_splits(const Shape& s, const int32_t* kv_len, int window, int sinks, bool bits4) {
+    const PastBlocks none{};
+    const AttnTiling tiling = bits4 ? attn4_tiling(s, none, kv_len, window, sinks) : attn_tiling(s, true);
+    int32_t n[CA_MAX_BATCH];
+    for (int b = 0; b < s.B; ++b) n[b] = attn_window_blocks(s, tiling.tile_rows, kv_len[b] - s.Lq, window, sinks);
+    SplitPlan plan;
+    attn_plan_counts(s, n, 0, tiling, &plan);
+    return plan.max;
+}
+
 int64_t attn_workspace_bytes(const Shape& s, int num_splits) {
     if (num_splits <= 1) return 0;
     const int64_t rows_all = (int64_t)s.B * s.Hkv * s.Lq * s.G;
@@ -1399,6 +1527,10 @@ void attn_fill(const AttnArgs& a, const AttnTiling& tiling, AttnParams* p, Split
     attn_positions(a.s, a.pb, a.kv_len, p->qpos0, nkb);
     for (int b = 0; b < CA_MAX_BATCH; ++b) p->nkb[b] = b < a.s.B ? nkb[b] : 0;
     for (int b = a.s.B; b < CA_MAX_BATCH; ++b) p->qpos0[b] = 0;
+    p->window = a.window;
+    p->sinks = a.sinks;
+    for (int b = 0; a.window > 0 && b < a.s.B; ++b)
+        nkb[b] = attn_window_blocks(a.s, tiling.tile_rows, p->qpos0[b], a.window, a.sinks);
     attn_plan(a.s, nkb, a.num_splits, tiling, plan);
     for (int b = 0; b < CA_MAX_BATCH; ++b) p->sp[b] = b < a.s.B ? plan->s[b] : 1;
     for (int b = 0; b <= CA_MAX_BATCH; ++b) p->ioff[b] = b <= a.s.B ? plan->off[b] : plan->off[a.s.B];
@@ -1458,7 +1590,9 @@ hipError_t launch_attn(const AttnArgs& a, hipStream_t stream) {
     };
     const bool streamed = kv_bytes >= kStreamBytes && !repeats(a.k) && !repeats(a.v);
     static_assert(kNW == kDecWaves, "one workgroup size for the attention kernels");
-    if (a.table)
+    if (a.window > 0)
+        attn_uses_decode_kernel(a.s, true) ? launch(attn_window_decode_kernel) : launch(attn_fwd_kernel<kNW, false, false, true>);
+    else if (a.table)
         row_res ? launch(attn_fwd_kernel<kNW, true, true>) : launch(attn_fwd_kernel<kNW, true, false>);
     else if (attn_uses_decode_kernel(a.s, true))
         !streamed                                    ? launch(attn_decode_kernel<kLoadsKept>)
@@ -1468,7 +1602,7 @@ hipError_t launch_attn(const AttnArgs& a, hipStream_t stream) {
         row_res ? launch(attn_fwd_kernel<kNW, false, true>) : launch(attn_fwd_kernel<kNW, false, false>);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || plan.max <= 1) return e;
-    return launch_attn_merge(p, false, stream);
+    return launch_attn_merge(p, a.window > 0, stream);
 }
 
 }  // namespace ca

@@ -26,6 +26,14 @@ constexpr int kNoKey = 0x7fffffff;
 
 __device__ __forceinline__ u32x4_t load16(const uint8_t* p) { return *reinterpret_cast<const u32x4_t*>(p); }
 
+// Whether a query sees one of the keys (a bit each) of a block under a window: at is its position and sinks the end of
+// the sinks, counted from the block's start.
+__device__ __forceinline__ bool sees(uint32_t lo, uint32_t hi, int at, int window, int sinks) {
+    auto below = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };  // keys 0 .. n - 1
+    const uint64_t seen = below(at + 1) & (~below(at + 1 - window) | below(sinks));
+    return ((static_cast<uint64_t>(hi) << 32 | lo) & seen) != 0;
+}
+
 // 8 values of one word of codes under one scale: a row of 8 dims, bf16
 __device__ __forceinline__ u32x4_t decode_row(uint32_t w, float s) {
     return u32x4_t{decode2<0>(w, s), decode2<1>(w, s), decode2<2>(w, s), decode2<3>(w, s)};
@@ -55,8 +63,8 @@ struct Page4 {
     int kb;                  // logical block
 };
 
-// One work item.  kStream: K and V are loaded with the non-temporal hint.
-template <int kN, bool kTab, bool kStream>
+// One work item.  kStream: K and V are loaded with the non-temporal hint.  kWin: the blocks of a window (WindowList).
+template <int kN, bool kTab, bool kStream, bool kWin = false>
 __device__ __forceinline__ void decode4_item(const Attn4Params& p4, const Item& it, float* mo, float* ml) {
     constexpr int kCache = kStream ? 2 : 0;  // cache policy of the loads: nt
     const AttnParams& p = p4.a;
@@ -80,7 +88,9 @@ __device__ __forceinline__ void decode4_item(const Attn4Params& p4, const Item& 
     // blocks from here on hold keys past the tile's first query
     const int mask_from = (qpos0 + (kN == 1 ? 0 : r0 / G) + 1) >> 6;
     const int32_t* tab = kTab ? p.table + (int64_t)row * p.table_stride : nullptr;
-    int n_vis = nkb;
+    const WindowList win(qpos0 + (kN == 1 ? 0 : r0 / G), qpos0 + (kN == 1 ? s.Lq - 1 : min(r0 + 16 * kN - 1, R - 1) / G),
+                         p.window, p.sinks);
+    int n_vis = kWin ? win.total : nkb;
     if (kTab) {  // entries up to the last one that the tile can see
         const int lim = (qpos0 + min(r0 + 16 * kN - 1, R - 1) / G) >> 6;
         n_vis = 0;
@@ -109,7 +119,7 @@ __device__ __forceinline__ void decode4_item(const Attn4Params& p4, const Item& 
     int kbid = 0, kid = 0, vid = 0;
     auto load_ids = [&](int c) {
         const int e = max(min(e0 + w + kWaves4 * (64 * c + l), e1 - 1), 0);
-        kbid = kTab ? min(max(tab[e], 0), nkb - 1) : e;
+        kbid = kTab ? min(max(tab[e], 0), nkb - 1) : kWin ? win.block(e) : e;
         const int kp = kpt[kbid], vp = vpt[kbid];
         kid = static_cast<int>(clamp_page(kp, p4.k.max_page));
         vid = static_cast<int>(clamp_page(vp, p4.v.max_page));
@@ -184,7 +194,8 @@ __device__ __forceinline__ void decode4_item(const Attn4Params& p4, const Item& 
             }
         }
         int nan_at = kNoKey;  // the first position with a NaN value in this lane's output dims
-        if (x.kb >= mask_from) {
+        uint32_t nan_lo = 0, nan_hi = 0;  // kWin: the block's keys with one, a bit each
+        if (kWin ? win.cut(x.kb) : x.kb >= mask_from) {
             // value i of tile kt is key 64 kb + 16 kt + 4 g + i
             const int first = 64 * x.kb + 4 * g;
 #pragma unroll
@@ -194,15 +205,32 @@ __device__ __forceinline__ void decode4_item(const Attn4Params& p4, const Item& 
                     const int key = first + 16 * kt + e;
 #pragma unroll
                     for (int u = 0; u < kN; ++u)
-                        if (key > qpos[u]) sc[u][kt][e] = kNegInf;
+                        if (key > qpos[u] || (kWin && key <= qpos[u] - p.window && key >= p.sinks)) sc[u][kt][e] = kNegInf;
                     const bool bad = ((x.vs[kt] >> (8 * e)) & 0xffu) == kScaleNan;
-                    if (bad && key < kv_tokens) nan_at = min(nan_at, key);
+                    if (kWin) {
+                        const uint32_t bit = bad && key < kv_tokens ? 1u << ((16 * kt + 4 * g + e) & 31) : 0u;
+                        (kt < 2 ? nan_lo : nan_hi) |= bit;
+                    } else if (bad && key < kv_tokens) {
+                        nan_at = min(nan_at, key);
+                    }
                     if (bad || key >= kv_tokens) {
                         x.v[kt][e] = 0;
                         x.vs[kt] &= ~(0xffu << (8 * e));
                     }
                 }
-            if (__ballot(nan_at != kNoKey)) {
+            if (kWin && __ballot((nan_lo | nan_hi) != 0)) {
+                // as below: over the lanes that hold this group of dims, then to those whose output dims these are
+                auto gather = [&](uint32_t m) {
+                    m |= __shfl_xor(m, 1, 64);
+                    m |= __shfl_xor(m, 2, 64);
+                    m |= __shfl_xor(m, 16, 64);
+                    m |= __shfl_xor(m, 32, 64);
+                    return static_cast<uint32_t>(__shfl(m, 4 * g, 64));
+                };
+                nan_lo = gather(nan_lo);
+                nan_hi = gather(nan_hi);
+            }
+            if (!kWin && __ballot(nan_at != kNoKey)) {
                 // over the four lanes and the four lane groups that hold this group of dims, then to the
                 // lanes whose output dims these are: 8 (4 g + i) + j, group g
                 nan_at = min(nan_at, __shfl_xor(nan_at, 1, 64));
@@ -269,7 +297,7 @@ __device__ __forceinline__ void decode4_item(const Attn4Params& p4, const Item& 
         }
 #pragma unroll
         for (int u = 0; u < kN; ++u)
-            if (nan_at <= qpos[u]) {
+            if (kWin ? sees(nan_lo, nan_hi, qpos[u] - 64 * x.kb, p.window, p.sinks - 64 * x.kb) : nan_at <= qpos[u]) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -346,7 +374,7 @@ __device__ __forceinline__ void decode4_item(const Attn4Params& p4, const Item& 
 // 30.5, 64 requests of 4096, 3 caches 55.5, 50.5.  Slower only for one cache near that size again and again (64
 // requests of 4096, 285 MB, 47.2, 48.9).
 enum { kLoadsKept, kLoadsStreamed, kLoadsStreamedUnshared };
-template <int kN, bool kTab, int kLoads>
+template <int kN, bool kTab, int kLoads, bool kWin = false>
 __global__ __launch_bounds__(kWaves4 * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn4_decode_kernel(Attn4Params p4) {
     __shared__ __attribute__((aligned(16))) float mo[kWaves4 * 16 * kOStride4];
     __shared__ float ml[kWaves4 * 16 * 2];
@@ -358,9 +386,9 @@ __global__ __launch_bounds__(kWaves4 * 64) __attribute__((amdgpu_waves_per_eu(2)
     it.tile = __builtin_amdgcn_readfirstlane(it.tile);
     if (kLoads == kLoadsStreamed ||
         (kLoads == kLoadsStreamedUnshared && !shares_pages(p4.a, it, p4.k.page_table, p4.k.pts)))
-        decode4_item<kN, kTab, true>(p4, it, mo, ml);
+        decode4_item<kN, kTab, true, kWin>(p4, it, mo, ml);
     else
-        decode4_item<kN, kTab, false>(p4, it, mo, ml);
+        decode4_item<kN, kTab, false, kWin>(p4, it, mo, ml);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -383,11 +411,13 @@ struct Int4C {
     static constexpr int value = N;
 };
 
-template <bool kTab>
+template <bool kTab, bool kWin = false>
 __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn4_fwd_kernel(Attn4Params p4) {
     __shared__ __attribute__((aligned(16))) uint8_t smem[2 * kVRing4];
-    // by block modulo 4 and group of dims: the first key in the block with a NaN value (masked blocks)
+    // by block modulo 4 and group of dims: the first key in the block with a NaN value (masked blocks), kWin: a
+    // bit for every key with one
     __shared__ int vnan[4][4];
+    __shared__ uint32_t vbits[4][4][2];
     __shared__ int late[kNW];
     const AttnParams& p = p4.a;
     const Shape& s = p.s;
@@ -431,9 +461,14 @@ __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) v
             qf[ds] = qvalid ? *reinterpret_cast<const bf16x8_t*>(qp + 16 * ds) : __builtin_bit_cast(bf16x8_t, z);
         }
     }
-    if (tid < 16) vnan[tid >> 2][tid & 3] = 64;
+    const WindowList win(first_q, qpos0 + t_last, p.window, p.sinks);
+    if (kWin) {
+        if (tid < 32) (&vbits[0][0][0])[tid] = 0;
+    } else if (tid < 16) {
+        vnan[tid >> 2][tid & 3] = 64;
+    }
     // entries up to the last one that the tile can see
-    int n_vis = kTab ? 0 : min(nkb, lim + 1);
+    int n_vis = kTab ? 0 : kWin ? win.total : min(nkb, lim + 1);
     if (kTab) {
         for (int end = min(max(sload(p.counts + row), 0), s.cap); end > 0; end -= 64) {
             const int e = end - 1 - l;
@@ -449,7 +484,7 @@ __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) v
     const int nblk = min(n_vis, e0 + chunk) - e0;
     // blocks before the first masked one; a list's order is not relied on: every wave looks through an eighth
     const int whole = (first_q + 1) >> 6;  // blocks [0, whole) hold no key past the tile's first query
-    int n_un = min(max(whole - e0, 0), nblk);
+    int n_un = min(max((kWin ? win.full : whole) - e0, 0), nblk);
     if (kTab) {
         int first = nblk;
         for (int at = 64 * w; at < nblk; at += 64 * kNW) {
@@ -479,10 +514,10 @@ __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) v
     int cur_page = 0, next_page = 0;
     auto load_pages = [&](int c) {
         const int e = e0 + min(64 * c + l, nblk - 1);
-        const int id = kTab ? min(max(tab[e], 0), nkb - 1) : e;
+        const int id = kTab ? min(max(tab[e], 0), nkb - 1) : kWin ? win.block(e) : e;
         next_page = static_cast<int>(clamp_page(pt[id], kv.max_page));
     };
-    auto id_of = [&](int i) { return kTab ? min(max(sload(tab + e0 + i), 0), nkb - 1) : e0 + i; };
+    auto id_of = [&](int i) { return kTab ? min(max(sload(tab + e0 + i), 0), nkb - 1) : kWin ? win.block(e0 + i) : e0 + i; };
     // ---- a block's codes: memory -> registers (of this wave's cache; i asked for in ascending order) ----
     const int u = tid & 255;
     const int st_t = is_v ? 4 * (u >> 4) : u >> 2;  // token (of V: the first of four)
@@ -520,7 +555,8 @@ __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) v
             for (int i = 0; i < 4; ++i) {
                 const bool bad = ((x.scale >> (8 * i)) & 0xffu) == kScaleNan;
                 const bool there = first + i < kv_tokens;
-                if (bad && there) atomicMin(&vnan[block & 3][st_c >> 2], st_t + i);
+                if (kWin && bad && there) atomicOr(&vbits[block & 3][st_c >> 2][(st_t + i) >> 5], 1u << ((st_t + i) & 31));
+                if (!kWin && bad && there) atomicMin(&vnan[block & 3][st_c >> 2], st_t + i);
                 if (bad || !there) {
                     x.code[i] = 0;
                     x.scale &= ~(0xffu << (8 * i));
@@ -579,12 +615,13 @@ __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) v
     };
     auto mask = [&](int kb) {
         const int vis = qpos - 64 * kb - 8 * h;
+        const int past = kWin ? vis - p.window : 0, sink = kWin ? p.sinks - 64 * kb - 8 * h : 0;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const int key = kt * 32 + 16 * (e >> 3) + 4 * ((e >> 2) & 1) + (e & 3);
-                if (key > vis) sc[kt][e] = kNegInf;
+                if (key > vis || (kWin && key <= past && key >= sink)) sc[kt][e] = kNegInf;
             }
     };
     auto rise = [&](float mx) {
@@ -631,8 +668,9 @@ __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) v
         if (j >= n_un) {
 #pragma unroll
             for (int dt = 0; dt < 4; ++dt) {
-                const int at = vnan[j & 3][dt];
-                if (at < 64 && 64 * kb + at <= qpos)
+                const int at = kWin ? 64 : vnan[j & 3][dt];
+                if (kWin ? sees(vbits[j & 3][dt][0], vbits[j & 3][dt][1], qpos - 64 * kb, p.window, p.sinks - 64 * kb)
+                         : at < 64 && 64 * kb + at <= qpos)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) oacc[dt][e] = __builtin_nanf("");
             }
@@ -766,10 +804,15 @@ __global__ __launch_bounds__(kNW * 64) __attribute__((amdgpu_waves_per_eu(2))) v
             if (j + 1 < nblk) {
                 scores(((j + 1) & 3) * kPlace4);
                 const int kb = id_of(j + 1);
-                if (64 * kb + 63 > first_q) mask(kb);
+                if (kWin ? j + 1 >= n_un : 64 * kb + 63 > first_q) mask(kb);
                 block_max();
                 mid_slot();
-                if (tid < 4) vnan[(j + 3) & 3][tid] = 64;  // read last for block j - 1, written next for j + 3
+                // read last for block j - 1, written next for j + 3
+                if (kWin) {
+                    if (tid < 8) vbits[(j + 3) & 3][tid >> 1][tid & 1] = 0;
+                } else if (tid < 4) {
+                    vnan[(j + 3) & 3][tid] = 64;
+                }
                 stage(j);
             }
         }
@@ -958,11 +1001,12 @@ __global__ __launch_bounds__(256) void attn4_merge_rows_kernel(Merge4Params p) {
 // 256 over 8 + 4 11.7, 26.8; 256 over 64 + 4 (8.5 blocks a CU) 26.5, 41; 256 over 256 + 4 (32.5) 78.4, 75.3,
 // with 30 % kept 32.7, 42.5; 512 over 128 + 8 (34) 87.5, 77.2, with 30 % kept 43.6, 43.0.  (Not always: 300 over
 // 40 + 5 with 28 / 4 heads, 6.3 blocks a CU, 39.3, 33.3.)
-AttnTiling attn4_tiling(const Shape& s, const PastBlocks& pb, const int32_t* kv_len) {
+AttnTiling attn4_tiling(const Shape& s, const PastBlocks& pb, const int32_t* kv_len, int window, int sinks) {
     const bool dense = kv_len != nullptr;
     const int rows = s.Lq * s.G;
     int32_t qpos0[CA_MAX_BATCH], nkb[CA_MAX_BATCH];
     attn_positions(s, pb, kv_len, qpos0, nkb);
+    for (int b = 0; window > 0 && b < s.B; ++b) nkb[b] = attn_window_blocks(s, kBM, qpos0[b], window, sinks);
     double blocks = 0.0;  // of 256 rows
     for (int b = 0; b < s.B; ++b) blocks += (double)s.Hkv * ((rows + kBM - 1) / kBM) * nkb[b];
     if (rows <= 160 || blocks <= 12.0 * 256)
@@ -975,14 +1019,18 @@ AttnTiling attn4_tiling(const Shape& s, const PastBlocks& pb, const int32_t* kv_
 hipError_t launch_attn4(const AttnArgs& a, const Kv4Addr& k, const Kv4Addr& v, hipStream_t stream) {
     Attn4Params p;
     SplitPlan plan;
-    const AttnTiling tiling = attn4_tiling(a.s, a.pb, a.kv_len);
+    const AttnTiling tiling = attn4_tiling(a.s, a.pb, a.kv_len, a.window, a.sinks);
     attn_fill(a, tiling, &p.a, &plan);
     p.a.ws_unsplit = nullptr;  // a launch with splits keeps them
     p.k = k;
     p.v = v;
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(plan.per_xcd * 8), dim3(kNW * 64), 0, stream, p); };
     static_assert(kNW == kWaves4, "one workgroup size");
-    if (a.table)
+    if (a.window > 0)
+        tiling.tile_rows == 16   ? launch(attn4_decode_kernel<1, false, kLoadsStreamed, true>)
+        : tiling.tile_rows == 32 ? launch(attn4_decode_kernel<2, false, kLoadsKept, true>)
+                                 : launch(attn4_fwd_kernel<false, true>);
+    else if (a.table)
         tiling.streams ? launch(attn4_decode_kernel<2, true, kLoadsKept>) : launch(attn4_fwd_kernel<true>);
     else if (tiling.tile_rows == 16)
         a.s.B > 1 ? launch(attn4_decode_kernel<1, false, kLoadsStreamedUnshared>)

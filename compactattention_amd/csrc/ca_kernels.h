@@ -124,6 +124,7 @@ struct AttnArgs {
     int num_splits;  // > 0: every request uses this many splits; 0: per-request plan
     void* workspace;
     const int32_t* kv_len;  // decode: host array of per-request KV lengths (tokens); else null
+    int window = 0, sinks = 0;  // with kv_len: attention under a window (window > 0), any q_len
 };
 
 constexpr int kMaxPrefillSplits = 16;
@@ -172,16 +173,59 @@ struct AttnTiling {
 // dense = identity block lists over kv_len tokens (decode); otherwise per-row tables.  decode: whether few
 // rows may take the decode kernel.
 AttnTiling attn_tiling(const Shape& s, bool dense, bool decode = true);
-AttnTiling attn4_tiling(const Shape& s, const PastBlocks& pb, const int32_t* kv_len);
+AttnTiling attn4_tiling(const Shape& s, const PastBlocks& pb, const int32_t* kv_len, int window = 0, int sinks = 0);
+// The blocks of a request's longest list under a window, with tiles of tile_rows packed rows
+int attn_window_blocks(const Shape& s, int tile_rows, int qpos0, int window, int sinks);
 void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling& tiling, SplitPlan* plan);
 bool attn_uses_decode_kernel(const Shape& s, bool dense);
 void attn_positions(const Shape& s, const PastBlocks& pb, const int32_t* kv_len, int32_t* qpos0, int32_t* nkb);
 int attn_pick_splits(const Shape& s, const PastBlocks& pb, const int32_t* kv_len);
 int attn_pick_splits(const Shape& s, const PastBlocks& pb, const int32_t* kv_len, const AttnTiling& tiling);
+// The splits of a launch under a window, over bf16 pages or (bits4) pages held in 4 bits
+int attn_window_splits(const Shape& s, const int32_t* kv_len, int window, int sinks, bool bits4);
 int64_t attn_workspace_bytes(const Shape& s, int num_splits);
 hipError_t launch_attn(const AttnArgs& a, hipStream_t stream);
 // The same over pages held in 4 bits (a.k and a.v unused; ca_attn4.hip)
 hipError_t launch_attn4(const AttnArgs& a, const Kv4Addr& k, const Kv4Addr& v, hipStream_t stream);
+
+// The attention weight that keys received (ca_mass.hip): over bf16 keys (k) or keys held in 4 bits (k4), all blocks or the
+// table's
+struct MassArgs {
+    Shape s;
+    SeqAddr q;
+    const KvAddr* k;
+    const Kv4Addr* k4;
+    const int32_t* start;  // host: the position of every request's first query
+    const float* lse;
+    int64_t lse_sb, lse_sh;
+    const float* mass;
+    int64_t mass_stride;
+    float* out;  // may be mass
+    int64_t out_stride;
+    const int32_t* table;
+    int64_t table_stride;
+    const int32_t* counts;
+    float scale;
+    int window, sinks;  // window 0: none
+};
+hipError_t launch_key_mass(const MassArgs& a, hipStream_t stream);
+
+// Eviction (ca_evict.hip): the positions of the tokens that stay, and the copy of tokens into other pages
+hipError_t launch_heavy_tokens(const float* mass, int64_t mass_stride, int B, int Hkv, const int32_t* len, int budget, int sinks,
+                               int recent, int32_t* keep, int64_t keep_stride, hipStream_t stream);
+struct MoveArgs {
+    int B, Hkv, n;       // n: places of a row; request b fills min(n, len[b])
+    const int32_t* len;  // host: tokens of every request
+    const KvAddr *k, *v, *k_dst, *v_dst;       // either these
+    const Kv4Addr *k4, *v4, *k4_dst, *v4_dst;  // or these
+    const int32_t* keep;
+    int64_t keep_stride;
+    const float* mass;  // with mass_out, or neither
+    int64_t mass_stride;
+    float* mass_out;
+    int64_t mass_out_stride;
+};
+hipError_t launch_move_tokens(const MoveArgs& a, hipStream_t stream);
 
 // model plumbing (ca_model.hip)
 // x2 / y2 (nullable): a second tensor of H2 heads over the same tokens

@@ -841,6 +841,160 @@ def attn_decode(q: torch.Tensor, k: AnyKV, v: AnyKV, kv_len: Sequence[int], scal
     return (out, lse) if with_lse else out
 
 
+# ----------------------------------------------------------------------------- caches of bounded size
+def _cache_launch(name: str, caches: Sequence[AnyKV], *tensors: Optional[torch.Tensor]):
+    """The entry point for these caches (all bf16 or all in 4 bits) and the context to call it in."""
+    bits4 = isinstance(caches[0], KV4)
+    if any(isinstance(kv, KV4) != bits4 for kv in caches):
+        raise ValueError("the caches of a call must all be bf16 or all be held in 4 bits")
+    guard = _on_device(*tensors, *(t for kv in caches for t in (kv.tensor, kv.page_table)))
+    return getattr(_hip.lib(), name + "_q4" if bits4 else name), guard
+
+
+def attn_window(q: torch.Tensor, k: AnyKV, v: AnyKV, start: Union[int, Sequence[int]], window: int, sinks: int, scale: float,
+                kv_cap: int, num_kv_heads: int, out: Optional[torch.Tensor] = None, with_lse: bool = False,
+                num_splits: int = 0, workspace: Optional[torch.Tensor] = None):
+    """Attention under a sliding window with sink tokens: q/out [B, L, Hq, 128] bf16, query t of request b at position
+    p = start[b] + t (one start for all, or one per request) sees the keys j <= p with p - j < window or j < sinks.
+    Any L >= 1: single tokens, drafts, chunks.  K and V are bf16 (KV) or held in 4 bits (KV4) and hold start + L
+    tokens; of a paged cache only the blocks with a visible key need pages.  What a query does not see changes
+    nothing, whatever the cache holds there.  with_lse also returns the log-sum-exp [B, Hq, L] fp32."""
+    B, L, Hq, _ = q.shape
+    ql = seq_layout(q, "q")
+    if out is None:
+        out = torch.empty_like(q)
+    elif tuple(out.shape) != tuple(q.shape):
+        raise ValueError(f"out {tuple(out.shape)} must have q's shape {tuple(q.shape)}")
+    ol = seq_layout(out, "out")
+    sa, blocks = _starts(start, B, L)
+    for name, kv in (("k", k), ("v", v)):
+        kv.check_blocks(name, B, num_kv_heads, blocks, tokens=max(sa) + L)
+    entry, guard = _cache_launch("ca_attn_window", (k, v), q, out, workspace)
+    if L == 0:
+        return (out, torch.empty((B, Hq, 0), dtype=torch.float32, device=q.device)) if with_lse else out
+    d = make_dims(B, L, Hq, num_kv_heads, kv_cap)
+    lib = _hip.lib()
+    size = lib.ca_attn_window_q4_workspace_size if isinstance(k, KV4) else lib.ca_attn_window_workspace_size
+    need = size(ctypes.byref(d), sa, int(window), int(sinks), int(num_splits))
+    if need < 0:
+        raise _hip.CaError(int(need), _hip.last_error())
+    if need > 0 and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
+    lse = torch.empty((B, Hq, L), dtype=torch.float32, device=q.device) if with_lse else None
+    with guard:
+        check(entry(ctypes.byref(d), ctypes.byref(ql), ctypes.byref(k.layout), ctypes.byref(v.layout), sa, int(window),
+                    int(sinks), float(scale), ctypes.byref(ol), _ptr(lse), int(num_splits), _ptr(workspace), int(need),
+                    _stream()))
+    return (out, lse) if with_lse else out
+
+
+def _rows(name: str, t: torch.Tensor, dtype: torch.dtype, rows: int, columns: int) -> int:
+    """Checks a [>= rows, >= columns] tensor with contiguous rows; its stride from row to row."""
+    _need_cuda(name, t, dtype)
+    if t.dim() != 2 or t.stride(1) != 1 and t.shape[1] > 1 or t.shape[0] < rows or t.shape[1] < columns:
+        raise ValueError(f"{name} {tuple(t.shape)} must be [>= {rows}, >= {columns}] with contiguous rows")
+    if t.stride(0) < t.shape[1] and t.shape[0] > 1:
+        raise ValueError(f"{name}'s rows must not overlap")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def key_mass(q: torch.Tensor, k: AnyKV, lse: torch.Tensor, mass: torch.Tensor, start: Union[int, Sequence[int]], scale: float,
+             kv_cap: int, num_kv_heads: int, window: int = 0, sinks: int = 0, table: Optional[torch.Tensor] = None,
+             counts: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The attention weight that every cached key receives from queries q [B, L, Hq, 128] at positions start[b] + t, added
+    to mass [B*Hkv, >= tokens] fp32: in place, or with ``out`` (of that form) written there for the start + L tokens of
+    every request.  A key's weight is summed over the queries and the query heads of its KV group, exp(q . k * scale -
+    lse) with the lse [B, Hq, L] that attention returned (any strides over requests and heads, so the last tokens of a
+    chunk may be passed alone).  window 0: every earlier key; else as ``attn_window``.  table and counts (as for
+    ``attn_fwd``, ascending): only the blocks that the attention ran over.  Returns out, or mass."""
+    B, L, Hq, _ = q.shape
+    ql = seq_layout(q, "q")
+    sa, blocks = _starts(start, B, L)
+    rows, tokens = B * num_kv_heads, max(sa) + L
+    k.check_blocks("k", B, num_kv_heads, blocks, tokens=tokens)
+    _need_cuda("lse", lse, torch.float32)
+    if tuple(lse.shape) != (B, Hq, L) or L > 1 and lse.stride(2) != 1:
+        raise ValueError(f"lse {tuple(lse.shape)} must be [{B}, {Hq}, {L}] with a contiguous last dim")
+    ms = _rows("mass", mass, torch.float32, rows, tokens)
+    to, os_ = (mass, ms) if out is None else (out, _rows("out", out, torch.float32, rows, tokens))
+    if (table is None) != (counts is None):
+        raise ValueError("table and counts must both be given or both be None")
+    if table is not None:
+        _need_cuda("table", table, torch.int32)
+        _need_cuda("counts", counts, torch.int32)
+        if table.dim() != 2 or table.stride(1) != 1 or table.shape[0] < rows or table.shape[1] < kv_cap:
+            raise ValueError("table must be [B*Hkv, >= kv_cap] with contiguous rows")
+        if counts.numel() < rows or not counts.is_contiguous():
+            raise ValueError("counts must hold B*Hkv entries")
+    entry, guard = _cache_launch("ca_key_mass", (k,), q, lse, mass, to, table, counts)
+    if L == 0:
+        if out is not None:
+            for b, n in enumerate(sa):
+                out[b * num_kv_heads:(b + 1) * num_kv_heads, :n] = mass[b * num_kv_heads:(b + 1) * num_kv_heads, :n]
+        return to
+    d = make_dims(B, L, Hq, num_kv_heads, kv_cap)
+    with guard:
+        check(entry(ctypes.byref(d), ctypes.byref(ql), ctypes.byref(k.layout), lse.data_ptr(), lse.stride(0), lse.stride(1), sa,
+                    int(window), int(sinks), _ptr(table), 0 if table is None else table.stride(0), _ptr(counts),
+                    float(scale), mass.data_ptr(), ms, to.data_ptr(), os_, _stream()))
+    return to
+
+
+def heavy_tokens(mass: torch.Tensor, lengths: Union[int, Sequence[int]], num_kv_heads: int, budget: int, sinks: int = 0,
+                 recent: int = 0) -> torch.Tensor:
+    """Which tokens of every row of a cache stay: keep [B*Hkv, budget] int32 holds, in ascending order, the positions of
+    the first ``sinks``, the last ``recent`` and the heaviest others of the request's lengths[b] tokens (one length for
+    all, or one per request), budget in all, by mass [B*Hkv, >= tokens] fp32.  Of equal weights the lower position
+    stays; NaN counts least.  Rows of at most budget tokens keep all; -1 stands in the places past them."""
+    rows = mass.shape[0]
+    if num_kv_heads < 1 or rows % num_kv_heads or rows == 0:
+        raise ValueError(f"mass has {rows} rows for {num_kv_heads} KV heads")
+    B = rows // num_kv_heads
+    la = past_array([lengths] * B if isinstance(lengths, (int, np.integer)) else lengths, B)
+    ms = _rows("mass", mass, torch.float32, rows, max(la))
+    lib = _hip.lib()
+    need = lib.ca_heavy_tokens_workspace_size(B, num_kv_heads, la, int(budget))
+    if need < 0:
+        raise _hip.CaError(int(need), _hip.last_error())
+    keep = torch.empty((rows, int(budget)), dtype=torch.int32, device=mass.device)
+    workspace = torch.empty((need,), dtype=torch.uint8, device=mass.device) if need > 0 else None
+    with _on_device(mass):
+        check(lib.ca_heavy_tokens(mass.data_ptr(), ms, B, num_kv_heads, la, int(budget), int(sinks), int(recent),
+                                  keep.data_ptr(), keep.stride(0), _ptr(workspace), int(need), _stream()))
+    return keep
+
+
+def move_tokens(k: AnyKV, v: AnyKV, k_dst: AnyKV, v_dst: AnyKV, keep: torch.Tensor, lengths: Union[int, Sequence[int]],
+                num_kv_heads: int, mass: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Token i of row r of k_dst and v_dst becomes token keep[r, i] of k and v, for i < min(keep's columns, lengths[b]);
+    keep [B*Hkv, n] int32 as ``heavy_tokens`` returns it.  All four caches are bf16 or all held in 4 bits (whose bytes
+    are copied, not quantised again).  Source and destination may lie in one pool, but no page (of a contiguous cache
+    no token) that is read may be written.  With mass [B*Hkv, >= tokens] the weights follow: returns [B*Hkv, n] fp32,
+    0 past a row's tokens."""
+    _need_cuda("keep", keep, torch.int32)
+    if keep.dim() != 2 or num_kv_heads < 1 or keep.shape[0] % num_kv_heads or keep.shape[0] == 0:
+        raise ValueError(f"keep {tuple(keep.shape)} must be [B*Hkv, n] for {num_kv_heads} KV heads")
+    rows, n = keep.shape
+    B = rows // num_kv_heads
+    ks = _rows("keep", keep, torch.int32, rows, n)
+    la = past_array([lengths] * B if isinstance(lengths, (int, np.integer)) else lengths, B)
+    longest = max(la)
+    to = min(n, longest)
+    for name, kv, tokens in (("k", k, longest), ("v", v, longest), ("k_dst", k_dst, to), ("v_dst", v_dst, to)):
+        kv.check_blocks(name, B, num_kv_heads, -(-tokens // BLOCK), tokens=tokens)
+    ms, moved = 0, None
+    if mass is not None:
+        ms = _rows("mass", mass, torch.float32, rows, longest)
+        moved = torch.empty((rows, n), dtype=torch.float32, device=mass.device)
+    entry, guard = _cache_launch("ca_move_tokens", (k, v, k_dst, v_dst), keep, mass)
+    if n == 0:
+        return moved
+    with guard:
+        check(entry(*(ctypes.byref(kv.layout) for kv in (k, v, k_dst, v_dst)), keep.data_ptr(), ks, B, num_kv_heads, la, n,
+                    _ptr(mass), ms, _ptr(moved), n, _stream()))
+    return moved
+
+
 # ----------------------------------------------------------------------------- model plumbing
 def _rope_tables(cos: torch.Tensor, sin: torch.Tensor, L: int) -> None:
     for name, t in (("cos", cos), ("sin", sin)):

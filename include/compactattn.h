@@ -483,6 +483,81 @@ int64_t ca_attn_fwd_q4_workspace_size(const ca_dims* dims, const int32_t* past_b
 int64_t ca_attn_decode_q4_workspace_size(const ca_dims* dims, const int32_t* kv_len_host, int32_t num_splits);
 
 /*
+ * Attention under a sliding window with sink tokens (bf16 in, fp32 accumulate, bf16 out): query t of
+ * request b at position p = start_host[b] + t sees key j where j <= p, and p - j < window or
+ * j < sinks.  Any q_len >= 1 (a single token, a draft, a chunk) and any start >= 0 with
+ * start + q_len <= 64 kv_cap; q_len * group <= 2^24.  Only the blocks that hold a visible key are read
+ * (page table entries of others may hold anything).  q, out, lse, splits and workspace as for
+ * ca_attn_decode (num_splits 0 to 64).  What a query does not see changes nothing, whatever the cache
+ * holds there; a query that sees a NaN key gets NaN and an lse of NaN, a value that is not finite goes
+ * into the dims of the queries that see it (in 4 bits a NaN value makes its group's dims NaN).
+ */
+int ca_attn_window(const ca_dims* dims, const ca_seq_layout* q, const ca_kv_layout* k, const ca_kv_layout* v,
+                   const int32_t* start_host, int32_t window, int32_t sinks, float scale,
+                   const ca_seq_layout* out, float* lse, int32_t num_splits, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+int ca_attn_window_q4(const ca_dims* dims, const ca_seq_layout* q, const ca_kv4_layout* k, const ca_kv4_layout* v,
+                      const int32_t* start_host, int32_t window, int32_t sinks, float scale,
+                      const ca_seq_layout* out, float* lse, int32_t num_splits, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+int64_t ca_attn_window_workspace_size(const ca_dims* dims, const int32_t* start_host, int32_t window, int32_t sinks,
+                                      int32_t num_splits);
+int64_t ca_attn_window_q4_workspace_size(const ca_dims* dims, const int32_t* start_host, int32_t window,
+                                         int32_t sinks, int32_t num_splits);
+
+/*
+ * The attention weight that every cached key received, added up:
+ *     out[row][j] = mass[row][j] + sum over t, g with key j visible of exp(q_tg . k_j * scale - lse_tg)
+ * for j < start_host[b] + q_len, row = b*Hkv + kv_head, g its group's query heads; fp32, keys and queries
+ * bf16 (or keys in 4 bits), fp32 products, in an order that depends on the sizes only.  Visible: j <= p =
+ * start_host[b] + t, and with window > 0 also p - j < window or j < sinks.  lse (element (b, h, t) at
+ * b*lse_stride_b + h*lse_stride_h + t) is the log-sum-exp that attention returned; a query whose lse is
+ * -inf adds nothing.  mass and out are [rows, stride] fp32, stride >= the tokens of a row; out may be
+ * mass (else they must not overlap).  With table and counts (both or neither) only the blocks of row's list add weight, as
+ * attention over that list gave it: ascending block ids, none twice; the other keys of out get mass.
+ * NaN: a key that is NaN gets a NaN weight where a query sees it, a query or lse that is NaN gives one
+ * to every key that it sees; what is hidden changes nothing.
+ */
+int ca_key_mass(const ca_dims* dims, const ca_seq_layout* q, const ca_kv_layout* k, const float* lse,
+                int64_t lse_stride_b, int64_t lse_stride_h, const int32_t* start_host, int32_t window, int32_t sinks,
+                const int32_t* table, int64_t table_stride, const int32_t* counts, float scale, const float* mass,
+                int64_t mass_stride, float* out, int64_t out_stride, void* stream);
+int ca_key_mass_q4(const ca_dims* dims, const ca_seq_layout* q, const ca_kv4_layout* k, const float* lse,
+                   int64_t lse_stride_b, int64_t lse_stride_h, const int32_t* start_host, int32_t window,
+                   int32_t sinks, const int32_t* table, int64_t table_stride, const int32_t* counts, float scale,
+                   const float* mass, int64_t mass_stride, float* out, int64_t out_stride, void* stream);
+
+/*
+ * Which tokens of a row stay: keep[row][0 .. budget) gets, in ascending order, the positions of the first
+ * `sinks` and the last `recent` of request b's len_host[b] tokens and of the budget - sinks - recent
+ * heaviest others by mass[row] (of equal weights the lower position; NaN counts least).  A row of at most
+ * budget tokens keeps them all; places past them get -1.  batch <= 64, len_host[b] in [0, 2^30],
+ * sinks + recent <= budget, mass_stride >= every len, keep_stride >= budget.
+ * ca_heavy_tokens_workspace_size: the bytes of workspace that the call needs (0: NULL will do).
+ */
+int64_t ca_heavy_tokens_workspace_size(int32_t batch, int32_t num_kv_heads, const int32_t* len_host, int32_t budget);
+int ca_heavy_tokens(const float* mass, int64_t mass_stride, int32_t batch, int32_t num_kv_heads,
+                    const int32_t* len_host, int32_t budget, int32_t sinks, int32_t recent, int32_t* keep,
+                    int64_t keep_stride, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Copies tokens into other blocks of a cache: token i of row r of k_dst and v_dst becomes token
+ * keep[r][i] of k and v, for i < min(n, len_host[b]); keep as ca_heavy_tokens writes it (positions are
+ * taken into [0, len)).  k and k_dst may be one pool; no page or token that is read may be written.  The
+ * tokens behind a row's last one stay as they were, and ids outside the pool are written through nowhere.
+ * With mass and mass_out (both or neither) mass_out[r][i] = mass[r][keep[r][i]], 0 for
+ * min(n, len) <= i < n.
+ */
+int ca_move_tokens(const ca_kv_layout* k, const ca_kv_layout* v, const ca_kv_layout* k_dst,
+                   const ca_kv_layout* v_dst, const int32_t* keep, int64_t keep_stride, int32_t batch,
+                   int32_t num_kv_heads, const int32_t* len_host, int32_t n, const float* mass, int64_t mass_stride,
+                   float* mass_out, int64_t mass_out_stride, void* stream);
+int ca_move_tokens_q4(const ca_kv4_layout* k, const ca_kv4_layout* v, const ca_kv4_layout* k_dst,
+                      const ca_kv4_layout* v_dst, const int32_t* keep, int64_t keep_stride, int32_t batch,
+                      int32_t num_kv_heads, const int32_t* len_host, int32_t n, const float* mass,
+                      int64_t mass_stride, float* mass_out, int64_t mass_out_stride, void* stream);
+
+/*
  * Copies n pages inside each of n_pools (at most CA_MAX_POOLS) pools: page dst_host[i] becomes page
  * src_host[i].  The ids are host arrays, read before the call returns.  Every id lies in every pool,
  * no page is written twice and none that is read is written, pools do not overlap but for a pool
