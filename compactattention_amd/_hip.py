@@ -75,6 +75,7 @@ EXPORTED = (
     "ca_attn_window_q4_workspace_size",
     "ca_key_mass",
     "ca_key_mass_q4",
+    "ca_key_mass_workspace_size",
     "ca_heavy_tokens",
     "ca_heavy_tokens_workspace_size",
     "ca_move_tokens",
@@ -215,16 +216,17 @@ _SIGNATURES = {
                                       _P(SeqLayout), _vp, _i32, _vp, _i64, _vp]),
     "ca_attn_window_workspace_size": (ctypes.c_int64, [_P(Dims), _vp, _i32, _i32, _i32]),
     "ca_key_mass": (ctypes.c_int, [_P(Dims), _P(SeqLayout), _P(KvLayout), _vp, _i64, _i64, _vp, _i32, _i32, _vp, _i64,
-                                   _vp, _f32, _vp, _i64, _vp, _i64, _vp]),
+                                   _vp, _f32, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
     "ca_move_tokens": (ctypes.c_int, [_P(KvLayout), _P(KvLayout), _P(KvLayout), _P(KvLayout), _vp, _i64, _i32, _i32, _vp,
                                       _i32, _vp, _i64, _vp, _i64, _vp]),
     "ca_attn_window_q4": (ctypes.c_int, [_P(Dims), _P(SeqLayout), _P(Kv4Layout), _P(Kv4Layout), _vp, _i32, _i32, _f32,
                                       _P(SeqLayout), _vp, _i32, _vp, _i64, _vp]),
     "ca_attn_window_q4_workspace_size": (ctypes.c_int64, [_P(Dims), _vp, _i32, _i32, _i32]),
     "ca_key_mass_q4": (ctypes.c_int, [_P(Dims), _P(SeqLayout), _P(Kv4Layout), _vp, _i64, _i64, _vp, _i32, _i32, _vp, _i64,
-                                   _vp, _f32, _vp, _i64, _vp, _i64, _vp]),
+                                   _vp, _f32, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
     "ca_move_tokens_q4": (ctypes.c_int, [_P(Kv4Layout), _P(Kv4Layout), _P(Kv4Layout), _P(Kv4Layout), _vp, _i64, _i32, _i32, _vp,
                                       _i32, _vp, _i64, _vp, _i64, _vp]),
+    "ca_key_mass_workspace_size": (ctypes.c_int64, [_P(Dims), _vp, _i32]),
     "ca_heavy_tokens": (ctypes.c_int, [_vp, _i64, _i32, _i32, _vp, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp]),
     "ca_heavy_tokens_workspace_size": (ctypes.c_int64, [_i32, _i32, _vp, _i32]),
     "ca_rmsnorm": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i32, _f32, _vp]),

@@ -957,7 +957,8 @@ int attn_window(const ca_dims* dims, const ca_seq_layout* q, const int32_t* star
 template <typename Keys>
 int key_mass(const ca_dims* dims, const ca_seq_layout* q, const float* lse, int64_t lse_sb, int64_t lse_sh, const int32_t* start,
              int32_t window, int32_t sinks, const int32_t* table, int64_t table_stride, const int32_t* counts, float scale,
-             const float* mass, int64_t mass_stride, float* out, int64_t out_stride, void* stream, const Keys& keys) {
+             const float* mass, int64_t mass_stride, float* out, int64_t out_stride, void* workspace, int64_t workspace_bytes,
+             void* stream, const Keys& keys) {
     ca::MassArgs a{};
     int32_t kv_len[CA_MAX_BATCH];
     int max_nkb = 0, rc;
@@ -984,9 +985,18 @@ int key_mass(const ca_dims* dims, const ca_seq_layout* q, const float* lse, int6
         const float *m1 = mass + (rows - 1) * mass_stride + tokens, *o1 = out + (rows - 1) * out_stride + tokens;
         if (mass < o1 && out < m1) return fail(CA_ERR_INVALID, "mass and out overlap");
     }
-    // eight blocks a workgroup of 512 threads, fewer only in launches of few blocks; a launch has less than 2^32 threads
-    if ((int64_t)(max_nkb / 8 + 2) * a.s.B * a.s.Hkv >= (int64_t)1 << 23)
+    // four blocks a workgroup of 256 threads, 16 times that in launches of few blocks; a launch has less than 2^32 threads
+    if ((int64_t)(max_nkb / 4 + 2) * a.s.B * a.s.Hkv >= (int64_t)1 << 24)
         return fail(CA_ERR_LIMIT, "%d rows of up to %d blocks are too many", a.s.B * a.s.Hkv, max_nkb);
+    // 32-bit offsets from a KV row's queries and lse (to a tile of 32 rows past the last one)
+    auto span = [&](int64_t st, int64_t sh) { return (a.s.Lq + 64) * st + (int64_t)a.s.G * sh < (int64_t)1 << 31; };
+    if (!span(2 * a.q.st, 2 * a.q.sh) || !span(4, 4 * lse_sh))
+        return fail(CA_ERR_LIMIT, "the queries or lse of a KV head span 2^31 bytes");
+    const int64_t need = ca::key_mass_workspace_bytes(a.s, start, table != nullptr);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
+        return fail(CA_ERR_WORKSPACE, "the call needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)need,
+                    (long long)workspace_bytes);
+    a.workspace = workspace;
     a.start = start;
     a.lse = lse;
     a.lse_sb = lse_sb;
@@ -1018,8 +1028,8 @@ int check_rows(int32_t batch, int32_t hkv, const int32_t* len, int32_t n, const 
         if (len[b] > 1 << 30) return fail(CA_ERR_LIMIT, "len[%d]=%d beyond 2^30", b, len[b]);
         *longest = max(*longest, len[b]);
     }
-    // a workgroup a block of 64 tokens
-    if ((int64_t)batch * hkv * ((max(n, *longest) + 63) / 64) >= (int64_t)1 << 24)
+    // a workgroup of 256 threads a block of 64 tokens, or at most 32 of 1024 a row
+    if ((int64_t)batch * hkv * ((max(n, *longest) + 63) / 64) >= (int64_t)1 << 24 || (int64_t)batch * hkv >= (int64_t)1 << 17)
         return fail(CA_ERR_LIMIT, "batch=%d x num_kv_heads=%d rows of %d tokens are too many", batch, hkv, max(n, *longest));
     return CA_OK;
 }
@@ -1098,13 +1108,21 @@ int ca_attn_window_q4(const ca_dims* dims, const ca_seq_layout* q, const ca_kv4_
                        });
 }
 
+int64_t ca_key_mass_workspace_size(const ca_dims* dims, const int32_t* start_host, int32_t lists) {
+    ca::Shape s;
+    int32_t kv_len[CA_MAX_BATCH];
+    int max_nkb = 0;
+    if (check_start_dims(dims, start_host, &s, kv_len, &max_nkb) != CA_OK) return -1;
+    return ca::key_mass_workspace_bytes(s, start_host, lists != 0);
+}
+
 int ca_key_mass(const ca_dims* dims, const ca_seq_layout* q, const ca_kv_layout* k, const float* lse, int64_t lse_stride_b,
                 int64_t lse_stride_h, const int32_t* start_host, int32_t window, int32_t sinks, const int32_t* table,
                 int64_t table_stride, const int32_t* counts, float scale, const float* mass, int64_t mass_stride,
-                float* out, int64_t out_stride, void* stream) {
+                float* out, int64_t out_stride, void* workspace, int64_t workspace_bytes, void* stream) {
     ca::KvAddr ka;
     return key_mass(dims, q, lse, lse_stride_b, lse_stride_h, start_host, window, sinks, table, table_stride, counts, scale, mass,
-                    mass_stride, out, out_stride, stream, [&](int max_nkb, ca::MassArgs* a) {
+                    mass_stride, out, out_stride, workspace, workspace_bytes, stream, [&](int max_nkb, ca::MassArgs* a) {
                         a->k = &ka;
                         return check_kv(k, "k", max_nkb, &ka);
                     });
@@ -1113,10 +1131,11 @@ int ca_key_mass(const ca_dims* dims, const ca_seq_layout* q, const ca_kv_layout*
 int ca_key_mass_q4(const ca_dims* dims, const ca_seq_layout* q, const ca_kv4_layout* k, const float* lse,
                    int64_t lse_stride_b, int64_t lse_stride_h, const int32_t* start_host, int32_t window, int32_t sinks,
                    const int32_t* table, int64_t table_stride, const int32_t* counts, float scale, const float* mass,
-                   int64_t mass_stride, float* out, int64_t out_stride, void* stream) {
+                   int64_t mass_stride, float* out, int64_t out_stride,
+                   void* workspace, int64_t workspace_bytes, void* stream) {
     ca::Kv4Addr ka;
     return key_mass(dims, q, lse, lse_stride_b, lse_stride_h, start_host, window, sinks, table, table_stride, counts, scale, mass,
-                    mass_stride, out, out_stride, stream, [&](int max_nkb, ca::MassArgs* a) {
+                    mass_stride, out, out_stride, workspace, workspace_bytes, stream, [&](int max_nkb, ca::MassArgs* a) {
                         a->k4 = &ka;
                         return check_kv4(k, "k", max_nkb, &ka);
                     });
@@ -1125,7 +1144,7 @@ int ca_key_mass_q4(const ca_dims* dims, const ca_seq_layout* q, const ca_kv4_lay
 int64_t ca_heavy_tokens_workspace_size(int32_t batch, int32_t num_kv_heads, const int32_t* len_host, int32_t budget) {
     int longest = 0;
     if (check_rows(batch, num_kv_heads, len_host, budget, "budget", &longest) != CA_OK) return -1;
-    return 0;
+    return ca::heavy_tokens_workspace_bytes(batch * num_kv_heads, longest, budget);
 }
 
 int ca_heavy_tokens(const float* mass, int64_t mass_stride, int32_t batch, int32_t num_kv_heads, const int32_t* len_host,
@@ -1141,10 +1160,12 @@ int ca_heavy_tokens(const float* mass, int64_t mass_stride, int32_t batch, int32
     if (mass_stride < longest || keep_stride < budget)
         return fail(CA_ERR_INVALID, "rows of mass (%lld) and keep (%lld) do not hold %d tokens and %d places",
                     (long long)mass_stride, (long long)keep_stride, longest, budget);
-    (void)workspace;
-    (void)workspace_bytes;
+    const int64_t need = ca::heavy_tokens_workspace_bytes(batch * num_kv_heads, longest, budget);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
+        return fail(CA_ERR_WORKSPACE, "the call needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)need,
+                    (long long)workspace_bytes);
     hipError_t e = ca::launch_heavy_tokens(mass, mass_stride, batch, num_kv_heads, len_host, budget, sinks, recent, keep,
-                                           keep_stride, static_cast<hipStream_t>(stream));
+                                           keep_stride, workspace, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail(e, "heavy_tokens launch");
     return ok();
 }

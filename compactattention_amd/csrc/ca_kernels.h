@@ -207,12 +207,15 @@ struct MassArgs {
     const int32_t* counts;
     float scale;
     int window, sinks;  // window 0: none
+    void* workspace;    // of key_mass_workspace_bytes
 };
+int64_t key_mass_workspace_bytes(const Shape& s, const int32_t* start, bool lists);
 hipError_t launch_key_mass(const MassArgs& a, hipStream_t stream);
 
 // Eviction (ca_evict.hip): the positions of the tokens that stay, and the copy of tokens into other pages
 hipError_t launch_heavy_tokens(const float* mass, int64_t mass_stride, int B, int Hkv, const int32_t* len, int budget, int sinks,
-                               int recent, int32_t* keep, int64_t keep_stride, hipStream_t stream);
+                               int recent, int32_t* keep, int64_t keep_stride, void* workspace, hipStream_t stream);
+int64_t heavy_tokens_workspace_bytes(int rows, int longest, int budget);
 struct MoveArgs {
     int B, Hkv, n;       // n: places of a row; request b fills min(n, len[b])
     const int32_t* len;  // host: tokens of every request

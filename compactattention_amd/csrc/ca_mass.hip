@@ -1,11 +1,10 @@
 // The attention weight that every cached key received: out[row][j] = mass[row][j] + the sum over the queries and the
 // query heads of the row's group that see key j of exp(q . k_j * scale - lse).
 //
-// The scores are S^T = K Q^T (32x32x16 bf16 MFMAs, fp32), so a lane holds 16 keys of one query row, and the sum over
-// query rows stays in the lane until the end: one fma, exp2 and add a score, and no atomics.  A wave keeps the 64 keys of
-// one block in registers and goes through the packed query rows r = t * G + g, 32 at a time; K is read once.
-// kParts waves of a workgroup share a block, each with every kParts-th tile of rows, and join in LDS in a fixed order, so
-// results do not depend on what runs when.
+// The scores are S^T = K Q^T (16x16x32 bf16 MFMAs, fp32), so a lane holds keys of one query row, and the sum over query
+// rows stays in the lane until the end: one fma, exp2 and add a score, and no atomics.  A wave keeps the 64 keys of one
+// block in registers and goes through the packed query rows r = t * G + g, 16 at a time; K is read once.
+// Where waves share a block they join in a fixed order, so results do not depend on what runs when.
 
 #include <type_traits>
 
@@ -15,7 +14,7 @@
 namespace ca {
 namespace {
 
-constexpr int kMassWaves = 8;
+constexpr int kMassWaves = 4;
 
 struct MassParams {
     Shape s;
@@ -33,194 +32,371 @@ struct MassParams {
     int64_t out_stride;
     float scale_log2;
     int window, sinks;
-    int items;  // workgroups of a row
+    int items;      // workgroups of a row (and part)
+    int parts;      // of the query rows, with workgroups of their own
+    int part_tiles;  // tiles of query tokens of a part
+    float* ws;      // the parts' sums [parts][rows][ws_stride], null where there is one
+    int64_t ws_stride;
     int32_t start[CA_MAX_BATCH];
 };
 
-// kQ4: keys held in 4 bits.  kTab: the blocks of per-row lists, else all of them.
-template <bool kQ4, bool kTab, int kParts>
-__global__ __launch_bounds__(kMassWaves * 64) __attribute__((amdgpu_waves_per_eu(2))) void key_mass_kernel(MassParams p) {
-    constexpr int kBlocks = kMassWaves / kParts;  // of a workgroup
-    __shared__ float part[kMassWaves][64];
-    const Shape& s = p.s;
-    const int rows = s.B * s.Hkv;
-    // a row's workgroups on one XCD, whose L2 then holds its queries once
-    int row, item;
+// A workgroup's row, place in the row's list and part of the query rows.  A row's workgroups run on one XCD, whose L2 then
+// holds its queries once, where the rows divide over the XCDs.
+__device__ __forceinline__ void find_rows(const MassParams& p, int* row, int* item, int* cut) {
+    const int rows = p.s.B * p.s.Hkv, per = p.items * p.parts;
+    int k;
     if (rows % 8 == 0) {
-        const int k = blockIdx.x >> 3;
-        const int u = k / p.items;
-        row = (blockIdx.x & 7) + 8 * u;
-        item = k - u * p.items;
+        k = blockIdx.x >> 3;
+        const int u = k / per;
+        *row = (blockIdx.x & 7) + 8 * u;
+        k -= u * per;
     } else {
-        row = blockIdx.x / p.items;
-        item = blockIdx.x - row * p.items;
+        *row = blockIdx.x / per;
+        k = blockIdx.x - *row * per;
     }
+    *item = k / p.parts;
+    *cut = k - *item * p.parts;
+}
+
+// Blocks that a list leaves out keep their weights: a wave copies those before its entry e (from the one before it on), the
+// wave after the last entry those behind it.
+template <bool kTab>
+__device__ __forceinline__ void copy_rest(const MassParams& p, int row, int e, int count, int nkb, int tokens, int l) {
+    if (!kTab || p.out == p.mass || e > count) return;
+    const int32_t* tab = p.table + (int64_t)row * p.table_stride;
+    const int from = e == 0 ? 0 : min(max(tab[e - 1], 0), nkb - 1) + 1;
+    const int to = e < count ? min(max(tab[e], 0), nkb - 1) : nkb;
+    const int end = min(64 * to, tokens);
+    constexpr int kAtOnce = 8;
+    for (int j0 = 64 * from + l; j0 < end; j0 += 64 * kAtOnce) {
+        float x[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) x[i] = j0 + 64 * i < end ? p.mass[(int64_t)row * p.mass_stride + j0 + 64 * i] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+            if (j0 + 64 * i < end) p.out[(int64_t)row * p.out_stride + j0 + 64 * i] = x[i];
+    }
+}
+
+// The 64 keys of a block, bf16: lane (n = l % 16, g = l / 16) holds key 16 kt + n, of the 32 dims of step j the eight of
+// chunk(j, g) (the order of a product's dims is free where both operands share it).
+template <bool kQ4>
+struct Keys {
+    bf16x8_t f[4][4];
+    static __device__ __forceinline__ int chunk(int j, int g) { return kQ4 ? 4 * g + j : 4 * j + g; }
+    __device__ __forceinline__ void load(const MassParams& p, int row, int b, int hk, int kb, int tokens, int n, int g) {
+        if (kQ4) {
+            const uint8_t* page = p.k4.data + clamp_page(sload(p.k4.page_table + (int64_t)row * p.k4.pts + kb), p.k4.max_page) * p.k4.stride;
+            const uint32_t scales = *reinterpret_cast<const uint32_t*>(page + k4_scale(n, g));  // of tokens n, 16 + n, 32 + n, 48 + n
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt) {
+                const u32x4_t code = *reinterpret_cast<const u32x4_t*>(page + 64 * (16 * kt + n) + 16 * g);
+                const float sc = scale_of(scales, kt);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const u32x4_t x = {decode2<0>(code[j], sc), decode2<1>(code[j], sc), decode2<2>(code[j], sc), decode2<3>(code[j], sc)};
+                    f[kt][j] = __builtin_bit_cast(bf16x8_t, x);
+                }
+            }
+        } else {
+            const int64_t phys = p.k.page_table ? clamp_page(sload(p.k.page_table + (int64_t)row * p.k.pts + kb), p.k.max_page) : kb;
+            const uint16_t* base = p.k.data + b * p.k.sb + hk * p.k.sh + phys * p.k.sblk;
+            const int last = min(64, tokens - 64 * kb) - 1;
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt) {
+                // (past the cache's end: its last token, for a sum that nobody writes)
+                const uint16_t* kp = base + (int64_t)min(16 * kt + n, last) * p.k.stok;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f[kt][j] = *reinterpret_cast<const bf16x8_t*>(kp + 8 * chunk(j, g));
+            }
+        }
+    }
+};
+
+// acc += the weights that 16 query rows give to the block: lane (n, g) has row n, value i of acc[kt] is key
+// 16 kt + 4 g + i.  neg: -lse of the row in log2 units.  kMask: the row at position pos may not see the whole block (pos
+// -1: it sees nothing).
+template <bool kQ4, bool kMask>
+__device__ __forceinline__ void add_weights(const MassParams& p, const Keys<kQ4>& keys, const bf16x8_t (&q)[4], float neg, int pos, int kb,
+                                            int g, f32x4_t (&acc)[4]) {
+    f32x4_t sc[4];
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) sc[kt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) sc[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(keys.f[kt][j], q[j], sc[kt], 0, 0, 0);
+    // a row sees keys [0, hi] of the block, under a window those from lo on or before sink
+    const int hi = pos - 64 * kb - 4 * g;
+    const int lo = p.window > 0 ? hi - p.window + 1 : -64, sink = p.sinks - 64 * kb - 4 * g;
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int key = 16 * kt + i;  // + 4 g
+            const float wt = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kt][i], p.scale_log2, neg));
+            // (dropped by a select: a hidden key may hold anything)
+            acc[kt][i] += !kMask || ((key <= hi) & ((key >= lo) | (key < sink))) ? wt : 0.0f;
+        }
+}
+
+// -lse in log2 units; a query without a key (lse -inf) gives weights of 0
+__device__ __forceinline__ float neg_lse(float lse) {
+    return lse == -__builtin_inff() ? lse : lse * -1.4426950408889634f;
+}
+
+// The sum over the 16 query rows of the lanes: of 16 values a lane gives half away at every step, and lane (n, g) ends
+// with that of key 16 (n / 4) + 4 g + n % 4.
+template <int kHalf>
+__device__ __forceinline__ void give_half(float (&v)[16], int n) {  // lanes n and n ^ kHalf; that with the bit keeps the upper values
+    const bool up = (n & kHalf) != 0;
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i) {
+        const float give = up ? v[i] : v[i + kHalf];
+        const float keep = up ? v[i + kHalf] : v[i];
+        v[i] = keep + __shfl_xor(give, kHalf, 64);
+    }
+}
+__device__ __forceinline__ float sum_rows(const f32x4_t (&acc)[4], int n) {
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = acc[i >> 2][i & 3];
+    give_half<8>(v, n);
+    give_half<4>(v, n);
+    give_half<2>(v, n);
+    give_half<1>(v, n);
+    return v[0];
+}
+
+// At most 16 query rows (single tokens): one tile, a wave a block.  Bound by memory, K's bytes read once: one token over
+// 131072 tokens of 8 KV heads (277 MB with the weights) takes 45 us, 6.1 TB/s.  With 32x32 products, whose operand takes 32
+// bytes of a key at a time where these take 64, it took 197 us.
+template <bool kQ4, bool kTab>
+__global__ __launch_bounds__(kMassWaves * 64) __attribute__((amdgpu_waves_per_eu(3))) void key_mass_token_kernel(MassParams p) {
+    const Shape& s = p.s;
+    const int row = blockIdx.x / p.items;
     const int b = row / s.Hkv;
     const int hk = row - b * s.Hkv;
     const int G = s.G;
-    const int R = s.Lq * G;
+    const int start = p.start[b];
+    const int tokens = start + s.Lq;
+    const int nkb = (tokens + 63) >> 6;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l = threadIdx.x & 63;
+    const int n = l & 15;
+    const int g = l >> 4;
+    const int count = kTab ? min(max(sload(p.counts + row), 0), min(s.cap, nkb)) : nkb;
+    const int e = (blockIdx.x - row * p.items) * kMassWaves + w;
+    copy_rest<kTab>(p, row, e, count, nkb, tokens, l);
+    if (e >= count) return;
+    const int kb = kTab ? min(max(sload(p.table + (int64_t)row * p.table_stride + e), 0), nkb - 1) : e;
+    Keys<kQ4> keys;
+    keys.load(p, row, b, hk, kb, tokens, n, g);
+    const bool valid = n < s.Lq * G;
+    const int t = valid ? n / G : 0;
+    const int hq = hk * G + (valid ? n - t * G : 0);
+    const uint16_t* qp = p.q.data + b * p.q.sb + (int64_t)t * p.q.st + (int64_t)hq * p.q.sh;
+    bf16x8_t q[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[j] = *reinterpret_cast<const bf16x8_t*>(qp + 8 * keys.chunk(j, g));
+    const float neg = neg_lse(p.lse[b * p.lse_sb + (int64_t)hq * p.lse_sh + t]);
+    // the key whose sum this lane ends with, and its weight so far
+    const int key_at = 64 * kb + 16 * (n >> 2) + 4 * g + (n & 3);
+    const float old = key_at < tokens ? p.mass[(int64_t)row * p.mass_stride + key_at] : 0.0f;
+    f32x4_t acc[4];
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) acc[kt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    add_weights<kQ4, true>(p, keys, q, neg, valid ? start + t : -1, kb, g, acc);
+    const float sum = sum_rows(acc, n);
+    if (key_at < tokens) p.out[(int64_t)row * p.out_stride + key_at] = old + sum;
+}
+
+// ---------------------------------------------------------------------------------------
+// Many query rows.  Four waves, each with the 64 keys of a block in registers, go through the packed rows together, the rows of
+// 32 / G tokens at a time from LDS (two places in turn: while one is read the next tile, already in registers, goes to the other and the
+// one after it is on its way).  A launch may cut the tiles into parts of p.part_tiles, each with workgroups of its own;
+// their sums go to p.ws and are joined in order by key_mass_join_kernel.
+constexpr int kTileRows = 32;
+
+template <bool kQ4, bool kTab>
+__global__ __launch_bounds__(kMassWaves * 64) __attribute__((amdgpu_waves_per_eu(3))) void key_mass_rows_kernel(MassParams p) {
+    __shared__ __attribute__((aligned(16))) uint8_t tile[2][kTileRows * 256];
+    __shared__ float tile_neg[2][kTileRows];
+    const Shape& s = p.s;
+    int row, item, cut;
+    find_rows(p, &row, &item, &cut);
+    const int b = row / s.Hkv;
+    const int hk = row - b * s.Hkv;
+    const int G = s.G;
     const int start = p.start[b];
     const int tokens = start + s.Lq;
     const int nkb = (tokens + 63) >> 6;
     const int tid = threadIdx.x;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l = tid & 63;
-    const int n = l & 31;
-    const int h = l >> 5;
+    const int n = l & 15;
+    const int g = l >> 4;
     const int32_t* tab = kTab ? p.table + (int64_t)row * p.table_stride : nullptr;
     const int count = kTab ? min(max(sload(p.counts + row), 0), min(s.cap, nkb)) : nkb;
-    const float* mass = p.mass + (int64_t)row * p.mass_stride;
-    float* out = p.out + (int64_t)row * p.out_stride;
-    const int e = item * kBlocks + w / kParts;
-    const int sub = w % kParts;
+    const int e0 = item * kMassWaves;
+    const int e = e0 + w;
+    if (p.ws == nullptr) copy_rest<kTab>(p, row, e, count, nkb, tokens, l);
+    if (e0 >= count) return;
     const bool here = e < count;
-    const int kb = !here ? 0 : kTab ? min(max(sload(tab + e), 0), nkb - 1) : e;
+    const int kb = kTab ? min(max(sload(tab + min(e, count - 1)), 0), nkb - 1) : min(e, count - 1);
+    const int first_kb = kTab ? min(max(sload(tab + e0), 0), nkb - 1) : e0;  // of the workgroup's blocks
+    const int last_kb = kTab ? min(max(sload(tab + min(e0 + kMassWaves, count) - 1), 0), nkb - 1) : min(e0 + kMassWaves, count) - 1;
 
-    // blocks that the list leaves out keep their weights: those before an entry (after the one before it) go with the
-    // entry, those after the last one with the place after it
-    if (kTab && p.out != p.mass && sub == 0 && e <= count) {
-        const int from = e == 0 ? 0 : min(max(sload(tab + e - 1), 0), nkb - 1) + 1;
-        const int to = here ? kb : nkb;
-        for (int j = 64 * from + l; j < min(64 * to, tokens); j += 64) out[j] = mass[j];
+    Keys<kQ4> keys;
+    keys.load(p, row, b, hk, kb, tokens, n, g);
+
+    // ---- the tiles that see a key of the workgroup's blocks; those in [ua, ub) see all of them whole ----
+    // a tile is T whole tokens' rows: its rows' heads and tokens are the same in every tile
+    const int T = kTileRows / G;
+    const int tiles = (s.Lq + T - 1) / T;
+    auto first_tile = [&](int t) { return t >= s.Lq ? tiles : max(t, 0) / T; };                     // with token t
+    auto tile_after = [&](int t) { return t >= s.Lq ? tiles : (max(t, 0) + T - 1) / T; };           // past the tokens before t
+    const bool edge = p.window > 0 && 64 * first_kb >= p.sinks;  // (blocks with sinks are seen to the end)
+    const int part0 = cut * p.part_tiles, part1 = part0 + p.part_tiles;
+    const int u0 = max(first_tile(64 * first_kb - start), part0);
+    const int u1 = max(min(edge ? tile_after(64 * last_kb - start + 63 + p.window) : tiles, part1), u0);
+    const int ua = min(max(tile_after(64 * last_kb - start + 63), u0), u1);
+    const bool always = p.window == 0 || 64 * last_kb + 64 <= p.sinks;
+    const int ub = max(min(always ? s.Lq / T : min(first_tile(64 * first_kb - start + p.window), s.Lq / T), u1), ua);
+    // Thread tid moves chunk tid % 16 of rows tid / 16 and 16 + tid / 16 of a tile, and tid < 32 the lse of row tid; chunk c
+    // of row r stands at chunk c ^ (r % 16), for reads without bank conflicts.  Rows past T tokens' (where the group does not
+    // divide 32) and past the last token are the last one's with weights of 0.
+    const int q_sh = static_cast<int>(p.q.sh) * 2, q_st = static_cast<int>(p.q.st) * 2;  // bytes (the host checks their range)
+    const int lse_sh = static_cast<int>(p.lse_sh) * 4;
+    const __amdgpu_buffer_rsrc_t q_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        p.q.data + b * p.q.sb + (int64_t)hk * G * p.q.sh, 0, (s.Lq - 1) * q_st + (G - 1) * q_sh + 256, 0x00020000);
+    const __amdgpu_buffer_rsrc_t lse_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<float*>(p.lse) + b * p.lse_sb + (int64_t)hk * G * p.lse_sh, 0, (s.Lq - 1) * 4 + (G - 1) * lse_sh + 4, 0x00020000);
+    const int c = tid & 15;
+    int at[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = min(16 * i + (tid >> 4), T * G - 1);
+        at[i] = r / G * q_st + r % G * q_sh + 16 * c;
     }
-
-    float acc[2][16];
+    const int lse_r = min(tid & 31, T * G - 1), lse_t = lse_r / G;
+    const int lse_at = lse_t * 4 + lse_r % G * lse_sh;
+    const bool lse_row = (tid & 31) < T * G;
+    u32x4_t held[2];
+    float held_neg = 0.0f;
+    auto fetch = [&](int u) {  // (a token past the last one: out of the range and zero, or another row's; the range check
+                                // covers the vector offset only)
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) acc[kt][j] = 0.0f;
-
-    if (here) {
-        // ---- keys: lane (n, h) holds key 32 kt + n, of the 16 dims of step ds the eight from dim(ds) on ----
-        auto dim = [&](int ds) { return kQ4 ? 32 * (2 * (ds >> 2) + h) + 8 * (ds & 3) : 16 * ds + 8 * h; };
-        bf16x8_t kf[2][8];
-        const int rows_here = min(64, tokens - 64 * kb);
-        if (kQ4) {
-            const uint8_t* page = p.k4.data + clamp_page(sload(p.k4.page_table + (int64_t)row * p.k4.pts + kb), p.k4.max_page) * p.k4.stride;
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int t = 32 * kt + n, g = 2 * c + h;
-                    const u32x4_t code = *reinterpret_cast<const u32x4_t*>(page + 64 * t + 16 * g);
-                    const float sc = scale_of(page[k4_scale(t, g)], 0);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const u32x4_t x = {decode2<0>(code[i], sc), decode2<1>(code[i], sc), decode2<2>(code[i], sc), decode2<3>(code[i], sc)};
-                        kf[kt][4 * c + i] = __builtin_bit_cast(bf16x8_t, x);
-                    }
-                }
-        } else {
-            const int64_t phys = p.k.page_table ? clamp_page(sload(p.k.page_table + (int64_t)row * p.k.pts + kb), p.k.max_page) : kb;
-            const uint16_t* base = p.k.data + b * p.k.sb + hk * p.k.sh + phys * p.k.sblk;
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                // (past the cache's end: its last token, whose place is written by nobody here)
-                const uint16_t* kp = base + (int64_t)min(32 * kt + n, rows_here - 1) * p.k.stok;
-#pragma unroll
-                for (int ds = 0; ds < 8; ++ds) kf[kt][ds] = *reinterpret_cast<const bf16x8_t*>(kp + dim(ds));
-            }
+        for (int i = 0; i < 2; ++i) held[i] = __builtin_amdgcn_raw_buffer_load_b128(q_rsrc, at[i] + u * T * q_st, 0, 0);
+        if (tid < kTileRows) {
+            const float lse = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(lse_rsrc, lse_at + u * T * 4, 0, 0));
+            held_neg = lse_row && u * T + lse_t < s.Lq ? neg_lse(lse) : -__builtin_inff();
         }
-        // ---- query tiles that see the block ----
-        // first: t >= 64 kb - start; last (windows): t <= 64 kb + 63 + window - 1 - start, unless sinks lie in it
-        const int tiles = (R + 31) >> 5;
-        const int t_from = max(64 * kb - start, 0);
-        const int t_to = p.window > 0 && 64 * kb >= p.sinks ? min(64 * kb - start + 62 + p.window, s.Lq - 1) : s.Lq - 1;
-        const int u0 = (int)(((int64_t)t_from * G) >> 5);
-        const int u1 = t_to < t_from ? 0 : min(tiles, (int)(((int64_t)(t_to + 1) * G + 31) >> 5));
-        struct Tile {
-            bf16x8_t q[8];
-            float neg;  // -lse in log2 units
-            int pos;    // the query's position, -1 where there is none or it sees no key
-        };
-        auto load = [&](int u) {
-            Tile x;
-            const int r = 32 * u + n;
-            const bool valid = r < R;
-            const int t = valid ? r / G : 0;
-            const int hq = hk * G + (valid ? r - t * G : 0);
-            const uint16_t* qp = p.q.data + b * p.q.sb + (int64_t)t * p.q.st + (int64_t)hq * p.q.sh;
+    };
+    const int to_lds = (tid >> 4) * 256 + ((c ^ (tid >> 4)) * 16);
+    auto put = [&](int to) {
 #pragma unroll
-            for (int ds = 0; ds < 8; ++ds) x.q[ds] = *reinterpret_cast<const bf16x8_t*>(qp + dim(ds));
-            const float lse = p.lse[b * p.lse_sb + (int64_t)hq * p.lse_sh + t];
-            x.neg = -lse * 1.4426950408889634f;
-            x.pos = valid && lse != -__builtin_inff() ? start + t : -1;
-            return x;
-        };
-        auto compute = [&](const Tile& x, int u) {
-            f32x16_t sc[2];
+        for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4_t*>(tile[to] + to_lds + 4096 * i) = held[i];
+        if (tid < kTileRows) tile_neg[to][tid] = held_neg;
+    };
+    int row_t[2];  // the token of the lane's rows in a tile, none's past T tokens' rows
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+    for (int i = 0; i < 2; ++i) row_t[i] = 16 * i + n < T * G ? (16 * i + n) / G : -(1 << 30);
+    f32x4_t acc[4];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) sc[kt][j] = 0.0f;
+    for (int kt = 0; kt < 4; ++kt) acc[kt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    auto run = [&](int u, int end, auto masked) {
+        constexpr bool kMask = decltype(masked)::value;
+        for (; u < end; ++u) {
+            const int from = (u - u0) & 1;
+            if (u + 1 < u1) put(from ^ 1);
+            if (u + 2 < u1) fetch(u + 2);
 #pragma unroll
-            for (int ds = 0; ds < 8; ++ds)
+            for (int i = 0; i < 2; ++i) {
+                bf16x8_t q[4];
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt) sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kt][ds], x.q[ds], sc[kt], 0, 0, 0);
-            // whole: every row of the tile sees the whole block
-            // (a row without a key, at -1, sees none)
-            const bool whole = x.pos >= 64 * kb + 63 && (p.window == 0 || x.pos - 64 * kb < p.window || 64 * kb + 63 < p.sinks);
-            if (__ballot(!whole) == 0) {
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) acc[kt][j] += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kt][j], p.scale_log2, x.neg));
-            } else {
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int key = 64 * kb + 32 * kt + 8 * (j >> 2) + 4 * h + (j & 3);
-                        const bool seen = key <= x.pos && (p.window == 0 || x.pos - key < p.window || key < p.sinks);
-                        const float wt = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kt][j], p.scale_log2, x.neg));
-                        acc[kt][j] += seen ? wt : 0.0f;
-                    }
+                for (int j = 0; j < 4; ++j)
+                    q[j] = *reinterpret_cast<const bf16x8_t*>(tile[from] + 4096 * i + n * 256 + ((keys.chunk(j, g) ^ n) * 16));
+                const int t = u * T + row_t[i];
+                add_weights<kQ4, kMask>(p, keys, q, tile_neg[from][16 * i + n], kMask && t >= 0 && t < s.Lq ? start + t : -1, kb, g, acc);
             }
-            (void)u;
-        };
-        int u = u0 + sub;
-        if (u < u1) {
-            Tile a = load(u);
-            for (; u < u1; u += kParts) {
-                Tile next = a;
-                if (u + kParts < u1) next = load(u + kParts);
-                compute(a, u);
-                a = next;
-            }
+            __syncthreads();
         }
-    }
-
-    // ---- the sum over the 32 query rows of the lanes: of 32 values a lane gives half away at every step ----
-    float v[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = acc[i >> 4][i & 15];
-#pragma unroll
-    for (int step = 0; step < 5; ++step) {
-        const int half = 16 >> step;  // lanes n and n ^ half; the one whose bit is set keeps the upper values
-        const bool up = (n & half) != 0;
-#pragma unroll
-        for (int i = 0; i < half; ++i) {
-            const float give = up ? v[i] : v[i + half];
-            const float keep = up ? v[i + half] : v[i];
-            v[i] = keep + __shfl_xor(give, half, 64);
-        }
-    }
-    // lane (n, h) now holds the sum of value n: kt = n / 16, j = n % 16
-    const int key = 32 * (n >> 4) + 8 * ((n & 15) >> 2) + 4 * h + (n & 3);
-    float sum = v[0];
-    if (kParts > 1) {
-        part[w][l] = sum;
+    };
+    if (u0 < u1) {
+        fetch(u0);
+        put(0);
+        if (u0 + 1 < u1) fetch(u0 + 1);
         __syncthreads();
-        if (sub != 0) return;
-        sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kParts; ++i) sum += part[w + i][l];
+        run(u0, ua, std::true_type{});
+        run(ua, ub, std::false_type{});
+        run(ub, u1, std::true_type{});
     }
-    const int j = 64 * kb + key;
-    if (here && j < tokens) out[j] = mass[j] + sum;
+    const float sum = sum_rows(acc, n);
+    if (!here) return;
+    const int key = 16 * (n >> 2) + 4 * g + (n & 3);
+    if (p.ws != nullptr) {
+        p.ws[((int64_t)cut * s.B * s.Hkv + row) * p.ws_stride + 64 * e + key] = sum;
+    } else if (64 * kb + key < tokens) {
+        const int64_t j = 64 * kb + key;
+        p.out[(int64_t)row * p.out_stride + j] = p.mass[(int64_t)row * p.mass_stride + j] + sum;
+    }
+}
+
+// The parts' sums added to the weights, a wave a block.
+template <bool kTab>
+__global__ __launch_bounds__(kMassWaves * 64) void key_mass_join_kernel(MassParams p) {
+    const Shape& s = p.s;
+    const int rows = s.B * s.Hkv;
+    const int row = blockIdx.x / p.items;
+    const int e = (blockIdx.x - row * p.items) * kMassWaves + (threadIdx.x >> 6);
+    const int l = threadIdx.x & 63;
+    const int tokens = p.start[row / s.Hkv] + s.Lq;
+    const int nkb = (tokens + 63) >> 6;
+    const int count = kTab ? min(max(p.counts[row], 0), min(s.cap, nkb)) : nkb;
+    copy_rest<kTab>(p, row, e, count, nkb, tokens, l);
+    if (e >= count) return;
+    const int kb = kTab ? min(max(p.table[(int64_t)row * p.table_stride + e], 0), nkb - 1) : e;
+    if (64 * kb + l >= tokens) return;
+    float sum = 0.0f;
+    for (int i = 0; i < p.parts; ++i) sum += p.ws[((int64_t)i * rows + row) * p.ws_stride + 64 * e + l];
+    const int64_t j = 64 * kb + l;
+    p.out[(int64_t)row * p.out_stride + j] = p.mass[(int64_t)row * p.mass_stride + j] + sum;
+}
+
+struct MassPlan {
+    bool rows;       // key_mass_rows_kernel, else a block a wave (key_mass_token_kernel)
+    int parts;       // rows: of the queries
+    int part_tiles;
+};
+
+// The query tiles are cut into parts where the blocks alone are too few to fill the CUs a few times over (a list is taken
+// to name a quarter of the blocks), with 8 tiles or more to a part.
+MassPlan key_mass_plan(const Shape& s, const int32_t* start, bool lists) {
+    int64_t blocks = 0;
+    for (int b = 0; b < s.B; ++b) blocks += (int64_t)s.Hkv * ((start[b] + s.Lq + 63) / 64);
+    if (lists) blocks = (blocks + 3) / 4;
+    MassPlan plan{s.Lq * s.G > 16, 1, 0};
+    const int T = kTileRows / s.G, tiles = (s.Lq + T - 1) / T;
+    const int64_t groups = (blocks + kMassWaves - 1) / kMassWaves;
+    int parts = 1;
+    while (plan.rows && parts < 16 && tiles >= 16 * parts && groups * parts < 2048) ++parts;
+    const int per = (tiles + parts - 1) / parts;
+    plan.parts = (tiles + per - 1) / per;
+    plan.part_tiles = per;
+    return plan;
 }
 
 }  // namespace
+
+int64_t key_mass_workspace_bytes(const Shape& s, const int32_t* start, bool lists) {
+    const MassPlan plan = key_mass_plan(s, start, lists);
+    if (!plan.rows || plan.parts <= 1) return 0;
+    int nkb = 1;
+    for (int b = 0; b < s.B; ++b) nkb = max(nkb, (start[b] + s.Lq + 63) / 64);
+    const int64_t items = (nkb + (lists ? 1 : 0) + kMassWaves - 1) / kMassWaves;
+    return (int64_t)plan.parts * s.B * s.Hkv * items * kMassWaves * 64 * (int64_t)sizeof(float);
+}
 
 hipError_t launch_key_mass(const MassArgs& a, hipStream_t stream) {
     MassParams p{};
@@ -242,34 +418,36 @@ hipError_t launch_key_mass(const MassArgs& a, hipStream_t stream) {
     p.window = a.window;
     p.sinks = a.sinks;
     int nkb = 1;
-    int64_t blocks = 0;
     for (int b = 0; b < a.s.B; ++b) {
         p.start[b] = a.start[b];
-        const int n = (a.start[b] + a.s.Lq + 63) / 64;
-        nkb = max(nkb, n);
-        blocks += (int64_t)a.s.Hkv * n;
+        nkb = max(nkb, (a.start[b] + a.s.Lq + 63) / 64);
     }
-    if (a.table) blocks = (blocks + 3) / 4;
-    const int tiles = (a.s.Lq * a.s.G + 31) / 32;
-    int parts = 1;
-    while (parts < 8 && tiles >= 2 * parts && blocks * parts < 8 * 512) parts *= 2;
-    const int per = kMassWaves / parts;
-    p.items = (nkb + (a.table ? 1 : 0) + per - 1) / per;  // (a list's last place copies what follows it)
-    const int64_t grid = (int64_t)p.items * a.s.B * a.s.Hkv;
-    auto launch = [&](auto kernel) {
+    const MassPlan plan = key_mass_plan(a.s, a.start, a.table != nullptr);
+    const int rows = a.s.B * a.s.Hkv;
+    const int entries = nkb + (a.table ? 1 : 0);  // (a list's last place copies what follows it)
+    p.items = (entries + kMassWaves - 1) / kMassWaves;
+    p.parts = plan.parts;
+    p.part_tiles = plan.part_tiles;
+    p.ws = plan.parts > 1 ? static_cast<float*>(a.workspace) : nullptr;
+    p.ws_stride = (int64_t)64 * kMassWaves * p.items;
+    auto launch = [&](auto kernel, int64_t grid) {
         hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(kMassWaves * 64), 0, stream, p);
     };
-    auto pick = [&](auto n) {
-        constexpr int kParts = decltype(n)::value;
+    const int64_t grid = (int64_t)p.items * rows;
+    if (!plan.rows) {
         if (a.k4)
-            a.table ? launch(key_mass_kernel<true, true, kParts>) : launch(key_mass_kernel<true, false, kParts>);
+            a.table ? launch(key_mass_token_kernel<true, true>, grid) : launch(key_mass_token_kernel<true, false>, grid);
         else
-            a.table ? launch(key_mass_kernel<false, true, kParts>) : launch(key_mass_kernel<false, false, kParts>);
-    };
-    if (parts == 1) pick(std::integral_constant<int, 1>{});
-    else if (parts == 2) pick(std::integral_constant<int, 2>{});
-    else if (parts == 4) pick(std::integral_constant<int, 4>{});
-    else pick(std::integral_constant<int, 8>{});
+            a.table ? launch(key_mass_token_kernel<false, true>, grid) : launch(key_mass_token_kernel<false, false>, grid);
+        return hipGetLastError();
+    }
+    if (a.k4)
+        a.table ? launch(key_mass_rows_kernel<true, true>, grid * p.parts) : launch(key_mass_rows_kernel<true, false>, grid * p.parts);
+    else
+        a.table ? launch(key_mass_rows_kernel<false, true>, grid * p.parts) : launch(key_mass_rows_kernel<false, false>, grid * p.parts);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.parts == 1) return e;
+    a.table ? launch(key_mass_join_kernel<true>, grid) : launch(key_mass_join_kernel<false>, grid);
     return hipGetLastError();
 }
 

@@ -900,7 +900,8 @@ def _rows(name: str, t: torch.Tensor, dtype: torch.dtype, rows: int, columns: in
 
 def key_mass(q: torch.Tensor, k: AnyKV, lse: torch.Tensor, mass: torch.Tensor, start: Union[int, Sequence[int]], scale: float,
              kv_cap: int, num_kv_heads: int, window: int = 0, sinks: int = 0, table: Optional[torch.Tensor] = None,
-             counts: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+             counts: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+             workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The attention weight that every cached key receives from queries q [B, L, Hq, 128] at positions start[b] + t, added
     to mass [B*Hkv, >= tokens] fp32: in place, or with ``out`` (of that form) written there for the start + L tokens of
     every request.  A key's weight is summed over the queries and the query heads of its KV group, exp(q . k * scale -
@@ -926,17 +927,22 @@ def key_mass(q: torch.Tensor, k: AnyKV, lse: torch.Tensor, mass: torch.Tensor, s
             raise ValueError("table must be [B*Hkv, >= kv_cap] with contiguous rows")
         if counts.numel() < rows or not counts.is_contiguous():
             raise ValueError("counts must hold B*Hkv entries")
-    entry, guard = _cache_launch("ca_key_mass", (k,), q, lse, mass, to, table, counts)
+    entry, guard = _cache_launch("ca_key_mass", (k,), q, lse, mass, to, table, counts, workspace)
     if L == 0:
         if out is not None:
             for b, n in enumerate(sa):
                 out[b * num_kv_heads:(b + 1) * num_kv_heads, :n] = mass[b * num_kv_heads:(b + 1) * num_kv_heads, :n]
         return to
     d = make_dims(B, L, Hq, num_kv_heads, kv_cap)
+    need = _hip.lib().ca_key_mass_workspace_size(ctypes.byref(d), sa, table is not None)
+    if need < 0:
+        raise _hip.CaError(int(need), _hip.last_error())
+    if need > 0 and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
     with guard:
         check(entry(ctypes.byref(d), ctypes.byref(ql), ctypes.byref(k.layout), lse.data_ptr(), lse.stride(0), lse.stride(1), sa,
                     int(window), int(sinks), _ptr(table), 0 if table is None else table.stride(0), _ptr(counts),
-                    float(scale), mass.data_ptr(), ms, to.data_ptr(), os_, _stream()))
+                    float(scale), mass.data_ptr(), ms, to.data_ptr(), os_, _ptr(workspace), int(need), _stream()))
     return to
 
 

@@ -515,17 +515,21 @@ int64_t ca_attn_window_q4_workspace_size(const ca_dims* dims, const int32_t* sta
  * -inf adds nothing.  mass and out are [rows, stride] fp32, stride >= the tokens of a row; out may be
  * mass (else they must not overlap).  With table and counts (both or neither) only the blocks of row's list add weight, as
  * attention over that list gave it: ascending block ids, none twice; the other keys of out get mass.
+ * ca_key_mass_workspace_size: the bytes of workspace that a call needs, with lists or without (0: NULL will do).
  * NaN: a key that is NaN gets a NaN weight where a query sees it, a query or lse that is NaN gives one
  * to every key that it sees; what is hidden changes nothing.
  */
 int ca_key_mass(const ca_dims* dims, const ca_seq_layout* q, const ca_kv_layout* k, const float* lse,
                 int64_t lse_stride_b, int64_t lse_stride_h, const int32_t* start_host, int32_t window, int32_t sinks,
                 const int32_t* table, int64_t table_stride, const int32_t* counts, float scale, const float* mass,
-                int64_t mass_stride, float* out, int64_t out_stride, void* stream);
+                int64_t mass_stride, float* out, int64_t out_stride, void* workspace, int64_t workspace_bytes,
+                void* stream);
 int ca_key_mass_q4(const ca_dims* dims, const ca_seq_layout* q, const ca_kv4_layout* k, const float* lse,
                    int64_t lse_stride_b, int64_t lse_stride_h, const int32_t* start_host, int32_t window,
                    int32_t sinks, const int32_t* table, int64_t table_stride, const int32_t* counts, float scale,
-                   const float* mass, int64_t mass_stride, float* out, int64_t out_stride, void* stream);
+                   const float* mass, int64_t mass_stride, float* out, int64_t out_stride, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+int64_t ca_key_mass_workspace_size(const ca_dims* dims, const int32_t* start_host, int32_t lists);
 
 /*
  * Which tokens of a row stay: keep[row][0 .. budget) gets, in ascending order, the positions of the first

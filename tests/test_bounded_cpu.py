@@ -89,7 +89,7 @@ def test_key_mass_refusals(bits4, change, code, text):
     a.update(change)
     entry = getattr(_hip.lib(), "ca_key_mass_q4" if bits4 else "ca_key_mass")
     refused(entry(dims(), seq(), kv4() if bits4 else kv(), a["lse"], a["lse_stride"], 50, a["start"], a["window"], a["sinks"], a["table"],
-                  a["table_stride"], a["counts"], a["scale"], a["mass"], a["mass_stride"], a["out"], a["out_stride"], None), code, text)
+                  a["table_stride"], a["counts"], a["scale"], a["mass"], a["mass_stride"], a["out"], a["out_stride"], None, 0, None), code, text)
 
 
 @pytest.mark.parametrize("change,code,text", [
