@@ -807,7 +807,8 @@ constexpr int kDecRows = 16;
 constexpr int kDecVBytes = 64 * 256;
 constexpr int kDecOStride = 132;  // floats per row of a wave's partial O in LDS (padded)
 
-// One work item.  kStream: K and V are loaded with the non-temporal hint.  kWin: the blocks of a window (WindowList).
+// One work item.  kStream: K and V are loaded with the non-temporal hint.  kWin: the blocks of a window (WindowList), and
+// more than 16 rows in tiles of 16.
 template <bool kStream, bool kWin = false>
 __device__ __forceinline__ void decode_item(const AttnParams& p, const Item& it, uint8_t* smem) {
     constexpr int kCache = kStream ? 2 : 0;  // cache policy of the loads: nt
@@ -820,7 +821,8 @@ __device__ __forceinline__ void decode_item(const AttnParams& p, const Item& it,
     const int G = s.G;
     const int R = p.rows_total;
     const int qpos0 = p.qpos0[b];
-    const WindowList win(qpos0, qpos0 + s.Lq - 1, p.window, p.sinks);
+    const int r0 = kWin ? kDecRows * it.tile : 0;
+    const WindowList win(qpos0 + r0 / G, qpos0 + min(r0 + kDecRows - 1, R - 1) / G, p.window, p.sinks);
     const int nkb = kWin ? win.total : p.nkb[b];  // the last query row sees every block
     const int chunk = (nkb + nsplit - 1) / nsplit;
     const int e0 = min(nkb, split * chunk);
@@ -834,9 +836,9 @@ __device__ __forceinline__ void decode_item(const AttnParams& p, const Item& it,
     const int g = l >> 4;  // lane group (K index block)
 
     // Q^T (B operand of S^T): lane (n, g) holds Q[row n][32 j + 8 g .. + 7] for step j
-    const bool qvalid = n < R;
-    const int qt = qvalid ? n / G : 0;
-    const int qg = qvalid ? n - qt * G : 0;
+    const bool qvalid = r0 + n < R;
+    const int qt = qvalid ? (r0 + n) / G : 0;
+    const int qg = qvalid ? r0 + n - qt * G : 0;
     bf16x8_t qf[4];
     {
         const uint16_t* qp = p.q.data + b * p.q.sb + (int64_t)qt * p.q.st + (int64_t)(hk * G + qg) * p.q.sh + 8 * g;
@@ -1051,21 +1053,22 @@ __device__ __forceinline__ void decode_item(const AttnParams& p, const Item& it,
         ml[(w * kDecRows + n) * 2 + 1] = l_run;
     }
     __syncthreads();
-    const int orow = tid >> 5;  // 16 rows x 32 threads, 4 head-dim values each
+    const int lrow = tid >> 5;  // 16 rows x 32 threads, 4 head-dim values each
+    const int orow = r0 + lrow;
     const int d4 = (tid & 31) * 4;
     if (orow >= R) return;
     float mx = -__builtin_inff();
 #pragma unroll
-    for (int v = 0; v < kDecWaves; ++v) mx = fmaxf(mx, ml[(v * kDecRows + orow) * 2]);
+    for (int v = 0; v < kDecWaves; ++v) mx = fmaxf(mx, ml[(v * kDecRows + lrow) * 2]);
     f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
     float wsum = 0.0f;
     if (kWin && mx == -__builtin_inff()) mx = 0.0f;  // (fmaxf drops NaN: a NaN sum stays)
     if (kWin || mx != -__builtin_inff()) {
 #pragma unroll
         for (int v = 0; v < kDecWaves; ++v) {
-            const float wv = __builtin_amdgcn_exp2f(ml[(v * kDecRows + orow) * 2] - mx);
-            wsum += wv * ml[(v * kDecRows + orow) * 2 + 1];
-            acc += wv * *reinterpret_cast<const f32x4_t*>(mo + (v * kDecRows + orow) * kDecOStride + d4);
+            const float wv = __builtin_amdgcn_exp2f(ml[(v * kDecRows + lrow) * 2] - mx);
+            wsum += wv * ml[(v * kDecRows + lrow) * 2 + 1];
+            acc += wv * *reinterpret_cast<const f32x4_t*>(mo + (v * kDecRows + lrow) * kDecOStride + d4);
         }
     }
     const bool some = kWin ? wsum != 0.0f : wsum > 0.0f;
@@ -1106,10 +1109,11 @@ __global__ __launch_bounds__(kDecWaves * 64) void attn_decode_kernel(AttnParams 
 __global__ __launch_bounds__(kDecWaves * 64) void attn_window_decode_kernel(AttnParams p) {
     __shared__ __attribute__((aligned(16))) uint8_t smem[kDecWaves * kDecVBytes];
     Item it;
-    if (!find_item(p, 1, &it)) return;
+    if (!find_item(p, p.ntiles, &it)) return;
     it.row = __builtin_amdgcn_readfirstlane(it.row);
     it.b = __builtin_amdgcn_readfirstlane(it.b);
     it.split = __builtin_amdgcn_readfirstlane(it.split);
+    it.tile = __builtin_amdgcn_readfirstlane(it.tile);
     decode_item<false, true>(p, it, smem);
 }
 
@@ -1122,6 +1126,42 @@ bool attn_uses_decode_kernel(const Shape& s, bool dense) {
 AttnTiling attn_tiling(const Shape& s, bool dense, bool decode) {
     if (decode && attn_uses_decode_kernel(s, dense)) return AttnTiling{kDecRows, true, false, false, 4, 32};
     return AttnTiling{kBM, false, false, !dense, 16, dense ? kMaxDecodeSplits : kMaxPrefillSplits};
+}
+
+// Windows in tiles of 256 rows: their lists are of about one length (nkb blocks), so one split count for all requests, the
+// one with the least time by what was measured (bf16 and 4 bits alike): a round of 256 items takes 10 us and 1.5 us a
+// block, a merge 7 us and what it reads and writes (1032 bytes a partial row at 5.5 TB/s).  1000 queries under 1500 (28 Q /
+// 4 KV heads) 65 us whole, 58 in 2; 512 under 4096 (32 / 8) 96 and 55 in 4; 100 under 4096 95 and 33 in 8 to 16.
+static double window_us(const Shape& s, int nkb, int max_splits, int* splits) {
+    const int rows = s.Lq * s.G;
+    const double units = (double)s.B * s.Hkv * ((rows + kBM - 1) / kBM);
+    double best = 0.0;
+    for (int c = 1; c <= max_splits && c <= nkb; ++c) {
+        const double us = ceil(units * c / 256) * (10.0 + 1.5 * ((nkb + c - 1) / c)) +
+                          (c > 1 ? 7.0 + 1.9e-4 * s.B * s.Hkv * rows * c : 0.0);
+        if (c == 1 || us < best) {
+            best = us;
+            *splits = c;
+        }
+    }
+    return best;
+}
+
+// Windows over bf16 caches: tiles of 16 rows, whose waves take blocks on their own, take 12 us and 0.7 us for every block
+// that a CU's items have, tiles of 256 rows the time above (16 queries under 2048, 32 Q / 8 KV heads, 12.9 and 21 us; 256
+// under 2048, 8 / 8 heads, 21 and 32; 64 under 8192, 32 / 8, 54 and 42).
+AttnTiling attn_window_tiling(const Shape& s, const int32_t* kv_len, int window, int sinks) {
+    AttnTiling small{kDecRows, true, false, false, 4, 32}, large{kBM, false, false, false, 1, kMaxDecodeSplits};
+    small.window = large.window = true;
+    const int rows = s.Lq * s.G;
+    if (rows <= kDecRows) return small;
+    double blocks = 0.0;
+    int nkb = 1, splits = 1;
+    for (int b = 0; b < s.B; ++b) {
+        blocks += (double)s.Hkv * ((rows + kDecRows - 1) / kDecRows) * attn_window_blocks(s, kDecRows, kv_len[b] - s.Lq, window, sinks);
+        nkb = max(nkb, attn_window_blocks(s, kBM, kv_len[b] - s.Lq, window, sinks));
+    }
+    return 12.0 + 0.7 * blocks / 256 < window_us(s, nkb, kMaxDecodeSplits, &splits) ? small : large;
 }
 
 // The plan's split counts (its placement: attn_plan).
@@ -1166,7 +1206,9 @@ static void attn_plan_counts(const Shape& s, const int32_t* nkb, int forced, con
     // from half on, 500 over 16 to 128, 28 / 4, 174 -> 183: fewer units balance the XCDs less).  Of 100 drawn launches
     // 16 are slower without, by 6 % on the average, none faster.
     int whole_if = 0;
-    if (!dec && forced <= 0) {
+    if (!dec && forced <= 0 && tiling.window) {
+        window_us(s, nkb_max, max_splits, &forced);
+    } else if (!dec && forced <= 0) {
         // attn_fwd_kernel: one split count for every request.  Splitting in proportion to
         // each request's blocks measured slower on ragged batches (config 4: 380 vs 319 us
         // sparse, 2386 vs 2077 us dense), and the blocks a request selects are device data
@@ -1349,6 +1391,9 @@ void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling&
     plan->unit_splits = 0;
     plan->per_xcd = (plan->off[s.B] + 7) / 8;
     if (rows > kPlanRows) return;
+    // Windows of several tiles: every tile has blocks of its own, so tiles are dealt in order, an eighth to every XCD
+    // (by rows, 2048 queries of 2 KV heads leave six XCDs idle).
+    if (tiling.window && ntiles > 1) return;
     // Placement units on the 8 XCDs.  A unit is a KV row and a range of its splits; the row
     // tiles of a unit stream the same blocks, so they share the XCD's L2, and different
     // split ranges of a row are disjoint parts of its block list (placing them apart
@@ -1494,7 +1539,7 @@ int attn_window_blocks(const Shape& s, int tile_rows, int qpos0, int window, int
 
 int attn_window_splits(const Shape& s, const int32_t* kv_len, int window, int sinks, bool bits4) {
     const PastBlocks none{};
-    const AttnTiling tiling = bits4 ? attn4_tiling(s, none, kv_len, window, sinks) : attn_tiling(s, true);
+    const AttnTiling tiling = bits4 ? attn4_tiling(s, none, kv_len, window, sinks) : attn_window_tiling(s, kv_len, window, sinks);
     int32_t n[CA_MAX_BATCH];
     for (int b = 0; b < s.B; ++b) n[b] = attn_window_blocks(s, tiling.tile_rows, kv_len[b] - s.Lq, window, sinks);
     SplitPlan plan;
@@ -1563,7 +1608,8 @@ hipError_t launch_attn_merge(const AttnParams& p, bool nan_lse, hipStream_t stre
 hipError_t launch_attn(const AttnArgs& a, hipStream_t stream) {
     AttnParams p;
     SplitPlan plan;
-    attn_fill(a, attn_tiling(a.s, a.kv_len != nullptr), &p, &plan);
+    const AttnTiling tiling = a.window > 0 ? attn_window_tiling(a.s, a.kv_len, a.window, a.sinks) : attn_tiling(a.s, a.kv_len != nullptr);
+    attn_fill(a, tiling, &p, &plan);
     bool row_res;
     {
         int max_tokens = 0;
@@ -1591,7 +1637,7 @@ hipError_t launch_attn(const AttnArgs& a, hipStream_t stream) {
     const bool streamed = kv_bytes >= kStreamBytes && !repeats(a.k) && !repeats(a.v);
     static_assert(kNW == kDecWaves, "one workgroup size for the attention kernels");
     if (a.window > 0)
-        attn_uses_decode_kernel(a.s, true) ? launch(attn_window_decode_kernel) : launch(attn_fwd_kernel<kNW, false, false, true>);
+        tiling.streams ? launch(attn_window_decode_kernel) : launch(attn_fwd_kernel<kNW, false, false, true>);
     else if (a.table)
         row_res ? launch(attn_fwd_kernel<kNW, true, true>) : launch(attn_fwd_kernel<kNW, true, false>);
     else if (attn_uses_decode_kernel(a.s, true))

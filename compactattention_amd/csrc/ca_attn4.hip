@@ -1013,6 +1013,7 @@ AttnTiling attn4_tiling(const Shape& s, const PastBlocks& pb, const int32_t* kv_
         return AttnTiling{dense && rows <= 16 ? 16 : 32, true, true, !dense, 0, dense ? 32 : kMaxPrefillSplits};
     AttnTiling t = attn_tiling(s, dense, false);
     t.steps = true;
+    t.window = window > 0;
     return t;
 }
 

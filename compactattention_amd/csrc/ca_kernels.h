@@ -169,10 +169,12 @@ struct AttnTiling {
     bool lists;        // block lists of the device's choosing (else every block)
     int min_blocks;    // least blocks of a split
     int max_splits;
+    bool window = false;  // under a window
 };
 // dense = identity block lists over kv_len tokens (decode); otherwise per-row tables.  decode: whether few
 // rows may take the decode kernel.
 AttnTiling attn_tiling(const Shape& s, bool dense, bool decode = true);
+AttnTiling attn_window_tiling(const Shape& s, const int32_t* kv_len, int window, int sinks);
 AttnTiling attn4_tiling(const Shape& s, const PastBlocks& pb, const int32_t* kv_len, int window = 0, int sinks = 0);
 // The blocks of a request's longest list under a window, with tiles of tile_rows packed rows
 int attn_window_blocks(const Shape& s, int tile_rows, int qpos0, int window, int sinks);
