@@ -26,6 +26,11 @@ A cache of ``bits=4`` holds its pages in 4 bits (``ops.KV4``: [num_pages, 4352] 
 bytes), quantised as tokens are appended.  The chunk summaries are still pooled from the bf16 keys; a
 mean-K that is recomputed from the cache (``refresh_kmean``) and the views are those of the stored values.
 
+A cache of bounded size.  ``with_mass`` keeps the attention weight that every key received (``add_mass``: fp32 by KV row and
+slot); ``evict`` leaves the first tokens, the last ones and the heaviest of the others, in order, in pages of their own.
+Slots then count what is held and ``position`` what was appended: keys keep the rotation of the position that they had.
+``drop_outside`` gives the pages back that a sliding window has left behind.
+
 Pages are reference-counted: ``fork`` lets a request share another's pages, and a decode
 append into a shared, partly filled page copies it first.  ``truncate`` gives the pages behind a
 length back, ``compact`` moves the pages in use to the front of the pool and gives the rest of its memory
@@ -148,9 +153,10 @@ class PagedKVCache:
 
     def __init__(self, batch: int, num_kv_heads: int, max_tokens: int, device, with_kmean: bool = True,
                  with_kgate: bool = False, kgate_heads: Optional[int] = None, pool_pages: Optional[int] = None,
-                 bits: int = 16):
+                 bits: int = 16, with_mass: bool = False):
         """max_tokens sizes the page table and summaries (they grow on demand); pool_pages
-        sizes the initial page pool (default: every row's max_tokens); bits is 16 (bf16 pages) or 4."""
+        sizes the initial page pool (default: every row's max_tokens); bits is 16 (bf16 pages) or 4; with_mass
+        keeps the keys' attention weights."""
         self.batch = batch
         self.num_kv_heads = num_kv_heads
         self.rows = batch * num_kv_heads
@@ -164,7 +170,11 @@ class PagedKVCache:
         self.kgate_heads = kgate_heads or num_kv_heads
         self.kmean = self._summary(num_kv_heads) if with_kmean else None
         self.kgate = self._summary(self.kgate_heads) if with_kgate else None
+        self.mass = self._weights() if with_mass else None  # [rows, cap * 64]; 0 from the length on
         self.length = 0  # tokens stored per request
+        self.evicted = 0  # tokens that evict has dropped per request
+        self._in_order_from = 0  # slots from here on hold consecutive positions (slot + evicted)
+        self._dropped = (0, 0, 0)  # drop_outside: blocks [a, b) have no pages, and the window that they were dropped for
         self.kmean_blocks = 0  # leading blocks with a valid kmean
         self.kgate_blocks = 0  # leading blocks with a valid kgate
         self.kgate_tokens = 0  # tokens that those pooled (the last block's may end inside it); 0: not known
@@ -172,6 +182,14 @@ class PagedKVCache:
     # -- layout ---------------------------------------------------------------------------
     def _summary(self, heads: int) -> torch.Tensor:
         return torch.zeros((self.batch, heads, self.cap, HEAD_DIM), dtype=torch.float32, device=self.device)
+
+    def _weights(self) -> torch.Tensor:
+        return torch.zeros((self.rows, self.cap * BLOCK), dtype=torch.float32, device=self.device)
+
+    @property
+    def position(self) -> int:
+        """Tokens appended so far per request, the evicted ones among them: the next token's position."""
+        return self.length + self.evicted
 
     @property
     def past_blocks(self) -> int:
@@ -205,7 +223,10 @@ class PagedKVCache:
                 t = torch.zeros((old.shape[0], old.shape[1], new, HEAD_DIM), dtype=torch.float32, device=self.device)
                 t[:, :, :self.cap].copy_(old)
                 setattr(self, name, t)
-        self.cap = new
+        old_cap, self.cap = self.cap, new
+        if self.mass is not None:
+            old, self.mass = self.mass, self._weights()
+            self.mass[:, :old_cap * BLOCK].copy_(old)
 
     def _upload(self, b0: int, b1: int) -> None:
         if b1 > b0:
@@ -319,6 +340,7 @@ class PagedKVCache:
         are the ones a chunk append of the same keys writes, bit for bit."""
         if self.kmean is None or self.kmean_blocks >= upto:
             return
+        self._need_pages()
         b0 = self.kmean_blocks
         if self.bits == 4:
             n = (upto - b0) * BLOCK
@@ -393,19 +415,35 @@ class PagedKVCache:
             self.pool.release(old)
             self._pt[rd] = -1
             self._pt[rd, :nb] = self._pt[rs, :nb]
-            self.pool.retain(self._pt[rs, :nb])
+            shared = self._pt[rs, :nb]
+            self.pool.retain(shared[shared >= 0])
         self._upload(0, self.cap)
         for t in (self.kmean, self.kgate):
             if t is not None:
                 t[dst].copy_(t[src])
+        if self.mass is not None:
+            self.mass[dst * H:(dst + 1) * H].copy_(self.mass[src * H:(src + 1) * H])
+
+    def check_truncate(self, tokens: int) -> None:
+        """Raise where ``truncate(tokens)`` cannot be."""
+        if not 0 <= tokens <= self.length:
+            raise ValueError(f"cannot truncate to {tokens} tokens: the cache holds {self.length}")
+        if tokens < self._in_order_from:
+            raise ValueError(f"cannot truncate to {tokens} slots: those before {self._in_order_from} were picked by eviction and "
+                             "no longer follow the sequence")
+        a, b, window = self._dropped
+        if a < b and max(0, tokens - window + 1) < b * BLOCK:
+            raise ValueError(f"cannot truncate to {tokens} tokens: a window of {window} there sees tokens before {b * BLOCK}, whose "
+                             "pages were dropped")
 
     def truncate(self, tokens: int, keep_pages: bool = False) -> None:
         """Forget what every request holds past ``tokens`` tokens (a rejected draft, a shorter prefix); the pages
         behind them go back to the pool.  With keep_pages those that a row owns alone stay mapped, as in
         ``reset``.  Summaries that pooled a token that goes are no longer valid: a rejected draft after a chunk that
         ended inside a block leaves that block's gate-K summary as it is."""
-        if not 0 <= tokens <= self.length:
-            raise ValueError(f"cannot truncate to {tokens} tokens: the cache holds {self.length}")
+        self.check_truncate(tokens)
+        if self.mass is not None:
+            self.mass[:, int(tokens):self.length] = 0.0
         nb = -(-int(tokens) // BLOCK)
         tail = self._pt[:, nb:]
         drop = tail >= 0
@@ -421,6 +459,100 @@ class PagedKVCache:
             self.kgate_blocks = min(self.kgate_blocks, self.length // BLOCK)
             self.kgate_tokens = min(self.kgate_tokens, BLOCK * self.kgate_blocks)
 
+    # -- bounded size ---------------------------------------------------------------------
+    def add_mass(self, q: torch.Tensor, lse: torch.Tensor, scale: float, table: Optional[torch.Tensor] = None,
+                 counts: Optional[torch.Tensor] = None) -> None:
+        """Add the attention weights of the queries q [B, L, Hq, 128] of the last L tokens to the keys' (``ops.key_mass``), with
+        the lse [B, Hq, L] that their attention returned, over all keys or the blocks of its table."""
+        if self.mass is None:
+            raise ValueError("cache built without the keys' weights (with_mass)")
+        L = q.shape[1]
+        if L > self.length:
+            raise ValueError(f"{L} queries over {self.length} tokens")
+        ops.key_mass(q, self.layouts()[0], lse, self.mass, self.length - L, scale, self.cap, self.num_kv_heads, table=table,
+                     counts=counts)
+
+    def _take_pages(self, blocks: int) -> np.ndarray:
+        """Pages [rows, blocks] for what eviction keeps: those that a row has mapped behind its tokens and owns alone, and new
+        ones."""
+        nb = -(-self.length // BLOCK)
+        out = np.full((self.rows, blocks), -1, np.int32)
+        tail = self._pt[:, nb:]
+        for r in range(self.rows):
+            own = [int(p) for p in tail[r] if p >= 0 and self.pool.refs[p] == 1][:blocks]
+            out[r, :len(own)] = own
+            tail[r][np.isin(tail[r], own)] = -1
+        need = out < 0
+        if need.any():
+            out[need] = self.pool.alloc(int(need.sum()))
+        return out
+
+    def evict(self, budget: int, sinks: int = 0, recent: int = 0, keep_pages: bool = False) -> int:
+        """Leave budget tokens in every row, each its own: the first ``sinks``, the last ``recent`` and the heaviest of the others
+        by the weights that they received.  They move, in order, into other pages (pages that a fork shares stay as they are), the
+        old ones go back to the pool, or with keep_pages stay mapped behind where a row owns them alone.  Mean-K summaries are
+        computed again before they are next read; a cache with gate-K summaries, which pool keys that it does not hold,
+        raises.  Returns how many tokens of a row went."""
+        if self.mass is None:
+            raise ValueError("cache built without the keys' weights (with_mass)")
+        if self.kgate is not None:
+            raise ValueError("a cache with gate-K summaries cannot evict: they pool pre-RoPE keys by block")
+        if self._dropped[0] < self._dropped[1]:
+            raise ValueError("the pages of some tokens were dropped (drop_outside)")
+        if not 0 < budget or sinks < 0 or recent < 0 or sinks + recent > budget:
+            raise ValueError(f"a budget of {budget} does not hold {sinks} sinks and {recent} recent tokens")
+        n = self.length
+        if n <= budget:
+            return 0
+        keep = ops.heavy_tokens(self.mass, n, self.num_kv_heads, budget, sinks, recent)
+        blocks = -(-budget // BLOCK)
+        pages = self._take_pages(blocks)
+        K, V = self.layouts()  # (of the pool as it is now: it may have grown)
+        table = torch.from_numpy(pages).to(self.device)
+        make = ops.KV4.paged if self.bits == 4 else ops.KV.paged
+        moved = ops.move_tokens(K, V, make(self.pool.k, table), make(self.pool.v, table), keep, n, self.num_kv_heads,
+                                mass=self.mass)
+        self.mass[:, :budget].copy_(moved)
+        self.mass[:, budget:n] = 0.0
+        old = self._pt
+        self._pt = np.full_like(old, -1)
+        self._pt[:, :blocks] = pages
+        for r in range(self.rows):
+            mapped = old[r][old[r] >= 0]
+            own = mapped[self.pool.refs[mapped] == 1][:self.cap - blocks] if keep_pages else mapped[:0]
+            self._pt[r, blocks:blocks + own.size] = own
+            self.pool.release(mapped[~np.isin(mapped, own)])
+        self._upload(0, self.cap)
+        self.length = budget
+        self.evicted += n - budget
+        self._in_order_from = budget - recent
+        self.kmean_blocks = 0
+        return n - budget
+
+    def drop_outside(self, window: int, sinks: int = 0, slack: int = 0) -> int:
+        """Give back the pages of the blocks that no query from the current length on sees under a window with sink tokens
+        (``ops.attn_window``), nor one up to ``slack`` tokens before it (a draft that may be rejected).  Returns how many
+        blocks of a row went; what is dropped can be read no more."""
+        if window < 1 or sinks < 0 or slack < 0:
+            raise ValueError(f"window={window}, sinks={sinks} and slack={slack}")
+        a, b = -(-sinks // BLOCK), max(0, self.length - slack - window + 1) // BLOCK
+        had = self._dropped
+        if had[0] < had[1]:
+            if had[0] != a or had[2] != window:
+                raise ValueError(f"pages were dropped for a window of {had[2]} with sinks in {had[0]} blocks")
+            first = had[1]
+        else:
+            first = a
+        if first >= b:
+            return 0
+        cols = self._pt[:, first:b]
+        self.pool.release(cols[cols >= 0])
+        cols[:] = -1
+        self._upload(first, b)
+        self._dropped = (a, b, window)
+        self.kmean_blocks = min(self.kmean_blocks, a)
+        return b - first
+
     def compact(self, shrink: bool = True) -> int:
         """Move the pages in use to the front of the pool (``ops.copy_pages``) and, with shrink, give the memory
         behind them back; returns how many pages moved.  Page ids, and with shrink the pools, change: graphs that
@@ -433,7 +565,12 @@ class PagedKVCache:
         return moved
 
     # -- views ----------------------------------------------------------------------------
+    def _need_pages(self) -> None:
+        if self._dropped[0] < self._dropped[1]:
+            raise ValueError(f"the pages of blocks [{self._dropped[0]}, {self._dropped[1]}) were dropped (drop_outside)")
+
     def _values(self, of_v: bool) -> torch.Tensor:
+        self._need_pages()
         if self.bits == 4:
             K, V = self.layouts()
             got = ops.gather_q4(None if of_v else K, V if of_v else None, self.batch, self.num_kv_heads, 0, self.length)
@@ -471,6 +608,10 @@ class PagedKVCache:
                 self.pool.release(mapped)
             self._pt[:] = -1
             self.page_table.fill_(-1)
+        if self.mass is not None:
+            self.mass[:, :self.length] = 0.0
         self.length = 0
+        self.evicted = self._in_order_from = 0
+        self._dropped = (0, 0, 0)
         self.kmean_blocks = 0
         self.set_kgate(0)

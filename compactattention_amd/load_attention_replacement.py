@@ -24,7 +24,7 @@ from __future__ import annotations
 import os
 import warnings
 from types import MethodType
-from typing import Optional, Union
+from typing import List, Optional, Union
 
 import torch
 from torch import nn
@@ -204,14 +204,23 @@ def load_llama_attention_replacement_model(
     flashprefill_last_n_block: int = 2,
     flashprefill_min_budget: int = 0,
     kv_cache_bits: int = 16,
+    sliding_window: int = 0,
+    sliding_window_sinks: int = 0,
+    sliding_window_layers: Optional[List[int]] = None,
+    kv_budget: int = 0,
+    kv_budget_sinks: int = 4,
+    kv_budget_recent: int = 0,
+    kv_budget_slack: int = 64,
+    kv_budget_observe: int = 64,
 ) -> nn.Module:
     """Returns the stock LlamaForCausalLM with compactattn attention in every layer.
 
     base_model: a transformers LlamaForCausalLM (moved to torch_dtype) or a local model
     directory (``from_pretrained(..., local_files_only=True)``).  model_id: optional local
     directory or file holding the Seer gate weights (``attn_gate_weights.pth``); a Seer variant whose
-    gate weights are not all there warns.  kv_cache_bits: 4 for a KV cache held in 4 bits (a keyword of
-    this build).
+    gate weights are not all there warns.  Keywords of this build: kv_cache_bits 4 for a KV cache held in 4 bits;
+    sliding_window (with its sinks, and the layers that have it; None: all) for queries that see the last tokens and the
+    first; kv_budget for KV heads that keep that many tokens by the attention weight that they received (FlashPrefill).
     """
     from transformers import LlamaForCausalLM
 
@@ -230,6 +239,11 @@ def load_llama_attention_replacement_model(
         flashprefill_window_size=flashprefill_window_size, flashprefill_last_n_block=flashprefill_last_n_block,
         flashprefill_min_budget=flashprefill_min_budget, gate=_gate_settings(model_id))
     seer_cfg.kv_cache_bits = int(kv_cache_bits)
+    seer_cfg.sliding_window, seer_cfg.sliding_window_sinks = int(sliding_window), int(sliding_window_sinks)
+    seer_cfg.sliding_window_layers = sliding_window_layers
+    seer_cfg.kv_budget, seer_cfg.kv_budget_sinks = int(kv_budget), int(kv_budget_sinks)
+    seer_cfg.kv_budget_recent, seer_cfg.kv_budget_slack = int(kv_budget_recent), int(kv_budget_slack)
+    seer_cfg.kv_budget_observe = int(kv_budget_observe)
     seer_cfg.validate()
     block_rope = _BlockRope(model.model.rotary_emb, seer_cfg.max_position_embeddings)
     cls = _VARIANTS[variant]

@@ -15,7 +15,7 @@ not have (BASELINE configs 1 and 3 ask for it); they default to 0.
 from __future__ import annotations
 
 from dataclasses import asdict, dataclass, fields
-from typing import Any, Dict, Optional
+from typing import Any, Dict, List, Optional
 
 
 @dataclass
@@ -68,6 +68,18 @@ class SeerAttnLlamaConfig:
     # RMS norm of every query and key head before the rotation (weights q_norm, k_norm [head_dim]; FlashPrefill
     # model)
     qk_norm: bool = False
+    # layers whose queries see the last sliding_window tokens and the first sliding_window_sinks (0: none; layers None: all)
+    sliding_window: int = 0
+    sliding_window_sinks: int = 0
+    sliding_window_layers: Optional[List[int]] = None
+    # tokens that every other layer's KV heads keep (0: all): the first kv_budget_sinks, the last kv_budget_recent and those that
+    # received most attention weight; dropped once there are kv_budget_slack more.  Weights are counted of the last
+    # kv_budget_observe queries of a chunk (0: all) and of every decoded token (FlashPrefill model)
+    kv_budget: int = 0
+    kv_budget_sinks: int = 4
+    kv_budget_recent: int = 0
+    kv_budget_slack: int = 64
+    kv_budget_observe: int = 64
 
     @classmethod
     def from_dict(cls, d: Dict[str, Any]) -> "SeerAttnLlamaConfig":
@@ -84,6 +96,10 @@ class SeerAttnLlamaConfig:
     def num_key_value_groups(self) -> int:
         return self.num_attention_heads // self.num_key_value_heads
 
+    def window_of(self, layer: int) -> int:
+        """The sliding window of a layer, 0 for none."""
+        return self.sliding_window if self.sliding_window_layers is None or layer in self.sliding_window_layers else 0
+
     def validate(self) -> None:
         if self.head_dim != 128:
             raise ValueError("the compactattn kernels run head_dim 128")
@@ -97,6 +113,19 @@ class SeerAttnLlamaConfig:
             raise ValueError("seerattn_flashprefill_score_mode must be 'pooled' or 'token'")
         if self.kv_cache_bits not in (4, 16):
             raise ValueError("kv_cache_bits must be 16 or 4")
+        if self.sliding_window < 0 or self.sliding_window_sinks < 0:
+            raise ValueError("sliding_window and sliding_window_sinks must not be negative")
+        if self.sliding_window_layers is not None:
+            bad = [i for i in self.sliding_window_layers if not 0 <= i < self.num_hidden_layers]
+            if bad or self.sliding_window == 0:
+                raise ValueError(f"sliding_window_layers {self.sliding_window_layers} need a sliding_window and layers below "
+                                 f"{self.num_hidden_layers}")
+        if self.kv_budget < 0 or self.kv_budget % self.seerattn_flashprefill_block_size:
+            raise ValueError("kv_budget must be a multiple of seerattn_flashprefill_block_size (a chunk that follows starts there)")
+        if min(self.kv_budget_sinks, self.kv_budget_recent, self.kv_budget_slack, self.kv_budget_observe) < 0:
+            raise ValueError("kv_budget_sinks, kv_budget_recent, kv_budget_slack and kv_budget_observe must not be negative")
+        if self.kv_budget and self.kv_budget_sinks + self.kv_budget_recent > self.kv_budget:
+            raise ValueError("kv_budget must hold kv_budget_sinks and kv_budget_recent")
         from ..attn_gate import parse_gate_type
 
         parse_gate_type(self.seerattn_gate_type)

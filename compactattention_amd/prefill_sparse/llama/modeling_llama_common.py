@@ -201,8 +201,38 @@ def dense_decode_forward(attn: nn.Module, hidden_states: torch.Tensor, position_
     query_states, key_states = position_qk(attn, q, k, cos, sin)
     cache.append_tokens(key_states, v)
     K, V = cache.layouts()
-    out = ops.attn_decode(query_states.contiguous(), K, V, [cache.length] * B, attn.scaling, cache.cap,
-                          attn.num_key_value_heads)
+    query_states = query_states.contiguous()
+    out = ops.attn_decode(query_states, K, V, [cache.length] * B, attn.scaling, cache.cap, attn.num_key_value_heads,
+                          with_lse=cache.mass is not None)
+    if cache.mass is not None:
+        out, lse = out
+        cache.add_mass(query_states, lse, attn.scaling)
+        keep_budget(attn.config, cache)
+    return attn.o_proj(out.reshape(B, L, -1))
+
+
+def keep_budget(config: SeerAttnLlamaConfig, cache: PagedKVCache) -> None:
+    """Evict down to the config's kv_budget once the cache holds kv_budget_slack tokens more (host work, so not while a graph
+    is captured)."""
+    if cache.length > config.kv_budget + config.kv_budget_slack and not torch.cuda.is_current_stream_capturing():
+        cache.evict(config.kv_budget, config.kv_budget_sinks, config.kv_budget_recent, keep_pages=True)
+
+
+def window_forward(attn: nn.Module, hidden_states: torch.Tensor, position_embeddings, cache: PagedKVCache, window: int
+                   ) -> torch.Tensor:
+    """A layer under a sliding window: any number of new tokens (a chunk, a draft, one token) is appended and attends to the last
+    ``window`` tokens and the config's sinks; pages that the window has left behind go back to the pool, but for those that
+    a rejected draft of up to 64 tokens would bring back."""
+    B, L, _ = hidden_states.shape
+    q, k, v = project_qkv(attn, hidden_states)
+    cos, sin = position_embeddings
+    query_states, key_states = position_qk(attn, q, k, cos, sin)
+    start = cache.append_tokens(key_states, v)
+    K, V = cache.layouts()
+    sinks = attn.config.sliding_window_sinks
+    out = ops.attn_window(query_states, K, V, start, window, sinks, attn.scaling, cache.cap, attn.num_key_value_heads)
+    if not torch.cuda.is_current_stream_capturing():
+        cache.drop_outside(window, sinks, slack=BLOCK)
     return attn.o_proj(out.reshape(B, L, -1))
 
 
@@ -227,21 +257,28 @@ class ChunkedPrefillCache:
         kgate_heads = gate_key_heads(config.seerattn_gate_type, config.seerattn_gate_force_double,
                                      config.seerattn_compactattn_kv_group_aware_gate, config.num_attention_heads,
                                      config.num_key_value_heads)
-        self.layers: List[PagedKVCache] = [
-            PagedKVCache(batch, config.num_key_value_heads, max_tokens, device, with_kmean=with_kmean,
-                         with_kgate=with_kgate, kgate_heads=kgate_heads, bits=config.kv_cache_bits)
-            for _ in range(config.num_hidden_layers)
-        ]
-        # pages for max_tokens up front, so a prefill of that length maps nothing on the way;
-        # a longer sequence grows the pool and the page tables on demand
-        for layer in self.layers:
-            layer.reserve(max_tokens)
+        rows = batch * config.num_key_value_heads
+        self.layers: List[PagedKVCache] = []
+        for i in range(config.num_hidden_layers):
+            window = config.window_of(i)
+            if window:  # no summaries, and pages for the sinks, the window and a chunk (the pool grows where more are needed)
+                held = min(max_tokens, window + config.sliding_window_sinks + 2048)
+                self.layers.append(PagedKVCache(batch, config.num_key_value_heads, max_tokens, device, with_kmean=False,
+                                                bits=config.kv_cache_bits, pool_pages=rows * (held // BLOCK + 4)))
+                continue
+            self.layers.append(PagedKVCache(batch, config.num_key_value_heads, max_tokens, device, with_kmean=with_kmean,
+                                            with_kgate=with_kgate, kgate_heads=kgate_heads, bits=config.kv_cache_bits,
+                                            with_mass=config.kv_budget > 0))
+            # pages for max_tokens up front, so a prefill of that length maps nothing on the way;
+            # a longer sequence grows the pool and the page tables on demand
+            self.layers[-1].reserve(max_tokens)
 
     def layer(self, idx: int) -> PagedKVCache:
         return self.layers[idx]
 
     def get_seq_length(self) -> int:
-        return self.layers[0].length
+        """Tokens of the sequence so far, those among them that a layer no longer holds."""
+        return self.layers[0].position
 
     def reset(self) -> None:
         """Start a new sequence in the same pages (pages shared by a fork are released)."""
@@ -249,9 +286,12 @@ class ChunkedPrefillCache:
             c.reset(keep_pages=True)
 
     def truncate(self, tokens: int, keep_pages: bool = False) -> None:
-        """Forget every layer's tokens past ``tokens`` (a rejected draft)."""
+        """Forget every layer's tokens past ``tokens`` of the sequence (a rejected draft).  A layer that has evicted tokens goes
+        back into its recent ones only, one under a window 64 tokens at least; else nothing is truncated and it raises."""
         for c in self.layers:
-            c.truncate(tokens, keep_pages)
+            c.check_truncate(tokens - c.evicted)
+        for c in self.layers:
+            c.truncate(tokens - c.evicted, keep_pages)
 
     def compact(self, shrink: bool = True) -> int:
         """``PagedKVCache.compact`` of every layer; returns how many pages moved in all."""

@@ -30,8 +30,8 @@ from ...modules._core import COMPACTATTN_VERSION
 from ...modules.flashprefill_prefill import flashprefill_rule, flashprefill_tables
 from .configuration_llama_seerattn import SeerAttnLlamaConfig
 from .modeling_llama_common import (ChunkedPrefillCache, CompactAttnLlamaForCausalLM, FusedProjections,
-                                     dense_decode_forward, event_span, is_decode_step, make_qk_norms, position_qk,
-                                     project_qkv)
+                                     dense_decode_forward, event_span, is_decode_step, keep_budget, make_qk_norms,
+                                     position_qk, project_qkv, window_forward)
 
 BLOCK = 64
 
@@ -73,6 +73,12 @@ class LlamaFlashPrefillCompactAttnAttention(nn.Module):
             raise ValueError("the compactattn prefill path needs a ChunkedPrefillCache")
         if attention_mask is not None and not bool(attention_mask.all()):
             raise ValueError("padded positions are not supported by the compactattn prefill path")
+        window = self.config.window_of(self.layer_idx)
+        if window:
+            with event_span(self.attention_timer):
+                out = window_forward(self, hidden_states, position_embeddings, past_key_value.layer(self.layer_idx), window)
+            self._compactattn_last_stats = {"path": "window"} if self.compactattn_debug else None
+            return out, 0.0, None, None, None
         if is_decode_step(hidden_states, past_key_value.layer(self.layer_idx)):
             out = dense_decode_forward(self, hidden_states, position_embeddings, past_key_value.layer(self.layer_idx))
             self._compactattn_last_stats = {"path": "decode_dense"} if self.compactattn_debug else None
@@ -100,7 +106,13 @@ class LlamaFlashPrefillCompactAttnAttention(nn.Module):
                                                     query_states=query_states)
             K, V = cache.layouts()
             out = ops.attn_fwd(query_states, K, V, table, counts, P, self.scaling, cache.cap,
-                               self.num_key_value_heads)
+                               self.num_key_value_heads, with_lse=cache.mass is not None)
+            if cache.mass is not None:
+                out, lse = out
+                seen = min(self.config.kv_budget_observe or L, L)  # the last queries vote for the keys that stay
+                cache.add_mass(query_states[:, L - seen:], lse[:, :, L - seen:], self.scaling, None if dense else table,
+                               None if dense else counts)
+                keep_budget(self.config, cache)
         if self.table_sink is not None:  # per-chunk block counts (device tensors), for FLOP accounting
             self.table_sink.append((counts, L, past))
         out = self.o_proj(out.reshape(B, L, -1))

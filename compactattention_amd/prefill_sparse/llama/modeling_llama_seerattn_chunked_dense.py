@@ -38,7 +38,8 @@ from ...modules.attention_forward_chunked_dense import (_compactattn_effective_t
 from ..attn_gate import ATTNGATE_CLASSES
 from .configuration_llama_seerattn import SeerAttnLlamaConfig
 from .modeling_llama_common import (ChunkedPrefillCache, CompactAttnLlamaForCausalLM, FusedProjections,
-                                     dense_decode_forward, event_span, is_decode_step, project_qkv, rope_qk)
+                                     dense_decode_forward, event_span, is_decode_step, project_qkv, rope_qk,
+                                     window_forward)
 
 BLOCK = 64
 
@@ -95,6 +96,8 @@ class LlamaSeerAttentionChunkedDense(nn.Module):
         super().__init__()
         if config.qk_norm:
             raise ValueError("qk_norm: the AttnGate pools queries and keys before their norm; the FlashPrefill model has it")
+        if config.kv_budget:
+            raise ValueError("kv_budget: the gate's block summaries pool keys that the cache does not hold; the FlashPrefill model has it")
         self.config = config
         self.layer_idx = layer_idx
         self.head_dim = config.head_dim
@@ -183,6 +186,12 @@ class LlamaSeerAttentionChunkedDense(nn.Module):
             raise ValueError("padded positions are not supported by the compactattn prefill path")
         if block_position_embeddings is None:
             raise ValueError("block_position_embeddings (per-block rotary tables) are required")
+        window = self.config.window_of(self.layer_idx)
+        if window:
+            with event_span(self.attention_timer):
+                out = window_forward(self, hidden_states, position_embeddings, past_key_value.layer(self.layer_idx), window)
+            self._compactattn_last_stats = {"path": "window"} if self.compactattn_debug else None
+            return out, 0.0, None, None, None
         if is_decode_step(hidden_states, past_key_value.layer(self.layer_idx)):
             out = dense_decode_forward(self, hidden_states, position_embeddings, past_key_value.layer(self.layer_idx))
             self._compactattn_last_stats = {"path": "decode_dense"} if self.compactattn_debug else None
