@@ -33,29 +33,36 @@ struct MassParams {
     float scale_log2;
     int window, sinks;
     int items;      // workgroups of a row (and part)
-    int parts;      // of the query rows, with workgroups of their own
-    int part_tiles;  // tiles of query tokens of a part
+    int parts;      // of the query tiles, every parts-th each, with workgroups of their own
     float* ws;      // the parts' sums [parts][rows][ws_stride], null where there is one
     int64_t ws_stride;
     int32_t start[CA_MAX_BATCH];
 };
 
-// A workgroup's row, place in the row's list and part of the query rows.  A row's workgroups run on one XCD, whose L2 then
-// holds its queries once, where the rows divide over the XCDs.
+// A workgroup's row, place in the row's list and part of the query tiles (p.parts is 1, 2, 4, 8 or 16).  Workgroup i runs on
+// XCD i % 8.  The parts of an item lie on XCDs of their own and the items of a row on all, so the XCDs carry equal work
+// whatever the lists' lengths, and the L2 of each holds its part of the queries (a chunk over 20 % of 32768 tokens 173 us
+// with a row's workgroups on one XCD, 158 so).  All blocks in one part: whole rows by XCD where they divide (64 queries over
+// 32768 tokens 40 us, 36 so).
 __device__ __forceinline__ void find_rows(const MassParams& p, int* row, int* item, int* cut) {
-    const int rows = p.s.B * p.s.Hkv, per = p.items * p.parts;
-    int k;
-    if (rows % 8 == 0) {
-        k = blockIdx.x >> 3;
-        const int u = k / per;
-        *row = (blockIdx.x & 7) + 8 * u;
-        k -= u * per;
-    } else {
-        *row = blockIdx.x / per;
-        k = blockIdx.x - *row * per;
+    const int x = blockIdx.x & 7, k = blockIdx.x >> 3;
+    if (p.parts == 1 && p.table == nullptr && (p.s.B * p.s.Hkv) % 8 == 0) {
+        *cut = 0;
+        *row = k / p.items;
+        *item = k - *row * p.items;
+        *row = x + 8 * *row;
+        return;
     }
-    *item = k / p.parts;
-    *cut = k - *item * p.parts;
+    int at;
+    if (p.parts <= 8) {
+        *cut = x & (p.parts - 1);
+        at = k * (8 / p.parts) + x / p.parts;
+    } else {
+        *cut = x + 8 * (k & 1);
+        at = k >> 1;
+    }
+    *row = at / p.items;
+    *item = at - *row * p.items;
 }
 
 // Blocks that a list leaves out keep their weights: a wave copies those before its entry e (from the one before it on), the
@@ -214,8 +221,12 @@ __global__ __launch_bounds__(kMassWaves * 64) __attribute__((amdgpu_waves_per_eu
 // ---------------------------------------------------------------------------------------
 // Many query rows.  Four waves, each with the 64 keys of a block in registers, go through the packed rows together, the rows of
 // 32 / G tokens at a time from LDS (two places in turn: while one is read the next tile, already in registers, goes to the other and the
-// one after it is on its way).  A launch may cut the tiles into parts of p.part_tiles, each with workgroups of its own;
-// their sums go to p.ws and are joined in order by key_mass_join_kernel.
+// one after it is on its way).  A launch may deal the tiles to p.parts, each with workgroups of its own; their sums go to
+// p.ws and are joined in order by key_mass_join_kernel.
+// Bound by vector instructions (one fma, exp2 and add a score, 16 of a wave's 64-lane cycles) beside 16 of the matrix cores:
+// 2048 queries over 32768 tokens (32 Q / 8 KV heads) 540 us, 0.98 PFLOP/s of the 1.21 that a large product reaches; 64 queries
+// 36 us, where a third is K's way from memory.  32x32x16 products, at two waves a SIMD where these run three, took 12 %
+// longer; products woven into the weights of the tile before, instruction by instruction, 10 %.
 constexpr int kTileRows = 32;
 
 template <bool kQ4, bool kTab>
@@ -225,6 +236,7 @@ __global__ __launch_bounds__(kMassWaves * 64) __attribute__((amdgpu_waves_per_eu
     const Shape& s = p.s;
     int row, item, cut;
     find_rows(p, &row, &item, &cut);
+    if (row >= s.B * s.Hkv) return;
     const int b = row / s.Hkv;
     const int hk = row - b * s.Hkv;
     const int G = s.G;
@@ -257,12 +269,12 @@ __global__ __launch_bounds__(kMassWaves * 64) __attribute__((amdgpu_waves_per_eu
     auto first_tile = [&](int t) { return t >= s.Lq ? tiles : max(t, 0) / T; };                     // with token t
     auto tile_after = [&](int t) { return t >= s.Lq ? tiles : (max(t, 0) + T - 1) / T; };           // past the tokens before t
     const bool edge = p.window > 0 && 64 * first_kb >= p.sinks;  // (blocks with sinks are seen to the end)
-    const int part0 = cut * p.part_tiles, part1 = part0 + p.part_tiles;
-    const int u0 = max(first_tile(64 * first_kb - start), part0);
-    const int u1 = max(min(edge ? tile_after(64 * last_kb - start + 63 + p.window) : tiles, part1), u0);
-    const int ua = min(max(tile_after(64 * last_kb - start + 63), u0), u1);
+    const int u1 = edge ? tile_after(64 * last_kb - start + 63 + p.window) : tiles;
+    // of those the part's: every p.parts-th
+    const int u0 = first_tile(64 * first_kb - start) + ((cut - first_tile(64 * first_kb - start)) & (p.parts - 1));
+    const int ua = tile_after(64 * last_kb - start + 63);
     const bool always = p.window == 0 || 64 * last_kb + 64 <= p.sinks;
-    const int ub = max(min(always ? s.Lq / T : min(first_tile(64 * first_kb - start + p.window), s.Lq / T), u1), ua);
+    const int ub = always ? s.Lq / T : min(first_tile(64 * first_kb - start + p.window), s.Lq / T);
     // Thread tid moves chunk tid % 16 of rows tid / 16 and 16 + tid / 16 of a tile, and tid < 32 the lse of row tid; chunk c
     // of row r stands at chunk c ^ (r % 16), for reads without bank conflicts.  Rows past T tokens' (where the group does not
     // divide 32) and past the last token are the last one's with weights of 0.
@@ -305,12 +317,12 @@ __global__ __launch_bounds__(kMassWaves * 64) __attribute__((amdgpu_waves_per_eu
     f32x4_t acc[4];
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) acc[kt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    auto run = [&](int u, int end, auto masked) {
+    int u = u0, from = 0;
+    auto run = [&](int end, auto masked) {
         constexpr bool kMask = decltype(masked)::value;
-        for (; u < end; ++u) {
-            const int from = (u - u0) & 1;
-            if (u + 1 < u1) put(from ^ 1);
-            if (u + 2 < u1) fetch(u + 2);
+        for (; u < end; u += p.parts) {
+            if (u + p.parts < u1) put(from ^ 1);
+            if (u + 2 * p.parts < u1) fetch(u + 2 * p.parts);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 bf16x8_t q[4];
@@ -321,16 +333,17 @@ __global__ __launch_bounds__(kMassWaves * 64) __attribute__((amdgpu_waves_per_eu
                 add_weights<kQ4, kMask>(p, keys, q, tile_neg[from][16 * i + n], kMask && t >= 0 && t < s.Lq ? start + t : -1, kb, g, acc);
             }
             __syncthreads();
+            from ^= 1;
         }
     };
     if (u0 < u1) {
         fetch(u0);
         put(0);
-        if (u0 + 1 < u1) fetch(u0 + 1);
+        if (u0 + p.parts < u1) fetch(u0 + p.parts);
         __syncthreads();
-        run(u0, ua, std::true_type{});
-        run(ua, ub, std::false_type{});
-        run(ub, u1, std::true_type{});
+        run(min(ua, u1), std::true_type{});
+        run(min(ub, u1), std::false_type{});
+        run(u1, std::true_type{});
     }
     const float sum = sum_rows(acc, n);
     if (!here) return;
@@ -366,24 +379,19 @@ __global__ __launch_bounds__(kMassWaves * 64) void key_mass_join_kernel(MassPara
 
 struct MassPlan {
     bool rows;       // key_mass_rows_kernel, else a block a wave (key_mass_token_kernel)
-    int parts;       // rows: of the queries
-    int part_tiles;
+    int parts;       // rows: of the query tiles, each with workgroups of its own
 };
 
-// The query tiles are cut into parts where the blocks alone are too few to fill the CUs a few times over (a list is taken
+// The query tiles are dealt to parts where the blocks alone are too few to fill the CUs a few times over (a list is taken
 // to name a quarter of the blocks), with 8 tiles or more to a part.
 MassPlan key_mass_plan(const Shape& s, const int32_t* start, bool lists) {
     int64_t blocks = 0;
     for (int b = 0; b < s.B; ++b) blocks += (int64_t)s.Hkv * ((start[b] + s.Lq + 63) / 64);
     if (lists) blocks = (blocks + 3) / 4;
-    MassPlan plan{s.Lq * s.G > 16, 1, 0};
+    MassPlan plan{s.Lq * s.G > 16, 1};
     const int T = kTileRows / s.G, tiles = (s.Lq + T - 1) / T;
     const int64_t groups = (blocks + kMassWaves - 1) / kMassWaves;
-    int parts = 1;
-    while (plan.rows && parts < 16 && tiles >= 16 * parts && groups * parts < 2048) ++parts;
-    const int per = (tiles + parts - 1) / parts;
-    plan.parts = (tiles + per - 1) / per;
-    plan.part_tiles = per;
+    while (plan.rows && plan.parts < 16 && tiles >= 16 * plan.parts && groups * plan.parts < 2048) plan.parts *= 2;
     return plan;
 }
 
@@ -427,13 +435,12 @@ hipError_t launch_key_mass(const MassArgs& a, hipStream_t stream) {
     const int entries = nkb + (a.table ? 1 : 0);  // (a list's last place copies what follows it)
     p.items = (entries + kMassWaves - 1) / kMassWaves;
     p.parts = plan.parts;
-    p.part_tiles = plan.part_tiles;
     p.ws = plan.parts > 1 ? static_cast<float*>(a.workspace) : nullptr;
     p.ws_stride = (int64_t)64 * kMassWaves * p.items;
     auto launch = [&](auto kernel, int64_t grid) {
         hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(kMassWaves * 64), 0, stream, p);
     };
-    const int64_t grid = (int64_t)p.items * rows;
+    const int64_t grid = (int64_t)p.items * rows, grid_parts = (grid * p.parts + 15) / 16 * 16;
     if (!plan.rows) {
         if (a.k4)
             a.table ? launch(key_mass_token_kernel<true, true>, grid) : launch(key_mass_token_kernel<true, false>, grid);
@@ -442,9 +449,9 @@ hipError_t launch_key_mass(const MassArgs& a, hipStream_t stream) {
         return hipGetLastError();
     }
     if (a.k4)
-        a.table ? launch(key_mass_rows_kernel<true, true>, grid * p.parts) : launch(key_mass_rows_kernel<true, false>, grid * p.parts);
+        a.table ? launch(key_mass_rows_kernel<true, true>, grid_parts) : launch(key_mass_rows_kernel<true, false>, grid_parts);
     else
-        a.table ? launch(key_mass_rows_kernel<false, true>, grid * p.parts) : launch(key_mass_rows_kernel<false, false>, grid * p.parts);
+        a.table ? launch(key_mass_rows_kernel<false, true>, grid_parts) : launch(key_mass_rows_kernel<false, false>, grid_parts);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.parts == 1) return e;
     a.table ? launch(key_mass_join_kernel<true>, grid) : launch(key_mass_join_kernel<false>, grid);
