@@ -175,7 +175,7 @@ __device__ __forceinline__ Found found_at(const PickParams& p, int row, int slic
     const int b0 = level_bins(level - 1) - 1 - 2 * tid;
     int h0 = 0, h1 = 0, p0 = 0, p1 = 0;  // this thread's two bins over all slices, and over those before
     const int* hist = slice_hist(p, row, level - 1, 0) + max(b0 - 1, 0);
-    constexpr int kAtOnce = 8;
+    constexpr int kAtOnce = 16;
     for (int k = 0; k < p.slices; k += kAtOnce) {
         int2 h[kAtOnce];
 #pragma unroll

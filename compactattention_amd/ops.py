@@ -183,12 +183,12 @@ class KV:
         """Global page pool [num_pages, 64, 128] and page_table [B*Hkv, blocks] int32."""
         _need_cuda("pool", pool, torch.bfloat16)
         _need_cuda("page_table", page_table, torch.int32)
-        if pool.dim() != 3 or pool.shape[1] != BLOCK or pool.shape[2] != HEAD_DIM or pool.stride(-1) != 1:
+        shape, st, pt = pool.shape, pool.stride(), page_table.stride()
+        if len(shape) != 3 or shape[1] != BLOCK or shape[2] != HEAD_DIM or st[2] != 1:
             raise ValueError("page pool must be [num_pages, 64, 128]")
-        if page_table.dim() != 2 or page_table.stride(1) != 1:
+        if len(pt) != 2 or pt[1] != 1:
             raise ValueError("page_table must be [rows, blocks] with contiguous rows")
-        return KV(pool, KvLayout(pool.data_ptr(), 0, 0, pool.stride(0), pool.stride(1), page_table.data_ptr(),
-                                 page_table.stride(0), pool.shape[0]), page_table)
+        return KV(pool, KvLayout(pool.data_ptr(), 0, 0, st[0], st[1], page_table.data_ptr(), pt[0], shape[0]), page_table)
 
     def check_blocks(self, name: str, batch: int, heads: int, blocks: int, tokens: Optional[int] = None) -> None:
         """Raise unless this layout covers ``blocks`` logical blocks of each of the ``batch`` x
@@ -845,10 +845,27 @@ def attn_decode(q: torch.Tensor, k: AnyKV, v: AnyKV, kv_len: Sequence[int], scal
 def _cache_launch(name: str, caches: Sequence[AnyKV], *tensors: Optional[torch.Tensor]):
     """The entry point for these caches (all bf16 or all in 4 bits) and the context to call it in."""
     bits4 = isinstance(caches[0], KV4)
-    if any(isinstance(kv, KV4) != bits4 for kv in caches):
-        raise ValueError("the caches of a call must all be bf16 or all be held in 4 bits")
-    guard = _on_device(*tensors, *(t for kv in caches for t in (kv.tensor, kv.page_table)))
-    return getattr(_hip.lib(), name + "_q4" if bits4 else name), guard
+    all_of = list(tensors)
+    for kv in caches:
+        if isinstance(kv, KV4) != bits4:
+            raise ValueError("the caches of a call must all be bf16 or all be held in 4 bits")
+        all_of.append(kv.tensor)
+        all_of.append(kv.page_table)
+    return getattr(_hip.lib(), name + "_q4" if bits4 else name), _on_device(*all_of)
+
+
+_INT32_MAX = (1 << 31) - 1
+
+
+def _span(tokens: int) -> int:
+    """A number of tokens as the C-ABI takes it: past 2^31 - 1 as good as that many; negative ones are refused there."""
+    return max(-1, min(int(tokens), _INT32_MAX))
+
+
+def _int32(name: str, value: int) -> int:
+    if not -_INT32_MAX <= int(value) <= _INT32_MAX:  # a ctypes argument would take it modulo 2^32
+        raise ValueError(f"{name}={value} must fit 32 bits")
+    return int(value)
 
 
 def attn_window(q: torch.Tensor, k: AnyKV, v: AnyKV, start: Union[int, Sequence[int]], window: int, sinks: int, scale: float,
@@ -875,27 +892,30 @@ def attn_window(q: torch.Tensor, k: AnyKV, v: AnyKV, start: Union[int, Sequence[
     d = make_dims(B, L, Hq, num_kv_heads, kv_cap)
     lib = _hip.lib()
     size = lib.ca_attn_window_q4_workspace_size if isinstance(k, KV4) else lib.ca_attn_window_workspace_size
-    need = size(ctypes.byref(d), sa, int(window), int(sinks), int(num_splits))
+    window, sinks, num_splits = _span(window), _span(sinks), _int32("num_splits", num_splits)
+    need = size(ctypes.byref(d), sa, window, sinks, num_splits)
     if need < 0:
         raise _hip.CaError(int(need), _hip.last_error())
     if need > 0 and (workspace is None or workspace.numel() * workspace.element_size() < need):
         workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
     lse = torch.empty((B, Hq, L), dtype=torch.float32, device=q.device) if with_lse else None
     with guard:
-        check(entry(ctypes.byref(d), ctypes.byref(ql), ctypes.byref(k.layout), ctypes.byref(v.layout), sa, int(window),
-                    int(sinks), float(scale), ctypes.byref(ol), _ptr(lse), int(num_splits), _ptr(workspace), int(need),
-                    _stream()))
+        check(entry(ctypes.byref(d), ctypes.byref(ql), ctypes.byref(k.layout), ctypes.byref(v.layout), sa, window,
+                    sinks, float(scale), ctypes.byref(ol), _ptr(lse), num_splits, _ptr(workspace), int(need), _stream()))
     return (out, lse) if with_lse else out
 
 
 def _rows(name: str, t: torch.Tensor, dtype: torch.dtype, rows: int, columns: int) -> int:
     """Checks a [>= rows, >= columns] tensor with contiguous rows; its stride from row to row."""
     _need_cuda(name, t, dtype)
-    if t.dim() != 2 or t.stride(1) != 1 and t.shape[1] > 1 or t.shape[0] < rows or t.shape[1] < columns:
-        raise ValueError(f"{name} {tuple(t.shape)} must be [>= {rows}, >= {columns}] with contiguous rows")
-    if t.stride(0) < t.shape[1] and t.shape[0] > 1:
+    shape, st = t.shape, t.stride()
+    if len(shape) != 2 or st[1] != 1 and shape[1] > 1 or shape[0] < rows or shape[1] < columns:
+        raise ValueError(f"{name} {tuple(shape)} must be [>= {rows}, >= {columns}] with contiguous rows")
+    if shape[0] < 2:
+        return shape[1]
+    if st[0] < shape[1]:
         raise ValueError(f"{name}'s rows must not overlap")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return st[0]
 
 
 def key_mass(q: torch.Tensor, k: AnyKV, lse: torch.Tensor, mass: torch.Tensor, start: Union[int, Sequence[int]], scale: float,
@@ -941,7 +961,7 @@ def key_mass(q: torch.Tensor, k: AnyKV, lse: torch.Tensor, mass: torch.Tensor, s
         workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
     with guard:
         check(entry(ctypes.byref(d), ctypes.byref(ql), ctypes.byref(k.layout), lse.data_ptr(), lse.stride(0), lse.stride(1), sa,
-                    int(window), int(sinks), _ptr(table), 0 if table is None else table.stride(0), _ptr(counts),
+                    _span(window), _span(sinks), _ptr(table), 0 if table is None else table.stride(0), _ptr(counts),
                     float(scale), mass.data_ptr(), ms, to.data_ptr(), os_, _ptr(workspace), int(need), _stream()))
     return to
 
@@ -958,15 +978,16 @@ def heavy_tokens(mass: torch.Tensor, lengths: Union[int, Sequence[int]], num_kv_
     B = rows // num_kv_heads
     la = past_array([lengths] * B if isinstance(lengths, (int, np.integer)) else lengths, B)
     ms = _rows("mass", mass, torch.float32, rows, max(la))
+    budget, sinks, recent = _int32("budget", budget), _int32("sinks", sinks), _int32("recent", recent)
     lib = _hip.lib()
-    need = lib.ca_heavy_tokens_workspace_size(B, num_kv_heads, la, int(budget))
+    need = lib.ca_heavy_tokens_workspace_size(B, num_kv_heads, la, budget)
     if need < 0:
         raise _hip.CaError(int(need), _hip.last_error())
-    keep = torch.empty((rows, int(budget)), dtype=torch.int32, device=mass.device)
+    keep = torch.empty((rows, budget), dtype=torch.int32, device=mass.device)
     workspace = torch.empty((need,), dtype=torch.uint8, device=mass.device) if need > 0 else None
     with _on_device(mass):
-        check(lib.ca_heavy_tokens(mass.data_ptr(), ms, B, num_kv_heads, la, int(budget), int(sinks), int(recent),
-                                  keep.data_ptr(), keep.stride(0), _ptr(workspace), int(need), _stream()))
+        check(lib.ca_heavy_tokens(mass.data_ptr(), ms, B, num_kv_heads, la, budget, sinks, recent, keep.data_ptr(),
+                                  keep.stride(0), _ptr(workspace), int(need), _stream()))
     return keep
 
 

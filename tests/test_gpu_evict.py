@@ -159,3 +159,61 @@ def test_captured():
         torch.cuda.synchronize()
         assert torch.equal(keep.cpu(), want_keep(mass, [3000], 4, 100, 4, 10))
         assert torch.equal(keep, ops.heavy_tokens(mass, 3000, 4, 100, 4, 10))
+
+
+def test_what_the_entry_points_refuse():
+    mass = masses(4, 300, "spread", 30)
+    with pytest.raises(ValueError, match="KV heads"):
+        ops.heavy_tokens(mass, 300, 3, 10)
+    with pytest.raises(ValueError, match="mass"):
+        ops.heavy_tokens(mass, 301, 4, 10)
+    with pytest.raises(ValueError, match="32 bits"):
+        ops.heavy_tokens(mass, 300, 4, (1 << 32) + 10)
+    for bad in (dict(budget=0), dict(budget=10, sinks=-1), dict(budget=10, sinks=6, recent=5)):
+        with pytest.raises(ops._hip.CaError):
+            ops.heavy_tokens(mass, 300, 4, **bad)
+    k, v = random_kv(1, 4, 300, 31)
+    cache = Cache(k, v, "paged", "cuda", 31)
+    q4 = Cache(k, v, "q4", "cuda", 31)
+    keep = ops.heavy_tokens(mass, 300, 4, 100)
+    (_, K2), (_, V2) = dest("paged", 1, 4, 100, 32)[0]
+    (_, K64), _ = dest("paged", 1, 4, 64, 32)[0]
+    with pytest.raises(ValueError, match="all be bf16 or all be held"):
+        ops.move_tokens(q4.K, q4.V, K2, V2, keep, 300, 4)
+    with pytest.raises(ValueError, match="k_dst"):
+        ops.move_tokens(cache.K, cache.V, K64, V2, keep, 300, 4)
+    with pytest.raises(ValueError, match="does not cover"):
+        ops.move_tokens(cache.K, cache.V, K2, V2, keep, 400, 4)
+    with pytest.raises(ValueError, match="int32"):
+        ops.move_tokens(cache.K, cache.V, K2, V2, keep.long(), 300, 4)
+    assert ops.move_tokens(cache.K, cache.V, K2, V2, keep, 300, 4) is None
+
+
+def test_two_calls_at_once():
+    a, b = masses(8, 50000, "spread", 40), masses(8, 40000, "ties", 41)
+    want = [ops.heavy_tokens(a, 50000, 8, 3000, 4, 100), ops.heavy_tokens(b, 40000, 8, 2000, 0, 50)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(8):
+        with torch.cuda.stream(streams[0]):
+            got[0].append(ops.heavy_tokens(a, 50000, 8, 3000, 4, 100))
+        with torch.cuda.stream(streams[1]):
+            got[1].append(ops.heavy_tokens(b, 40000, 8, 2000, 0, 50))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+def test_long_rows_captured():
+    """The launches of rows in slices, replayed with other weights in place."""
+    mass = masses(4, 40000, "spread", 50)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        keep = ops.heavy_tokens(mass, [40000, 17000], 2, 1000, 4, 10)
+    for i in range(4):
+        mass.copy_(masses(4, 40000, ("ties", "spread", "close", "odd")[i], 60 + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(keep.cpu(), want_keep(mass, [40000, 17000], 2, 1000, 4, 10))
+        assert torch.equal(keep, ops.heavy_tokens(mass, [40000, 17000], 2, 1000, 4, 10))

@@ -165,3 +165,52 @@ def test_weights_of_a_query_add_up_to_its_heads():
     ops.key_mass(q, cache.K, lse, mass, 2999, SCALE, cache.cap, 2)
     # the lse is that of weights rounded to bf16, off by 2^-8 each at most
     assert ((mass.double().sum(1) - 4).abs() <= 4 * 1.1 * 2.0 ** -8).all()
+
+
+def test_what_the_entry_point_refuses():
+    cache, q, lse, mass = setup([100], 3, 8, 2, "paged", seed=16)
+    args = ([100], SCALE, cache.cap, 2)
+    for bad, text in ((dict(lse=lse[:, :4]), "lse"), (dict(lse=lse.double()), "float32"), (dict(mass=mass[:1]), "mass"),
+                      (dict(mass=mass[:, :102]), "mass"), (dict(mass=mass.half()), "float32"), (dict(mass=mass[:1].expand(2, -1)), "overlap")):
+        a = dict(q=q, k=cache.K, lse=lse, mass=mass)
+        a.update(bad)
+        with pytest.raises(ValueError, match=text):
+            ops.key_mass(a["q"], a["k"], a["lse"], a["mass"], *args)
+    table = torch.zeros((2, cache.cap), dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="both"):
+        ops.key_mass(q, cache.K, lse, mass, *args, table=table)
+    with pytest.raises(ops._hip.CaError, match="overlap"):
+        ops.key_mass(q, cache.K, lse, mass[:, :110], *args, out=mass[:, 5:115])
+    with pytest.raises(ops._hip.CaError, match="window"):
+        ops.key_mass(q, cache.K, lse, mass, *args, window=-1)
+    old = mass.clone()
+    assert ops.key_mass(q[:, :0], cache.K, lse[:, :, :0], mass, *args) is mass and torch.equal(mass, old)
+    out = torch.zeros_like(mass)
+    ops.key_mass(q[:, :0], cache.K, lse[:, :, :0], mass, *args, out=out)
+    assert torch.equal(out[:, :100], mass[:, :100]) and (out[:, 100:] == 0).all()
+
+
+def test_parts_of_a_long_chunk():
+    """Enough query tiles over few blocks that parts of them have workgroups of their own, with lists and without."""
+    for kind in ("paged", "q4"):
+        cache, q, lse, mass = setup([130], 600, 16, 2, kind, seed=17)
+        old = mass.clone()
+        ops.key_mass(q, cache.K, lse, mass, [130], SCALE, cache.cap, 2)
+        check(mass, old, q, cache, lse, [130])
+        table = torch.full((2, cache.cap), -1, dtype=torch.int32)
+        lists = [[0, 2, 5, 11], list(range(1, 12))]
+        for r, x in enumerate(lists):
+            table[r, :len(x)] = torch.tensor(x, dtype=torch.int32)
+        counts = torch.tensor([4, 11], dtype=torch.int32).cuda()
+        out = torch.zeros_like(old)
+        out[:, 730:] = old[:, 730:]
+        ops.key_mass(q, cache.K, lse, old, [130], SCALE, cache.cap, 2, window=400, sinks=3, table=table.cuda(), counts=counts, out=out)
+        check(out, old, q, cache, lse, [130], 400, 3, lists)
+
+
+def test_the_largest_groups_and_odd_ones():
+    for Hq, Hkv in ((11, 1), (13, 1), (30, 2), (16, 1), (5, 5)):
+        cache, q, lse, mass = setup([70, 200], 37, Hq, Hkv, "heads", seed=Hq)
+        old = mass.clone()
+        ops.key_mass(q, cache.K, lse, mass, [70, 200], SCALE, cache.cap, Hkv)
+        check(mass, old, q, cache, lse, [70, 200])

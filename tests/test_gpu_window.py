@@ -172,3 +172,54 @@ def test_pages_past_4_gib(L):
         pools.append(pool)
     got = ops.attn_window(q, ops.KV.paged(pools[0], table), ops.KV.paged(pools[1], table), [start], W, S, SCALE, cache.cap, Hkv)
     assert torch.equal(got, want)
+
+
+def test_windows_and_positions_past_32_bits():
+    """A window or sinks past 2^31 are as good as everything; nothing is taken modulo 2^32."""
+    cache, q = setup([300], 2, 8, 2, HUGE, 0, "paged")
+    want = ops.attn_window(q, cache.K, cache.V, [300], 10 ** 6, 0, SCALE, cache.cap, 2)
+    for W, S in ((1 << 31, 0), ((1 << 32) + 5, 0), (1, (1 << 32) + 1), (10 ** 12, 10 ** 12)):
+        assert torch.equal(ops.attn_window(q, cache.K, cache.V, [300], W, S, SCALE, cache.cap, 2), want)
+    for kw in (dict(window=-(1 << 32) + 5), dict(window=0), dict(sinks=-(1 << 32))):
+        with pytest.raises(ops._hip.CaError):
+            ops.attn_window(q, cache.K, cache.V, [300], **{"window": 5, "sinks": 0, **kw}, scale=SCALE, kv_cap=cache.cap, num_kv_heads=2)
+    for bad in (dict(start=[(1 << 32) + 300]), dict(num_splits=1 << 32)):
+        with pytest.raises(ValueError):
+            ops.attn_window(q, cache.K, cache.V, **{"start": [300], **bad}, window=5, sinks=0, scale=SCALE, kv_cap=cache.cap, num_kv_heads=2)
+
+
+def test_what_the_entry_point_refuses():
+    cache, q = setup([100], 3, 8, 2, 50, 0, "paged")
+    q4, _ = setup([100], 3, 8, 2, 50, 0, "q4")
+    args = (50, 0, SCALE, cache.cap, 2)
+    with pytest.raises(ValueError, match="all be bf16 or all be held"):
+        ops.attn_window(q, cache.K, q4.V, [100], *args)
+    with pytest.raises(ValueError, match="does not cover"):
+        ops.attn_window(q, cache.K, cache.V, [200], *args)
+    with pytest.raises(ValueError, match="per-request"):
+        ops.attn_window(q, cache.K, cache.V, [100, 100], *args)
+    with pytest.raises(ValueError, match="q's shape"):
+        ops.attn_window(q, cache.K, cache.V, [100], *args, out=q[:, :2])
+    with pytest.raises(ValueError, match="bfloat16"):
+        ops.attn_window(q.float(), cache.K, cache.V, [100], *args)
+    empty, lse = ops.attn_window(q[:, :0], cache.K, cache.V, [100], *args, with_lse=True)
+    assert empty.shape == (1, 0, 8, 128) and lse.shape == (1, 8, 0)
+
+
+def test_two_calls_at_once():
+    """Calls on two streams have workspaces of their own."""
+    a, qa = setup([3000], 40, 8, 2, 2000, 5, "paged", seed=1)
+    b, qb = setup([2500], 40, 8, 2, 1500, 5, "paged", seed=2)
+    run = [lambda o=None: ops.attn_window(qa, a.K, a.V, [3000], 2000, 5, SCALE, a.cap, 2, num_splits=8, out=o),
+           lambda o=None: ops.attn_window(qb, b.K, b.V, [2500], 1500, 5, SCALE, b.cap, 2, num_splits=8, out=o)]
+    want = [f() for f in run]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(run[i]())
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
