@@ -220,19 +220,40 @@ __global__ __launch_bounds__(kMassWaves * 64) __attribute__((amdgpu_waves_per_eu
 
 // ---------------------------------------------------------------------------------------
 // Many query rows.  Four waves, each with the 64 keys of a block in registers, go through the packed rows together, the rows of
-// 32 / G tokens at a time from LDS (two places in turn: while one is read the next tile, already in registers, goes to the other and the
-// one after it is on its way).  A launch may deal the tiles to p.parts, each with workgroups of its own; their sums go to
-// p.ws and are joined in order by key_mass_join_kernel.
+// 32 / G tokens at a time from LDS (four places in turn: while one is read the next three tiles are on their way; through
+// registers and two places a chunk over 20 % of 32768 tokens took 161 us where it takes 150).  A launch may deal the tiles to
+// p.parts, each with workgroups of its own; their sums go to p.ws and are joined in order by key_mass_join_kernel.
 // Bound by vector instructions (one fma, exp2 and add a score, 16 of a wave's 64-lane cycles) beside 16 of the matrix cores:
 // 2048 queries over 32768 tokens (32 Q / 8 KV heads) 540 us, 0.98 PFLOP/s of the 1.21 that a large product reaches; 64 queries
-// 36 us, where a third is K's way from memory.  32x32x16 products, at two waves a SIMD where these run three, took 12 %
+// 34 us, where a third is K's way from memory.  32x32x16 products, at two waves a SIMD where these run three, took 12 %
 // longer; products woven into the weights of the tile before, instruction by instruction, 10 %.
 constexpr int kTileRows = 32;
+constexpr int kPlaces = 4;                   // tiles in LDS
+constexpr int kTileBytes = kTileRows * 256;
+
+// Words of a raw buffer resource over `bytes` bytes at base (wave-uniform).
+__device__ __forceinline__ u32x4_t range_of(const void* base, int bytes) {
+    const uint64_t a = reinterpret_cast<uint64_t>(base);
+    return u32x4_t{static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(a))),
+                   static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(a >> 32) & 0xffff)),
+                   static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(bytes)), 0x00020000u};
+}
+// Loads that write LDS: lane L's 16 (4) bytes at byte off of the resource go to LDS byte dst + 16 L (4 L); out of its range
+// they write zeros.  (Five wait states from a vector instruction that writes the resource to its use: s_mov and s_nop 3.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void to_lds16(u32x4_t rsrc, uint32_t off, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(off), "s"(rsrc), "s"(dst) : "memory", "m0");
+}
+__device__ __forceinline__ void to_lds4(u32x4_t rsrc, uint32_t off, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dword %0, %1, 0 offen lds" : : "v"(off), "s"(rsrc), "s"(dst) : "memory", "m0");
+}
+#pragma clang diagnostic pop
 
 template <bool kQ4, bool kTab>
 __global__ __launch_bounds__(kMassWaves * 64) __attribute__((amdgpu_waves_per_eu(3))) void key_mass_rows_kernel(MassParams p) {
-    __shared__ __attribute__((aligned(16))) uint8_t tile[2][kTileRows * 256];
-    __shared__ float tile_neg[2][kTileRows];
+    __shared__ __attribute__((aligned(16))) uint8_t tile[kPlaces][kTileBytes];
+    __shared__ float tile_lse[kPlaces][kMassWaves][64];
     const Shape& s = p.s;
     int row, item, cut;
     find_rows(p, &row, &item, &cut);
@@ -275,41 +296,29 @@ __global__ __launch_bounds__(kMassWaves * 64) __attribute__((amdgpu_waves_per_eu
     const int ua = tile_after(64 * last_kb - start + 63);
     const bool always = p.window == 0 || 64 * last_kb + 64 <= p.sinks;
     const int ub = always ? s.Lq / T : min(first_tile(64 * first_kb - start + p.window), s.Lq / T);
-    // Thread tid moves chunk tid % 16 of rows tid / 16 and 16 + tid / 16 of a tile, and tid < 32 the lse of row tid; chunk c
-    // of row r stands at chunk c ^ (r % 16), for reads without bank conflicts.  Rows past T tokens' (where the group does not
-    // divide 32) and past the last token are the last one's with weights of 0.
+    // Wave w moves rows 4 w + 16 i + l / 16 of a tile (i = 0, 1) and its own copy of the rows' lse; chunk c of row r stands at
+    // chunk c ^ (r % 16), for reads without bank conflicts.  Rows past T tokens' (where the group does not divide 32) and
+    // past the last token count nowhere.
     const int q_sh = static_cast<int>(p.q.sh) * 2, q_st = static_cast<int>(p.q.st) * 2;  // bytes (the host checks their range)
     const int lse_sh = static_cast<int>(p.lse_sh) * 4;
-    const __amdgpu_buffer_rsrc_t q_rsrc = __builtin_amdgcn_make_buffer_rsrc(
-        p.q.data + b * p.q.sb + (int64_t)hk * G * p.q.sh, 0, (s.Lq - 1) * q_st + (G - 1) * q_sh + 256, 0x00020000);
-    const __amdgpu_buffer_rsrc_t lse_rsrc = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<float*>(p.lse) + b * p.lse_sb + (int64_t)hk * G * p.lse_sh, 0, (s.Lq - 1) * 4 + (G - 1) * lse_sh + 4, 0x00020000);
-    const int c = tid & 15;
+    const int q_bytes = (s.Lq - 1) * q_st + (G - 1) * q_sh + 256, lse_bytes = (s.Lq - 1) * 4 + (G - 1) * lse_sh + 4;
+    const u32x4_t q_rsrc = range_of(p.q.data + b * p.q.sb + (int64_t)hk * G * p.q.sh, q_bytes);
+    const u32x4_t lse_rsrc = range_of(p.lse + b * p.lse_sb + (int64_t)hk * G * p.lse_sh, lse_bytes);
     int at[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int r = min(16 * i + (tid >> 4), T * G - 1);
-        at[i] = r / G * q_st + r % G * q_sh + 16 * c;
+        at[i] = r / G * q_st + r % G * q_sh + 16 * ((tid & 15) ^ (tid >> 4));
     }
-    const int lse_r = min(tid & 31, T * G - 1), lse_t = lse_r / G;
-    const int lse_at = lse_t * 4 + lse_r % G * lse_sh;
-    const bool lse_row = (tid & 31) < T * G;
-    u32x4_t held[2];
-    float held_neg = 0.0f;
-    auto fetch = [&](int u) {  // (a token past the last one: out of the range and zero, or another row's; the range check
-                                // covers the vector offset only)
+    const int lse_r = min(l & 31, T * G - 1), lse_at = lse_r / G * 4 + lse_r % G * lse_sh;
+    const uint32_t tile0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to_lds(tile[0]))) + w * 1024;
+    const uint32_t lse0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to_lds(reinterpret_cast<const uint8_t*>(tile_lse[0][w]))));
+    auto fetch = [&](int u, int to) {  // (a tile past the last one: out of the ranges, no access; the range check covers the
+                                       // vector offset only)
+        const uint32_t qo = u < u1 ? u * T * q_st : q_bytes, lo = u < u1 ? u * T * 4 : lse_bytes;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) held[i] = __builtin_amdgcn_raw_buffer_load_b128(q_rsrc, at[i] + u * T * q_st, 0, 0);
-        if (tid < kTileRows) {
-            const float lse = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(lse_rsrc, lse_at + u * T * 4, 0, 0));
-            held_neg = lse_row && u * T + lse_t < s.Lq ? neg_lse(lse) : -__builtin_inff();
-        }
-    };
-    const int to_lds = (tid >> 4) * 256 + ((c ^ (tid >> 4)) * 16);
-    auto put = [&](int to) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4_t*>(tile[to] + to_lds + 4096 * i) = held[i];
-        if (tid < kTileRows) tile_neg[to][tid] = held_neg;
+        for (int i = 0; i < 2; ++i) to_lds16(q_rsrc, at[i] + qo, tile0 + to * kTileBytes + 4096 * i);
+        to_lds4(lse_rsrc, lse_at + lo, lse0 + to * (kMassWaves * 256));
     };
     int row_t[2];  // the token of the lane's rows in a tile, none's past T tokens' rows
 #pragma unroll
@@ -321,8 +330,11 @@ __global__ __launch_bounds__(kMassWaves * 64) __attribute__((amdgpu_waves_per_eu
     auto run = [&](int end, auto masked) {
         constexpr bool kMask = decltype(masked)::value;
         for (; u < end; u += p.parts) {
-            if (u + p.parts < u1) put(from ^ 1);
-            if (u + 2 * p.parts < u1) fetch(u + 2 * p.parts);
+            // the tile is there (the six loads of the two behind it may be on their way), and the last one's reads are over
+            asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            fetch(u + 3 * p.parts, (from + 3) & 3);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 bf16x8_t q[4];
@@ -330,20 +342,18 @@ __global__ __launch_bounds__(kMassWaves * 64) __attribute__((amdgpu_waves_per_eu
                 for (int j = 0; j < 4; ++j)
                     q[j] = *reinterpret_cast<const bf16x8_t*>(tile[from] + 4096 * i + n * 256 + ((keys.chunk(j, g) ^ n) * 16));
                 const int t = u * T + row_t[i];
-                add_weights<kQ4, kMask>(p, keys, q, tile_neg[from][16 * i + n], kMask && t >= 0 && t < s.Lq ? start + t : -1, kb, g, acc);
+                const float neg = row_t[i] >= 0 ? neg_lse(tile_lse[from][w][16 * i + n]) : -__builtin_inff();
+                add_weights<kQ4, kMask>(p, keys, q, neg, kMask && t >= 0 && t < s.Lq ? start + t : -1, kb, g, acc);
             }
-            __syncthreads();
-            from ^= 1;
+            from = (from + 1) & 3;
         }
     };
     if (u0 < u1) {
-        fetch(u0);
-        put(0);
-        if (u0 + p.parts < u1) fetch(u0 + p.parts);
-        __syncthreads();
+        for (int i = 0; i < 3; ++i) fetch(u0 + i * p.parts, i);
         run(min(ua, u1), std::true_type{});
         run(min(ub, u1), std::false_type{});
         run(u1, std::true_type{});
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (loads into LDS end before the workgroup)
     }
     const float sum = sum_rows(acc, n);
     if (!here) return;
@@ -383,7 +393,9 @@ struct MassPlan {
 };
 
 // The query tiles are dealt to parts where the blocks alone are too few to fill the CUs a few times over (a list is taken
-// to name a quarter of the blocks), with 8 tiles or more to a part.
+// to name a quarter of the blocks), with 8 tiles or more to a part, or 3 where there are fewer workgroups than CUs (100 queries
+// over 500 tokens, 32 Q / 8 KV heads, 20.2 -> 11.9 us; 235 over 10 % of 28955, 16 / 2, 34.7 -> 26.2; where they are more, 64
+// over 32768, 34 -> 44).
 MassPlan key_mass_plan(const Shape& s, const int32_t* start, bool lists) {
     int64_t blocks = 0;
     for (int b = 0; b < s.B; ++b) blocks += (int64_t)s.Hkv * ((start[b] + s.Lq + 63) / 64);
@@ -391,7 +403,8 @@ MassPlan key_mass_plan(const Shape& s, const int32_t* start, bool lists) {
     MassPlan plan{s.Lq * s.G > 16, 1};
     const int T = kTileRows / s.G, tiles = (s.Lq + T - 1) / T;
     const int64_t groups = (blocks + kMassWaves - 1) / kMassWaves;
-    while (plan.rows && plan.parts < 16 && tiles >= 16 * plan.parts && groups * plan.parts < 2048) plan.parts *= 2;
+    auto few = [&](int least, int places) { return tiles >= 2 * least * plan.parts && groups * plan.parts < places; };
+    while (plan.rows && plan.parts < 16 && (few(8, 2048) || few(3, 256))) plan.parts *= 2;
     return plan;
 }
 
@@ -402,7 +415,7 @@ int64_t key_mass_workspace_bytes(const Shape& s, const int32_t* start, bool list
     if (!plan.rows || plan.parts <= 1) return 0;
     int nkb = 1;
     for (int b = 0; b < s.B; ++b) nkb = max(nkb, (start[b] + s.Lq + 63) / 64);
-    const int64_t items = (nkb + (lists ? 1 : 0) + kMassWaves - 1) / kMassWaves;
+    const int64_t items = (nkb + (lists ? 1 : 0) + kMassWaves - 1) / kMassWaves | (lists ? 1 : 0);
     return (int64_t)plan.parts * s.B * s.Hkv * items * kMassWaves * 64 * (int64_t)sizeof(float);
 }
 
@@ -434,6 +447,9 @@ hipError_t launch_key_mass(const MassArgs& a, hipStream_t stream) {
     const int rows = a.s.B * a.s.Hkv;
     const int entries = nkb + (a.table ? 1 : 0);  // (a list's last place copies what follows it)
     p.items = (entries + kMassWaves - 1) / kMassWaves;
+    // (lists: the rows' first items are those with blocks, an odd count deals them to all XCDs; 142 queries of 14 requests
+    // 41.7 -> 39.5 us)
+    if (a.table) p.items |= 1;
     p.parts = plan.parts;
     p.ws = plan.parts > 1 ? static_cast<float*>(a.workspace) : nullptr;
     p.ws_stride = (int64_t)64 * kMassWaves * p.items;
