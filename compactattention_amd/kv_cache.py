@@ -245,8 +245,12 @@ class PagedKVCache:
             self._upload(b0, b1)
 
     def reserve(self, tokens: int) -> None:
-        """Map pages for the first ``tokens`` tokens of every request ahead of time."""
-        self._map(0, -(-int(tokens) // BLOCK))
+        """Map pages for the first ``tokens`` tokens of every request ahead of time (those that were dropped stay so)."""
+        a, b, _ = self._dropped
+        nb = -(-int(tokens) // BLOCK)
+        if a < b:
+            self._map(0, min(a, nb))
+        self._map(b if a < b else 0, nb)
 
     def _unshare(self, kb: int) -> None:
         """Copy-on-write of logical block kb: rows (in order) whose page still has other holders
@@ -466,6 +470,7 @@ class PagedKVCache:
         the lse [B, Hq, L] that their attention returned, over all keys or the blocks of its table."""
         if self.mass is None:
             raise ValueError("cache built without the keys' weights (with_mass)")
+        self._need_pages()
         L = q.shape[1]
         if L > self.length:
             raise ValueError(f"{L} queries over {self.length} tokens")

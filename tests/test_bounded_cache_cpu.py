@@ -47,6 +47,15 @@ def test_drop_outside_gives_back_what_no_later_query_sees():
     assert c.k_hf().shape == (2, 2, 5, 128) and consistent(c)
 
 
+def test_dropped_pages_stay_dropped():
+    c = cache(600, with_mass=True)
+    c.drop_outside(100, 3)
+    c.reserve(64 * 12)
+    assert (c._pt[:, 1:7] == -1).all() and (c._pt[:, 7:12] >= 0).all() and consistent(c)
+    with pytest.raises(ValueError, match="were dropped"):  # the weights of keys that are gone
+        c.add_mass(torch.zeros((2, 1, 4, 128), dtype=torch.bfloat16), torch.zeros((2, 4, 1)), 0.1)
+
+
 def test_slack_keeps_what_a_rejected_draft_brings_back():
     c = cache(600)
     c.drop_outside(100, 0, slack=64)
