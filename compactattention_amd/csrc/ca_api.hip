@@ -932,8 +932,8 @@ int attn_window(const ca_dims* dims, const ca_seq_layout* q, const int32_t* star
     if (!(scale > 0.0f) || scale > 3.0e38f) return fail(CA_ERR_INVALID, "scale must be positive and finite");
     if (num_splits < 0 || num_splits > ca::kMaxDecodeSplits)
         return fail(CA_ERR_INVALID, "num_splits=%d outside [0, %d]", num_splits, ca::kMaxDecodeSplits);
-    // a launch has less than 2^32 threads: 512 for a split of at least 32 rows (or of all there are)
-    if ((int64_t)a.s.B * a.s.Hkv * (((int64_t)a.s.Lq * a.s.G + 31) / 32) * max(num_splits, 1) >= (int64_t)1 << 23)
+    // a launch has less than 2^32 threads: 512 for a split of at least 16 rows (or of all there are)
+    if ((int64_t)a.s.B * a.s.Hkv * (((int64_t)a.s.Lq * a.s.G + 15) / 16) * max(num_splits, 1) >= (int64_t)1 << 23)
         return fail(CA_ERR_LIMIT, "%d rows of %d queries in %d splits are too many", a.s.B * a.s.Hkv, a.s.Lq * a.s.G, num_splits);
     const int splits = num_splits == 0 ? ca::attn_window_splits(a.s, kv_len, window, sinks, bits4) : num_splits;
     const int64_t need = ca::attn_workspace_bytes(a.s, splits);
@@ -1042,8 +1042,9 @@ int move_tokens(const int32_t* keep, int64_t keep_stride, int32_t batch, int32_t
     if ((rc = check_rows(batch, hkv, len, n, "n", &longest)) != CA_OK) return rc;
     if (keep == nullptr || !aligned4(keep)) return fail(CA_ERR_INVALID, "keep is NULL or misaligned");
     if (keep_stride < n) return fail(CA_ERR_INVALID, "keep_stride=%lld < n=%d", (long long)keep_stride, n);
-    if ((mass == nullptr) != (mass_out == nullptr)) return fail(CA_ERR_INVALID, "mass and mass_out must both be given or both be NULL");
-    if (mass != nullptr && (mass_stride < longest || mass_out_stride < n || !aligned4(mass) || !aligned4(mass_out)))
+    if ((mass == nullptr) != (mass_out == nullptr) && (mass != nullptr || longest > 0))
+        return fail(CA_ERR_INVALID, "mass and mass_out must both be given or both be NULL");
+    if (mass_out != nullptr && (mass_stride < longest || mass_out_stride < n || !aligned4(mass) || !aligned4(mass_out)))
         return fail(CA_ERR_INVALID, "rows of mass (%lld) and mass_out (%lld) do not hold %d and %d tokens, or are misaligned",
                     (long long)mass_stride, (long long)mass_out_stride, longest, n);
     if (mass != nullptr) {
@@ -1152,7 +1153,7 @@ int ca_heavy_tokens(const float* mass, int64_t mass_stride, int32_t batch, int32
                     int64_t workspace_bytes, void* stream) {
     int longest = 0, rc;
     if ((rc = check_rows(batch, num_kv_heads, len_host, budget, "budget", &longest)) != CA_OK) return rc;
-    if (mass == nullptr || keep == nullptr || !aligned4(mass) || !aligned4(keep))
+    if ((mass == nullptr && longest > 0) || keep == nullptr || !aligned4(mass) || !aligned4(keep))
         return fail(CA_ERR_INVALID, "mass or keep is NULL or misaligned");
     if (sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget)
         return fail(CA_ERR_INVALID, "sinks=%d and recent=%d must not be negative nor more than budget=%d together", sinks, recent,

@@ -65,6 +65,13 @@ def test_window_refusals(bits4, change, code, text):
                   None), code, text)
 
 
+def test_a_window_launch_has_less_than_2_32_threads():
+    # 2^20 queries of 64 x 2 rows in tiles of 16, which short windows take: 2^23 workgroups of 512
+    d = dims(batch=64, q_len=1 << 20, num_q_heads=2, kv_cap=1 << 14)
+    refused(_hip.lib().ca_attn_window(d, seq(), kv(pts=1 << 14), kv(pts=1 << 14), ints(*[0] * 64), 1, 0, 0.1, seq(), None, 1, None, 0, None), LIMIT,
+            "too many")
+
+
 @pytest.mark.parametrize("k,text", [(kv(pts=11), "page_table_stride"), (kv(pages=0), "num_pages"), (kv(stok=4), "strides"),
                                     (kv(data=FAKE + 8), "aligned")])
 def test_window_cache_refusals(k, text):

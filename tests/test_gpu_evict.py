@@ -52,6 +52,17 @@ def test_heavy_tokens(kind, lens, Hkv, budget, sinks, recent):
     assert torch.equal(keep.cpu(), want_keep(mass, lens, Hkv, budget, sinks, recent))
 
 
+@pytest.mark.parametrize("columns", [0, 5])
+def test_requests_without_tokens(columns):
+    mass = torch.ones((4, columns), device="cuda")
+    keep = ops.heavy_tokens(mass, [0, 0], 2, 70, 2, 3)
+    assert torch.equal(keep.cpu(), torch.full((4, 70), -1, dtype=torch.int32))
+    pool = torch.ones((8, 64, 128), dtype=torch.bfloat16, device="cuda")
+    K = ops.KV.paged(pool, torch.arange(8, dtype=torch.int32, device="cuda").view(4, 2))
+    moved = ops.move_tokens(K, K, K, K, keep, [0, 0], 2, mass=mass)
+    assert torch.equal(moved.cpu(), torch.zeros((4, 70))) and bool((pool == 1).all())
+
+
 def test_strided_mass_and_many_rows():
     mass = masses(64 * 8, 300, "ties", 1)
     lens = [37 + 4 * b for b in range(64)]
