@@ -995,9 +995,9 @@ def move_tokens(k: AnyKV, v: AnyKV, k_dst: AnyKV, v_dst: AnyKV, keep: torch.Tens
                 num_kv_heads: int, mass: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Token i of row r of k_dst and v_dst becomes token keep[r, i] of k and v, for i < min(keep's columns, lengths[b]);
     keep [B*Hkv, n] int32 as ``heavy_tokens`` returns it.  All four caches are bf16 or all held in 4 bits (whose bytes
-    are copied, not quantised again).  Source and destination may lie in one pool, but no page (of a contiguous cache
-    no token) that is read may be written.  With mass [B*Hkv, >= tokens] the weights follow: returns [B*Hkv, n] fp32,
-    0 past a row's tokens."""
+    are copied, not quantised again).  Source and destination may lie in one pool, but no destination page may be
+    named twice and no page (of a contiguous cache no token) that is read may be written.  With mass [B*Hkv, >= tokens]
+    the weights follow: returns [B*Hkv, n] fp32, 0 past a row's tokens."""
     _need_cuda("keep", keep, torch.int32)
     if keep.dim() != 2 or num_kv_heads < 1 or keep.shape[0] % num_kv_heads or keep.shape[0] == 0:
         raise ValueError(f"keep {tuple(keep.shape)} must be [B*Hkv, n] for {num_kv_heads} KV heads")

@@ -512,9 +512,10 @@ int64_t ca_attn_window_q4_workspace_size(const ca_dims* dims, const int32_t* sta
  * bf16 (or keys in 4 bits), fp32 products, in an order that depends on the sizes only.  Visible: j <= p =
  * start_host[b] + t, and with window > 0 also p - j < window or j < sinks.  lse (element (b, h, t) at
  * b*lse_stride_b + h*lse_stride_h + t) is the log-sum-exp that attention returned; a query whose lse is
- * -inf adds nothing.  mass and out are [rows, stride] fp32, stride >= the tokens of a row; out may be
- * mass (else they must not overlap).  With table and counts (both or neither) only the blocks of row's list add weight, as
- * attention over that list gave it: ascending block ids, none twice; the other keys of out get mass.
+ * -inf adds nothing to keys that are finite.  mass and out are [rows, stride] fp32, stride >= the tokens of
+ * a row; out may be mass (else they must not overlap).  With table and counts (both or neither) only the
+ * blocks of row's list add weight, as attention over that list gave it: ascending block ids, none twice; the
+ * other keys of out get mass.
  * ca_key_mass_workspace_size: the bytes of workspace that a call needs, with lists or without (0: NULL will do).
  * NaN: a key that is NaN gets a NaN weight where a query sees it, a query or lse that is NaN gives one
  * to every key that it sees; what is hidden changes nothing.
@@ -547,9 +548,9 @@ int ca_heavy_tokens(const float* mass, int64_t mass_stride, int32_t batch, int32
 /*
  * Copies tokens into other blocks of a cache: token i of row r of k_dst and v_dst becomes token
  * keep[r][i] of k and v, for i < min(n, len_host[b]); keep as ca_heavy_tokens writes it (positions are
- * taken into [0, len)).  k and k_dst may be one pool; no page or token that is read may be written.  The
- * tokens behind a row's last one stay as they were, and ids outside the pool are written through nowhere.
- * With mass and mass_out (both or neither) mass_out[r][i] = mass[r][keep[r][i]], 0 for
+ * taken into [0, len)).  k and k_dst may be one pool; no destination page may be named twice, and no page or
+ * token that is read may be written.  The tokens behind a row's last one stay as they were, and ids outside
+ * the pool are written through nowhere.  With mass and mass_out (both or neither) mass_out[r][i] = mass[r][keep[r][i]], 0 for
  * min(n, len) <= i < n.
  */
 int ca_move_tokens(const ca_kv_layout* k, const ca_kv_layout* v, const ca_kv_layout* k_dst,
