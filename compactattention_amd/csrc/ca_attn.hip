@@ -94,9 +94,14 @@ __device__ __forceinline__ void wait_dma() {
 // kTab: block lists come from the per-row table (prefill); otherwise they are the identity
 // 0 .. nkb-1 (dense decode), or kWin the blocks of a window (WindowList).  Under a window what is hidden has no
 // effect, whatever it holds (finish).
-template <int NW, bool kTab, bool kRow, bool kWin = false>
+// kPair (windows of few tiles): BM = 16 * NW rows, two waves to each 32 of them, which take a block each of every two and
+// join at the end, so twice as many workgroups share the work and no second launch joins parts: 1000 queries under 1500 (28
+// Q / 4 KV heads) 41 us in 220 workgroups, where 112 of 256 rows take 58 whole and 57 in two splits; 2000 under 1000 (8 / 1)
+// 29 against 45.  Where the tiles of 256 rows fill the CUs they are faster (2048 under 4096, 32 / 8, 140 and 156).
+template <int NW, bool kTab, bool kRow, bool kWin = false, bool kPair = false>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) void attn_fwd_kernel(AttnParams p) {
-    constexpr int BM = 32 * NW;
+    static_assert(!kPair || kWin, "pairs of waves take windows");
+    constexpr int BM = kPair ? 16 * NW : 32 * NW;
     __shared__ __attribute__((aligned(16))) uint8_t smem[kStages * (kKBytes + kVBytes)];  // K ring, then V ring
 
     // Ragged launches whose row tiles fill 3/4 of the CUs: one round of row tiles is enough
@@ -181,9 +186,11 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     const int l = tid & 63;
     const int h = l >> 5;
     const int n = l & 31;
+    const int rw = kPair ? w & (NW / 2 - 1) : w;  // which 32 rows
+    const int grp = kPair ? __builtin_amdgcn_readfirstlane(w / (NW / 2)) : 0;  // and which block of two
 
     // ---- Q fragments (B operand of S^T = K Q^T); the loads are in flight while the lists are read ----
-    const int qrow = r0 + 32 * w + n;
+    const int qrow = r0 + 32 * rw + n;
     const bool qvalid = qrow < rows_total;
     const int qt = qvalid ? qrow / G : 0;
     const int qg = qvalid ? qrow - qt * G : 0;
@@ -345,13 +352,13 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     const int k_r = swap23(n);
     int k_off[8];
 #pragma unroll
-    for (int ds = 0; ds < 8; ++ds) k_off[ds] = k_r * 256 + (((2 * ds + h) ^ (k_r & 15)) * 16);
+    for (int ds = 0; ds < 8; ++ds) k_off[ds] = k_r * 256 + (((2 * ds + h) ^ (k_r & 15)) * 16) + grp * 16384;
     const int v_rq = (l & 15) >> 2;
     const int v_x = 2 * ((l >> 4) & 1) + ((l & 3) >> 1);
     int v_off[4];
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt)
-        v_off[dt] = kVRing + (8 * h + v_rq) * 256 + (4 * (dt ^ v_rq) + v_x) * 16 + (l & 1) * 8;
+        v_off[dt] = kVRing + (8 * h + v_rq) * 256 + (4 * (dt ^ v_rq) + v_x) * 16 + (l & 1) * 8 + grp * 16384;
     // The normaliser sums the bf16-rounded weights the PV product uses: the 16-block 4x4x4 MFMA
     // with a ones A operand adds each lane's own four values (its column of its block) to every
     // element of the lane's accumulator.  (v_dot2 does the same in the VALU's encoding but waits
@@ -473,7 +480,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
                     const uint32_t both = ((key >> 3) & 1) == h ? mine : other;
                     const float wt = __uint_as_float((key & 1) ? both & 0xffff0000u : both << 16);
                     const bool seen = key <= vis && (key > vis - p.window || key < p.sinks - kb * 64);
-                    const uint8_t* vr = smem + kVRing + vbase + key * 256 + 8 * h;
+                    const uint8_t* vr = smem + kVRing + vbase + grp * 16384 + key * 256 + 8 * h;
 #pragma unroll
                     for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
@@ -504,6 +511,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     // each load makes its resource (!kRow) the prologue and the other slots leave out what the list
     // does not have, and then wait for all: 8 / 8 heads, 200 tokens on 6 blocks 21.0 -> 20.5 us.
     Blk vq0, vq1;  // the two entries whose K is issued and V is not
+    Blk vq2, vq3;  // (kPair: four, the next two pairs')
     auto issue_k = [&](int i, int half, const Blk& b) {
         load_half(kbase_row, k_rsrc, p.k.sblk, kstok_b, k_goff, b.id, b.kp, half, lds0 + (i & 3) * 16384);
     };
@@ -539,7 +547,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
     bf16x8_t kf[16];
     auto fused = [&](f32x16_t(&sc)[2], f32x16_t(&sn)[2], auto place, int j) {
         constexpr int R = decltype(place)::value;
-        constexpr int kK = ((R + 1) & 3) * 16384, kV = R * 16384, kN = ((R + 2) & 3) * 16384;
+        constexpr int kK = kPair ? ((R + 1) & 1) * 32768 : ((R + 1) & 3) * 16384, kV = kPair ? R * 32768 : R * 16384;
+        constexpr int kN = kPair ? kV : ((R + 2) & 3) * 16384;
         bf16x8_t vf[16];
         uint32_t pw[16];  // packed weights, two per word
         float y[33], x[34];
@@ -563,17 +572,21 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             if (i + kAhead < 16) kf[i + kAhead] = k_frag(kK, i + kAhead);
-            if (i >= 16 - kVAhead) vf[i - 16 + kVAhead] = v_frag(kV, i - 16 + kVAhead);
+            if (!kPair && i >= 16 - kVAhead) vf[i - 16 + kVAhead] = v_frag(kV, i - 16 + kVAhead);
             sn[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i], qf[i >> 1], i < 2 ? zero : sn[i & 1], 0, 0, 0);
             stage(e++);
             if (i < kEarly) stage(e++);
             asm volatile("" : "+v"(sn[i & 1]), "+v"(y[e - 1]), "+v"(x[e - 2]), "+v"(rs), "+v"(sc[e >> 4]) : : "memory");
             __builtin_amdgcn_sched_barrier(0);
         }
-        mid_slot(false);
+        mid_slot(kPair);
+        if (kPair) {
+#pragma unroll
+            for (int i = 0; i < kVAhead; ++i) vf[i] = v_frag(kV, i);
+        }
         // a wave in its PV half, whose groups are shorter, goes before one in its scores (-0.5 %)
         __builtin_amdgcn_s_setprio(1);
-        const Blk nb = next_blk(j + 5);
+        const Blk nb = next_blk(kPair ? 2 * j + 6 : j + 5), nb1 = kPair ? next_blk(2 * j + 7) : nb;
         float mx = -__builtin_inff();
         bool up = false;
 #pragma unroll
@@ -596,20 +609,137 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
             if (i == 13) up = __ballot(mx > m_run + kRescale) != 0;
             if (i == 14) l_run += rs[0];  // this lane's half of the row; combined across lanes n, n+32 at the end
             asm volatile("" : "+v"(oacc[i & 3]), "+v"(mx), "+v"(l_run) : : "memory");
-            if (i == 1) issue_v(j + 3, 0, vq0);
-            if (i == 4) issue_v(j + 3, 1, vq0);
-            if (i == 7) issue_k(j + 5, 0, nb);
-            if (i == 10) issue_k(j + 5, 1, nb);
+            if (kPair) {
+                if (i < 4) issue_v(2 * j + 2 + (i >> 1), i & 1, i < 2 ? vq0 : vq1);
+                if (i >= 4 && i < 8) issue_k(2 * j + 6 + ((i - 4) >> 1), i & 1, i < 6 ? nb : nb1);
+            } else {
+                if (i == 1) issue_v(j + 3, 0, vq0);
+                if (i == 4) issue_v(j + 3, 1, vq0);
+                if (i == 7) issue_k(j + 5, 0, nb);
+                if (i == 10) issue_k(j + 5, 1, nb);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
-        vq0 = vq1;
-        vq1 = nb;
+        if (kPair) {
+            vq0 = vq2;
+            vq1 = vq3;
+            vq2 = nb;
+            vq3 = nb1;
+        } else {
+            vq0 = vq1;
+            vq1 = nb;
+        }
         __builtin_amdgcn_s_setprio(0);
         if (up) rise(mx);
     };
 
     const int n_un = e_mask - e0;  // blocks before the first masked one
-    if (nblk > 0) {
+    if constexpr (kPair) {
+        // Two blocks a slot, places 2 (i % 2) and the next one of both rings for pair i.  The barrier of slot i stands for: K of
+        // pair i + 2 and V of pair i have landed, and every wave has read K of pair i + 1 and V of pair i - 1; so behind it V
+        // of pair i + 1 and K of pair i + 3 are issued, and all are waited for at the next one.  An entry past the list's end
+        // loads zeros, and its scores are hidden.
+        const int pairs = (nblk + 1) >> 1, whole_pairs = n_un >> 1;
+        auto pair_k = [&](int i, const Blk& b0, const Blk& b1) {
+            if (i >= pairs) return;
+            for (int half = 0; half < 2; ++half) issue_k(2 * i, half, b0);
+            for (int half = 0; half < 2; ++half) issue_k(2 * i + 1, half, b1);
+        };
+        auto pair_v = [&](int i, const Blk& b0, const Blk& b1) {
+            if (i >= pairs) return;
+            for (int half = 0; half < 2; ++half) issue_v(2 * i, half, b0);
+            for (int half = 0; half < 2; ++half) issue_v(2 * i + 1, half, b1);
+        };
+        auto hide = [&](int i) {  // of pair i what the rows do not see
+            const int e = e0 + 2 * i + grp;
+            if (e >= e1) {
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) sc[kt][j] = -__builtin_inff();
+            } else if (e >= e_mask) {
+                mask(block_id(e));
+            }
+        };
+        if (pairs > 0) {
+            const Blk b0 = next_blk(0), b1 = next_blk(1);
+            vq0 = next_blk(2);
+            vq1 = next_blk(3);
+            vq2 = next_blk(4);
+            vq3 = next_blk(5);
+            pair_k(0, b0, b1);
+            pair_k(1, vq0, vq1);
+            pair_v(0, b0, b1);
+            mid_slot(true);
+            scores(0);
+            hide(0);
+            block_max();
+            mid_slot(true);
+            pair_k(2, vq2, vq3);
+            int j = 0;
+            f32x16_t sn[2];
+            if (2 < whole_pairs) {
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) kf[i] = k_frag(32768, i);
+            }
+            for (; j + 2 < whole_pairs; j += 2) {
+                fused(sc, sn, IntC<0>{}, j);
+                fused(sn, sc, IntC<1>{}, j + 1);
+            }
+            const int j0 = j;
+            for (; j < pairs; ++j) {
+                mid_slot(true);
+                pair_v(j + 1, vq0, vq1);
+                if (j == j0) {  // (K of pair j + 2 is on its way)
+                    vq0 = vq2;
+                    vq1 = vq3;
+                } else {
+                    vq0 = next_blk(2 * j + 4);
+                    vq1 = next_blk(2 * j + 5);
+                    pair_k(j + 2, vq0, vq1);
+                }
+                const int e = e0 + 2 * j + grp;
+                const bool cut = e >= e_mask && e < e1;
+                finish((j & 1) * 32768, cut, cut ? block_id(e) : 0);
+                if (j + 1 < pairs) {
+                    scores(((j + 1) & 1) * 32768);
+                    hide(j + 1);
+                    block_max();
+                }
+            }
+        }
+        // the upper waves' sums through LDS, to the lower waves of the same rows
+        wait_dma();
+        __syncthreads();
+        float4* const joined = reinterpret_cast<float4*>(smem) + rw * 1024 + l;
+        float2* const stats = reinterpret_cast<float2*>(smem + 16384 * (NW / 2)) + rw * 64 + l;
+        if (grp == 1) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                joined[64 * i] = float4{oacc[i >> 2][4 * (i & 3)], oacc[i >> 2][4 * (i & 3) + 1], oacc[i >> 2][4 * (i & 3) + 2],
+                                        oacc[i >> 2][4 * (i & 3) + 3]};
+            *stats = float2{m_run, l_run};
+        }
+        __syncthreads();
+        if (grp == 1) return;
+        const float2 other = *stats;
+        const float top = fmaxf(m_run, other.x);
+        // (a row without a key in both: sums of 0, or NaN, stay)
+        const float wa = m_run == top ? 1.0f : __builtin_amdgcn_exp2f(m_run - top);
+        const float wb = other.x == top ? 1.0f : __builtin_amdgcn_exp2f(other.x - top);
+        l_run = l_run * wa + other.y * wb;
+        m_run = top;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float4 o = joined[64 * i];
+            const float from[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int at = 4 * (i & 3) + c;
+                oacc[i >> 2][at] = oacc[i >> 2][at] * wa + from[c] * wb;
+            }
+        }
+    } else if (nblk > 0) {
         const Blk b0 = next_blk(0), b1 = next_blk(1);
         vq0 = next_blk(2);
         vq1 = next_blk(3);
@@ -1128,16 +1258,17 @@ AttnTiling attn_tiling(const Shape& s, bool dense, bool decode) {
     return AttnTiling{kBM, false, false, !dense, 16, dense ? kMaxDecodeSplits : kMaxPrefillSplits};
 }
 
-// Windows in tiles of 256 rows: their lists are of about one length (nkb blocks), so one split count for all requests, the
-// one with the least time by what was measured (bf16 and 4 bits alike): a round of 256 items takes 10 us and 1.5 us a
-// block, a merge 7 us and what it reads and writes (1032 bytes a partial row at 5.5 TB/s).  1000 queries under 1500 (28 Q /
-// 4 KV heads) 65 us whole, 58 in 2; 512 under 4096 (32 / 8) 96 and 55 in 4; 100 under 4096 95 and 33 in 8 to 16.
-static double window_us(const Shape& s, int nkb, int max_splits, int* splits) {
+// Windows in tiles of 256 or 128 rows: their lists are of about one length (nkb blocks), so one split count for all requests,
+// the one with the least time by what was measured (bf16 and 4 bits alike): a round of 256 items takes 10 us and 1.5 us a
+// block, or pair of blocks in tiles of 128 rows (attn_fwd_kernel's kPair), a merge 7 us and what it reads and writes (1032
+// bytes a partial row at 5.5 TB/s).
+static double window_us(const Shape& s, int tile_rows, int nkb, int max_splits, int* splits) {
     const int rows = s.Lq * s.G;
-    const double units = (double)s.B * s.Hkv * ((rows + kBM - 1) / kBM);
+    const double units = (double)s.B * s.Hkv * ((rows + tile_rows - 1) / tile_rows);
     double best = 0.0;
     for (int c = 1; c <= max_splits && c <= nkb; ++c) {
-        const double us = ceil(units * c / 256) * (10.0 + 1.5 * ((nkb + c - 1) / c)) +
+        const int blocks = (nkb + c - 1) / c;
+        const double us = ceil(units * c / 256) * (10.0 + 1.5 * (tile_rows < kBM ? (blocks + 1) / 2 : blocks)) +
                           (c > 1 ? 7.0 + 1.9e-4 * s.B * s.Hkv * rows * c : 0.0);
         if (c == 1 || us < best) {
             best = us;
@@ -1147,21 +1278,62 @@ static double window_us(const Shape& s, int nkb, int max_splits, int* splits) {
     return best;
 }
 
-// Windows over bf16 caches: tiles of 16 rows, whose waves take blocks on their own, take 12 us and 0.7 us for every block
-// that a CU's items have, tiles of 256 rows the time above (16 queries under 2048, 32 Q / 8 KV heads, 12.9 and 21 us; 256
-// under 2048, 8 / 8 heads, 21 and 32; 64 under 8192, 32 / 8, 54 and 42).
-AttnTiling attn_window_tiling(const Shape& s, const int32_t* kv_len, int window, int sinks) {
-    AttnTiling small{kDecRows, true, false, false, 4, 32}, large{kBM, false, false, false, 1, kMaxDecodeSplits};
-    small.window = large.window = true;
-    const int rows = s.Lq * s.G;
-    if (rows <= kDecRows) return small;
-    double blocks = 0.0;
-    int nkb = 1, splits = 1;
+// Windows in several tiles of 16 rows, whose waves take blocks on their own: an item takes 2 us and 4.5 for every eight blocks,
+// a merge 4 us and its reads.  whole: few blocks are better left so where their splits need a second round (90 queries under
+// 900, 28 Q / 4 KV heads, 160 items of 16 blocks, 16.1 us whole, 23.3 in 2).
+static int small_splits(int nb, double item_blocks, const AttnTiling& t) {
+    return max(1, min(min(static_cast<int>(nb / item_blocks + 0.5), max(1, nb / t.min_blocks)), t.max_splits));
+}
+static double small_window_us(const Shape& s, const int32_t* nkb, const AttnTiling& t, bool* whole) {
+    const int rows = s.Lq * s.G, ntiles = (rows + t.tile_rows - 1) / t.tile_rows;
+    double total = 0.0;
+    bool even = true;
     for (int b = 0; b < s.B; ++b) {
-        blocks += (double)s.Hkv * ((rows + kDecRows - 1) / kDecRows) * attn_window_blocks(s, kDecRows, kv_len[b] - s.Lq, window, sinks);
-        nkb = max(nkb, attn_window_blocks(s, kBM, kv_len[b] - s.Lq, window, sinks));
+        total += (double)s.Hkv * ntiles * nkb[b];
+        even = even && nkb[b] == nkb[0];
     }
-    return 12.0 + 0.7 * blocks / 256 < window_us(s, nkb, kMaxDecodeSplits, &splits) ? small : large;
+    auto time = [&](bool split) {
+        double all = 0.0, longest = 0.0, parts = 0.0;
+        for (int b = 0; b < s.B; ++b) {
+            const int c = split ? small_splits(nkb[b], total / 256, t) : 1;
+            const double us = 2.0 + 4.5 * (((nkb[b] + c - 1) / c + 7) / 8);
+            all += (double)s.Hkv * ntiles * c * us;
+            longest = fmax(longest, us);
+            if (c > 1) parts += (double)s.Hkv * rows * c;
+        }
+        // (rounds of 256 items; short ones fill the last)
+        return longest * fmax(1.0, ceil(all / (256 * longest) - (even ? 0.0 : 0.25))) + (parts > 0.0 ? 4.0 + 1.9e-4 * parts : 0.0);
+    };
+    const double one = time(false), cut = time(true);
+    *whole = one <= cut;
+    return fmin(one, cut);
+}
+
+// Windows over bf16 caches: of tiles of 16, 256 and 128 rows those with the least time by the above (of 16, 256 and 128 rows:
+// 16 queries under 2048, 32 Q / 8 KV heads, 12.3, 19, 20 us; 256 under 2048, 8 / 8 heads, 20, 30, 25; 64 under 8192, 32 / 8, 51,
+// 39, 31; 1000 under 1500, 28 / 4, 137, 60, 41; 2048 under 4096, 32 / 8, 664, 140, 156).
+AttnTiling attn_window_tiling(const Shape& s, const int32_t* kv_len, int window, int sinks) {
+    AttnTiling tiling[3] = {{kDecRows, true, false, false, 4, 32},
+                            {kBM, false, false, false, 1, kMaxDecodeSplits},
+                            {kBM / 2, false, false, false, 1, kMaxDecodeSplits}};
+    for (AttnTiling& t : tiling) t.window = true;
+    const int rows = s.Lq * s.G;
+    if (rows <= kDecRows) return tiling[0];
+    int32_t n[CA_MAX_BATCH];
+    for (int b = 0; b < s.B; ++b) n[b] = attn_window_blocks(s, kDecRows, kv_len[b] - s.Lq, window, sinks);
+    int best = 0;
+    bool whole;
+    double best_us = small_window_us(s, n, tiling[0], &whole);
+    for (int i = 1; i < 3; ++i) {
+        int nkb = 1, splits = 1;
+        for (int b = 0; b < s.B; ++b) nkb = max(nkb, attn_window_blocks(s, tiling[i].tile_rows, kv_len[b] - s.Lq, window, sinks));
+        const double us = window_us(s, tiling[i].tile_rows, nkb, kMaxDecodeSplits, &splits);
+        if (us < best_us) {
+            best = i;
+            best_us = us;
+        }
+    }
+    return tiling[best];
 }
 
 // The plan's split counts (its placement: attn_plan).
@@ -1207,7 +1379,7 @@ static void attn_plan_counts(const Shape& s, const int32_t* nkb, int forced, con
     // 16 are slower without, by 6 % on the average, none faster.
     int whole_if = 0;
     if (!dec && forced <= 0 && tiling.window) {
-        window_us(s, nkb_max, max_splits, &forced);
+        window_us(s, tiling.tile_rows, nkb_max, max_splits, &forced);
     } else if (!dec && forced <= 0) {
         // attn_fwd_kernel: one split count for every request.  Splitting in proportion to
         // each request's blocks measured slower on ragged batches (config 4: 380 vs 319 us
@@ -1359,6 +1531,9 @@ static void attn_plan_counts(const Shape& s, const int32_t* nkb, int forced, con
             }
         }
     }
+    bool whole = false;
+    if (dec && tiling.window && ntiles > 1 && forced <= 0) small_window_us(s, nkb, tiling, &whole);
+    if (whole) forced = 1;
     plan->max = 1;
     plan->off[0] = 0;
     for (int b = 0; b < s.B; ++b) {
@@ -1371,9 +1546,7 @@ static void attn_plan_counts(const Shape& s, const int32_t* nkb, int forced, con
         } else if (turns > 0) {
             sb = max(1, (expected(nb) + kTurn * turns - 1) / (kTurn * turns));
         } else if (forced <= 0) {
-            sb = static_cast<int>(nb / item_blocks + 0.5);
-            sb = min(sb, max(1, nb / min_blocks));
-            sb = max(1, min(sb, max_splits));
+            sb = small_splits(nb, item_blocks, tiling);
         }
         plan->s[b] = sb;
         plan->max = max(plan->max, sb);
@@ -1647,7 +1820,9 @@ hipError_t launch_attn(const AttnArgs& a, hipStream_t stream) {
     const bool streamed = kv_bytes >= kStreamBytes && !repeats(a.k) && !repeats(a.v);
     static_assert(kNW == kDecWaves, "one workgroup size for the attention kernels");
     if (a.window > 0)
-        tiling.streams ? launch(attn_window_decode_kernel) : launch(attn_fwd_kernel<kNW, false, false, true>);
+        tiling.streams              ? launch(attn_window_decode_kernel)
+        : tiling.tile_rows == kBM / 2 ? launch(attn_fwd_kernel<kNW, false, false, true, true>)
+                                      : launch(attn_fwd_kernel<kNW, false, false, true>);
     else if (a.table)
         row_res ? launch(attn_fwd_kernel<kNW, true, true>) : launch(attn_fwd_kernel<kNW, true, false>);
     else if (attn_uses_decode_kernel(a.s, true))
