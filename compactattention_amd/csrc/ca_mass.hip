@@ -223,7 +223,7 @@ __global__ __launch_bounds__(kMassWaves * 64) __attribute__((amdgpu_waves_per_eu
 // 32 / G tokens at a time from LDS (four places in turn: while one is read the next three tiles are on their way; through
 // registers and two places a chunk over 20 % of 32768 tokens took 161 us where it takes 150).  A launch may deal the tiles to
 // p.parts, each with workgroups of its own; their sums go to p.ws and are joined in order by key_mass_join_kernel.
-// Bound by vector instructions (one fma, exp2 and add a score, 16 of a wave's 64-lane cycles) beside 16 of the matrix cores:
+// Bound by vector instructions (one fma, exp2 and add a score: 24 cycles of a wave, beside 16 of the matrix cores):
 // 2048 queries over 32768 tokens (32 Q / 8 KV heads) 540 us, 0.98 PFLOP/s of the 1.21 that a large product reaches; 64 queries
 // 34 us, where a third is K's way from memory.  32x32x16 products, at two waves a SIMD where these run three, took 12 %
 // longer; products woven into the weights of the tile before, instruction by instruction, 10 %.
