@@ -1262,7 +1262,7 @@ AttnTiling attn_tiling(const Shape& s, bool dense, bool decode) {
 // the one with the least time by what was measured (bf16 and 4 bits alike): a round of 256 items takes 10 us and 1.5 us a
 // block, or pair of blocks in tiles of 128 rows (attn_fwd_kernel's kPair), a merge 7 us and what it reads and writes (1032
 // bytes a partial row at 5.5 TB/s).
-static double window_us(const Shape& s, int tile_rows, int nkb, int max_splits, int* splits) {
+double attn_window_us(const Shape& s, int tile_rows, int nkb, int max_splits, int* splits) {
     const int rows = s.Lq * s.G;
     const double units = (double)s.B * s.Hkv * ((rows + tile_rows - 1) / tile_rows);
     double best = 0.0;
@@ -1327,7 +1327,7 @@ AttnTiling attn_window_tiling(const Shape& s, const int32_t* kv_len, int window,
     for (int i = 1; i < 3; ++i) {
         int nkb = 1, splits = 1;
         for (int b = 0; b < s.B; ++b) nkb = max(nkb, attn_window_blocks(s, tiling[i].tile_rows, kv_len[b] - s.Lq, window, sinks));
-        const double us = window_us(s, tiling[i].tile_rows, nkb, kMaxDecodeSplits, &splits);
+        const double us = attn_window_us(s, tiling[i].tile_rows, nkb, kMaxDecodeSplits, &splits);
         if (us < best_us) {
             best = i;
             best_us = us;
@@ -1379,7 +1379,7 @@ static void attn_plan_counts(const Shape& s, const int32_t* nkb, int forced, con
     // 16 are slower without, by 6 % on the average, none faster.
     int whole_if = 0;
     if (!dec && forced <= 0 && tiling.window) {
-        window_us(s, tiling.tile_rows, nkb_max, max_splits, &forced);
+        attn_window_us(s, tiling.tile_rows, nkb_max, max_splits, &forced);
     } else if (!dec && forced <= 0) {
         // attn_fwd_kernel: one split count for every request.  Splitting in proportion to
         // each request's blocks measured slower on ragged batches (config 4: 380 vs 319 us

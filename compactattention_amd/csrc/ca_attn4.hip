@@ -1001,15 +1001,31 @@ __global__ __launch_bounds__(256) void attn4_merge_rows_kernel(Merge4Params p) {
 // 256 over 8 + 4 11.7, 26.8; 256 over 64 + 4 (8.5 blocks a CU) 26.5, 41; 256 over 256 + 4 (32.5) 78.4, 75.3,
 // with 30 % kept 32.7, 42.5; 512 over 128 + 8 (34) 87.5, 77.2, with 30 % kept 43.6, 43.0.  (Not always: 300 over
 // 40 + 5 with 28 / 4 heads, 6.3 blocks a CU, 39.3, 33.3.)
+// Under a window lists are short and tiles many: a round of 256 small tiles takes 7.3 us and 0.3 us a block, tiles of 256 rows
+// what they take of bf16 pages and 5 us (2021 queries under 71, 24 Q / 6 KV heads, small and large, 51.7, 22.7 us; 397 of 5
+// requests under 131, 32 / 8, 77.7, 52.6; 1000 under 1024, 8 / 8, 14.4, 39.1; 512 under 4096, 32 / 8, 54.6, 55.9).
 AttnTiling attn4_tiling(const Shape& s, const PastBlocks& pb, const int32_t* kv_len, int window, int sinks) {
     const bool dense = kv_len != nullptr;
     const int rows = s.Lq * s.G;
     int32_t qpos0[CA_MAX_BATCH], nkb[CA_MAX_BATCH];
     attn_positions(s, pb, kv_len, qpos0, nkb);
-    for (int b = 0; window > 0 && b < s.B; ++b) nkb[b] = attn_window_blocks(s, kBM, qpos0[b], window, sinks);
-    double blocks = 0.0;  // of 256 rows
-    for (int b = 0; b < s.B; ++b) blocks += (double)s.Hkv * ((rows + kBM - 1) / kBM) * nkb[b];
-    if (rows <= 160 || blocks <= 12.0 * 256)
+    bool small = rows <= 160;
+    if (window == 0) {
+        double blocks = 0.0;  // of 256 rows
+        for (int b = 0; b < s.B; ++b) blocks += (double)s.Hkv * ((rows + kBM - 1) / kBM) * nkb[b];
+        small = small || blocks <= 12.0 * 256;
+    } else if (!small) {
+        int most = 1, most_small = 1, splits;
+        for (int b = 0; b < s.B; ++b) {
+            most = max(most, attn_window_blocks(s, kBM, qpos0[b], window, sinks));
+            most_small = max(most_small, attn_window_blocks(s, 32, qpos0[b], window, sinks));
+        }
+        const double items = (double)s.B * s.Hkv * ((rows + 31) / 32);
+        const int c = max(1, static_cast<int>(256 / items));
+        const double us = ceil(items * c / 256) * (7.3 + 0.3 * ((most_small + c - 1) / c)) + (c > 1 ? 4.0 + 1.9e-4 * s.B * s.Hkv * rows * c : 0.0);
+        small = us < attn_window_us(s, kBM, most, kMaxDecodeSplits, &splits) + 5.0;
+    }
+    if (small)
         return AttnTiling{dense && rows <= 16 ? 16 : 32, true, true, !dense, 0, dense ? 32 : kMaxPrefillSplits};
     AttnTiling t = attn_tiling(s, dense, false);
     t.steps = true;

@@ -178,6 +178,8 @@ AttnTiling attn_window_tiling(const Shape& s, const int32_t* kv_len, int window,
 AttnTiling attn4_tiling(const Shape& s, const PastBlocks& pb, const int32_t* kv_len, int window = 0, int sinks = 0);
 // The blocks of a request's longest list under a window, with tiles of tile_rows packed rows
 int attn_window_blocks(const Shape& s, int tile_rows, int qpos0, int window, int sinks);
+// The time of a launch under a window in tiles of 256 (128) rows, of lists of nkb blocks, and its split count
+double attn_window_us(const Shape& s, int tile_rows, int nkb, int max_splits, int* splits);
 void attn_plan(const Shape& s, const int32_t* nkb, int forced, const AttnTiling& tiling, SplitPlan* plan);
 bool attn_uses_decode_kernel(const Shape& s, bool dense);
 void attn_positions(const Shape& s, const PastBlocks& pb, const int32_t* kv_len, int32_t* qpos0, int32_t* nkb);

@@ -65,7 +65,7 @@ def test_splits(kind, L, splits):
 CHUNKS = [([900, 64], 600, 16, 2, 400, 3), ([0], 1300, 8, 1, 900, 0), ([500], 2000, 7, 7, 100, 3), ([300], 2100, 16, 8, 200, 3)]
 
 
-@pytest.mark.parametrize("kind", ["paged", "heads"])
+@pytest.mark.parametrize("kind", ["paged", "heads", "q4"])
 @pytest.mark.parametrize("starts,L,Hq,Hkv,W,S", CHUNKS)
 def test_chunks(starts, L, Hq, Hkv, W, S, kind):
     cache, q = setup(starts, L, Hq, Hkv, W, S, kind, seed=L, strided=True)
@@ -73,18 +73,19 @@ def test_chunks(starts, L, Hq, Hkv, W, S, kind):
     check(out, lse, cache, q, starts, W, S)
 
 
-@pytest.mark.parametrize("case,splits", [(0, 2), (0, 3), (0, 64), (1, 5), (3, 3)])
-def test_splits_of_chunks(case, splits):
+@pytest.mark.parametrize("case,splits,kind", [(0, 2, "paged"), (0, 3, "paged"), (0, 64, "paged"), (1, 5, "paged"), (3, 3, "paged"), (0, 5, "q4"),
+                                              (3, 3, "q4")])
+def test_splits_of_chunks(case, splits, kind):
     starts, L, Hq, Hkv, W, S = CHUNKS[case]
-    cache, q = setup(starts, L, Hq, Hkv, W, S, "paged", seed=splits)
+    cache, q = setup(starts, L, Hq, Hkv, W, S, kind, seed=splits)
     out, lse = ops.attn_window(q, cache.K, cache.V, starts, W, S, SCALE, cache.cap, Hkv, with_lse=True, num_splits=splits)
     check(out, lse, cache, q, starts, W, S)
 
 
-@pytest.mark.parametrize("splits", [0, 2])
-@pytest.mark.parametrize("case", [0, 3])
-def test_chunks_with_values_that_are_not_finite(case, splits):
-    """Hidden from all queries: no effect.  Visible: a value in its dims, a NaN key in the whole output and the lse."""
+@pytest.mark.parametrize("case,splits,kind", [(0, 0, "paged"), (0, 2, "paged"), (3, 0, "paged"), (3, 2, "paged"), (0, 0, "q4"), (3, 0, "q4")])
+def test_chunks_with_values_that_are_not_finite(case, splits, kind):
+    """Hidden from all queries: no effect.  Visible: a value in its dims (in 4 bits NaN in its group's), a NaN key in the whole
+    output and the lse."""
     starts, L, Hq, Hkv, W, S = CHUNKS[case]
     k, v = random_kv(len(starts), Hkv, max(starts) + L, 8)
     for b, start in enumerate(starts):
@@ -94,12 +95,12 @@ def test_chunks_with_values_that_are_not_finite(case, splits):
         for i, j in enumerate((1, start + 5, start + L // 3, start + L - 70, start + L - 1)):
             v[b, i % Hkv, j, 17 * i] = (math.inf, -math.inf, math.nan)[i % 3]
     k[-1, 0, starts[-1] + L // 2, 9] = math.nan
-    cache, q = Cache(k, v, "paged", "cuda", 8), random_q(len(starts), L, Hq, 8, "cuda")
+    cache, q = Cache(k, v, kind, "cuda", 8), random_q(len(starts), L, Hq, 8, "cuda")
     out, lse = ops.attn_window(q, cache.K, cache.V, starts, W, S, SCALE, cache.cap, Hkv, with_lse=True, num_splits=splits)
     out, lse = out.cpu().double(), lse.cpu().double()
     ref, rlse, _, ltol = attention(q, cache, starts, W, S)
     assert torch.equal(torch.isnan(out), torch.isnan(ref)) and torch.equal(torch.isnan(lse), torch.isnan(rlse))
-    assert torch.isnan(rlse).any() and torch.isfinite(rlse).any() and torch.isinf(ref).any()
+    assert torch.isnan(rlse).any() and torch.isfinite(rlse).any() and (kind == "q4" or torch.isinf(ref).any())
     there = torch.isfinite(rlse)
     assert ((lse - rlse).abs()[there] <= ltol[there]).all()
     fin = torch.isfinite(ref)
