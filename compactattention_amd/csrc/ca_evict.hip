@@ -41,6 +41,31 @@ struct Found {
     int left;
 };
 
+// Weights of 0 are counted a wave at a time: keys of blocks that no table listed have none, and their lanes would wait for each
+// other at one bin (16384 tokens, four fifths of them 0 by blocks: 25 us a value at a time, 16 so; without zeros 16 and 17).
+constexpr uint32_t kZero = 0x80000000u;  // rank_bits(0)
+template <int kN, typename Value, typename In>
+__device__ __forceinline__ void count_values(int* hist, uint32_t prefix, int level, const Value& value, const In& in) {
+    const uint32_t high = level_high(level);
+    auto bin = [&](uint32_t u) { return (u >> level_shift(level)) & (level_bins(level) - 1); };
+    if ((kZero & high) == prefix) {
+        int zeros = 0;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const uint32_t u = value(i);
+            zeros += __popcll(__ballot(in(i) && u == kZero));
+            if (in(i) && u != kZero && (u & high) == prefix) atomicAdd(&hist[bin(u)], 1);
+        }
+        if ((threadIdx.x & 63) == 0 && zeros > 0) atomicAdd(&hist[bin(kZero)], zeros);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const uint32_t u = value(i);
+            if (in(i) && (u & high) == prefix) atomicAdd(&hist[bin(u)], 1);
+        }
+    }
+}
+
 // The bin that holds the left-th value from above, of the counts h0, h1 that thread i holds of bins - 1 - 2 i and the one
 // below (0 past the lowest); every thread gets the result.  sums: kPickWaves ints, got: 2 ints.
 __device__ __forceinline__ Found next_digit(Found f, int level, int h0, int h1, int* sums, int* got) {
@@ -105,10 +130,7 @@ __global__ __launch_bounds__(kPickThreads) void heavy_tokens_kernel(PickParams p
     for (int level = 0; level < kLevels; ++level) {
         for (int i = tid; i < kBins; i += kPickThreads) hist[i] = 0;
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            if (j0 + 64 * i + l < j1 && (u[i] & level_high(level)) == f.prefix)
-                atomicAdd(&hist[(u[i] >> level_shift(level)) & (level_bins(level) - 1)], 1);
+        count_values<kPer>(hist, f.prefix, level, [&](int i) { return u[i]; }, [&](int i) { return j0 + 64 * i + l < j1; });
         __syncthreads();
         const int b0 = level_bins(level) - 1 - 2 * tid;
         f = next_digit(f, level, b0 >= 1 ? hist[b0] : 0, b0 >= 1 ? hist[b0 - 1] : 0, sums, got);
@@ -240,15 +262,11 @@ __global__ __launch_bounds__(kPickThreads) void heavy_count_kernel(PickParams p)
         if (tid == 0) *slice_state(p, row, kLevel, slice) = SliceState{f.prefix, f.left, above, 0};
     }
     __syncthreads();
-    for (int j = j0 + tid; j < j1;) {
-#pragma unroll
-        for (int i = 0; i < kSliceAtOnce; ++i) {
-            const uint32_t u = rank_bits(x[i]);
-            if (j + kPickThreads * i < j1 && (u & level_high(kLevel)) == f.prefix)
-                atomicAdd(&hist[(u >> level_shift(kLevel)) & (level_bins(kLevel) - 1)], 1);
-        }
+    for (int j = j0; j < j1;) {
+        count_values<kSliceAtOnce>(hist, f.prefix, kLevel, [&](int i) { return rank_bits(x[i]); },
+                                   [&](int i) { return j + tid + kPickThreads * i < j1; });
         j += kPickThreads * kSliceAtOnce;
-        if (j < j1) load(j);
+        if (j < j1) load(j + tid);
     }
     __syncthreads();
     int* out = slice_hist(p, row, kLevel, slice);

@@ -52,6 +52,17 @@ def test_heavy_tokens(kind, lens, Hkv, budget, sinks, recent):
     assert torch.equal(keep.cpu(), want_keep(mass, lens, Hkv, budget, sinks, recent))
 
 
+@pytest.mark.parametrize("share", [0.0, 0.05, 0.2, 0.9])  # of the blocks of 64 keys that any query gave weight
+@pytest.mark.parametrize("n", [70, 3000, 16384, 20000, 70000])
+def test_weights_of_zero(n, share):
+    g = torch.Generator().manual_seed(n)
+    some = (torch.rand((2, n // 64 + 1), generator=g) < share).repeat_interleave(64, 1)[:, :n]
+    mass = (masses(2, n, "spread", n).cpu() * some * torch.randint(-1, 2, (2, n), generator=g).abs()).cuda()
+    for budget in (n // 10, n // 2, n - 5):
+        keep = ops.heavy_tokens(mass, n, 2, budget, 3, 4)
+        assert torch.equal(keep.cpu(), want_keep(mass, [n], 2, budget, 3, 4)), budget
+
+
 @pytest.mark.parametrize("columns", [0, 5])
 def test_requests_without_tokens(columns):
     mass = torch.ones((4, columns), device="cuda")
