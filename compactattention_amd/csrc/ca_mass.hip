@@ -43,7 +43,7 @@ struct MassParams {
 // XCD i % 8.  The parts of an item lie on XCDs of their own and the items of a row on all, so the XCDs carry equal work
 // whatever the lists' lengths, and the L2 of each holds its part of the queries (a chunk over 20 % of 32768 tokens 173 us
 // with a row's workgroups on one XCD, 158 so).  All blocks in one part: whole rows by XCD where they divide (64 queries over
-// 32768 tokens 40 us, 36 so).
+// 32768 tokens 40 us, 36 so; all four with tiles through registers).
 __device__ __forceinline__ void find_rows(const MassParams& p, int* row, int* item, int* cut) {
     const int x = blockIdx.x & 7, k = blockIdx.x >> 3;
     if (p.parts == 1 && p.table == nullptr && (p.s.B * p.s.Hkv) % 8 == 0) {
@@ -224,7 +224,7 @@ __global__ __launch_bounds__(kMassWaves * 64) __attribute__((amdgpu_waves_per_eu
 // registers and two places a chunk over 20 % of 32768 tokens took 161 us where it takes 150).  A launch may deal the tiles to
 // p.parts, each with workgroups of its own; their sums go to p.ws and are joined in order by key_mass_join_kernel.
 // Bound by vector instructions (one fma, exp2 and add a score: 24 cycles of a wave, beside 16 of the matrix cores):
-// 2048 queries over 32768 tokens (32 Q / 8 KV heads) 540 us, 0.98 PFLOP/s of the 1.21 that a large product reaches; 64 queries
+// 2048 queries over 32768 tokens (32 Q / 8 KV heads) 523 us, 1.02 PFLOP/s of the 1.21 that a large product reaches; 64 queries
 // 34 us, where a third is K's way from memory.  32x32x16 products, at two waves a SIMD where these run three, took 12 %
 // longer; products woven into the weights of the tile before, instruction by instruction, 10 %.
 constexpr int kTileRows = 32;
