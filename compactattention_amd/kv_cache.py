@@ -530,7 +530,8 @@ class PagedKVCache:
         self._upload(0, self.cap)
         self.length = budget
         self.evicted += n - budget
-        self._in_order_from = budget - recent
+        # (recent tokens that an earlier eviction picked do not follow the sequence)
+        self._in_order_from = budget - min(recent, n - self._in_order_from)
         self.kmean_blocks = 0
         return n - budget
 
