@@ -73,6 +73,13 @@ def token_mass_rowmask(query_states: torch.Tensor, khat: torch.Tensor, past: Seq
     return ops.select_scores(scores, rule, past, num_kv_heads, cap, 64 * scores.shape[2])
 
 
+def check_score_blocks(block_size: int, past_blocks: int) -> None:
+    """A selecting chunk starts at a whole score block."""
+    if block_size == 128 and past_blocks % 2:
+        raise ValueError(f"128-token FlashPrefill blocks need a chunk that starts at a multiple of 128 tokens "
+                         f"(past {64 * past_blocks} tokens)")
+
+
 def flashprefill_tables(qhat: torch.Tensor, khat: torch.Tensor, past_blocks: Sequence[int], q_len: int,
                         num_kv_heads: int, kv_cap: int, rule: ops.Rule, block_size: int,
                         khat_block_size: int = 64, score_mode: str = "pooled",
@@ -97,9 +104,9 @@ def flashprefill_tables(qhat: torch.Tensor, khat: torch.Tensor, past_blocks: Seq
             rowmask, _ = ops.score_select(qhat, khat, scale, rule, P, num_kv_heads, kv_cap)
         table, counts, _, _ = ops.union_compact(rowmask, P, num_kv_heads, kv_cap, last_n_block=rule.last_n_block)
         return table, counts
-    if len(set(P)) != 1 or P[0] % 2:
-        raise ValueError(f"128-token FlashPrefill blocks need a chunk that starts at a multiple of 128 tokens "
-                         f"(past {64 * P[0]} tokens)")
+    if len(set(P)) != 1:
+        raise ValueError("128-token FlashPrefill blocks need requests of one past length")
+    check_score_blocks(block_size, P[0])
     qb64 = -(-q_len // 64)
     last = q_len - 64 * (qb64 - 1)  # tokens of the chunk's last 64-token block
     kb64 = P[0] + qb64

@@ -23,6 +23,7 @@ from torch import nn
 
 from ... import ops
 from ...kv_cache import PagedKVCache
+from ...modules.flashprefill_prefill import check_score_blocks
 from .configuration_llama_seerattn import SeerAttnLlamaConfig
 
 BLOCK = 64
@@ -188,14 +189,18 @@ def position_qk(attn: nn.Module, q: torch.Tensor, k: torch.Tensor, cos: torch.Te
                             sin.float().contiguous())
 
 
+def check_decode_tokens(tokens: int) -> None:
+    if tokens > BLOCK:
+        raise ValueError(f"decode steps take at most {BLOCK} tokens per call (got {tokens})")
+
+
 def dense_decode_forward(attn: nn.Module, hidden_states: torch.Tensor, position_embeddings, cache: PagedKVCache):
     """Decode step(s) of a compactattn attention module: up to 64 new tokens per request
     attend densely to the whole cache (the reference routes q_len == 1 to dense attention,
     compact_attn/prefill_sparse/llama/modeling_llama_seerattn_chunked_dense.py:878-894).
     K/V of the new tokens are appended at the cache's current length."""
     B, L, _ = hidden_states.shape
-    if L > BLOCK:
-        raise ValueError(f"decode steps take at most {BLOCK} tokens per call (got {L})")
+    check_decode_tokens(L)
     q, k, v = project_qkv(attn, hidden_states)
     cos, sin = position_embeddings
     query_states, key_states = position_qk(attn, q, k, cos, sin)
@@ -253,6 +258,7 @@ class ChunkedPrefillCache:
                  with_kgate: bool):
         from ..attn_gate import gate_key_heads
 
+        self.config = config
         max_tokens = -(-max_tokens // BLOCK) * BLOCK
         kgate_heads = gate_key_heads(config.seerattn_gate_type, config.seerattn_gate_force_double,
                                      config.seerattn_compactattn_kv_group_aware_gate, config.num_attention_heads,
@@ -279,6 +285,23 @@ class ChunkedPrefillCache:
     def get_seq_length(self) -> int:
         """Tokens of the sequence so far, those among them that a layer no longer holds."""
         return self.layers[0].position
+
+    def check_step(self, tokens: int) -> None:
+        """Raise where some layer refuses a call of this many tokens (one under a window takes any).  Layer 0 asks before it
+        appends, so a refused call leaves all layers as they were, of one length."""
+        if tokens == 1:
+            return
+        c = self.config
+        for i, layer in enumerate(self.layers):
+            if c.window_of(i):
+                continue
+            past = layer.past_blocks
+            if layer.length % BLOCK:
+                check_decode_tokens(tokens)
+            elif past and not c.seerattn_chunked_prefill_force_dense:
+                layer.require_kgate(past)
+                if layer.kmean is not None:
+                    check_score_blocks(c.seerattn_flashprefill_block_size, past)
 
     def reset(self) -> None:
         """Start a new sequence in the same pages (pages shared by a fork are released)."""

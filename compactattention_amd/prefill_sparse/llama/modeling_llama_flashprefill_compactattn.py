@@ -73,6 +73,8 @@ class LlamaFlashPrefillCompactAttnAttention(nn.Module):
             raise ValueError("the compactattn prefill path needs a ChunkedPrefillCache")
         if attention_mask is not None and not bool(attention_mask.all()):
             raise ValueError("padded positions are not supported by the compactattn prefill path")
+        if self.layer_idx == 0:
+            past_key_value.check_step(hidden_states.shape[1])
         window = self.config.window_of(self.layer_idx)
         if window:
             with event_span(self.attention_timer):

@@ -186,6 +186,8 @@ class LlamaSeerAttentionChunkedDense(nn.Module):
             raise ValueError("padded positions are not supported by the compactattn prefill path")
         if block_position_embeddings is None:
             raise ValueError("block_position_embeddings (per-block rotary tables) are required")
+        if self.layer_idx == 0:
+            past_key_value.check_step(hidden_states.shape[1])
         window = self.config.window_of(self.layer_idx)
         if window:
             with event_span(self.attention_timer):

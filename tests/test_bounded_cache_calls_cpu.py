@@ -90,3 +90,66 @@ def test_slots_that_follow_the_sequence_after_two_evictions(plain, first, more, 
     want = torch.arange(float(c.position - follows), float(c.position))
     assert torch.equal(positions(c)[:, c.length - follows:], want.expand(2, follows))
     consistent(c)
+
+
+def models():
+    from compactattention_amd.prefill_sparse.llama.modeling_llama_flashprefill_compactattn import LlamaFlashPrefillCompactAttnAttention
+    from compactattention_amd.prefill_sparse.llama.modeling_llama_seerattn_chunked_dense import LlamaSeerAttentionChunkedDense
+
+    return {"flash": LlamaFlashPrefillCompactAttnAttention, "seer": LlamaSeerAttentionChunkedDense}
+
+
+@pytest.mark.parametrize("model,held,tokens,message", [
+    ("flash", 100, 200, "at most 64 tokens"), ("seer", 100, 65, "at most 64 tokens"),  # decoded tokens left it inside a block
+    ("flash", 192, 128, "multiple of 128 tokens"), ("seer", 128, 64, "gate-K summaries are missing"),
+])
+@pytest.mark.parametrize("windows", [[0], [0, 2], []])
+def test_a_refused_call_leaves_every_layer_as_it_was(model, held, tokens, message, windows):
+    """Layer 0 raises before it appends, also where it is under a window itself and another layer refuses."""
+    from compactattention_amd.prefill_sparse.llama import SeerAttnLlamaConfig
+    from compactattention_amd.prefill_sparse.llama.modeling_llama_common import ChunkedPrefillCache
+
+    kw = dict(sliding_window=40, sliding_window_layers=windows) if windows else {}
+    config = SeerAttnLlamaConfig(vocab_size=64, hidden_size=256, intermediate_size=128, num_hidden_layers=3, num_attention_heads=2,
+                                 num_key_value_heads=1, **kw)
+    config.validate()
+    attn = models()[model](config, 0)
+    caches = ChunkedPrefillCache(config, 1, 512, "cpu", with_kmean=model == "flash", with_kgate=model == "seer")
+    for layer in caches.layers:
+        x = torch.zeros((1, held, 1, 128), dtype=torch.bfloat16)
+        layer.append_tokens(x, x)
+    before = [(c.length, c.position, c._pt.copy(), c.pool.refs.copy()) for c in caches.layers]
+    cos = torch.zeros((tokens, 128))
+    blocks = torch.zeros((8, 128))
+    with pytest.raises(ValueError, match=message):
+        attn(torch.zeros((1, tokens, 256), dtype=torch.bfloat16), (cos, cos), past_key_value=caches, block_position_embeddings=(blocks, blocks))
+    for c, (length, position, pt, refs) in zip(caches.layers, before):
+        assert (c.length, c.position) == (length, position)
+        assert np.array_equal(c._pt, pt) and np.array_equal(c.pool.refs, refs)
+    assert caches.get_seq_length() == held
+
+
+def test_calls_that_no_layer_refuses():
+    from compactattention_amd.prefill_sparse.llama import SeerAttnLlamaConfig
+    from compactattention_amd.prefill_sparse.llama.modeling_llama_common import ChunkedPrefillCache
+
+    kw = dict(vocab_size=64, hidden_size=256, intermediate_size=128, num_hidden_layers=2, num_attention_heads=2, num_key_value_heads=1)
+    for extra in (dict(), dict(sliding_window=40, sliding_window_layers=[0])):
+        caches = ChunkedPrefillCache(SeerAttnLlamaConfig(**kw, **extra), 1, 512, "cpu", with_kmean=True, with_kgate=False)
+        for held, calls in ((0, (1, 2, 64, 300)), (100, (1, 64)), (128, (1, 2, 300)), (192, (1,))):
+            for layer in caches.layers:
+                x = torch.zeros((1, held - layer.length, 1, 128), dtype=torch.bfloat16)
+                layer.append_tokens(x, x)
+            for tokens in calls:
+                caches.check_step(tokens)
+    caches = ChunkedPrefillCache(SeerAttnLlamaConfig(**kw, sliding_window=40), 1, 512, "cpu", with_kmean=True, with_kgate=False)
+    for layer in caches.layers:
+        x = torch.zeros((1, 100, 1, 128), dtype=torch.bfloat16)
+        layer.append_tokens(x, x)
+    caches.check_step(300)  # windows alone
+    caches = ChunkedPrefillCache(SeerAttnLlamaConfig(**kw, seerattn_chunked_prefill_force_dense=True), 1, 512, "cpu", with_kmean=False,
+                                 with_kgate=True)
+    for layer in caches.layers:
+        x = torch.zeros((1, 192, 1, 128), dtype=torch.bfloat16)
+        layer.append_tokens(x, x)
+    caches.check_step(64)  # chunks that do not select
