@@ -73,8 +73,9 @@ class SeerAttnLlamaConfig:
     sliding_window_sinks: int = 0
     sliding_window_layers: Optional[List[int]] = None
     # tokens that every other layer's KV heads keep (0: all): the first kv_budget_sinks, the last kv_budget_recent and those that
-    # received most attention weight; dropped once there are kv_budget_slack more.  Weights are counted of the last
-    # kv_budget_observe queries of a chunk (0: all) and of every decoded token (FlashPrefill model)
+    # received most attention weight; the others go, where there are more than kv_budget_slack of them, before the next tokens
+    # are appended.  Weights are counted of the last kv_budget_observe queries of a chunk (0: all) and of every decoded token
+    # (FlashPrefill model)
     kv_budget: int = 0
     kv_budget_sinks: int = 4
     kv_budget_recent: int = 0

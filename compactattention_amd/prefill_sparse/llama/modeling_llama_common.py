@@ -212,14 +212,19 @@ def dense_decode_forward(attn: nn.Module, hidden_states: torch.Tensor, position_
     if cache.mass is not None:
         out, lse = out
         cache.add_mass(query_states, lse, attn.scaling)
-        keep_budget(attn.config, cache)
     return attn.o_proj(out.reshape(B, L, -1))
 
 
+def over_budget(config: SeerAttnLlamaConfig, cache: PagedKVCache) -> bool:
+    """Whether the layer evicts before its next tokens are appended (host work, so not while a graph is captured)."""
+    return (cache.mass is not None and cache.length > config.kv_budget + config.kv_budget_slack
+            and not torch.cuda.is_current_stream_capturing())
+
+
 def keep_budget(config: SeerAttnLlamaConfig, cache: PagedKVCache) -> None:
-    """Evict down to the config's kv_budget once the cache holds kv_budget_slack tokens more (host work, so not while a graph
-    is captured)."""
-    if cache.length > config.kv_budget + config.kv_budget_slack and not torch.cuda.is_current_stream_capturing():
+    """Evict down to the config's kv_budget where the cache holds more than kv_budget_slack tokens above it.  Called before new
+    tokens are appended, so that those of the last call, which may be a rejected draft, can still be truncated."""
+    if over_budget(config, cache):
         cache.evict(config.kv_budget, config.kv_budget_sinks, config.kv_budget_recent, keep_pages=True)
 
 
@@ -295,8 +300,9 @@ class ChunkedPrefillCache:
         for i, layer in enumerate(self.layers):
             if c.window_of(i):
                 continue
-            past = layer.past_blocks
-            if layer.length % BLOCK:
+            length = c.kv_budget if over_budget(c, layer) else layer.length
+            past = length // BLOCK
+            if length % BLOCK:
                 check_decode_tokens(tokens)
             elif past and not c.seerattn_chunked_prefill_force_dense:
                 layer.require_kgate(past)
@@ -310,7 +316,8 @@ class ChunkedPrefillCache:
 
     def truncate(self, tokens: int, keep_pages: bool = False) -> None:
         """Forget every layer's tokens past ``tokens`` of the sequence (a rejected draft).  A layer that has evicted tokens goes
-        back into its recent ones only, one under a window 64 tokens at least; else nothing is truncated and it raises."""
+        back to the start of the call before which it did and then into its recent ones, one under a window 64 tokens at least;
+        else nothing is truncated and it raises."""
         for c in self.layers:
             c.check_truncate(tokens - c.evicted)
         for c in self.layers:

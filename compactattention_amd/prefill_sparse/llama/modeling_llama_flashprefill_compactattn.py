@@ -81,6 +81,7 @@ class LlamaFlashPrefillCompactAttnAttention(nn.Module):
                 out = window_forward(self, hidden_states, position_embeddings, past_key_value.layer(self.layer_idx), window)
             self._compactattn_last_stats = {"path": "window"} if self.compactattn_debug else None
             return out, 0.0, None, None, None
+        keep_budget(self.config, past_key_value.layer(self.layer_idx))
         if is_decode_step(hidden_states, past_key_value.layer(self.layer_idx)):
             out = dense_decode_forward(self, hidden_states, position_embeddings, past_key_value.layer(self.layer_idx))
             self._compactattn_last_stats = {"path": "decode_dense"} if self.compactattn_debug else None
@@ -114,7 +115,6 @@ class LlamaFlashPrefillCompactAttnAttention(nn.Module):
                 seen = min(self.config.kv_budget_observe or L, L)  # the last queries vote for the keys that stay
                 cache.add_mass(query_states[:, L - seen:], lse[:, :, L - seen:], self.scaling, None if dense else table,
                                None if dense else counts)
-                keep_budget(self.config, cache)
         if self.table_sink is not None:  # per-chunk block counts (device tensors), for FLOP accounting
             self.table_sink.append((counts, L, past))
         out = self.o_proj(out.reshape(B, L, -1))

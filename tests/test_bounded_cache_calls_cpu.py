@@ -153,3 +153,22 @@ def test_calls_that_no_layer_refuses():
         x = torch.zeros((1, 192, 1, 128), dtype=torch.bfloat16)
         layer.append_tokens(x, x)
     caches.check_step(64)  # chunks that do not select
+
+
+def test_the_check_of_a_call_counts_the_eviction_before_it(monkeypatch):
+    from compactattention_amd.prefill_sparse.llama import SeerAttnLlamaConfig
+    from compactattention_amd.prefill_sparse.llama.modeling_llama_common import ChunkedPrefillCache
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    config = SeerAttnLlamaConfig(vocab_size=64, hidden_size=256, intermediate_size=128, num_hidden_layers=2, num_attention_heads=2,
+                                 num_key_value_heads=1, kv_budget=128)
+    caches = ChunkedPrefillCache(config, 1, 512, "cpu", with_kmean=True, with_kgate=False)
+    for held, refused in ((150, True), (192, True), (193, False), (300, False)):
+        for layer in caches.layers:
+            x = torch.zeros((1, held - layer.length, 1, 128), dtype=torch.bfloat16)
+            layer.append_tokens(x, x)
+        if refused:
+            with pytest.raises(ValueError):
+                caches.check_step(100)
+        else:
+            caches.check_step(100)

@@ -43,3 +43,49 @@ def test_a_refused_turn_can_be_sent_again_in_pieces(gpu, cls):
         for c in cache.layers:
             check_pool(c)
     assert torch.equal(*out)
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("draft", [2, 17, 64])
+def test_a_draft_past_the_budget_can_be_rejected(gpu, bits, draft):
+    """With the settings' defaults: a draft that takes the cache past budget and slack leaves all its tokens to be rejected, and the
+    next call evicts."""
+    m = model_of(FLASH, gpu, kv_budget=256, kv_cache_bits=bits)
+    ids = synthetic_prompt(2, 512, m.config.vocab_size, 5, gpu)
+    cache = m.new_cache(2, 512)
+    m(ids[:, :256], cache)
+    for t in range(256, 319):
+        m(ids[:, t:t + 1], cache)
+    m(ids[:, 319:319 + draft], cache)  # (319: inside a block, where more than one token is a draft)
+    assert all(c.length == 319 + draft and c.evicted == 0 for c in cache.layers)
+    for kept in (draft - 1, 1, 0):
+        cache.truncate(319 + kept)
+        assert cache.get_seq_length() == 319 + kept
+    m(ids[:, 319:319 + draft], cache)
+    cache.truncate(321)
+    logits = m(ids[:, 321:321 + draft], cache)  # the first call past the budget: it evicts before it appends
+    assert torch.isfinite(logits).all() and all(c.length == 256 + draft and c.evicted == 65 for c in cache.layers)
+    cache.truncate(321)
+    assert all(c.length == 256 for c in cache.layers) and cache.get_seq_length() == 321
+    for t in range(321, 500):
+        logits = m(ids[:, t:t + 1], cache)
+        assert all(256 < c.length <= 256 + 64 + 1 for c in cache.layers)
+    assert torch.isfinite(logits).all()
+    for c in cache.layers:
+        check_pool(c)
+
+
+def test_a_long_turn_after_an_eviction(gpu):
+    """A chunk that starts past the budget starts at it, so also where decoded tokens left the cache inside a block."""
+    m = model_of(FLASH, gpu, kv_budget=256)
+    ids = synthetic_prompt(1, 1024, m.config.vocab_size, 6, gpu)
+    cache = m.new_cache(1, 1024)
+    m(ids[:, :300], cache)
+    with pytest.raises(ValueError, match="at most 64"):
+        m(ids[:, 300:400], cache)  # 300 is within the slack
+    m(ids[:, 300:350], cache)
+    assert all(c.length == c.position == 350 for c in cache.layers)
+    logits = m(ids[:, 350:550], cache)  # evicted to 256, a whole block
+    assert torch.isfinite(logits).all() and all(c.length == 256 + 200 and c.position == 550 for c in cache.layers)
+    for c in cache.layers:
+        check_pool(c)
