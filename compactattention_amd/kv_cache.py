@@ -43,7 +43,7 @@ step must be recorded after the cache holds its pages (``reserve``).
 """
 from __future__ import annotations
 
-from typing import List, Optional, Tuple
+from typing import List, NamedTuple, Optional, Tuple
 
 import numpy as np
 import torch
@@ -148,6 +148,19 @@ class PagePool:
         return new_id
 
 
+class _Draft(NamedTuple):
+    """What takes the weights that a draft's queries gave back out of the keys' (truncate)."""
+
+    start: int  # slots [start, end) hold its tokens
+    end: int
+    before: torch.Tensor  # the weights [rows, start] without its queries'
+    q: torch.Tensor
+    lse: torch.Tensor
+    scale: float
+    table: Optional[torch.Tensor]
+    counts: Optional[torch.Tensor]
+
+
 class PagedKVCache:
     """One layer's paged K/V cache for ``batch`` requests that advance together."""
 
@@ -175,6 +188,7 @@ class PagedKVCache:
         self.evicted = 0  # tokens that evict has dropped per request
         self._in_order_from = 0  # slots from here on hold consecutive positions (slot + evicted)
         self._dropped = (0, 0, 0)  # drop_outside: blocks [a, b) have no pages, and the window that they were dropped for
+        self._draft: Optional[_Draft] = None  # the last add_mass, where it was a draft's
         self.kmean_blocks = 0  # leading blocks with a valid kmean
         self.kgate_blocks = 0  # leading blocks with a valid kgate
         self.kgate_tokens = 0  # tokens that those pooled (the last block's may end inside it); 0: not known
@@ -427,6 +441,15 @@ class PagedKVCache:
                 t[dst].copy_(t[src])
         if self.mass is not None:
             self.mass[dst * H:(dst + 1) * H].copy_(self.mass[src * H:(src + 1) * H])
+        if self._draft is not None:
+            d, of = self._draft, list(range(self.batch))
+            of[dst] = src
+            d.before[dst * H:(dst + 1) * H].copy_(d.before[src * H:(src + 1) * H])
+            table, counts = d.table, d.counts
+            if table is not None:
+                row = [b * H + h for b in of for h in range(H)]
+                table, counts = table[row], counts[row]
+            self._draft = d._replace(q=d.q[of], lse=d.lse[of], table=table, counts=counts)
 
     def check_truncate(self, tokens: int) -> None:
         """Raise where ``truncate(tokens)`` cannot be."""
@@ -444,8 +467,11 @@ class PagedKVCache:
         """Forget what every request holds past ``tokens`` tokens (a rejected draft, a shorter prefix); the pages
         behind them go back to the pool.  With keep_pages those that a row owns alone stay mapped, as in
         ``reset``.  Summaries that pooled a token that goes are no longer valid: a rejected draft after a chunk that
-        ended inside a block leaves that block's gate-K summary as it is."""
+        ended inside a block leaves that block's gate-K summary as it is.  The weights that the tokens' queries gave to
+        the keys that stay go too where they were the last that ``add_mass`` added, with draft; else they stay."""
         self.check_truncate(tokens)
+        if self._draft is not None and tokens < self._draft.end:
+            self._take_back(int(tokens))
         if self.mass is not None:
             self.mass[:, int(tokens):self.length] = 0.0
         nb = -(-int(tokens) // BLOCK)
@@ -465,17 +491,36 @@ class PagedKVCache:
 
     # -- bounded size ---------------------------------------------------------------------
     def add_mass(self, q: torch.Tensor, lse: torch.Tensor, scale: float, table: Optional[torch.Tensor] = None,
-                 counts: Optional[torch.Tensor] = None) -> None:
+                 counts: Optional[torch.Tensor] = None, draft: bool = False) -> None:
         """Add the attention weights of the queries q [B, L, Hq, 128] of the last L tokens to the keys' (``ops.key_mass``), with
-        the lse [B, Hq, L] that their attention returned, over all keys or the blocks of its table."""
+        the lse [B, Hq, L] that their attention returned, over all keys or the blocks of its table.  draft: these tokens may be
+        rejected; q, lse, table and counts are held until the next call, not to be changed, so that a ``truncate`` that takes
+        some of the tokens takes their weights too (not while a graph is captured)."""
         if self.mass is None:
             raise ValueError("cache built without the keys' weights (with_mass)")
         self._need_pages()
         L = q.shape[1]
         if L > self.length:
             raise ValueError(f"{L} queries over {self.length} tokens")
-        ops.key_mass(q, self.layouts()[0], lse, self.mass, self.length - L, scale, self.cap, self.num_kv_heads, table=table,
-                     counts=counts)
+        start, self._draft = self.length - L, None
+        if draft and not (self.mass.is_cuda and torch.cuda.is_current_stream_capturing()):
+            held = _Draft(start, self.length, self.mass[:, :start].clone(), q, lse, scale, table, counts)
+        else:
+            held = None
+        ops.key_mass(q, self.layouts()[0], lse, self.mass, start, scale, self.cap, self.num_kv_heads, table=table, counts=counts)
+        self._draft = held
+
+    def _take_back(self, tokens: int) -> None:
+        """Leave of the draft's weights those of its queries before slot ``tokens``."""
+        d, self._draft = self._draft, None
+        self.mass[:, :d.start].copy_(d.before)
+        self.mass[:, d.start:d.end] = 0.0
+        n = tokens - d.start
+        if n > 0:
+            d = d._replace(end=tokens, q=d.q[:, :n], lse=d.lse[:, :, :n])
+            ops.key_mass(d.q, self.layouts()[0], d.lse, self.mass, d.start, d.scale, self.cap, self.num_kv_heads, table=d.table,
+                         counts=d.counts)
+            self._draft = d
 
     def _take_pages(self, blocks: int) -> np.ndarray:
         """Pages [rows, blocks] for what eviction keeps: those that a row has mapped behind its tokens and owns alone, and new
@@ -509,6 +554,7 @@ class PagedKVCache:
         n = self.length
         if n <= budget:
             return 0
+        self._draft = None
         keep = ops.heavy_tokens(self.mass, n, self.num_kv_heads, budget, sinks, recent)
         blocks = -(-budget // BLOCK)
         pages = self._take_pages(blocks)
@@ -619,5 +665,6 @@ class PagedKVCache:
         self.length = 0
         self.evicted = self._in_order_from = 0
         self._dropped = (0, 0, 0)
+        self._draft = None
         self.kmean_blocks = 0
         self.set_kgate(0)

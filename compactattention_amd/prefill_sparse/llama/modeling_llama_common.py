@@ -211,7 +211,7 @@ def dense_decode_forward(attn: nn.Module, hidden_states: torch.Tensor, position_
                           with_lse=cache.mass is not None)
     if cache.mass is not None:
         out, lse = out
-        cache.add_mass(query_states, lse, attn.scaling)
+        cache.add_mass(query_states, lse, attn.scaling, draft=L > 1)
     return attn.o_proj(out.reshape(B, L, -1))
 
 

@@ -114,7 +114,7 @@ class LlamaFlashPrefillCompactAttnAttention(nn.Module):
                 out, lse = out
                 seen = min(self.config.kv_budget_observe or L, L)  # the last queries vote for the keys that stay
                 cache.add_mass(query_states[:, L - seen:], lse[:, :, L - seen:], self.scaling, None if dense else table,
-                               None if dense else counts)
+                               None if dense else counts, draft=1 < L <= BLOCK)  # (a draft at a block's start)
         if self.table_sink is not None:  # per-chunk block counts (device tensors), for FLOP accounting
             self.table_sink.append((counts, L, past))
         out = self.o_proj(out.reshape(B, L, -1))

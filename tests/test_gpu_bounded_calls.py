@@ -4,10 +4,13 @@ from __future__ import annotations
 import pytest
 import torch
 
+from compactattention_amd import ops
 from compactattention_amd.chunked_prefill import synthetic_prompt
+from compactattention_amd.kv_cache import PagedKVCache
 from compactattention_amd.prefill_sparse.llama import (SeerAttnLlamaChunkedDenseForCausalLM,
                                                        SeerAttnLlamaFlashPrefillCompactAttnForCausalLM)
-from tests.test_gpu_bounded_cache import check_pool
+from tests.bounded_oracle import SCALE
+from tests.test_gpu_bounded_cache import _rand, check_pool
 from tests.test_gpu_model import tiny_config
 
 pytestmark = pytest.mark.gpu
@@ -89,3 +92,86 @@ def test_a_long_turn_after_an_eviction(gpu):
     assert torch.isfinite(logits).all() and all(c.length == 256 + 200 and c.position == 550 for c in cache.layers)
     for c in cache.layers:
         check_pool(c)
+
+
+def drafted(gpu, bits, past, L, lists, draft=True, seed=0):
+    """A cache of past tokens with weights, and a draft of L tokens whose queries voted."""
+    B, H, Hq = 2, 2, 8
+    g = torch.Generator().manual_seed(seed)
+    c = PagedKVCache(B, H, 512, gpu, bits=bits, with_mass=True, with_kmean=False)
+    c.append_tokens(_rand(g, gpu, B, past, H, 128), _rand(g, gpu, B, past, H, 128))
+    c.mass[:, :past] = torch.rand((B * H, past), generator=g).to(gpu)
+    base = c.mass.clone()
+    c.append_tokens(_rand(g, gpu, B, L, H, 128), _rand(g, gpu, B, L, H, 128))
+    q = _rand(g, gpu, B, L, Hq, 128)
+    _, lse = ops.attn_decode(q, *c.layouts(), [c.length] * B, SCALE, c.cap, H, with_lse=True)
+    table = counts = None
+    if lists:
+        table = torch.zeros((B * H, c.cap), dtype=torch.int32, device=gpu)
+        table[:, :3] = torch.tensor([[0, 2, past // 64]], dtype=torch.int32)
+        counts = torch.full((B * H,), 3, dtype=torch.int32, device=gpu)
+        counts[1] = 2
+    c.add_mass(q, lse, SCALE, table, counts, draft=draft)
+    return c, base, q, lse, table, counts
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("past,L,lists", [(200, 20, False), (192, 20, True), (0, 7, False), (250, 64, False)])
+def test_the_weights_of_a_rejected_draft_go(gpu, bits, past, L, lists):
+    c, base, q, lse, table, counts = drafted(gpu, bits, past, L, lists)
+    for stays in (L - 1, 5, 5, 1, 0):
+        want = base.clone()
+        if stays:
+            ops.key_mass(q[:, :stays].clone(), c.layouts()[0], lse[:, :, :stays].clone(), want, past, SCALE, c.cap, c.num_kv_heads,
+                         table=table, counts=counts)
+        assert (want != base).any() == (stays > 0)
+        c.truncate(past + stays)
+        assert torch.equal(c.mass, want), stays
+    if past:
+        c.truncate(past - 5)
+        base[:, past - 5:] = 0
+        assert torch.equal(c.mass, base)
+
+
+def test_weights_of_drafts_between_other_calls(gpu):
+    L, past = 9, 130
+    # several calls back at once; and what is not called a draft stays
+    c, base, *_ = drafted(gpu, 16, past, L, False)
+    c.truncate(past - 1)
+    base[:, past - 1:] = 0
+    assert torch.equal(c.mass, base)
+    c, base, *_ = drafted(gpu, 16, past, L, False, draft=False)
+    after = c.mass.clone()
+    c.truncate(past)
+    assert torch.equal(c.mass[:, :past], after[:, :past]) and (c.mass[:, past:] == 0).all()
+    # tokens appended behind a draft that stays, and rejected
+    c, base, q, lse, _, _ = drafted(gpu, 16, past, L, False)
+    after = c.mass.clone()
+    x = torch.zeros((2, 3, 2, 128), dtype=torch.bfloat16, device=gpu)
+    c.append_tokens(x, x)
+    c.truncate(past + L)
+    assert torch.equal(c.mass, after)
+    # a later call's weights are added to those of the draft, which then stay
+    c.append_tokens(x, x)
+    c.add_mass(q[:, :3], lse[:, :, :3], SCALE)
+    after = c.mass.clone()
+    c.truncate(past + 2)
+    assert torch.equal(c.mass[:, :past + 2], after[:, :past + 2])
+    # a fork's weights go with those of the request that it shares
+    c, base, *_ = drafted(gpu, 16, past, L, True)
+    c.fork(1, 0)
+    c.truncate(past + 4)
+    one, base, *_ = drafted(gpu, 16, past, L, True)
+    one.truncate(past + 4)
+    assert torch.equal(c.mass[:2], c.mass[2:]) and torch.equal(c.mass[2:], one.mass[2:])
+    # an eviction or a new sequence forgets the draft
+    c, base, *_ = drafted(gpu, 16, past, L, False)
+    c.evict(100, recent=30)
+    mass = c.mass.clone()
+    c.truncate(80)
+    assert torch.equal(c.mass[:, :80], mass[:, :80])
+    c, base, *_ = drafted(gpu, 16, past, L, False)
+    c.reset(keep_pages=True)
+    c.append_tokens(x, x)
+    c.truncate(1)
+    assert (c.mass == 0).all()
