@@ -9,8 +9,8 @@ from compactattention_amd.chunked_prefill import synthetic_prompt
 from compactattention_amd.kv_cache import PagedKVCache
 from compactattention_amd.prefill_sparse.llama import (SeerAttnLlamaChunkedDenseForCausalLM,
                                                        SeerAttnLlamaFlashPrefillCompactAttnForCausalLM)
-from tests.bounded_oracle import SCALE
-from tests.test_gpu_bounded_cache import _rand, check_pool
+from tests.bounded_oracle import SCALE, kept, weights
+from tests.test_gpu_bounded_cache import _rand, check_pool, held
 from tests.test_gpu_model import tiny_config
 
 pytestmark = pytest.mark.gpu
@@ -175,3 +175,89 @@ def test_weights_of_drafts_between_other_calls(gpu):
     c.append_tokens(x, x)
     c.truncate(1)
     assert (c.mass == 0).all()
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("dense", [False, True])
+def test_the_weights_of_a_model_and_what_it_keeps(gpu, bits, dense, monkeypatch):
+    """Every call's weights against 64 bits on the cache's own keys, over the queries, log-sum-exps and lists of the attention itself;
+    every eviction against the weights; a rejected draft."""
+    m = model_of(FLASH, gpu, kv_budget=256, kv_budget_sinks=4, kv_budget_recent=30, kv_budget_slack=20, kv_budget_observe=50,
+                 kv_cache_bits=bits, seerattn_chunked_prefill_force_dense=dense, seerattn_flashprefill_block_size=64,
+                 seerattn_flashprefill_alpha=0.9, seerattn_flashprefill_attention_sink=0, seerattn_flashprefill_window_size=1,
+                 seerattn_flashprefill_last_n_block=0)
+    with torch.no_grad():
+        for layer in m.model.layers:  # block scores that differ
+            layer.self_attn.q_proj.weight.mul_(8)
+            layer.self_attn.k_proj.weight.mul_(8)
+    seen = {"attention": None, "votes": 0, "evictions": 0, "listed": 0, "last": {}}
+    reals = {n: getattr(ops, n) for n in ("attn_fwd", "attn_decode")}
+
+    def attention(name):
+        def call(q, K, V, *a, **kw):
+            out, lse = reals[name](q, K, V, *a, **kw)
+            seen["attention"] = (q, lse, a[0] if name == "attn_fwd" else None, a[1] if name == "attn_fwd" else None)
+            return out, lse
+        return call
+
+    add, evict = PagedKVCache.add_mass, PagedKVCache.evict
+
+    def add_mass(self, q, lse, scale, table=None, counts=None, draft=False):
+        L, n, before = q.shape[1], self.length, self.mass.clone()
+        add(self, q, lse, scale, table, counts, draft)
+        aq, alse, atable, acounts = seen["attention"]
+        assert L == min(aq.shape[1], 50) and torch.equal(q, aq[:, -L:]) and torch.equal(lse, alse[:, :, -L:])
+        lists = None
+        if table is not None:
+            assert torch.equal(table, atable) and torch.equal(counts, acounts)
+            lists = [table[r, :counts[r]].tolist() for r in range(self.rows)]
+            seen["listed"] += any(len(x) < -(-n // 64) for x in lists)
+        start = [n - L] * self.batch
+        want, tol = weights(q, held(self), lse, before[:, :n], start, 0, 0, lists=lists, scale=scale)
+        assert ((self.mass[:, :n].double().cpu() - want).abs() <= tol).all() and (self.mass[:, n:] == 0).all()
+        # a query's weights over the keys that it saw are a softmax: the sums of a KV head are its group's queries (the
+        # log-sum-exp is that of weights rounded to bf16, off by 2^-8 at most)
+        votes = L * m.config.num_key_value_groups
+        sums = (self.mass - before)[:, :n].double().sum(1).cpu()
+        slack = 2.0 ** -24 * self.mass[:, :n].double().sum(1).cpu() + tol.sum(1)
+        assert ((sums - votes).abs() <= votes * 2.0 ** -8 + slack).all()
+        seen["votes"] += 1
+        seen["last"][id(self)] = (before, q, lse, scale, lists, n - L)
+
+    def evicts(self, budget, sinks=0, recent=0, keep_pages=False):
+        n, k, v, w = self.length, self.k_hf().clone(), self.v_hf().clone(), self.mass.cpu().numpy().copy()
+        assert n > 256 + 20 and (budget, sinks, recent) == (256, 4, 30)
+        gone = evict(self, budget, sinks, recent, keep_pages)
+        for r in range(self.rows):
+            ids = torch.tensor(kept(w[r], n, budget, sinks, recent), device=gpu)
+            b, h = divmod(r, self.num_kv_heads)
+            assert torch.equal(self.k_hf()[b, h], k[b, h, ids]) and torch.equal(self.v_hf()[b, h], v[b, h, ids])
+            assert torch.equal(self.mass[r, :budget].cpu(), torch.from_numpy(w[r])[ids.cpu()])
+        seen["evictions"] += 1
+        return gone
+
+    for name in reals:
+        monkeypatch.setattr(ops, name, attention(name))
+    monkeypatch.setattr(PagedKVCache, "add_mass", add_mass)
+    monkeypatch.setattr(PagedKVCache, "evict", evicts)
+    ids = synthetic_prompt(1, 1280, m.config.vocab_size, 9, gpu)
+    cache = m.new_cache(1, 1280)
+    m(ids[:, :256], cache)
+    for a in range(256, 768, 64):  # (one query block each, so lists leave blocks out)
+        m(ids[:, a:a + 64], cache)
+    for t in range(768, 794):
+        m(ids[:, t:t + 1], cache)
+    # drafts, inside a block and past budget and slack: of 7 tokens 2 stay, of 9 none
+    for draft, stays in ((7, 2), (9, 0)):
+        at = cache.get_seq_length()
+        m(ids[:, at:at + draft], cache)
+        cache.truncate(at + stays)
+        for c in cache.layers:
+            before, q, lse, scale, lists, start = seen["last"][id(c)]
+            n = start + stays
+            want, tol = before[:, :n].double().cpu(), torch.zeros((c.rows, n))
+            if stays:
+                want, tol = weights(q[:, :stays], held(c), lse[:, :, :stays], before[:, :n], [start], 0, 0, lists=lists, scale=scale)
+            assert c.length == n and ((c.mass[:, :n].double().cpu() - want).abs() <= tol).all() and (c.mass[:, n:] == 0).all()
+    m(ids[:, 900:901], cache)
+    assert seen["votes"] == 2 * (9 + 26 + 2 + 1) and seen["evictions"] >= 2 * 2 and (seen["listed"] > 0) == (not dense)
