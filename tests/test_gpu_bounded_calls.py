@@ -108,7 +108,7 @@ def drafted(gpu, bits, past, L, lists, draft=True, seed=0):
     table = counts = None
     if lists:
         table = torch.zeros((B * H, c.cap), dtype=torch.int32, device=gpu)
-        table[:, :3] = torch.tensor([[0, 2, past // 64]], dtype=torch.int32)
+        table[:, :3] = torch.tensor([[0, 1, past // 64]], dtype=torch.int32)
         counts = torch.full((B * H,), 3, dtype=torch.int32, device=gpu)
         counts[1] = 2
     c.add_mass(q, lse, SCALE, table, counts, draft=draft)
