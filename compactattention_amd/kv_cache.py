@@ -159,6 +159,8 @@ class _Draft(NamedTuple):
     scale: float
     table: Optional[torch.Tensor]
     counts: Optional[torch.Tensor]
+    window: int
+    sinks: int
 
 
 class PagedKVCache:
@@ -491,9 +493,10 @@ class PagedKVCache:
 
     # -- bounded size ---------------------------------------------------------------------
     def add_mass(self, q: torch.Tensor, lse: torch.Tensor, scale: float, table: Optional[torch.Tensor] = None,
-                 counts: Optional[torch.Tensor] = None, draft: bool = False) -> None:
+                 counts: Optional[torch.Tensor] = None, draft: bool = False, window: int = 0, sinks: int = 0) -> None:
         """Add the attention weights of the queries q [B, L, Hq, 128] of the last L tokens to the keys' (``ops.key_mass``), with
-        the lse [B, Hq, L] that their attention returned, over all keys or the blocks of its table.  draft: these tokens may be
+        the lse [B, Hq, L] that their attention returned, over all keys or the blocks of its table, and under its window and
+        sinks (0: none; of slots, as the attention's).  draft: these tokens may be
         rejected; q, lse, table and counts are held until the next call, not to be changed, so that a ``truncate`` that takes
         some of the tokens takes their weights too (not while a graph is captured)."""
         if self.mass is None:
@@ -504,10 +507,11 @@ class PagedKVCache:
             raise ValueError(f"{L} queries over {self.length} tokens")
         start, self._draft = self.length - L, None
         if draft and not (self.mass.is_cuda and torch.cuda.is_current_stream_capturing()):
-            held = _Draft(start, self.length, self.mass[:, :start].clone(), q, lse, scale, table, counts)
+            held = _Draft(start, self.length, self.mass[:, :start].clone(), q, lse, scale, table, counts, window, sinks)
         else:
             held = None
-        ops.key_mass(q, self.layouts()[0], lse, self.mass, start, scale, self.cap, self.num_kv_heads, table=table, counts=counts)
+        ops.key_mass(q, self.layouts()[0], lse, self.mass, start, scale, self.cap, self.num_kv_heads, window=window, sinks=sinks,
+                     table=table, counts=counts)
         self._draft = held
 
     def _take_back(self, tokens: int) -> None:
@@ -518,8 +522,8 @@ class PagedKVCache:
         n = tokens - d.start
         if n > 0:
             d = d._replace(end=tokens, q=d.q[:, :n], lse=d.lse[:, :, :n])
-            ops.key_mass(d.q, self.layouts()[0], d.lse, self.mass, d.start, d.scale, self.cap, self.num_kv_heads, table=d.table,
-                         counts=d.counts)
+            ops.key_mass(d.q, self.layouts()[0], d.lse, self.mass, d.start, d.scale, self.cap, self.num_kv_heads, window=d.window,
+                         sinks=d.sinks, table=d.table, counts=d.counts)
             self._draft = d
 
     def _take_pages(self, blocks: int) -> np.ndarray:

@@ -178,6 +178,34 @@ def test_weights_of_drafts_between_other_calls(gpu):
 
 
 @pytest.mark.parametrize("bits", [4, 16])
+def test_the_weights_of_attention_under_a_window(gpu, bits):
+    """Keys that the window hid get none; eviction by them; a draft's taken back."""
+    B, H, Hq, W, S = 2, 2, 8, 70, 5
+    g = torch.Generator().manual_seed(bits)
+    c = PagedKVCache(B, H, 512, gpu, bits=bits, with_mass=True, with_kmean=False)
+    for L in (150, 1, 9, 1):
+        start = c.append_tokens(_rand(g, gpu, B, L, H, 128), _rand(g, gpu, B, L, H, 128))
+        q = _rand(g, gpu, B, L, Hq, 128)
+        _, lse = ops.attn_window(q, *c.layouts(), start, W, S, SCALE, c.cap, H, with_lse=True)
+        before, n = c.mass.clone(), c.length
+        c.add_mass(q, lse, SCALE, window=W, sinks=S, draft=L == 9)
+        want, tol = weights(q, held(c), lse, before[:, :n], [start] * B, W, S)
+        assert ((c.mass[:, :n].double().cpu() - want).abs() <= tol).all()
+        if start >= S + W:
+            assert torch.equal(c.mass[:, S:start - W + 1], before[:, S:start - W + 1])
+        if L == 9:
+            c.truncate(start + 4)
+            want, tol = weights(q[:, :4], held(c), lse[:, :, :4], before[:, :start + 4], [start] * B, W, S)
+            assert ((c.mass[:, :start + 4].double().cpu() - want).abs() <= tol).all()
+    w, n = c.mass.cpu().numpy().copy(), c.length
+    c.evict(100, S, W)
+    for r in range(B * H):
+        assert torch.equal(c.mass[r, :100].cpu(), torch.from_numpy(w[r])[kept(w[r], n, 100, S, W)])
+    with pytest.raises(ops._hip.CaError, match="window"):
+        c.add_mass(q[:, :1], lse[:, :, :1], SCALE, window=-1)
+
+
+@pytest.mark.parametrize("bits", [4, 16])
 @pytest.mark.parametrize("dense", [False, True])
 def test_the_weights_of_a_model_and_what_it_keeps(gpu, bits, dense, monkeypatch):
     """Every call's weights against 64 bits on the cache's own keys, over the queries, log-sum-exps and lists of the attention itself;
