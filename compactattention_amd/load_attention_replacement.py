@@ -209,7 +209,7 @@ def load_llama_attention_replacement_model(
     sliding_window_layers: Optional[List[int]] = None,
     kv_budget: int = 0,
     kv_budget_sinks: int = 4,
-    kv_budget_recent: int = 0,
+    kv_budget_recent: Optional[int] = None,
     kv_budget_slack: int = 64,
     kv_budget_observe: int = 64,
 ) -> nn.Module:
@@ -242,8 +242,8 @@ def load_llama_attention_replacement_model(
     seer_cfg.sliding_window, seer_cfg.sliding_window_sinks = int(sliding_window), int(sliding_window_sinks)
     seer_cfg.sliding_window_layers = sliding_window_layers
     seer_cfg.kv_budget, seer_cfg.kv_budget_sinks = int(kv_budget), int(kv_budget_sinks)
-    seer_cfg.kv_budget_recent, seer_cfg.kv_budget_slack = int(kv_budget_recent), int(kv_budget_slack)
-    seer_cfg.kv_budget_observe = int(kv_budget_observe)
+    seer_cfg.kv_budget_recent = None if kv_budget_recent is None else int(kv_budget_recent)
+    seer_cfg.kv_budget_slack, seer_cfg.kv_budget_observe = int(kv_budget_slack), int(kv_budget_observe)
     seer_cfg.validate()
     block_rope = _BlockRope(model.model.rotary_emb, seer_cfg.max_position_embeddings)
     cls = _VARIANTS[variant]

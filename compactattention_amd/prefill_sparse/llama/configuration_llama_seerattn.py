@@ -74,11 +74,12 @@ class SeerAttnLlamaConfig:
     sliding_window_layers: Optional[List[int]] = None
     # tokens that every other layer's KV heads keep (0: all): the first kv_budget_sinks, the last kv_budget_recent and those that
     # received most attention weight; the others go, where there are more than kv_budget_slack of them, before the next tokens
-    # are appended.  Weights are counted of the last kv_budget_observe queries of a chunk (0: all) and of every decoded token
-    # (FlashPrefill model)
+    # are appended.  kv_budget_recent None: 64, or what the sinks leave of the budget (with none, tokens just decoded compete
+    # with the weights of thousands of queries and go first).  Weights are counted of the last kv_budget_observe queries of a
+    # chunk (0: all) and of every decoded token (FlashPrefill model)
     kv_budget: int = 0
     kv_budget_sinks: int = 4
-    kv_budget_recent: int = 0
+    kv_budget_recent: Optional[int] = None
     kv_budget_slack: int = 64
     kv_budget_observe: int = 64
 
@@ -100,6 +101,10 @@ class SeerAttnLlamaConfig:
     def window_of(self, layer: int) -> int:
         """The sliding window of a layer, 0 for none."""
         return self.sliding_window if self.sliding_window_layers is None or layer in self.sliding_window_layers else 0
+
+    def budget_recent(self) -> int:
+        """The recent tokens that a layer with a budget keeps."""
+        return min(64, self.kv_budget - self.kv_budget_sinks) if self.kv_budget_recent is None else self.kv_budget_recent
 
     def validate(self) -> None:
         if self.head_dim != 128:
@@ -123,9 +128,9 @@ class SeerAttnLlamaConfig:
                                  f"{self.num_hidden_layers}")
         if self.kv_budget < 0 or self.kv_budget % self.seerattn_flashprefill_block_size:
             raise ValueError("kv_budget must be a multiple of seerattn_flashprefill_block_size (a chunk that follows starts there)")
-        if min(self.kv_budget_sinks, self.kv_budget_recent, self.kv_budget_slack, self.kv_budget_observe) < 0:
+        if min(self.kv_budget_sinks, self.kv_budget_recent or 0, self.kv_budget_slack, self.kv_budget_observe) < 0:
             raise ValueError("kv_budget_sinks, kv_budget_recent, kv_budget_slack and kv_budget_observe must not be negative")
-        if self.kv_budget and self.kv_budget_sinks + self.kv_budget_recent > self.kv_budget:
+        if self.kv_budget and self.kv_budget_sinks + max(self.budget_recent(), 0) > self.kv_budget:
             raise ValueError("kv_budget must hold kv_budget_sinks and kv_budget_recent")
         from ..attn_gate import parse_gate_type
 

@@ -225,7 +225,7 @@ def keep_budget(config: SeerAttnLlamaConfig, cache: PagedKVCache) -> None:
     """Evict down to the config's kv_budget where the cache holds more than kv_budget_slack tokens above it.  Called before new
     tokens are appended, so that those of the last call, which may be a rejected draft, can still be truncated."""
     if over_budget(config, cache):
-        cache.evict(config.kv_budget, config.kv_budget_sinks, config.kv_budget_recent, keep_pages=True)
+        cache.evict(config.kv_budget, config.kv_budget_sinks, config.budget_recent(), keep_pages=True)
 
 
 def window_forward(attn: nn.Module, hidden_states: torch.Tensor, position_embeddings, cache: PagedKVCache, window: int

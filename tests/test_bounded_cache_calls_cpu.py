@@ -172,3 +172,32 @@ def test_the_check_of_a_call_counts_the_eviction_before_it(monkeypatch):
                 caches.check_step(100)
         else:
             caches.check_step(100)
+
+
+@pytest.mark.parametrize("settings,recent", [(dict(), 64), (dict(kv_budget_recent=0), 0), (dict(kv_budget_sinks=100), 28),
+                                             (dict(kv_budget_sinks=128), 0), (dict(kv_budget=1024, kv_budget_recent=500), 500)])
+def test_recent_tokens_that_a_budget_keeps(settings, recent):
+    """Tokens just decoded have had few queries: where the setting says nothing, the last ones stay whatever their weights."""
+    from compactattention_amd.prefill_sparse.llama import SeerAttnLlamaConfig
+
+    config = SeerAttnLlamaConfig(**{"kv_budget": 128, **settings})
+    config.validate()
+    assert config.budget_recent() == recent
+    again = SeerAttnLlamaConfig.from_dict(config.to_dict())
+    assert again.budget_recent() == recent
+    with pytest.raises(ValueError, match="kv_budget"):
+        SeerAttnLlamaConfig(kv_budget=128, kv_budget_sinks=129).validate()
+
+
+def test_a_layer_evicts_with_its_settings(plain, monkeypatch):
+    from compactattention_amd.prefill_sparse.llama import SeerAttnLlamaConfig
+    from compactattention_amd.prefill_sparse.llama.modeling_llama_common import keep_budget
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    c = cache(200)
+    c.mass[:, 136:] = 0  # decoded tokens without a query yet
+    keep_budget(SeerAttnLlamaConfig(kv_budget=128, kv_budget_slack=72), c)
+    assert c.length == 200
+    keep_budget(SeerAttnLlamaConfig(kv_budget=128, kv_budget_slack=71), c)
+    assert c.length == 128 and torch.equal(positions(c)[:, 64:], torch.arange(136.0, 200.0).expand(2, 64))
+    assert torch.equal(positions(c)[:, :4], torch.arange(4.0).expand(2, 4))
