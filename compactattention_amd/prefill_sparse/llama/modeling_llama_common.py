@@ -27,6 +27,7 @@ from ...modules.flashprefill_prefill import check_score_blocks
 from .configuration_llama_seerattn import SeerAttnLlamaConfig
 
 BLOCK = 64
+CHUNK_TOKENS = 2048  # of a chunk, as caches of bounded size are planned (longer ones grow them)
 
 
 class FusedProjections:
@@ -215,6 +216,15 @@ def dense_decode_forward(attn: nn.Module, hidden_states: torch.Tensor, position_
     return attn.o_proj(out.reshape(B, L, -1))
 
 
+def budget_tokens(config: SeerAttnLlamaConfig, max_tokens: int) -> int:
+    """Slots of a layer with a budget: budget, slack and a chunk, and behind them the pages that an eviction moves the budget into."""
+    most = config.kv_budget + config.kv_budget_slack
+    if max_tokens <= most:  # never evicts
+        return max_tokens
+    whole = lambda n: -(-n // BLOCK) * BLOCK
+    return whole(min(max_tokens, most + CHUNK_TOKENS)) + whole(config.kv_budget)
+
+
 def over_budget(config: SeerAttnLlamaConfig, cache: PagedKVCache) -> bool:
     """Whether the layer evicts before its next tokens are appended (host work, so not while a graph is captured)."""
     return (cache.mass is not None and cache.length > config.kv_budget + config.kv_budget_slack
@@ -273,16 +283,17 @@ class ChunkedPrefillCache:
         for i in range(config.num_hidden_layers):
             window = config.window_of(i)
             if window:  # no summaries, and pages for the sinks, the window and a chunk (the pool grows where more are needed)
-                held = min(max_tokens, window + config.sliding_window_sinks + 2048)
+                held = min(max_tokens, window + config.sliding_window_sinks + CHUNK_TOKENS)
                 self.layers.append(PagedKVCache(batch, config.num_key_value_heads, max_tokens, device, with_kmean=False,
                                                 bits=config.kv_cache_bits, pool_pages=rows * (held // BLOCK + 4)))
                 continue
-            self.layers.append(PagedKVCache(batch, config.num_key_value_heads, max_tokens, device, with_kmean=with_kmean,
+            held = budget_tokens(config, max_tokens) if config.kv_budget else max_tokens
+            self.layers.append(PagedKVCache(batch, config.num_key_value_heads, held, device, with_kmean=with_kmean,
                                             with_kgate=with_kgate, kgate_heads=kgate_heads, bits=config.kv_cache_bits,
                                             with_mass=config.kv_budget > 0))
-            # pages for max_tokens up front, so a prefill of that length maps nothing on the way;
+            # pages for what it holds up front, so a prefill of that length maps nothing on the way;
             # a longer sequence grows the pool and the page tables on demand
-            self.layers[-1].reserve(max_tokens)
+            self.layers[-1].reserve(held)
 
     def layer(self, idx: int) -> PagedKVCache:
         return self.layers[idx]

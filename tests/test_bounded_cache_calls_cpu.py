@@ -201,3 +201,46 @@ def test_a_layer_evicts_with_its_settings(plain, monkeypatch):
     keep_budget(SeerAttnLlamaConfig(kv_budget=128, kv_budget_slack=71), c)
     assert c.length == 128 and torch.equal(positions(c)[:, 64:], torch.arange(136.0, 200.0).expand(2, 64))
     assert torch.equal(positions(c)[:, :4], torch.arange(4.0).expand(2, 4))
+
+
+def budget_caches(max_tokens, **kw):
+    from compactattention_amd.prefill_sparse.llama import SeerAttnLlamaConfig
+    from compactattention_amd.prefill_sparse.llama.modeling_llama_common import ChunkedPrefillCache
+
+    config = SeerAttnLlamaConfig(vocab_size=64, hidden_size=256, intermediate_size=128, num_hidden_layers=1, num_attention_heads=2,
+                                 num_key_value_heads=2, **{"kv_budget": 256, **kw})
+    config.validate()
+    return config, ChunkedPrefillCache(config, 1, max_tokens, "cpu", with_kmean=False, with_kgate=False)
+
+
+@pytest.mark.parametrize("budget,slack,max_tokens,slots", [(256, 64, 131072, 256 + 64 + 2048 + 256), (256, 0, 1000, 1024 + 256), (256, 100, 356, 384 + 256),
+                                                           (256, 64, 320, 320), (256, 64, 8192, 256 + 64 + 2048 + 256),
+                                                           (1024, 8192, 4096, 4096), (4096, 70, 131072, 6272 + 4096)])
+def test_a_layer_with_a_budget_holds_pages_for_it(budget, slack, max_tokens, slots):
+    """Not for the sequence: budget, slack, a chunk of 2048 and the pages that an eviction moves the budget into."""
+    _, caches = budget_caches(max_tokens, kv_budget=budget, kv_budget_slack=slack)
+    c = caches.layer(0)
+    assert c.cap == slots // 64 and c.pool.num_pages == 2 * (slots // 64) and c.mass.shape == (2, slots)
+    assert c.pool.free_pages == 0 and (c._pt >= 0).all()
+
+
+def test_a_long_run_with_a_budget_takes_no_more_pages(plain, monkeypatch):
+    from compactattention_amd.prefill_sparse.llama.modeling_llama_common import keep_budget
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    config, caches = budget_caches(131072)
+    c = caches.layer(0)
+    pages, cap = c.pool.num_pages, c.cap
+    g = torch.Generator().manual_seed(0)
+    for n in [2048, 2048, 2048, 700, 1, 64, 2048] + [1] * 70 + [64] * 6 + [2048, 300, 21, 64, 2048]:
+        keep_budget(config, c)
+        x = torch.randn((1, n, 2, 128), generator=g).to(torch.bfloat16)
+        c.append_tokens(x, x)
+        c.mass[:, :c.length] += torch.rand((2, c.length), generator=g)
+        consistent(c)
+    assert (c.pool.num_pages, c.cap) == (pages, cap) and c.position > 5 * 2048
+    keep_budget(config, c)
+    assert c.length == 256
+    c.reset(keep_pages=True)
+    consistent(c)
+    assert c.pool.num_pages == pages
