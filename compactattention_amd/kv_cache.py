@@ -111,10 +111,10 @@ class PagePool:
     def _grow(self, need: int) -> None:
         old = self.num_pages
         new = max(2 * old, old + need)
-        for name in ("k", "v"):
-            t = self._pages(new)
-            t[:old].copy_(getattr(self, name))
-            setattr(self, name, t)
+        k, v = self._pages(new), self._pages(new)  # (both or neither, should memory run out)
+        k[:old].copy_(self.k)
+        v[:old].copy_(self.v)
+        self.k, self.v = k, v
         self.refs = np.concatenate([self.refs, np.zeros(new - old, np.int32)])
         self._free = list(range(new - 1, old - 1, -1)) + self._free
 
@@ -185,7 +185,8 @@ class PagedKVCache:
         self.kgate_heads = kgate_heads or num_kv_heads
         self.kmean = self._summary(num_kv_heads) if with_kmean else None
         self.kgate = self._summary(self.kgate_heads) if with_kgate else None
-        self.mass = self._weights() if with_mass else None  # [rows, cap * 64]; 0 from the length on
+        # the keys' weights, 0 from the length on
+        self.mass = torch.zeros((self.rows, self.cap * BLOCK), dtype=torch.float32, device=self.device) if with_mass else None
         self.length = 0  # tokens stored per request
         self.evicted = 0  # tokens that evict has dropped per request
         self._in_order_from = 0  # slots from here on hold consecutive positions (slot + evicted)
@@ -198,9 +199,6 @@ class PagedKVCache:
     # -- layout ---------------------------------------------------------------------------
     def _summary(self, heads: int) -> torch.Tensor:
         return torch.zeros((self.batch, heads, self.cap, HEAD_DIM), dtype=torch.float32, device=self.device)
-
-    def _weights(self) -> torch.Tensor:
-        return torch.zeros((self.rows, self.cap * BLOCK), dtype=torch.float32, device=self.device)
 
     @property
     def position(self) -> int:
@@ -226,23 +224,22 @@ class PagedKVCache:
     def _grow_cap(self, blocks: int) -> None:
         if blocks <= self.cap:
             return
-        new = max(2 * self.cap, blocks)
+        old, new = self.cap, max(2 * self.cap, blocks)
         pt = np.full((self.rows, new), -1, np.int32)
-        pt[:, :self.cap] = self._pt
-        self._pt = pt
-        dev_pt = torch.full((self.rows, new), -1, dtype=torch.int32, device=self.device)
-        dev_pt[:, :self.cap].copy_(self.page_table)
-        self.page_table = dev_pt
+        pt[:, :old] = self._pt
+        grown = {"page_table": torch.full((self.rows, new), -1, dtype=torch.int32, device=self.device)}
+        grown["page_table"][:, :old].copy_(self.page_table)
         for name in ("kmean", "kgate"):
-            old = getattr(self, name)
-            if old is not None:
-                t = torch.zeros((old.shape[0], old.shape[1], new, HEAD_DIM), dtype=torch.float32, device=self.device)
-                t[:, :, :self.cap].copy_(old)
-                setattr(self, name, t)
-        old_cap, self.cap = self.cap, new
+            t = getattr(self, name)
+            if t is not None:
+                grown[name] = torch.zeros((t.shape[0], t.shape[1], new, HEAD_DIM), dtype=torch.float32, device=self.device)
+                grown[name][:, :, :old].copy_(t)
         if self.mass is not None:
-            old, self.mass = self.mass, self._weights()
-            self.mass[:, :old_cap * BLOCK].copy_(old)
+            grown["mass"] = torch.zeros((self.rows, new * BLOCK), dtype=torch.float32, device=self.device)
+            grown["mass"][:, :old * BLOCK].copy_(self.mass)
+        for name, t in grown.items():  # (all or none, should memory run out)
+            setattr(self, name, t)
+        self._pt, self.cap = pt, new
 
     def _upload(self, b0: int, b1: int) -> None:
         if b1 > b0:
@@ -535,10 +532,11 @@ class PagedKVCache:
         for r in range(self.rows):
             own = [int(p) for p in tail[r] if p >= 0 and self.pool.refs[p] == 1][:blocks]
             out[r, :len(own)] = own
-            tail[r][np.isin(tail[r], own)] = -1
         need = out < 0
         if need.any():
-            out[need] = self.pool.alloc(int(need.sum()))
+            out[need] = self.pool.alloc(int(need.sum()))  # (may raise, so before the table changes)
+        for r in range(self.rows):
+            tail[r][np.isin(tail[r], out[r])] = -1
         return out
 
     def evict(self, budget: int, sinks: int = 0, recent: int = 0, keep_pages: bool = False) -> int:
@@ -546,7 +544,7 @@ class PagedKVCache:
         by the weights that they received.  They move, in order, into other pages (pages that a fork shares stay as they are), the
         old ones go back to the pool, or with keep_pages stay mapped behind where a row owns them alone.  Mean-K summaries are
         computed again before they are next read; a cache with gate-K summaries, which pool keys that it does not hold,
-        raises.  Returns how many tokens of a row went."""
+        raises.  Where memory runs out the cache stays as it was.  Returns how many tokens of a row went."""
         if self.mass is None:
             raise ValueError("cache built without the keys' weights (with_mass)")
         if self.kgate is not None:
@@ -558,15 +556,21 @@ class PagedKVCache:
         n = self.length
         if n <= budget:
             return 0
-        self._draft = None
         keep = ops.heavy_tokens(self.mass, n, self.num_kv_heads, budget, sinks, recent)
         blocks = -(-budget // BLOCK)
+        was = self._pt.copy()
         pages = self._take_pages(blocks)
-        K, V = self.layouts()  # (of the pool as it is now: it may have grown)
-        table = torch.from_numpy(pages).to(self.device)
-        make = ops.KV4.paged if self.bits == 4 else ops.KV.paged
-        moved = ops.move_tokens(K, V, make(self.pool.k, table), make(self.pool.v, table), keep, n, self.num_kv_heads,
-                                mass=self.mass)
+        try:
+            K, V = self.layouts()  # (of the pool as it is now: it may have grown)
+            table = torch.from_numpy(pages).to(self.device)
+            make = ops.KV4.paged if self.bits == 4 else ops.KV.paged
+            moved = ops.move_tokens(K, V, make(self.pool.k, table), make(self.pool.v, table), keep, n, self.num_kv_heads,
+                                    mass=self.mass)
+        except BaseException:
+            self.pool.release(pages[~np.isin(pages, was)])
+            self._pt = was
+            raise
+        self._draft = None
         self.mass[:, :budget].copy_(moved)
         self.mass[:, budget:n] = 0.0
         old = self._pt

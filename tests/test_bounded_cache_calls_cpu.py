@@ -244,3 +244,62 @@ def test_a_long_run_with_a_budget_takes_no_more_pages(plain, monkeypatch):
     c.reset(keep_pages=True)
     consistent(c)
     assert c.pool.num_pages == pages
+
+
+# reserved: pages behind the tokens (none, some of those that move, all)
+@pytest.mark.parametrize("where,reserved", [("alloc", 0), ("alloc", 320), ("pool", 0), ("pool", 320), ("move", 0), ("move", 320), ("move", 640)])
+def test_an_eviction_without_memory_leaves_the_cache_as_it_was(plain, monkeypatch, where, reserved):
+    c = PagedKVCache(1, 2, 640, "cpu", with_kmean=False, with_mass=True, pool_pages=8)
+    append(c, 250)
+    c.mass[:, :250] = torch.rand((2, 250), generator=torch.Generator().manual_seed(1))
+    if reserved:
+        c.reserve(reserved)
+
+    def out_of_memory(*a, **kw):
+        raise torch.OutOfMemoryError("none left")
+
+    old = (c.length, c.position, c._pt.copy(), c.pool.refs.copy(), c.mass.clone(), c.k_hf().clone())
+    with monkeypatch.context() as m:
+        if where == "alloc":
+            m.setattr(c.pool, "alloc", out_of_memory)
+        elif where == "pool":  # the second of a larger pool's two tensors
+            real, calls = c.pool._pages, []
+            m.setattr(c.pool, "_pages", lambda n: calls.append(n) or (real(n) if len(calls) == 1 else out_of_memory()))
+            c.pool._free, free = [], c.pool._free
+        else:
+            m.setattr(ops, "move_tokens", out_of_memory)
+        with pytest.raises(torch.OutOfMemoryError):
+            c.evict(190)
+        if where == "pool":
+            c.pool._free = free
+    assert (c.length, c.position) == old[:2] and np.array_equal(c._pt, old[2]) and torch.equal(c.mass, old[4])
+    assert np.array_equal(c.pool.refs[:old[3].size], old[3]) and (c.pool.refs[old[3].size:] == 0).all()
+    assert c.pool.k.shape == c.pool.v.shape and torch.equal(c.k_hf(), old[5])
+    consistent(c)
+    assert c.evict(190) == 60
+    consistent(c)
+
+
+@pytest.mark.parametrize("fails", [1, 2, 3])
+def test_tables_and_weights_that_cannot_grow_stay(monkeypatch, fails):
+    """The page table on the device, the mean keys and the weights grow together."""
+    c = PagedKVCache(1, 2, 64, "cpu", with_mass=True)
+    full, zeros, calls = torch.full, torch.zeros, []
+
+    def counted(real):
+        def make(*a, **kw):
+            calls.append(1)
+            if len(calls) == fails:
+                raise torch.OutOfMemoryError("none left")
+            return real(*a, **kw)
+        return make
+
+    with monkeypatch.context() as m:
+        m.setattr(torch, "full", counted(full))
+        m.setattr(torch, "zeros", counted(zeros))
+        with pytest.raises(torch.OutOfMemoryError):
+            c.reserve(320)
+    assert c.cap == 1 and c._pt.shape == (2, 1) and c.page_table.shape == (2, 1)
+    assert c.kmean.shape[2] == 1 and c.mass.shape == (2, 64)
+    c.reserve(320)
+    assert c.cap == 5 and c.page_table.shape == (2, 5) and c.kmean.shape[2] == 5 and c.mass.shape == (2, 320)
