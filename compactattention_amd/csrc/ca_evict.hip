@@ -443,7 +443,8 @@ __global__ __launch_bounds__(256) void move_tokens_kernel(MoveParams p) {
 
 }  // namespace
 
-// Rows of up to 16384 tokens are held in one workgroup's registers, longer ones are cut into slices of about 8192.
+// Rows of up to 16384 tokens are held in one workgroup's registers, longer ones are cut into slices of about 8192, at most 32 of
+// them: past 262144 tokens slices are longer, and their workgroups go through them in several loads.
 static int heavy_slices(int longest) { return longest <= 16 * kPickThreads ? 1 : min((longest + kSlice - 1) / kSlice, 32); }
 
 int64_t heavy_tokens_workspace_bytes(int rows, int longest, int budget) {
