@@ -513,15 +513,15 @@ class PagedKVCache:
 
     def _take_back(self, tokens: int) -> None:
         """Leave of the draft's weights those of its queries before slot ``tokens``."""
-        d, self._draft = self._draft, None
-        self.mass[:, :d.start].copy_(d.before)
-        self.mass[:, d.start:d.end] = 0.0
-        n = tokens - d.start
+        d, n = self._draft, tokens - self._draft.start
+        left = torch.zeros((self.rows, d.end), dtype=torch.float32, device=self.device)
+        left[:, :d.start].copy_(d.before)
         if n > 0:
             d = d._replace(end=tokens, q=d.q[:, :n], lse=d.lse[:, :, :n])
-            ops.key_mass(d.q, self.layouts()[0], d.lse, self.mass, d.start, d.scale, self.cap, self.num_kv_heads, window=d.window,
+            ops.key_mass(d.q, self.layouts()[0], d.lse, left, d.start, d.scale, self.cap, self.num_kv_heads, window=d.window,
                          sinks=d.sinks, table=d.table, counts=d.counts)
-            self._draft = d
+        self.mass[:, :left.shape[1]].copy_(left)
+        self._draft = d if n > 0 else None
 
     def _take_pages(self, blocks: int) -> np.ndarray:
         """Pages [rows, blocks] for what eviction keeps: those that a row has mapped behind its tokens and owns alone, and new

@@ -177,6 +177,25 @@ def test_weights_of_drafts_between_other_calls(gpu):
     assert (c.mass == 0).all()
 
 
+def test_weights_of_a_captured_draft(gpu):
+    """A graph adds in place at every replay and holds nothing to take back; a draft before it is forgotten."""
+    c, base, q, lse, _, _ = drafted(gpu, 16, 130, 9, False)
+    with torch.cuda.device(gpu):
+        graph = torch.cuda.CUDAGraph()
+        before = c.mass.clone()
+        with torch.cuda.graph(graph):
+            c.add_mass(q, lse, SCALE, draft=True)
+        assert c._draft is None and torch.equal(c.mass, before)
+        want = before.clone()
+        for _ in range(3):
+            graph.replay()
+            ops.key_mass(q, c.layouts()[0], lse, want, 130, SCALE, c.cap, c.num_kv_heads)
+            torch.cuda.synchronize()
+            assert torch.equal(c.mass, want)
+        c.truncate(130)
+        assert torch.equal(c.mass[:, :130], want[:, :130]) and (c.mass[:, 130:] == 0).all()
+
+
 @pytest.mark.parametrize("bits", [4, 16])
 def test_the_weights_of_attention_under_a_window(gpu, bits):
     """Keys that the window hid get none; eviction by them; a draft's taken back."""
