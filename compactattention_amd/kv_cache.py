@@ -653,14 +653,19 @@ class PagedKVCache:
     def reset(self, keep_pages: bool = False) -> None:
         """Empty the cache.  By default every request's pages go back to the pool (which keeps
         its size); with keep_pages the pages a row owns alone stay mapped for the next
-        sequence (no allocation or page-table upload when it refills them), while pages
-        shared with another request are released so a refill never writes into them."""
+        sequence (no allocation or page-table upload when it refills them; those of a cache that
+        dropped pages move to its start), while pages shared with another request are released
+        so a refill never writes into them."""
         if keep_pages:
             mapped = self._pt >= 0
             shared = mapped & (self.pool.refs[np.where(mapped, self._pt, 0)] > 1)
             if shared.any():
                 self.pool.release(self._pt[shared])
                 self._pt[shared] = -1
+            if self._dropped[0] < self._dropped[1]:  # what a window left mapped at its end goes to the start
+                order = np.argsort(self._pt < 0, axis=1, kind="stable")
+                self._pt = np.take_along_axis(self._pt, order, axis=1)
+            if shared.any() or self._dropped[0] < self._dropped[1]:
                 self._upload(0, self.cap)
         else:
             mapped = self._pt[self._pt >= 0]

@@ -303,3 +303,29 @@ def test_tables_and_weights_that_cannot_grow_stay(monkeypatch, fails):
     assert c.kmean.shape[2] == 1 and c.mass.shape == (2, 64)
     c.reserve(320)
     assert c.cap == 5 and c.page_table.shape == (2, 5) and c.kmean.shape[2] == 5 and c.mass.shape == (2, 320)
+
+
+@pytest.mark.parametrize("sinks", [0, 70])
+def test_sequences_under_a_window_start_again_in_the_same_pages(sinks):
+    """Pages that a window has left behind leave those of its end mapped far from the start, where a new sequence begins."""
+    window, chunk = 200, 300
+    blocks = -(-sinks // 64) + (window + chunk) // 64 + 3
+    c = PagedKVCache(2, 2, 4096, "cpu", with_kmean=False, pool_pages=4 * blocks)
+    for _ in range(3):
+        for n in [chunk] * 9 + [1] * 5 + [64, 1]:
+            x = torch.zeros((2, n, 2, 128), dtype=torch.bfloat16)
+            c.append_tokens(x, x)
+            c.drop_outside(window, sinks, slack=64)
+        assert c.pool.num_pages == 4 * blocks
+        used = c.pool.refs.sum()
+        c.reset(keep_pages=True)
+        consistent(c)
+        assert c.pool.refs.sum() == used and (c._pt[:, :used // 4] >= 0).all()
+    c.fork(0, 1)
+    x = torch.zeros((2, 900, 2, 128), dtype=torch.bfloat16)
+    c.append_tokens(x, x)
+    c.drop_outside(window, sinks)
+    c.fork(0, 1)  # pages that two requests share go back
+    c.reset(keep_pages=True)
+    consistent(c)
+    assert c.pool.refs.max() <= 1
