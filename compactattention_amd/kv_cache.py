@@ -493,9 +493,9 @@ class PagedKVCache:
                  counts: Optional[torch.Tensor] = None, draft: bool = False, window: int = 0, sinks: int = 0) -> None:
         """Add the attention weights of the queries q [B, L, Hq, 128] of the last L tokens to the keys' (``ops.key_mass``), with
         the lse [B, Hq, L] that their attention returned, over all keys or the blocks of its table, and under its window and
-        sinks (0: none; of slots, as the attention's).  draft: these tokens may be
-        rejected; q, lse, table and counts are held until the next call, not to be changed, so that a ``truncate`` that takes
-        some of the tokens takes their weights too (not while a graph is captured)."""
+        sinks (0: none; of slots, as the attention's).  draft: these tokens may be rejected; q, lse, table and counts are held
+        until the next call, not to be changed, so that a ``truncate`` that takes some of the tokens takes their weights too
+        (not while a graph is captured)."""
         if self.mass is None:
             raise ValueError("cache built without the keys' weights (with_mass)")
         self._need_pages()

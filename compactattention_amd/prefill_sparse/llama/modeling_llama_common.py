@@ -221,13 +221,13 @@ def budget_tokens(config: SeerAttnLlamaConfig, max_tokens: int) -> int:
     most = config.kv_budget + config.kv_budget_slack
     if max_tokens <= most:  # never evicts
         return max_tokens
-    whole = lambda n: -(-n // BLOCK) * BLOCK
-    return whole(min(max_tokens, most + CHUNK_TOKENS)) + whole(config.kv_budget)
+    held, moved = min(max_tokens, most + CHUNK_TOKENS), config.kv_budget
+    return BLOCK * (-(-held // BLOCK) - (-moved // BLOCK))
 
 
 def over_budget(config: SeerAttnLlamaConfig, cache: PagedKVCache) -> bool:
     """Whether the layer evicts before its next tokens are appended (host work, so not while a graph is captured)."""
-    return (cache.mass is not None and cache.length > config.kv_budget + config.kv_budget_slack
+    return (cache.mass is not None and 0 < config.kv_budget < cache.length - config.kv_budget_slack
             and not torch.cuda.is_current_stream_capturing())
 
 
